@@ -217,6 +217,129 @@ int qvx_qmatmul_swiglu(float* d_out, const void* d_w_gu, uint32_t type, const fl
 int qvx_interleave_rows16(void* d_dst, const void* d_a, const void* d_b, uint32_t type, int rows, int cols,
                           void* stream);
 
+/* ---- attention: the paged key / value cache, and an encoder's states ----------------------- */
+/* What a serving step does between the q / k / v and the o projections (runtime/src/text_model.cpp:
+ * 150-158): page tables, rotary positions with the append to the cache, attention of the new token;
+ * and a decoder's attention to an encoder's states.  Activations are fp32, softmax statistics and sums
+ * at least that.  All four calls are asynchronous on `stream`, allocate nothing and keep nothing between
+ * calls, so they can be captured into a graph and replayed while the device data they read changes;
+ * calls that may overlap need workspaces of their own (two graphs too).  Row lengths, page ids, slots
+ * and positions are read on the device and checked there: what lies outside is left out as described,
+ * never read or written. */
+
+/* A paged cache of one layer: pages of page_size tokens, page p at d_k + p * page_stride bytes (and
+ * d_v), each [kv_heads][page_size][head_dim] values.  type: F32, F16, BF16, or Q8_0 with a page's int8
+ * quants in that order first and the fp16 scales of their blocks of 32, [kv_heads][page_size]
+ * [head_dim / 32], behind them (Q8_0's values with rows on aligned addresses).  head_dim: a
+ * multiple of 8 (Q8_0: 32) up to 256.  page_stride: a multiple of 16 of at least qvx_kv_page_bytes, 0
+ * for exactly that; larger strides interleave layers, or K and V.  The descriptions are host memory,
+ * read during the call. */
+typedef struct qvx_kv_cache {
+  void* d_k;
+  void* d_v;
+  int64_t page_stride;
+  uint32_t type;
+  int32_t n_pages, page_size, kv_heads, head_dim;
+} qvx_kv_cache;
+
+/* Bytes of a page of K (or V), a multiple of 16; 0 for a type or shape that the cache does not take. */
+size_t qvx_kv_page_bytes(uint32_t type, int kv_heads, int page_size, int head_dim);
+
+/* Status bits of qvx_kv_map, stored on the device. */
+#define QVX_MAP_PAGES 1    /* the free list does not reach */
+#define QVX_MAP_COLUMNS 2  /* a sequence would outgrow its row of the table */
+#define QVX_MAP_ROWS 4     /* more new tokens than max_tokens */
+#define QVX_MAP_NEGATIVE 8 /* a negative length or count */
+/* Page tables and slots of a step's new tokens, from the sequences' lengths (the reference grows a
+ * session's page list on the host, memory/include/qorvix/memory/kv_cache.hpp:36-59).  Sequence b of
+ * n_seqs (1 .. 16384) holds d_held[b] tokens and gets d_new[b] more (0 allowed).  Its new pages, columns
+ * ceil(held / page_size) .. ceil((held + new) / page_size) - 1 of its row of d_table [n_seqs,
+ * table_width], are taken from d_free [n_free] in sequence order, behind the d_taken_in[0] that earlier
+ * calls took.  The new tokens of all sequences, one behind the other, are the rows t < max_tokens of
+ *   d_slots[t] = page id * page_size + position % page_size (what qvx_rope_kv takes), -1 if the table's
+ *                id is negative or the slot passes 31 bits,
+ *   d_pos[t]   = the token's position, d_seq[t] = its sequence (either may be NULL);
+ * rows behind the last token get -1, 0 and -1.  d_lens[b] = held + new, d_offsets[0 .. n_seqs] = each
+ * sequence's first row and their number, d_taken_out[0] = pages taken so far, d_taken_out[1] = status.
+ * All or nothing: unless the status is 0 no table entry changes, the lengths are d_held's, the count
+ * d_taken_in's, and every row is one behind the last token.  d_lens may be d_held and d_taken_out may
+ * be d_taken_in (2 values; then a second launch stores them), any other overlap of the outputs with d_held, d_new
+ * or d_taken_in -> QVX_E_RANGE. */
+int qvx_kv_map(const int32_t* d_held, const int32_t* d_new, int n_seqs, int32_t* d_table, int table_width,
+               int page_size, const int32_t* d_free, int n_free, const int32_t* d_taken_in, int32_t* d_taken_out,
+               int32_t* d_lens, int32_t* d_offsets, int32_t* d_slots, int32_t* d_pos, int32_t* d_seq,
+               int max_tokens, void* stream);
+
+/* A rotation: pair i < rot_dim / 2 of a head turns by position[axis[i]] * inv_freq[i] radians, its
+ * cosine and sine times `scale`.  d_inv_freq [rot_dim / 2] doubles (any scaling of frequencies, per pair,
+ * is the caller's); d_axis [rot_dim / 2], NULL: all on axis 0, ids past n_axes - 1 count as that one.
+ * pairing QVX_ROPE_HALVES: values i and i + rot_dim / 2; QVX_ROPE_PAIRS: values 2 i and 2 i + 1.
+ * Values from rot_dim on pass unturned.  rot_dim: a multiple of 8 up to head_dim (0: none turns);
+ * n_axes 1 .. 4. */
+#define QVX_ROPE_HALVES 0
+#define QVX_ROPE_PAIRS 1
+typedef struct qvx_rope {
+  const double* d_inv_freq;
+  const uint8_t* d_axis;
+  int32_t rot_dim, n_axes, pairing;
+  float scale;
+} qvx_rope;
+
+/* Rotary positions with several axes, and the append to the cache, in one launch (rope and the cache
+ * store of cuda/src/cuda_backend.cu:249-272, 274-346).  q_out[t] = rotated q[t]; rotated k[t] and v[t] are
+ * stored in the cache at d_slots[t], rounded once to its type (Q8_0: scale = max|x| / 127 of a block in
+ * fp16, quants to the nearest of x / scale).  Token t's heads lie side by side at d_q + t * q_stride
+ * (elements; likewise q_out, k, v), so parts of one stacked product can be passed.  d_pos [n_axes]
+ * [pos_stride] int32; angles are formed in 64 bits.  A token whose slot is negative or past the cache
+ * is padding: none of its rows is written, q_out's neither.  q_out may be q itself (the same stride);
+ * slots of one call are distinct, else which token's values a row holds is not specified.
+ * cache NULL: q alone is rotated (d_k, d_v, d_slots are not read), as an image encoder's q and k. */
+int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t q_stride, int q_heads,
+                const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens, int head_dim,
+                const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
+                const int32_t* d_slots, void* stream);
+
+/* Attention of one new token a sequence over the paged cache (attentionDecodeKernel,
+ * cuda/src/cuda_backend.cu:347-409): out[b, h] = softmax(scale q[b, h] . K)  V over the first d_lens[b] tokens
+ * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head
+ * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and
+ * out_stride elements apart; out may be q.  Long sequences are split over workgroups and joined in a
+ * second launch, in the same order in every run: equal inputs give equal bits.  A length of 0 gives zeros; lengths
+ * are cut to table_width * page_size; tokens on page ids outside the cache do not count; rows of the
+ * cache behind a sequence's last token are not read.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less -> QVX_E_RANGE; its
+ * contents need not be kept or cleared). */
+int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q_stride, int q_heads,
+                   const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens,
+                   int n_seqs, float scale, void* d_ws, size_t ws_bytes, void* stream);
+/* Workspace of that call; 0 also where it needs none, or would be refused. */
+size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width);
+
+/* An encoder's keys and values: value i of head h of state j of sequence b at d_k[b * batch_stride +
+ * j * row_stride + h * head_stride + i] (elements; d_v alike), F32, F16 or BF16, max_len states a sequence at most.
+ * Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and under 64 Mi bytes.  head_dim: a multiple of 8
+ * up to 256. */
+typedef struct qvx_kv_states {
+  const void* d_k;
+  const void* d_v;
+  int64_t batch_stride, row_stride, head_stride;
+  uint32_t type;
+  int32_t max_len, kv_heads, head_dim;
+} qvx_kv_states;
+
+/* Cross attention to an encoder's states of another length (a speech decoder's second attention, an
+ * image model's attention to text): the queries d_offsets[b] .. d_offsets[b + 1] - 1 of n_q attend the
+ * first d_lens[b] states of sequence b (0: zeros; NULL: all max_len), none masked by position.
+ * d_offsets NULL: n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  Rows behind the last
+ * sequence's are left as they were.  q and out share q_type: F32, F16 or BF16, rows and heads as in
+ * qvx_attn_paged.  Where q and the states share a 16-bit type and there are many queries, both
+ * products run on the 16-bit matrix cores and the softmax weights are rounded to that type (sums
+ * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout. */
+int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                   const int32_t* d_offsets, int n_q, const qvx_kv_states* states, const int32_t* d_lens, int n_seqs,
+                   float scale, void* d_ws, size_t ws_bytes, void* stream);
+/* Workspace of that call; 0 also where it needs none, or would be refused. */
+size_t qvx_attn_cross_ws(const qvx_kv_states* states, uint32_t q_type, int q_heads, int n_q, int n_seqs);
+
 /* Prefill GEMM: out[m * rows + r] = sum_k X[m, k] * dequant(W)[r, k] for m < M, X fp16 [M, cols].
  * No reference counterpart (the reference prefills token by token); semantics are qmatmulN's
  * with X converted fp16 -> fp32 exactly.  variant = QVX_GEMM_BF16 | QVX_GEMM_F16 | QVX_GEMM_I8;

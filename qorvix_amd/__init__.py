@@ -34,8 +34,13 @@ E_FORMAT, E_IO, E_LIB = -9, -10, -11
 # GEMM variants
 GEMM_BF16, GEMM_I8, GEMM_F16 = 0, 1, 2
 
+# pairings of a rotation, and the status bits of kv_map
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+MAP_PAGES, MAP_COLUMNS, MAP_ROWS, MAP_NEGATIVE = 1, 2, 4, 8
+
 # The C ABI: name -> (argtypes, restype).  tests/test_capi.py checks this table against qvx.h.
 _vp, _u32, _i32, _sz, _u64, _f32 = C.c_void_p, C.c_uint32, C.c_int, C.c_size_t, C.c_uint64, C.c_float
+_i64 = C.c_int64
 SIGNATURES = {
     "qvx_version": ([], C.c_char_p),
     "qvx_strerror": ([_i32], C.c_char_p),
@@ -55,6 +60,13 @@ SIGNATURES = {
     "qvx_swiglu": ([_vp, _vp, _vp, _sz, _vp], _i32),
     "qvx_dequantize": ([_u32, _vp, _vp, _sz, _vp], _i32),
     "qvx_dequant_row": ([_vp, _u32, _i32, _i32, _vp, _vp], _i32),
+    "qvx_kv_page_bytes": ([_u32, _i32, _i32, _i32], _sz),
+    "qvx_kv_map": ([_vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
+    "qvx_rope_kv": ([_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _vp], _i32),
+    "qvx_attn_paged": ([_vp, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
+    "qvx_attn_paged_ws": ([_vp, _i32, _i32, _i32], _sz),
+    "qvx_attn_cross": ([_vp, _i64, _vp, _i64, _u32, _i32, _vp, _i32, _vp, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
+    "qvx_attn_cross_ws": ([_vp, _u32, _i32, _i32, _i32], _sz),
     "qvx_qgemm_f16": ([_vp, _vp, _u32, _vp, _i32, _i32, _i32, _i32, _vp], _i32),
     "qvx_qgemm_f16_noalloc": ([_vp, _vp, _u32, _vp, _i32, _i32, _i32, _i32, _vp], _i32),
     "qvx_qgemm_plan_q4k": ([_i32, _i32, _i32, _i32, _vp, _i32], _i32),
@@ -248,6 +260,129 @@ def swiglu(out: int, gate: int, up: int, n: int, stream: int = 0) -> int:
     return lib().qvx_swiglu(out, gate, up, n, stream)
 
 
+# ---- attention: the paged cache and an encoder's states (raw device pointers; include/qvx.h) -------------
+
+def _torch_types():
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+class KvCache(C.Structure):
+    """A paged cache of one layer (qvx_kv_cache): K and V pages of ``page_size`` tokens, each page
+    [kv_heads][page_size][head_dim] values of a ggml type (Q8_0: the quants, then the scales)."""
+
+    _fields_ = [("d_k", _vp), ("d_v", _vp), ("page_stride", _i64), ("type", _u32), ("n_pages", _i32),
+                ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32)]
+
+    @classmethod
+    def of(cls, k, v, ggml_type: int, page_size: int, kv_heads: int, head_dim: int) -> "KvCache":
+        """The cache in two device tensors whose first dimension is the page (any strides between
+        pages, K and V alike; each page contiguous)."""
+        need = kv_page_bytes(ggml_type, kv_heads, page_size, head_dim)
+        strides = []
+        for x in (k, v):
+            held = x.element_size() * (x.numel() // max(x.shape[0], 1))
+            inner = x[0] if x.shape[0] else x
+            if need == 0 or held < need or not inner.is_contiguous() or not x.is_cuda:
+                raise ValueError("KvCache.of: device pages of kv_page_bytes(...) bytes, each contiguous")
+            strides.append(x.stride(0) * x.element_size())
+        if strides[0] != strides[1] or k.shape[0] != v.shape[0] or k.device != v.device:
+            raise ValueError("KvCache.of: K and V must have as many pages, equally far apart, on one device")
+        c = cls(k.data_ptr(), v.data_ptr(), strides[0], ggml_type, k.shape[0], page_size, kv_heads, head_dim)
+        c.tensors = (k, v)
+        return c
+
+
+class Rope(C.Structure):
+    """A rotation (qvx_rope): per pair of a head an inverse frequency (float64) and the axis whose
+    positions turn it (uint8)."""
+
+    _fields_ = [("d_inv_freq", _vp), ("d_axis", _vp), ("rot_dim", _i32), ("n_axes", _i32), ("pairing", _i32),
+                ("scale", _f32)]
+
+    @classmethod
+    def of(cls, inv_freq, axis=None, n_axes: int = 1, pairing: int = ROPE_HALVES, scale: float = 1.0) -> "Rope":
+        import torch
+        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not inv_freq.is_cuda:
+            raise ValueError("Rope.of: inv_freq is a contiguous float64 device vector, one value a pair")
+        if axis is not None and (axis.dtype != torch.uint8 or axis.shape != inv_freq.shape or not axis.is_contiguous()
+                                 or axis.device != inv_freq.device):
+            raise ValueError("Rope.of: axis is a uint8 vector beside inv_freq")
+        c = cls(inv_freq.data_ptr(), axis.data_ptr() if axis is not None else None, 2 * inv_freq.shape[0], n_axes,
+                pairing, scale)
+        c.tensors = (inv_freq, axis)
+        return c
+
+
+class KvStates(C.Structure):
+    """An encoder's keys and values (qvx_kv_states)."""
+
+    _fields_ = [("d_k", _vp), ("d_v", _vp), ("batch_stride", _i64), ("row_stride", _i64), ("head_stride", _i64),
+                ("type", _u32), ("max_len", _i32), ("kv_heads", _i32), ("head_dim", _i32)]
+
+    @classmethod
+    def of(cls, k, v) -> "KvStates":
+        """Keys and values [sequences, states, heads, head_dim] of one dtype, of any strides alike but
+        for the last dimension's 1 (views of a stacked projection, or head by head)."""
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("KvStates.of: keys and values [sequences, states, heads, head_dim] laid out alike")
+        if k.dtype not in _torch_types() or not k.is_cuda or (k.shape[3] > 1 and k.stride(3) != 1):
+            raise ValueError("KvStates.of: float32, float16 or bfloat16 device tensors with values side by side")
+        s = [k.stride(i) if k.shape[i] > 1 else n for i, n in
+             enumerate((k.shape[1] * k.shape[2] * k.shape[3], k.shape[2] * k.shape[3], k.shape[3]))]
+        c = cls(k.data_ptr(), v.data_ptr(), *s, _torch_types()[k.dtype], k.shape[1], k.shape[2], k.shape[3])
+        c.tensors = (k, v)
+        return c
+
+
+def kv_page_bytes(ggml_type: int, kv_heads: int, page_size: int, head_dim: int) -> int:
+    """Bytes of a cache page of K (or V); 0 for what the cache does not take."""
+    return lib().qvx_kv_page_bytes(ggml_type, kv_heads, page_size, head_dim)
+
+
+def kv_map(held: int, new: int, n_seqs: int, table: int, table_width: int, page_size: int, free: int, n_free: int,
+           taken_in: int, taken_out: int, lens: int, offsets: int, slots: int, pos: int, seq: int, max_tokens: int,
+           stream: int = 0) -> int:
+    """Page tables, slots and positions of a step's new tokens from the sequences' lengths. Status."""
+    return lib().qvx_kv_map(held, new, n_seqs, table, table_width, page_size, free, n_free, taken_in, taken_out, lens,
+                            offsets, slots, pos or None, seq or None, max_tokens, stream)
+
+
+def rope_kv(q_out: int, q_out_stride: int, q: int, q_stride: int, q_heads: int, k: int, k_stride: int, v: int,
+            v_stride: int, n_tokens: int, head_dim: int, rope: Rope, pos: int, pos_stride: int, cache: KvCache | None,
+            slots: int, stream: int = 0) -> int:
+    """Rotary positions of q and k, and the append of k and v to the paged cache. Status."""
+    return lib().qvx_rope_kv(q_out, q_out_stride, q, q_stride, q_heads, k, k_stride, v, v_stride, n_tokens, head_dim,
+                             C.byref(rope), pos, pos_stride, C.byref(cache) if cache is not None else None, slots,
+                             stream)
+
+
+def attn_paged(out: int, out_stride: int, q: int, q_stride: int, q_heads: int, cache: KvCache, table: int,
+               table_width: int, lens: int, n_seqs: int, scale: float, ws: int, ws_bytes: int, stream: int = 0) -> int:
+    """Attention of one new token a sequence over the paged cache. Status."""
+    return lib().qvx_attn_paged(out, out_stride, q, q_stride, q_heads, C.byref(cache), table, table_width, lens, n_seqs,
+                                scale, ws, ws_bytes, stream)
+
+
+def attn_paged_ws(cache: KvCache, q_heads: int, n_seqs: int, table_width: int) -> int:
+    """Bytes of attn_paged's workspace."""
+    return lib().qvx_attn_paged_ws(C.byref(cache), q_heads, n_seqs, table_width)
+
+
+def attn_cross(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, offsets: int, n_q: int,
+               states: KvStates, lens: int, n_seqs: int, scale: float, ws: int, ws_bytes: int, stream: int = 0) -> int:
+    """Cross attention of (ragged) queries to an encoder's states. Status."""
+    return lib().qvx_attn_cross(out, out_stride, q, q_stride, q_type, q_heads, offsets or None, n_q, C.byref(states),
+                                lens or None, n_seqs, scale, ws, ws_bytes, stream)
+
+
+def attn_cross_ws(states: KvStates, q_type, q_heads: int, n_q: int, n_seqs: int) -> int:
+    """Bytes of attn_cross's workspace; q_type a ggml type id or a torch dtype."""
+    if not isinstance(q_type, int):
+        q_type = _torch_types()[q_type]
+    return lib().qvx_attn_cross_ws(C.byref(states), q_type, q_heads, n_q, n_seqs)
+
+
 def dequantize(ggml_type: int, src: int, dst: int, n: int, stream: int = 0) -> int:
     """dequantize (runtime/src/dequant.cpp:277-296) on device pointers. Status."""
     return lib().qvx_dequantize(ggml_type, src, dst, n, stream)
@@ -400,6 +535,111 @@ def qmatmul_swiglu_t(w_gu, ggml_type: int, x, ffn: int, cols: int, norm_w=None, 
     nw = norm_w.data_ptr() if norm_w is not None else None
     _check(lib().qvx_qmatmul_swiglu(out.data_ptr(), w_gu.data_ptr(), ggml_type, x.data_ptr(), nw, eps, nvec, ffn,
                                     cols, _stream()), "qvx_qmatmul_swiglu")
+    return out
+
+
+def _rows(x, what: str):
+    """(address, elements from row to row) of a device tensor [rows, heads, head_dim] or [rows, heads *
+    head_dim] whose rows are contiguous."""
+    width = x[0].numel() if x.shape[0] else 0
+    if not x.is_cuda or (x.shape[0] and not x[0].is_contiguous()):
+        raise ValueError(f"{what}: device rows with their heads side by side")
+    return x.data_ptr(), (x.stride(0) if x.shape[0] > 1 else width)
+
+
+def _int32(x, shape, device, what: str):
+    import torch
+    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape) or not x.is_contiguous() or x.device != device:
+        raise ValueError(f"{what}: contiguous int32 {tuple(shape)} on {device}")
+    return x.data_ptr()
+
+
+def kv_map_t(held, new, table, page_size: int, free, taken, max_tokens: int):
+    """kv_map on int32 device tensors: held, new [n]; table [n, width] (new pages are stored in it); free
+    list; taken [2].  Returns (lens, offsets, slots, pos, seq, taken)."""
+    import torch
+    n, dev = held.shape[0], held.device
+    i32 = dict(dtype=torch.int32, device=dev)
+    lens, offsets, out = torch.empty(n, **i32), torch.empty(n + 1, **i32), torch.empty(2, **i32)
+    slots, pos, seq = (torch.empty(max_tokens, **i32) for _ in range(3))
+    args = [_int32(held, (n,), dev, "held"), _int32(new, (n,), dev, "new"), n,
+            _int32(table, (n, table.shape[-1]), dev, "table"), table.shape[-1], page_size,
+            _int32(free, free.shape[:1], dev, "free"), free.shape[0], _int32(taken, (2,), dev, "taken")]
+    with torch.cuda.device(dev):
+        _check(kv_map(*args, out.data_ptr(), lens.data_ptr(), offsets.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+                      seq.data_ptr(), max_tokens, _stream()), "qvx_kv_map")
+    return lens, offsets, slots, pos, seq, out
+
+
+def rope_kv_t(q, k, v, pos, rope: Rope, cache: KvCache | None = None, slots=None, out=None):
+    """rope_kv on device tensors: q [tokens, heads, head_dim] fp32 (rows of any stride), k and v [tokens, kv_heads,
+    head_dim] (None without a cache), pos [tokens] or [axes, tokens] int32, slots [tokens] int32.  Returns q_out."""
+    import torch
+    n, heads, d = q.shape
+    if out is None:
+        out = torch.empty((n, heads, d), dtype=torch.float32, device=q.device)
+    for x, what, h in ((q, "q", heads), (out, "out", heads), (k, "k", cache.kv_heads if cache is not None else 0),
+                       (v, "v", cache.kv_heads if cache is not None else 0)):
+        if (cache is None and what in "kv") or (what in ("q", "out") and x is None):
+            continue
+        if x is None or x.dtype != torch.float32 or tuple(x.shape) != (n, h, d) or x.device != q.device:
+            raise ValueError(f"rope_kv_t: {what} is float32 [{n}, {h}, {d}] on {q.device}")
+    axes = pos.reshape(-1, n)
+    pp = _int32(axes, (rope.n_axes, n), q.device, "pos")
+    kv = (*_rows(k, "k"), *_rows(v, "v")) if cache is not None else (0, 0, 0, 0)
+    if cache is not None and slots is None:
+        raise ValueError("rope_kv_t: a cache needs slots")
+    sl = _int32(slots, (n,), q.device, "slots") if cache is not None else 0
+    with torch.cuda.device(q.device):
+        _check(rope_kv(*_rows(out, "out"), *_rows(q, "q"), heads, *kv, n, d, rope, pp, n, cache, sl, _stream()),
+               "qvx_rope_kv")
+    return out
+
+
+def attn_paged_t(q, cache: KvCache, table, lens, scale: float | None = None, out=None, ws=None):
+    """attn_paged on device tensors: q [n, heads, head_dim] fp32, table [n, width] and lens [n] int32; scale
+    1 / sqrt(head_dim) unless given.  Without ws the workspace is torch memory of the call."""
+    import torch
+    n, heads, d = q.shape
+    if q.dtype != torch.float32 or d != cache.head_dim:
+        raise ValueError("attn_paged_t: q is float32 [n, heads, the cache's head_dim]")
+    if out is None:
+        out = torch.empty((n, heads, d), dtype=torch.float32, device=q.device)
+    elif out.dtype != torch.float32 or out.shape != q.shape or out.device != q.device:
+        raise ValueError("attn_paged_t: out is float32 and as q")
+    width = table.shape[-1]
+    tp, lp = _int32(table, (n, width), q.device, "table"), _int32(lens, (n,), q.device, "lens")
+    with torch.cuda.device(q.device):
+        if ws is None:
+            ws = torch.empty(attn_paged_ws(cache, heads, n, width), dtype=torch.uint8, device=q.device)
+        _check(attn_paged(*_rows(out, "out"), *_rows(q, "q"), heads, cache, tp, width, lp, n,
+                          d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(),
+                          _stream()), "qvx_attn_paged")
+    return out
+
+
+def attn_cross_t(q, states: KvStates, lens=None, offsets=None, scale: float | None = None, out=None, ws=None):
+    """attn_cross on device tensors: q [rows, heads, head_dim] in float32, float16 or bfloat16, offsets [n + 1]
+    and lens [n] int32 (None: equal parts, all states).  Rows past offsets[n] keep out's values."""
+    import torch
+    n_q, heads, d = q.shape
+    if q.dtype not in _torch_types() or d != states.head_dim:
+        raise ValueError("attn_cross_t: q is float32, float16 or bfloat16 [rows, heads, the states' head_dim]")
+    if out is None:
+        out = torch.zeros((n_q, heads, d), dtype=q.dtype, device=q.device) if offsets is not None else \
+            torch.empty((n_q, heads, d), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device:
+        raise ValueError("attn_cross_t: out is as q")
+    n = states.tensors[0].shape[0]
+    op = _int32(offsets, (n + 1,), q.device, "offsets") if offsets is not None else 0
+    lp = _int32(lens, (n,), q.device, "lens") if lens is not None else 0
+    t = _torch_types()[q.dtype]
+    with torch.cuda.device(q.device):
+        if ws is None:
+            ws = torch.empty(attn_cross_ws(states, t, heads, n_q, n), dtype=torch.uint8, device=q.device)
+        _check(attn_cross(*_rows(out, "out"), *_rows(q, "q"), t, heads, op, n_q, states, lp, n,
+                          d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(),
+                          _stream()), "qvx_attn_cross")
     return out
 
 

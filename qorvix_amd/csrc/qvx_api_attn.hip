@@ -1,0 +1,322 @@
+// qvx_api_attn.hip -- the extern "C" boundary of the attention calls (include/qvx.h): argument checks,
+// which run before any device work, and the bounds that the kernels' partition of the work needs.
+#include "qvx_attn.hpp"
+#include "qvx_kv.hpp"
+
+#include <cstdio>
+
+namespace qvx {
+bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
+bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s);
+void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s);
+}  // namespace qvx
+
+using namespace qvx;
+
+namespace {
+
+constexpr int kAttnMaxSeqs = 65536, kMapMaxSeqs = 16384;
+constexpr int64_t kMaxPitch = 64ll << 20;  // sixteen rows stay far inside 32-bit offsets
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int attn_status(bool launched) {
+  const hipError_t e = hipGetLastError();
+  if (launched && e == hipSuccess) return QVX_OK;
+  std::fprintf(stderr, "qvx: HIP error %d (%s)\n", (int)e, hipGetErrorString(e));
+  return QVX_E_HIP;
+}
+
+// Bytes of n values of a cache or states type; 0 for another type.
+int64_t value_bytes(uint32_t type, int64_t n) {
+  switch (type) {
+    case T_F32: return 4 * n;
+    case T_F16: case T_BF16: return 2 * n;
+    case T_Q8_0: return n + n / 16;
+    default: return 0;
+  }
+}
+
+bool head_dim_ok(uint32_t type, int d) { return d > 0 && d <= 256 && d % (type == T_Q8_0 ? 32 : 8) == 0; }
+
+int64_t page_bytes(uint32_t type, int kv_heads, int page_size, int head_dim) {
+  if (!value_bytes(type, 1) || kv_heads <= 0 || page_size <= 0 || !head_dim_ok(type, head_dim)) return 0;
+  const int64_t rows = (int64_t)kv_heads * page_size;
+  if (rows > (1ll << 40)) return 0;
+  return (value_bytes(type, rows * head_dim) + 15) / 16 * 16;
+}
+
+int check_cache(const qvx_kv_cache* c, int64_t* stride) {
+  if (!c) return QVX_E_NULL;
+  if (!value_bytes(c->type, 1)) return QVX_E_TYPE;
+  const int64_t packed = page_bytes(c->type, c->kv_heads, c->page_size, c->head_dim);
+  if (!packed || c->n_pages <= 0) return QVX_E_SHAPE;
+  if ((int64_t)c->n_pages * c->page_size > 0x7fffffffll) return QVX_E_RANGE;
+  if (c->page_stride && (c->page_stride < packed || c->page_stride % 16)) return QVX_E_RANGE;
+  if (!c->d_k || !c->d_v) return QVX_E_NULL;
+  if (!aligned(c->d_k, 16) || !aligned(c->d_v, 16)) return QVX_E_RANGE;
+  *stride = c->page_stride ? c->page_stride : packed;
+  return QVX_OK;
+}
+
+// The partition of a call whose heads, pages and sequences are filled in: how many work items are
+// aimed at, and the bounds that grid and workspace are sized by.  Workgroups to fill the chip: four a CU.
+// A chunk has at least 8 tiles (128 keys), two a wave: shorter ones are all launch and join.
+constexpr int kAttnWgs = 1024, kMinChunk = 8;
+
+// False: the partition passes 31 bits.
+bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
+  const int64_t tiles = (int64_t)c.max_len / c.page_size * c.page_tiles +
+                        (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
+  c.min_chunk = kMinChunk;
+  c.target = std::max(1, kAttnWgs / c.kv_heads);
+  *join = tiles > c.min_chunk;
+  const int64_t items = std::min(row_tiles + c.target, row_tiles * std::max<int64_t>((tiles + kMinChunk - 1) / kMinChunk, 1));
+  if (items > 0x7fffffffll || tiles > 0x7fffffffll) return false;
+  c.items = (int)items;
+  const int d16 = (c.head_dim + 15) / 16 * 16;
+  *ws_bytes = *join ? (size_t)attn_slots(c) * c.kv_heads * attn_part(c.lds_rows, d16) * sizeof(float) : 0;
+  return true;
+}
+
+int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width, AttnCall& c, bool* join,
+                size_t* ws_bytes) {
+  if (n_seqs <= 0) return QVX_E_NVEC;
+  if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
+  if (q_heads <= 0 || q_heads % cache->kv_heads || table_width <= 0) return QVX_E_SHAPE;
+  if (n_seqs > kAttnMaxSeqs || cache->kv_heads > 65535 || (int64_t)table_width * cache->page_size > 0x7fffffffll)
+    return QVX_E_RANGE;
+  const int d = cache->head_dim;
+  c.k = static_cast<const uint8_t*>(cache->d_k);
+  c.v = static_cast<const uint8_t*>(cache->d_v);
+  c.pitch = cache->type == T_Q8_0 ? d : (int)value_bytes(cache->type, d);
+  c.head_stride = (int64_t)cache->page_size * c.pitch;
+  c.scale_off = (int64_t)cache->kv_heads * c.head_stride;
+  c.table_width = table_width;
+  c.n_pages = cache->n_pages;
+  c.page_size = cache->page_size;
+  c.page_tiles = (cache->page_size + kAttnTile - 1) / kAttnTile;
+  c.max_len = table_width * cache->page_size;
+  c.n_seqs = c.n_q = n_seqs;
+  c.q_each = 1;
+  c.kv_heads = cache->kv_heads;
+  c.group = q_heads / cache->kv_heads;
+  c.head_dim = d;
+  c.lds_rows = std::min(kAttnRows, c.group);
+  const int64_t row_tiles = (int64_t)n_seqs * ((c.group + kAttnRows - 1) / kAttnRows);
+  return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+}
+
+int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, AttnCall& c,
+                bool* join, size_t* ws_bytes) {
+  if (!st) return QVX_E_NULL;
+  if (n_seqs <= 0) return QVX_E_NVEC;
+  if ((q_type != T_F32 && q_type != T_F16 && q_type != T_BF16) ||
+      (st->type != T_F32 && st->type != T_F16 && st->type != T_BF16))
+    return QVX_E_TYPE;
+  if (n_q < 0 || (!ragged && n_q % n_seqs) || q_heads <= 0 || st->kv_heads <= 0 || q_heads % st->kv_heads ||
+      st->max_len < 0 || !head_dim_ok(st->type, st->head_dim) || st->row_stride < st->head_dim || st->batch_stride < 0 ||
+      st->head_stride < 0)
+    return QVX_E_SHAPE;
+  const int64_t es = value_bytes(st->type, 1);
+  constexpr int64_t kMost = 1ll << 56;
+  if (n_seqs > kAttnMaxSeqs || st->kv_heads > 65535 || st->batch_stride > kMost || st->head_stride > kMost ||
+      st->row_stride > kMaxPitch / es || (st->row_stride * es) % 16 || (st->batch_stride * es) % 16 ||
+      (st->head_stride * es) % 16)
+    return QVX_E_RANGE;
+  if (!st->d_k || !st->d_v) return QVX_E_NULL;
+  if (!aligned(st->d_k, 16) || !aligned(st->d_v, 16)) return QVX_E_RANGE;
+  c.q_type = q_type;
+  c.k = static_cast<const uint8_t*>(st->d_k);
+  c.v = static_cast<const uint8_t*>(st->d_v);
+  c.page_stride = st->batch_stride * es;
+  c.head_stride = st->head_stride * es;
+  c.pitch = (int)(st->row_stride * es);
+  c.n_pages = n_seqs;
+  c.page_tiles = std::max(1, st->max_len / kAttnTile + (st->max_len % kAttnTile != 0));
+  c.page_size = std::max(1, st->max_len);
+  c.max_len = st->max_len;
+  c.n_seqs = n_seqs;
+  c.n_q = n_q;
+  c.q_each = ragged ? 0 : n_q / n_seqs;
+  c.kv_heads = st->kv_heads;
+  c.group = q_heads / st->kv_heads;
+  c.head_dim = st->head_dim;
+  const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
+  if ((int64_t)n_q * c.group > 0x7fffffffll - kAttnRows) return QVX_E_RANGE;
+  c.lds_rows = (int)std::max<int64_t>(1, std::min<int64_t>(kAttnRows, rows));
+  const int64_t row_tiles = ragged ? (int64_t)n_q * c.group / kAttnRows + n_seqs : n_seqs * ((rows + kAttnRows - 1) / kAttnRows);
+  return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+}  // namespace
+
+#pragma GCC visibility push(default)
+extern "C" {
+
+size_t qvx_kv_page_bytes(uint32_t type, int kv_heads, int page_size, int head_dim) {
+  return (size_t)page_bytes(type, kv_heads, page_size, head_dim);
+}
+
+int qvx_kv_map(const int32_t* d_held, const int32_t* d_new, int n_seqs, int32_t* d_table, int table_width,
+               int page_size, const int32_t* d_free, int n_free, const int32_t* d_taken_in, int32_t* d_taken_out,
+               int32_t* d_lens, int32_t* d_offsets, int32_t* d_slots, int32_t* d_pos, int32_t* d_seq,
+               int max_tokens, void* stream) {
+  if (n_seqs <= 0) return QVX_E_NVEC;
+  if (table_width <= 0 || page_size <= 0 || n_free < 0 || max_tokens < 0) return QVX_E_SHAPE;
+  if (n_seqs > kMapMaxSeqs) return QVX_E_RANGE;
+  if (!d_held || !d_new || !d_table || (!d_free && n_free) || !d_taken_in || !d_taken_out || !d_lens || !d_offsets ||
+      (!d_slots && max_tokens))
+    return QVX_E_NULL;
+  const struct {
+    const int32_t* p;
+    int64_t n;
+  } ins[] = {{d_held, n_seqs}, {d_new, n_seqs}, {d_taken_in, 2}},
+    outs[] = {{d_lens, n_seqs}, {d_taken_out, 2}, {d_offsets, n_seqs + 1}, {d_slots, max_tokens}, {d_pos, max_tokens},
+              {d_seq, max_tokens}};
+  bool alias = false;
+  for (const auto& i : ins)
+    for (const auto& o : outs) {
+      const auto a = reinterpret_cast<uintptr_t>(i.p), b = reinterpret_cast<uintptr_t>(o.p);
+      if (!b || a + 4 * i.n <= b || b + 4 * o.n <= a) continue;
+      if (i.p == o.p && ((i.p == d_held && o.p == d_lens) || (i.p == d_taken_in && o.p == d_taken_out)))
+        alias = true;
+      else
+        return QVX_E_RANGE;
+    }
+  const MapCall c{d_held, d_new,  n_seqs,    d_table, table_width, page_size, d_free, n_free,
+                  d_taken_in, d_taken_out, d_lens, d_offsets, d_slots, d_pos, d_seq, max_tokens};
+  return attn_status(launch_kv_map(c, alias, static_cast<hipStream_t>(stream)));
+}
+
+int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t q_stride, int q_heads,
+                const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens, int head_dim,
+                const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
+                const int32_t* d_slots, void* stream) {
+  if (n_tokens <= 0) return QVX_E_NVEC;
+  if (!rope) return QVX_E_NULL;
+  RopeCall c{};
+  uint32_t type = T_F32;
+  if (cache) {
+    if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
+    if (cache->head_dim != head_dim) return QVX_E_SHAPE;
+    type = cache->type;
+    c.kv_heads = cache->kv_heads;
+    c.k_pages = static_cast<uint8_t*>(cache->d_k);
+    c.v_pages = static_cast<uint8_t*>(cache->d_v);
+    c.scale_off = (int64_t)cache->kv_heads * cache->page_size * head_dim;
+    c.page_size = cache->page_size;
+    c.n_slots = (int64_t)cache->n_pages * cache->page_size;
+  }
+  if (rope->pairing != QVX_ROPE_HALVES && rope->pairing != QVX_ROPE_PAIRS) return QVX_E_VARIANT;
+  if (q_heads < 0 || q_heads + c.kv_heads <= 0 || !head_dim_ok(T_F32, head_dim) || rope->rot_dim < 0 ||
+      rope->rot_dim > head_dim || rope->rot_dim % 8 || rope->n_axes < 1 || rope->n_axes > 4)
+    return QVX_E_SHAPE;
+  const int64_t q_row = (int64_t)q_heads * head_dim, kv_row = (int64_t)c.kv_heads * head_dim;
+  if (q_stride < 0 || q_out_stride < q_row || (cache && (k_stride < 0 || v_stride < 0)) || pos_stride < 0 ||
+      (rope->n_axes > 1 && pos_stride < n_tokens))
+    return QVX_E_SHAPE;
+  if (q_row > 0x7fffffffll / 16 || kv_row > 0x7fffffffll / 16) return QVX_E_RANGE;
+  if ((q_heads && (!d_q || !d_q_out)) || (cache && (!d_k || !d_v || !d_slots)) ||
+      (rope->rot_dim && (!rope->d_inv_freq || !d_pos)))
+    return QVX_E_NULL;
+  if (d_q == d_q_out && q_stride != q_out_stride) return QVX_E_RANGE;
+  c.q_out = d_q_out;
+  c.q = d_q;
+  c.q_out_stride = q_out_stride;
+  c.q_stride = q_stride;
+  c.q_heads = q_heads;
+  c.head_dim = head_dim;
+  c.n_tokens = n_tokens;
+  c.inv_freq = rope->d_inv_freq;
+  c.axis = rope->d_axis;
+  c.rot_dim = rope->rot_dim;
+  c.n_axes = rope->n_axes;
+  c.halves = rope->pairing == QVX_ROPE_HALVES;
+  c.scale = rope->scale;
+  c.pos = d_pos;
+  c.pos_stride = pos_stride;
+  bool vec = q_stride % 4 == 0 && q_out_stride % 4 == 0 && aligned(d_q, 16) && aligned(d_q_out, 16);
+  if (cache) {
+    c.k = d_k;
+    c.v = d_v;
+    c.k_stride = k_stride;
+    c.v_stride = v_stride;
+    c.slots = d_slots;
+    vec = vec && k_stride % 4 == 0 && v_stride % 4 == 0 && aligned(d_k, 16) && aligned(d_v, 16);
+  }
+  launch_rope_kv(c, type, vec, static_cast<hipStream_t>(stream));
+  return attn_status(true);
+}
+
+size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width) {
+  AttnCall c{};
+  bool join = false;
+  size_t bytes = 0;
+  return check_paged(cache, q_heads, n_seqs, table_width, c, &join, &bytes) == QVX_OK ? bytes : 0;
+}
+
+int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q_stride, int q_heads,
+                   const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens,
+                   int n_seqs, float scale, void* d_ws, size_t ws_bytes, void* stream) {
+  AttnCall c{};
+  bool join = false;
+  size_t need = 0;
+  if (int rc = check_paged(cache, q_heads, n_seqs, table_width, c, &join, &need); rc != QVX_OK) return rc;
+  if (q_stride < 0 || out_stride < (int64_t)q_heads * cache->head_dim) return QVX_E_SHAPE;
+  if (!d_out || !d_q || !d_table || !d_lens || (need && !d_ws)) return QVX_E_NULL;
+  if (ws_bytes < need || !aligned(d_ws, 16) || (d_out == d_q && q_stride != out_stride)) return QVX_E_RANGE;
+  c.q = d_q;
+  c.out = d_out;
+  c.q_stride = q_stride;
+  c.out_stride = out_stride;
+  c.q_type = T_F32;
+  c.table = d_table;
+  c.lens = d_lens;
+  c.scale2 = scale * kLog2e;
+  c.ws = static_cast<float*>(d_ws);
+  return attn_status(launch_attn_split(c, cache->type, join, static_cast<hipStream_t>(stream)));
+}
+
+size_t qvx_attn_cross_ws(const qvx_kv_states* states, uint32_t q_type, int q_heads, int n_q, int n_seqs) {
+  // Ragged and equal queries differ in their bounds: the larger need serves both.
+  size_t most = 0;
+  for (int ragged = 0; ragged < 2; ++ragged) {
+    AttnCall c{};
+    bool join = false;
+    size_t bytes = 0;
+    if (check_cross(states, q_type, q_heads, ragged != 0, n_q, n_seqs, c, &join, &bytes) == QVX_OK)
+      most = std::max(most, bytes);
+  }
+  return most;
+}
+
+int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                   const int32_t* d_offsets, int n_q, const qvx_kv_states* states, const int32_t* d_lens, int n_seqs,
+                   float scale, void* d_ws, size_t ws_bytes, void* stream) {
+  AttnCall c{};
+  bool join = false;
+  size_t need = 0;
+  if (int rc = check_cross(states, q_type, q_heads, d_offsets != nullptr, n_q, n_seqs, c, &join, &need); rc != QVX_OK)
+    return rc;
+  if (q_stride < 0 || out_stride < (int64_t)q_heads * states->head_dim) return QVX_E_SHAPE;
+  if (n_q == 0) return QVX_OK;
+  if (!d_out || !d_q || (need && !d_ws)) return QVX_E_NULL;
+  if (!aligned(d_out, q_type == T_F32 ? 4 : 2) || !aligned(d_q, q_type == T_F32 ? 4 : 2) || ws_bytes < need ||
+      !aligned(d_ws, 16) || (d_out == d_q && q_stride != out_stride))
+    return QVX_E_RANGE;
+  c.q = d_q;
+  c.out = d_out;
+  c.q_stride = q_stride;
+  c.out_stride = out_stride;
+  c.q_offsets = d_offsets;
+  c.lens = d_lens;
+  c.scale2 = scale * kLog2e;
+  c.ws = static_cast<float*>(d_ws);
+  return attn_status(launch_attn_split(c, states->type, join, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
+#pragma GCC visibility pop

@@ -1,0 +1,10 @@
+// qvx_attn_bf16.hip -- the split attention kernel over BF16 keys and values (qvx_attn_split.hpp).
+#include "qvx_attn_split.hpp"
+
+namespace qvx {
+
+bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, size_t lds, hipStream_t s) {
+  return attn_split_dt<T_BF16>(c, grid, lds, s);
+}
+
+}  // namespace qvx

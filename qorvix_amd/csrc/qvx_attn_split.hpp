@@ -1,0 +1,316 @@
+// qvx_attn_split.hpp -- attention of few query rows over many keys on gfx950: the kernel behind
+// qvx_attn_paged and behind qvx_attn_cross for single tokens and fp32 queries.
+//
+//   out[row] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q[row] . k_j
+//
+// for any m, here a running reference that follows the largest s_j seen (below).  The sum is one pass
+// over the keys, so the cache is read once and that read bounds the kernel.
+//
+// Arithmetic.  Keys and values are widened to fp32 in registers (Q8_0: times their scale) and both
+// products run on the fp32 matrix instruction (16x16x4): queries, weights and sums are never rounded
+// below 32 bits, whatever the cache holds.
+//
+// Layout.  S^T = K Q^T puts key 4 g + r (g = lane / 16) and row lane % 16 into register r; the second
+// product reads its left operand, P, with row lane % 16 and key index g.  So the weights go from one
+// product to the next in place, without a lane exchange or LDS, when the values of key 4 g + r are
+// loaded by the lanes of group g: 16 lanes cover a token's values in consecutive pieces.
+//
+// The reference m.  A row's weights may use any common m; m moves only when a logit exceeds it by
+// more than 2^kSlack, which after the first tiles is rare, so a step costs a compare and a wave vote
+// instead of a lane reduction and a rescale.  Weights reach at most 2^kSlack, sums of 2^20 of them
+// 2^40: far from fp32's range, and the relative error of each stays that of fp32.
+//
+// Split.  A work item is a chunk of a sequence's tiles (qvx_attn.hpp); its four waves take tiles in
+// turn and join through LDS.  Items of a sequence that has several leave their sums, their maxima
+// and values in the workspace, and k_attn_join adds them up in the order of the chunks.
+#pragma once
+
+#include "qvx_attn.hpp"
+
+namespace qvx {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kSlack = 20.0f;
+constexpr uint32_t kPastEnd = 0x7fffff00u;  // an offset no descriptor reaches: the load gives zeros
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const uint8_t* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
+// N consecutive values of type T, N in 4, 8, 16: the raw words as loaded, and their fp32 values.
+template <uint32_t T, int N> struct AttnRaw;
+
+template <int W> struct AttnWords {
+  uint32_t w[W];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (W == 1) {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    } else if constexpr (W == 2) {
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+      w[0] = x[0], w[1] = x[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0);
+        w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
+      }
+    }
+  }
+};
+
+template <int N> struct AttnRaw<T_F32, N> : AttnWords<N> {
+  static constexpr int kBytes = 4 * N;
+  __device__ __forceinline__ float at(int i, float) const { return __builtin_bit_cast(float, this->w[i]); }
+};
+template <int N> struct AttnRaw<T_F16, N> : AttnWords<N / 2> {
+  static constexpr int kBytes = 2 * N;
+  __device__ __forceinline__ float at(int i, float) const {
+    const f16x2 h = __builtin_bit_cast(f16x2, this->w[i / 2]);
+    return i % 2 ? (float)h.y : (float)h.x;
+  }
+};
+template <int N> struct AttnRaw<T_BF16, N> : AttnWords<N / 2> {
+  static constexpr int kBytes = 2 * N;
+  __device__ __forceinline__ float at(int i, float) const {
+    return __builtin_bit_cast(float, i % 2 ? this->w[i / 2] & 0xffff0000u : this->w[i / 2] << 16);
+  }
+};
+template <int N> struct AttnRaw<T_Q8_0, N> : AttnWords<N / 4> {
+  static constexpr int kBytes = N;
+  __device__ __forceinline__ float at(int i, float step) const {
+    return (float)((int32_t)(this->w[i / 4] << (24 - 8 * (i % 4))) >> 24) * step;
+  }
+};
+
+// One element of a query or an output row, by type.
+__device__ __forceinline__ float attn_load(const void* p, int64_t i, uint32_t type) {
+  if (type == T_F32) return static_cast<const float*>(p)[i];
+  const uint16_t h = static_cast<const uint16_t*>(p)[i];
+  if (type == T_F16) return (float)__builtin_bit_cast(_Float16, h);
+  return __builtin_bit_cast(float, (uint32_t)h << 16);
+}
+__device__ __forceinline__ void attn_store(void* p, int64_t i, uint32_t type, float x) {
+  if (type == T_F32) {
+    static_cast<float*>(p)[i] = x;
+  } else if (type == T_F16) {
+    static_cast<_Float16*>(p)[i] = (_Float16)x;
+  } else {
+    static_cast<__bf16*>(p)[i] = (__bf16)x;
+  }
+}
+
+// Element offset of a row's head in q (stride: q_stride) or out, and whether the row exists.
+__device__ __forceinline__ int64_t attn_row(const AttnCall& c, const AttnItem& it, int row, int kvh, int64_t stride) {
+  const int query = row / c.group, head = row - query * c.group;
+  return (int64_t)(it.q0 + query) * stride + (int64_t)(kvh * c.group + head) * c.head_dim;
+}
+
+__device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.
+template <uint32_t T, int DT>
+__global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
+  constexpr int KS = DT / 32;  // 32 values of a key at a time
+  constexpr int VB = DT / 16;  // consecutive values of a lane in the second product
+  constexpr int VU = VB < 8 ? VB : 8, VN = VB / VU;
+  using KRaw = AttnRaw<T, 8>;
+  using VRaw = AttnRaw<T, VU>;
+  constexpr bool kQ8 = T == T_Q8_0;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, d = c.head_dim;
+  const AttnItem it = attn_item(c, blockIdx.x, reinterpret_cast<int*>(lds));
+  if (!it.any) return;
+
+  // This lane's query values: row col, for the key loads' pieces 32 s + 8 g + j.
+  float q[KS][8];
+  const int row = it.row0 + col;
+  {
+    const int64_t at = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = 32 * s + 8 * g + j;
+        q[s][j] = row < it.rows && i < d ? attn_load(c.q, at + i, c.q_type) * c.scale2 : 0.0f;
+      }
+  }
+  uint32_t koff[KS], voff[VN], soff = 0, svoff = 0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    koff[s] = 32 * s + 8 * g < d ? (uint32_t)(col * c.pitch + (32 * s + 8 * g) * KRaw::kBytes / 8) : kPastEnd;
+#pragma unroll
+  for (int u = 0; u < VN; ++u) {
+    const int i = col * VB + u * VU;
+    voff[u] = i < d ? (uint32_t)(4 * g * c.pitch + i * VRaw::kBytes / VU) : kPastEnd;
+  }
+  const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
+  if constexpr (kQ8) {
+    soff = (uint32_t)(col * spitch);
+    svoff = col * VB < d ? (uint32_t)(4 * g * spitch + col * VB / 32 * 2) : kPastEnd;
+  }
+
+  float m = -INFINITY, l = 0.0f;
+  f32x4 acc[VB];
+#pragma unroll
+  for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
+  const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
+  int page = 0, tok = 0, live = 0;
+  for (int n = 0; n < tiles; ++n) {
+    if ((n & 63) == 0) {
+      const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
+      live = 0;
+      if (t < it.tile1) {
+        const int p = t / c.page_tiles;
+        tok = (t - p * c.page_tiles) * kAttnTile;
+        page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
+        live = min(min(kAttnTile, c.page_size - tok), it.len - p * c.page_size - tok);
+        if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
+      }
+    }
+    const int64_t pg = __builtin_amdgcn_readlane(page, n & 63);
+    const int tk = __builtin_amdgcn_readlane(tok, n & 63), nk = __builtin_amdgcn_readlane(live, n & 63);
+    const int64_t at = pg * c.page_stride + (int64_t)kvh * c.head_stride + (int64_t)tk * c.pitch;
+    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(nk * c.pitch));
+    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(nk * c.pitch));
+    KRaw kw[KS];
+    VRaw vw[4][VN];
+    float kstep[KS], vstep[4];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kw[s].load(kr, koff[s]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int u = 0; u < VN; ++u) vw[r][u].load(vr, voff[u] + r * c.pitch);
+    if constexpr (kQ8) {
+      const int64_t sat = pg * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tk) * spitch;
+      const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + sat, (uint32_t)(nk * spitch));
+      const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + sat, (uint32_t)(nk * spitch));
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        kstep[s] = (float)__builtin_bit_cast(
+            _Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + 2 * s : kPastEnd, 0, 0));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        vstep[r] = (float)__builtin_bit_cast(
+            _Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vs, svoff + r * spitch, 0, 0));
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kstep[s] = 1.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) vstep[r] = 1.0f;
+    }
+    f32x4 sc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kw[s].at(j, kstep[s]), q[s][j], sc, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r >= nk) sc[r] = -INFINITY;
+    const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+    if (__any(top > m + kSlack)) {  // m + slack is -inf at the start: any finite logit moves it
+      float t = fmaxf(top, __shfl_xor(top, 16));
+      t = fmaxf(t, __shfl_xor(t, 32));
+      const float now = fmaxf(m, t);
+      const float f = m == now ? 1.0f : attn_pow2(m - now);
+      m = now;
+      l *= f;
+      float fr[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
+#pragma unroll
+      for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] *= fr[r];
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = attn_pow2(sc[r] - ref);
+      l += p[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int u = 0; u < VN; ++u)
+#pragma unroll
+        for (int j = 0; j < VU; ++j)
+          acc[u * VU + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], vw[r][u].at(j, vstep[r]), acc[u * VU + j], 0, 0, 0);
+  }
+
+  // The lane groups hold sums over their own keys.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  // Join the waves: m, l and the values of the rows that exist, through LDS.
+  const int d16 = (d + 15) & ~15, nrow = min(kAttnRows, it.rows - it.row0);
+  float* lm = lds;                           // [wave][16]
+  float* ll = lds + kAttnWaves * kAttnRows;  // [wave][16]
+  float* lv = lds + 2 * kAttnWaves * kAttnRows + (size_t)wave * c.lds_rows * d16;
+  __syncthreads();  // attn_item's words have been read
+  if (lane < 16) {
+    lm[wave * kAttnRows + lane] = m;
+    ll[wave * kAttnRows + lane] = l;
+  }
+#pragma unroll
+  for (int j = 0; j < VB; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r < nrow && col * VB + j < d) lv[(4 * g + r) * d16 + col * VB + j] = acc[j][r];
+  __syncthreads();
+  const float* v0 = lds + 2 * kAttnWaves * kAttnRows;
+  const int vstride = c.lds_rows * d16;
+  float* part = it.chunks > 1 ? c.ws + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(c.lds_rows, d16) : nullptr;
+  for (int e = threadIdx.x; e < nrow * d; e += 64 * kAttnWaves) {
+    const int r = e / d, i = e - r * d;
+    float top = lm[r];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, lm[w * kAttnRows + r]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, val = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+      const float f = attn_pow2(lm[w * kAttnRows + r] - ref);
+      sum += ll[w * kAttnRows + r] * f;
+      val += v0[w * vstride + r * d16 + i] * f;
+    }
+    if (it.chunks == 1) {
+      attn_store(c.out, attn_row(c, it, it.row0 + r, kvh, c.out_stride) + i, c.q_type, it.len ? val / sum : 0.0f);
+    } else {
+      part[r * d16 + i] = val;
+      if (i == 0) {
+        part[c.lds_rows * d16 + r] = top;
+        part[c.lds_rows * (d16 + 1) + r] = sum;
+      }
+    }
+  }
+}
+
+template <uint32_t T> bool attn_split_dt(const AttnCall& c, dim3 grid, size_t lds, hipStream_t s) {
+  static LdsLimit lim64, lim128, lim256;
+  if (c.head_dim <= 64) {
+    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 64>), lim64, lds)) return false;
+    k_attn_split<T, 64><<<grid, 64 * kAttnWaves, lds, s>>>(c);
+  } else if (c.head_dim <= 128) {
+    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 128>), lim128, lds)) return false;
+    k_attn_split<T, 128><<<grid, 64 * kAttnWaves, lds, s>>>(c);
+  } else {
+    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 256>), lim256, lds)) return false;
+    k_attn_split<T, 256><<<grid, 64 * kAttnWaves, lds, s>>>(c);
+  }
+  return true;
+}
+
+}  // namespace qvx
