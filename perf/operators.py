@@ -230,9 +230,8 @@ def _own_handles(s, c):
     import qorvix_amd as qvx
     s.qvx = qvx
     if c["op"] == "map":
-        s.lens, s.offsets = _ints([0] * c["n"]), _ints([0] * (c["n"] + 1))
-        s.slots, s.pos, s.seq = (_ints([0] * s.rows) for _ in range(3))
-        s.taken_out = _ints([0, 0])
+        s.lens, s.offsets, s.slots, s.pos, s.seq, s.taken_out = (
+            torch.empty(n, dtype=torch.int32, device=DEVICE) for n in (c["n"], c["n"] + 1, s.rows, s.rows, s.rows, 2))
     if c["op"] in ("rope", "paged"):
         s.cache = qvx.KvCache.of(s.k_cache, s.v_cache, TYPES[c["type"]], c["page"], c["kv_heads"], c["d"])
     if c["op"] == "rope":
