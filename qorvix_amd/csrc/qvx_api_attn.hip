@@ -7,6 +7,8 @@
 
 namespace qvx {
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
+int attn16_rows();
+bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s);
 bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s);
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s);
 }  // namespace qvx
@@ -147,6 +149,17 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   c.lds_rows = (int)std::max<int64_t>(1, std::min<int64_t>(kAttnRows, rows));
   const int64_t row_tiles = ragged ? (int64_t)n_q * c.group / kAttnRows + n_seqs : n_seqs * ((rows + kAttnRows - 1) / kAttnRows);
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+}
+
+// Whether a checked cross call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a
+// 16-bit type and there are row tiles enough.
+bool cross16(const AttnCall& c, uint32_t type, bool ragged, float scale, int* items) {
+  if (c.q_type != type || type == T_F32 || !(scale >= 0.0f)) return false;
+  const int64_t r = attn16_rows(), rows = (int64_t)(ragged ? c.n_q : c.q_each) * c.group;
+  const int64_t tiles = ragged ? rows / r + c.n_seqs : c.n_seqs * ((rows + r - 1) / r);
+  if ((int64_t)c.n_q * c.group < 32 * (int64_t)c.n_seqs || tiles > 0x7fffffffll) return false;
+  *items = (int)tiles;
+  return true;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -315,6 +328,13 @@ int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_s
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
   c.ws = static_cast<float*>(d_ws);
+  if (int items; cross16(c, states->type, d_offsets != nullptr, scale, &items)) {
+    c.items = items;
+    c.min_chunk = 0x7ffffff0;  // a row tile takes all keys
+    c.q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
+    c.out_wide = aligned(d_out, 8) && out_stride % 4 == 0;
+    return attn_status(launch_attn16(c, states->type, static_cast<hipStream_t>(stream)));
+  }
   return attn_status(launch_attn_split(c, states->type, join, static_cast<hipStream_t>(stream)));
 }
 

@@ -17,7 +17,7 @@ namespace {
 __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
   __shared__ __attribute__((aligned(16))) float lds[3 * 256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kvh = blockIdx.y;
-  const AttnItem it = attn_item(c, blockIdx.x, reinterpret_cast<int*>(lds));
+  const AttnItem it = attn_item<kAttnRows>(c, blockIdx.x, reinterpret_cast<int*>(lds));
   if (!it.any || it.chunks == 1) return;
   const int d = c.head_dim, d16 = (d + 15) & ~15, nrow = min(kAttnRows, it.rows - it.row0);
   const size_t size = attn_part(c.lds_rows, d16), step = (size_t)c.kv_heads * size;

@@ -21,6 +21,7 @@ struct AttnCall {
   void* out;
   int64_t q_stride, out_stride;  // elements from one query's heads to the next query's
   uint32_t q_type;               // T_F32, T_F16 or T_BF16, the output's type too
+  bool q_wide, out_wide;         // 16-bit rows of q on 16-byte, of out on 8-byte addresses
   const int32_t* q_offsets;      // [n_seqs + 1], or null: q_each queries a sequence
   int q_each, n_q;
   const uint8_t *k, *v;
@@ -56,7 +57,7 @@ __device__ inline int attn_tiles(const AttnCall& c, int len) {
   return full * c.page_tiles + (len - full * c.page_size + kAttnTile - 1) / kAttnTile;
 }
 
-// One work item: rows [row0, row0 + 16) of sequence seq over tiles [tile0, tile1); `chunk` of `chunks`.
+// One work item: rows [row0, row0 + R) of sequence seq over tiles [tile0, tile1); `chunk` of `chunks`.
 struct AttnItem {
   bool any;
   int seq, len, q0, rows, row0;  // q0: the sequence's first query; rows: of the whole sequence
@@ -68,7 +69,8 @@ struct AttnSeq {
   int len, q0, nq, row_tiles, tiles;
 };
 
-__device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
+// R: query rows of a row tile, here and below.
+template <int R> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
   AttnSeq s{0, 0, 0, 0, 0};
   if (b >= c.n_seqs) return s;
   int len = c.lens ? c.lens[b] : c.max_len;
@@ -80,7 +82,7 @@ __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
     s.q0 = b * c.q_each;
     s.nq = c.q_each;
   }
-  s.row_tiles = (s.nq * c.group + kAttnRows - 1) / kAttnRows;
+  s.row_tiles = (s.nq * c.group + R - 1) / R;
   s.tiles = attn_tiles(c, s.len);
   return s;
 }
@@ -91,6 +93,7 @@ __device__ inline int attn_chunk(const AttnCall& c, long long total) {
   return (int)min(max((long long)c.min_chunk, (per + 3) / 4 * 4), 0x7ffffff0ll);
 }
 
+template <int R>
 __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b, int chunk, int i, int slot0) {
   AttnItem it;
   it.seq = b;
@@ -100,7 +103,7 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   const int rt = i / it.chunks;
   it.chunk = i - rt * it.chunks;
   it.rows = s.nq;
-  it.row0 = rt * kAttnRows;
+  it.row0 = rt * R;
   it.tile0 = it.chunk * chunk;
   it.tile1 = min(it.tile0 + chunk, s.tiles);
   it.slot = slot0 + i;
@@ -112,10 +115,10 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
 // The work item of number `item`, the same in every thread of the workgroup (256 threads); `lds`:
 // 20 words that the caller does not use across the call.  Sequences that fit a wave are looked
 // through by every wave for itself, more by the workgroup together.
-__device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
+template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (c.n_seqs <= 64) {
-    const AttnSeq s = attn_seq(c, lane);
+    const AttnSeq s = attn_seq<R>(c, lane);
     long long total = (long long)s.row_tiles * s.tiles;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2)
@@ -140,7 +143,7 @@ __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
     t.q0 = __builtin_amdgcn_readlane(s.q0, b);
     t.nq = __builtin_amdgcn_readlane(s.nq, b) * c.group;
     t.tiles = __builtin_amdgcn_readlane(s.tiles, b);
-    return attn_take(c, t, b, chunk, item - __builtin_amdgcn_readlane(upto - mine, b),
+    return attn_take<R>(c, t, b, chunk, item - __builtin_amdgcn_readlane(upto - mine, b),
                      __builtin_amdgcn_readlane(slots - split, b));
   }
   // Every thread takes a run of sequences; the runs' sums are scanned through LDS.
@@ -148,7 +151,7 @@ __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
   const int b0 = (int)threadIdx.x * per, b1 = min(b0 + per, c.n_seqs);
   long long total = 0;
   for (int b = b0; b < b1; ++b) {
-    const AttnSeq s = attn_seq(c, b);
+    const AttnSeq s = attn_seq<R>(c, b);
     total += (long long)s.row_tiles * s.tiles;
   }
 #pragma unroll
@@ -159,7 +162,7 @@ __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
   const int chunk = attn_chunk(c, sums[0] + sums[1] + sums[2] + sums[3]);
   int mine = 0, split = 0;
   for (int b = b0; b < b1; ++b) {
-    const AttnSeq s = attn_seq(c, b);
+    const AttnSeq s = attn_seq<R>(c, b);
     const int parts = (s.tiles + chunk - 1) / chunk, n = s.row_tiles * max(parts, 1);
     mine += n;
     split += parts > 1 ? n : 0;
@@ -177,7 +180,7 @@ __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
   if (item >= upto - mine && item < upto) {
     int first = upto - mine, slot0 = slots - split;
     for (int b = b0; b < b1; ++b) {
-      const AttnSeq s = attn_seq(c, b);
+      const AttnSeq s = attn_seq<R>(c, b);
       const int parts = (s.tiles + chunk - 1) / chunk, n = s.row_tiles * max(parts, 1);
       if (item < first + n) {
         lds[16] = b;
@@ -194,9 +197,9 @@ __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
   const int slot0 = __builtin_amdgcn_readfirstlane(lds[18]);
   AttnItem none{};
   if (b < 0) return none;
-  AttnSeq s = attn_seq(c, b);
+  AttnSeq s = attn_seq<R>(c, b);
   s.nq *= c.group;
-  return attn_take(c, s, b, chunk, i, slot0);
+  return attn_take<R>(c, s, b, chunk, i, slot0);
 }
 
 }  // namespace qvx

@@ -1,0 +1,273 @@
+// qvx_attn16.hip -- cross attention of many queries in fp16 / bf16 on gfx950's 16-bit matrix cores.
+//
+//   out[row] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (q[row] . k_j) - m),  c = scale log2(e)
+//
+// in one pass over the keys, 128 query rows a workgroup (32 a wave) against key and value tiles that
+// the workgroup stages in LDS, the next tile in flight while the present one is multiplied.
+//
+// Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction, fp32 sums.  The weights are
+// rounded to the operands' type (to the nearest) before the second product: each by at most half a
+// step, and the denominator sums them unrounded in fp32.  The reference m follows the largest logit
+// lazily, as in qvx_attn_split.hpp, at most 2^kSlack16 behind: weights to 2^8 are as exact in fp16 as
+// those to 1, and those of 2^-22 of the largest are still above its smallest normal number.
+//
+// Layout.  In S^T a lane holds query row lane % 32 and, with h = lane / 32, the keys 8 (r / 4) + 4 h + r % 4
+// in registers r = 0 .. 15.  The second product's right operand wants, for 16 keys, eight of them in
+// lane half h: registers 8 n .. 8 n + 7 are such eight for one order of the keys, so the weights are
+// only rounded and packed, and V^T is read with its keys in the same order: quads 4 h .. 4 h + 3 and
+// 8 + 4 h .. of a 16-key step, each by one transposing LDS read.  A lane's row is the same in S^T, P^T
+// and O^T, so maxima, sums and rescales need no lane exchange but that of the two halves.
+//
+// LDS rows are swizzled: 16-byte units of K by the row, so that sixteen rows' equal units cover the
+// banks, 64-byte runs of V by the row, so that the four rows of a transposing read do.
+#include "qvx_attn_split.hpp"
+
+namespace qvx {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kRows16 = 128;  // query rows of a workgroup
+constexpr float kSlack16 = 8.0f;
+
+typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
+
+template <uint32_t T> __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (T == T_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <uint32_t T> __device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (T == T_F16) {
+    const f16x2 h = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(uint32_t, h);
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 h = {(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(uint32_t, h);
+  }
+}
+
+// DP: head_dim rounded up to a multiple of 32; KT: keys of a tile.
+template <uint32_t T, int DP, int KT> struct Tile16 {
+  static constexpr int kPitch = 2 * DP;       // bytes of a row
+  static constexpr int kUnits = DP / 8;       // 16-byte units of a row
+  static constexpr int kBanks = kPitch / 4 % 64;
+  static constexpr int kBytes = KT * kPitch;  // of a tile of K, or of V
+  static constexpr int kLoads = (KT * kUnits + 255) / 256;  // units a thread stages
+  // Byte offset of unit u of row r.
+  static __device__ __forceinline__ int k_at(int r, int u) {
+    const int x = kBanks == 0 ? r & 15 : kBanks == 32 ? (r >> 1) & 7 : (r >> 2) & 3;
+    return r * kPitch + 16 * (u ^ x);
+  }
+  static __device__ __forceinline__ int v_at(int r, int u) {
+    const int x = kBanks == 0 ? r & 3 : kBanks == 32 ? (r >> 1) & 1 : 0;
+    return r * kPitch + 16 * (u ^ (4 * x));
+  }
+};
+
+template <uint32_t T, int DP, int KT>
+__global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
+  using L = Tile16<T, DP, KT>;
+  constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds16[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.y, d = c.head_dim;
+  const AttnItem it = attn_item<kRows16>(c, blockIdx.x, reinterpret_cast<int*>(lds16));
+  if (!it.any) return;
+  __syncthreads();  // the item's words are read before tiles overwrite them
+  const LdsPtr lds = (LdsPtr)lds16;
+
+  const int row = it.row0 + 32 * wave + col;
+  const bool live = row < it.rows;
+  const int64_t qat = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
+  u32x4 q[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int i = 16 * s + 8 * h;
+    q[s] = u32x4{0, 0, 0, 0};
+    if (live && i < d) {  // element by element where rows are not on 16-byte addresses
+      const uint16_t* p = static_cast<const uint16_t*>(c.q) + qat + i;
+      if (c.q_wide) {
+        q[s] = *reinterpret_cast<const u32x4*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[s][j] = (uint32_t)p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
+      }
+    }
+  }
+
+  // Staging: unit e = tid + 256 i of a tile is unit e % kUnits of its row e / kUnits.
+  uint32_t goff[L::kLoads];
+  int kst[L::kLoads], vst[L::kLoads];
+#pragma unroll
+  for (int i = 0; i < L::kLoads; ++i) {
+    const int e = tid + 256 * i, r = e / L::kUnits, u = e - r * L::kUnits;
+    goff[i] = 8 * u < d && r < KT ? (uint32_t)(r * c.pitch + 16 * u) : kPastEnd;
+    kst[i] = L::k_at(r, u);
+    vst[i] = L::v_at(r, u);
+  }
+  const int64_t base = (int64_t)it.seq * c.page_stride + (int64_t)kvh * c.head_stride;
+  u32x4 kreg[L::kLoads], vreg[L::kLoads];
+  auto fetch = [&](int t) {
+    const int n = min(KT, it.len - t * KT);
+    const int64_t at = base + (int64_t)t * KT * c.pitch;
+    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(n * c.pitch));
+    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(n * c.pitch));
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, goff[i], 0, 0);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, goff[i], 0, 0);
+  };
+  auto stage = [&](int buf) {
+    const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i)
+      if (KT * L::kUnits % 256 == 0 || tid + 256 * i < KT * L::kUnits) {
+        *(__attribute__((address_space(3))) u32x4*)(kb + kst[i]) = kreg[i];
+        *(__attribute__((address_space(3))) u32x4*)(vb + vst[i]) = vreg[i];
+      }
+  };
+
+  // Lane addresses of the transposing reads: row 4 h + lane % 16 / 4 and column quad lane % 4 of the
+  // sixteen columns that this group of sixteen lanes gets.
+  const int vrow = 4 * h + (lane & 15) / 4, vcol = 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+
+  float m = -INFINITY, l = 0.0f;
+  f32x16 acc[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
+
+  const int tiles = (it.len + KT - 1) / KT;
+  if (tiles > 0) {
+    fetch(0);
+    stage(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < tiles; ++t) {
+    if (t + 1 < tiles) fetch(t + 1);
+    const LdsPtr kb = lds + (t & 1) * 2 * L::kBytes, vb = kb + L::kBytes;
+    f32x16 s[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        const u32x4 a = *(__attribute__((address_space(3))) u32x4*)(kb + L::k_at(32 * b + col, 2 * i + h));
+        s[b] = mma32<T>(a, q[i], s[b]);
+      }
+    const int left = it.len - t * KT;
+    if (left < KT) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * b + 8 * (r / 4) + 4 * h + r % 4 >= left) s[b][r] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    top *= c.scale2;  // scale2 >= 0: the order stays
+    if (__any(top > m + kSlack16)) {
+      const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float f = m == now ? 1.0f : attn_pow2(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    u32x4 p[KB][2];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float x = attn_pow2(__builtin_fmaf(s[b][r], c.scale2, -ref));
+        const float y = attn_pow2(__builtin_fmaf(s[b][r + 1], c.scale2, -ref));
+        l += x;
+        l += y;
+        p[b][r / 8][r / 2 % 4] = pack2<T>(x, y);
+      }
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < DB; ++e) {
+          const int r0 = 32 * b + 16 * n + vrow, cc = 32 * e + vcol;
+          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) i16x4*)(vb + L::v_at(r0, cc / 8) + 2 * (cc & 7)));
+          const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) i16x4*)(vb + L::v_at(r0 + 8, cc / 8) + 2 * (cc & 7)));
+          const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[e] = mma32<T>(__builtin_bit_cast(u32x4, v), p[b][n], acc[e]);
+        }
+    if (t + 1 < tiles) stage((t + 1) & 1);  // the buffer that everyone left a barrier ago
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32);
+  if (!live) return;
+  const float inv = it.len ? 1.0f / l : 0.0f;  // no keys: zeros (acc is zero)
+  uint16_t* o = static_cast<uint16_t*>(c.out) + attn_row(c, it, row, kvh, c.out_stride);
+#pragma unroll
+  for (int e = 0; e < DB; ++e)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int i = 32 * e + 8 * (r / 4) + 4 * h;
+      if (i >= d) continue;
+      const u32x2 w = {pack2<T>(acc[e][r] * inv, acc[e][r + 1] * inv), pack2<T>(acc[e][r + 2] * inv, acc[e][r + 3] * inv)};
+      if (c.out_wide) {
+        *reinterpret_cast<u32x2*>(o + i) = w;
+      } else {
+        o[i] = (uint16_t)w[0], o[i + 1] = (uint16_t)(w[0] >> 16);
+        o[i + 2] = (uint16_t)w[1], o[i + 3] = (uint16_t)(w[1] >> 16);
+      }
+    }
+}
+
+template <uint32_t T, int DP, int KT> bool attn16(const AttnCall& c, dim3 grid, hipStream_t s) {
+  static LdsLimit lim;
+  const size_t lds = 4 * (size_t)Tile16<T, DP, KT>::kBytes;
+  if (!lds_ready(reinterpret_cast<const void*>(&k_attn16<T, DP, KT>), lim, lds)) return false;
+  k_attn16<T, DP, KT><<<grid, 256, lds, s>>>(c);
+  return true;
+}
+
+template <uint32_t T> bool attn16_dp(const AttnCall& c, dim3 grid, hipStream_t s) {
+  const int d = c.head_dim;
+  if (d <= 32) return attn16<T, 32, 64>(c, grid, s);
+  if (d <= 64) return attn16<T, 64, 64>(c, grid, s);
+  if (d <= 96) return attn16<T, 96, 64>(c, grid, s);
+  if (d <= 128) return attn16<T, 128, 64>(c, grid, s);
+  if (d <= 160) return attn16<T, 160, 32>(c, grid, s);
+  return attn16<T, 256, 32>(c, grid, s);
+}
+
+}  // namespace
+
+int attn16_rows() { return kRows16; }
+
+bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s) {
+  const dim3 grid((unsigned)c.items, (unsigned)c.kv_heads);
+  return type == T_F16 ? attn16_dp<T_F16>(c, grid, s) : attn16_dp<T_BF16>(c, grid, s);
+}
+
+}  // namespace qvx

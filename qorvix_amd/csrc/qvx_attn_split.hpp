@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.y, d = c.head_dim;
-  const AttnItem it = attn_item(c, blockIdx.x, reinterpret_cast<int*>(lds));
+  const AttnItem it = attn_item<kAttnRows>(c, blockIdx.x, reinterpret_cast<int*>(lds));
   if (!it.any) return;
 
   // This lane's query values: row col, for the key loads' pieces 32 s + 8 g + j.
