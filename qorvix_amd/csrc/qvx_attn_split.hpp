@@ -6,9 +6,10 @@
 // for any m, here a running reference that follows the largest s_j seen (below).  The sum is one pass
 // over the keys, so the cache is read once and that read bounds the kernel.
 //
-// Arithmetic.  Keys and values are widened to fp32 in registers (Q8_0: times their scale) and both
-// products run on the fp32 matrix instruction (16x16x4): queries, weights and sums are never rounded
-// below 32 bits, whatever the cache holds.
+// Arithmetic: fp32 throughout, whatever the cache holds.  The first product takes 16-bit keys as they are
+// and the queries in 16-bit parts that add up to the fp32 values (below); fp32 keys, and the values of
+// every type widened in registers, run on the fp32 matrix instruction (16x16x4), so the weights are
+// never rounded.
 //
 // Layout.  S^T = K Q^T puts key 4 g + r (g = lane / 16) and row lane % 16 into register r; the second
 // product reads its left operand, P, with row lane % 16 and key index g.  So the weights go from one
@@ -86,16 +87,31 @@ template <int N> struct AttnRaw<T_BF16, N> : AttnWords<N / 2> {
 template <int N> struct AttnRaw<T_Q8_0, N> : AttnWords<N / 4> {
   static constexpr int kBytes = N;
   __device__ __forceinline__ float at(int i, float step) const {
-    return (float)((int32_t)(this->w[i / 4] << (24 - 8 * (i % 4))) >> 24) * step;
+    // the byte as b + 128, unsigned: one conversion and one multiply-add a value
+    const uint32_t u = this->w[i / 4] ^ 0x80808080u;
+    return __builtin_fmaf((float)(u >> (8 * (i % 4)) & 255u), step, -128.0f * step);
   }
 };
 
-// One element of a query or an output row, by type.
-__device__ __forceinline__ float attn_load(const void* p, int64_t i, uint32_t type) {
-  if (type == T_F32) return static_cast<const float*>(p)[i];
-  const uint16_t h = static_cast<const uint16_t*>(p)[i];
-  if (type == T_F16) return (float)__builtin_bit_cast(_Float16, h);
-  return __builtin_bit_cast(float, (uint32_t)h << 16);
+// Eight consecutive elements of a query row, on any address of their type.
+__device__ __forceinline__ void attn_load8(float (&x)[8], const void* p, int64_t at, uint32_t type) {
+  if (type == T_F32) {
+    struct __attribute__((packed, aligned(4))) Eight {
+      float v[8];
+    };
+    const Eight e = *reinterpret_cast<const Eight*>(static_cast<const float*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = e.v[i];
+  } else {
+    struct __attribute__((packed, aligned(2))) Eight {
+      uint16_t v[8];
+    };
+    const Eight e = *reinterpret_cast<const Eight*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = type == T_F16 ? (float)__builtin_bit_cast(_Float16, e.v[i])
+                           : __builtin_bit_cast(float, (uint32_t)e.v[i] << 16);
+  }
 }
 __device__ __forceinline__ void attn_store(void* p, int64_t i, uint32_t type, float x) {
   if (type == T_F32) {
@@ -115,14 +131,88 @@ __device__ __forceinline__ int64_t attn_row(const AttnCall& c, const AttnItem& i
 
 __device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The queries as the first product's right operand, KS pieces of 32 values.  F32: fp32 itself, eight
+// values a lane for eight 16x16x4 instructions a piece.  Otherwise 16-bit parts that add up to the fp32
+// value, each multiplied by the keys in its own 16x16x32 instruction: fp16 twice (11 + 11 bits), bf16
+// three times (8 + 8 + 8); products of 16-bit values are exact in the instruction's fp32 sums.  The
+// row is first brought to a largest magnitude of 2^14 (a power of two, undone in the exponent), so
+// that no part overflows fp16 and the small part of every value that matters stays normal.
+template <uint32_t T, int KS> struct AttnQuery {
+  typedef _Float16 Key __attribute__((ext_vector_type(8)));
+  Key hi[KS], lo[KS];
+  __device__ __forceinline__ void set(int s, const float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hi[s][j] = (_Float16)x[j];
+      lo[s][j] = (_Float16)(x[j] - (float)hi[s][j]);
+    }
+  }
+  __device__ __forceinline__ f32x4 mul(int s, Key k, f32x4 c) const {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, lo[s], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(k, hi[s], c, 0, 0, 0);
+  }
+};
+template <int KS> struct AttnQuery<T_BF16, KS> {
+  typedef __bf16 Key __attribute__((ext_vector_type(8)));
+  Key part[3][KS];
+  __device__ __forceinline__ void set(int s, const float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float rest = x[j];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        part[i][s][j] = (__bf16)rest;
+        rest -= (float)part[i][s][j];
+      }
+    }
+  }
+  __device__ __forceinline__ f32x4 mul(int s, Key k, f32x4 c) const {
+#pragma unroll
+    for (int i = 2; i >= 0; --i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, part[i][s], c, 0, 0, 0);
+    return c;
+  }
+};
+template <int KS> struct AttnQuery<T_F32, KS> {
+  float v[KS][8];
+  __device__ __forceinline__ void set(int s, const float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[s][j] = x[j];
+  }
+};
+
+// A tile of 16 keys and their values as loaded: lane (col, g) holds pieces 32 s + 8 g of key col, and
+// values col * VB .. of keys 4 g .. 4 g + 3.
+template <uint32_t T, int DT> struct AttnTile {
+  static constexpr int KS = DT / 32, VB = DT / 16, VU = VB < 8 ? VB : 8, VN = VB / VU;
+  // The next tile is loaded during the present one where both fit the registers of two waves a SIMD
+  // (up to 8 KB a tile); larger tiles are loads enough by themselves.
+  static constexpr bool kAhead = DT * AttnRaw<T, 8>::kBytes * 4 <= 8192;
+  AttnRaw<T, 8> k[KS];
+  AttnRaw<T, VU> v[4][VN];
+  uint16_t kstep[T == T_Q8_0 ? KS : 1], vstep[T == T_Q8_0 ? 4 : 1];
+  int live;
+};
+
+__device__ __forceinline__ float attn_half(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+
+// Eight int8 as fp16: each byte b becomes the fp16 number 1024 + (b + 128), less 1152: exact.
+__device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&w)[2]) {
+  uint32_t x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = w[i / 2] ^ 0x80808080u;
+    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u, i % 2 ? 0x04030402u : 0x04010400u);
+    x[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
+  }
+  return __builtin_bit_cast(AttnQuery<T_F16, 1>::Key, u32x4{x[0], x[1], x[2], x[3]});
+}
+
 // DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.
 template <uint32_t T, int DT>
-__global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
-  constexpr int KS = DT / 32;  // 32 values of a key at a time
-  constexpr int VB = DT / 16;  // consecutive values of a lane in the second product
-  constexpr int VU = VB < 8 ? VB : 8, VN = VB / VU;
-  using KRaw = AttnRaw<T, 8>;
-  using VRaw = AttnRaw<T, VU>;
+__global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_split(AttnCall c) {
+  using Tile = AttnTile<T, DT>;
+  constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN;
+  constexpr int kKeyBytes = AttnRaw<T, 8>::kBytes, kValBytes = AttnRaw<T, VU>::kBytes / VU;
   constexpr bool kQ8 = T == T_Q8_0;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -131,32 +221,98 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
   const AttnItem it = attn_item<kAttnRows>(c, blockIdx.x, reinterpret_cast<int*>(lds));
   if (!it.any) return;
 
-  // This lane's query values: row col, for the key loads' pieces 32 s + 8 g + j.
-  float q[KS][8];
-  const int row = it.row0 + col;
-  {
-    const int64_t at = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = 32 * s + 8 * g + j;
-        q[s][j] = row < it.rows && i < d ? attn_load(c.q, at + i, c.q_type) * c.scale2 : 0.0f;
-      }
-  }
+  // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
+  const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
+  int page = 0, tok = 0, live = 0;
+  auto look_up = [&](int n) {
+    const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
+    live = 0;
+    if (t < it.tile1) {
+      const int p = t / c.page_tiles;
+      tok = (t - p * c.page_tiles) * kAttnTile;
+      page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
+      live = min(min(kAttnTile, c.page_size - tok), it.len - p * c.page_size - tok);
+      if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
+    }
+  };
+  look_up(0);
+
   uint32_t koff[KS], voff[VN], soff = 0, svoff = 0;
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    koff[s] = 32 * s + 8 * g < d ? (uint32_t)(col * c.pitch + (32 * s + 8 * g) * KRaw::kBytes / 8) : kPastEnd;
+    koff[s] = 32 * s + 8 * g < d ? (uint32_t)(col * c.pitch + (4 * s + g) * kKeyBytes) : kPastEnd;
 #pragma unroll
   for (int u = 0; u < VN; ++u) {
     const int i = col * VB + u * VU;
-    voff[u] = i < d ? (uint32_t)(4 * g * c.pitch + i * VRaw::kBytes / VU) : kPastEnd;
+    voff[u] = i < d ? (uint32_t)(4 * g * c.pitch + i * kValBytes) : kPastEnd;
   }
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   if constexpr (kQ8) {
     soff = (uint32_t)(col * spitch);
     svoff = col * VB < d ? (uint32_t)(4 * g * spitch + col * VB / 32 * 2) : kPastEnd;
+  }
+  // Tile n of the wave's, none (and no memory) past the last.
+  auto load = [&](Tile& x, int n) {
+    if (n && (n & 63) == 0) look_up(n);
+    const int64_t pg = __builtin_amdgcn_readlane(page, n & 63);
+    const int tk = __builtin_amdgcn_readlane(tok, n & 63);
+    x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
+    const int64_t at = pg * c.page_stride + (int64_t)kvh * c.head_stride + (int64_t)tk * c.pitch;
+    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(x.live * c.pitch));
+    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(x.live * c.pitch));
+#pragma unroll
+    for (int s = 0; s < KS; ++s) x.k[s].load(kr, koff[s]);
+    if constexpr (kQ8) {
+      const int64_t sat = pg * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tk) * spitch;
+      const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + sat, (uint32_t)(x.live * spitch));
+      const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + sat, (uint32_t)(x.live * spitch));
+#pragma unroll
+      for (int s = 0; s < KS; ++s)  // the scales of the keys that this lane gets in the product: 4 g .. 4 g + 3
+        x.kstep[s] = __builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + 2 * s : kPastEnd, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x.vstep[r] = __builtin_amdgcn_raw_buffer_load_b16(vs, svoff + r * spitch, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int u = 0; u < VN; ++u) x.v[r][u].load(vr, voff[u] + r * c.pitch);
+  };
+  Tile even, odd;
+  load(even, 0);
+
+  // This lane's query values: row col, pieces 32 s + 8 g; rows and values that are not there are zeros.
+  AttnQuery<T, KS> q;
+  float mul = 1.0f;
+  {
+    const int row = it.row0 + col;
+    const int64_t at = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
+    float x[KS][8];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int i = 32 * s + 8 * g;
+      attn_load8(x[s], c.q, at + (i < d ? i : 0), c.q_type);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[s][j] = row < it.rows && i < d ? x[s][j] * c.scale2 : 0.0f;
+    }
+    if constexpr (T != T_F32) {
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // 2^e <= top < 2^(e + 1) to 2^14; a row with an infinite value as it is
+      const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+      const int up = e < 128 ? 14 - e : 0;
+      mul = __builtin_ldexpf(1.0f, -up);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] = __builtin_ldexpf(x[s][j], up);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q.set(s, x[s]);
   }
 
   float m = -INFINITY, l = 0.0f;
@@ -164,62 +320,31 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
 #pragma unroll
   for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
-  const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
-  int page = 0, tok = 0, live = 0;
-  for (int n = 0; n < tiles; ++n) {
-    if ((n & 63) == 0) {
-      const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
-      live = 0;
-      if (t < it.tile1) {
-        const int p = t / c.page_tiles;
-        tok = (t - p * c.page_tiles) * kAttnTile;
-        page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
-        live = min(min(kAttnTile, c.page_size - tok), it.len - p * c.page_size - tok);
-        if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
-      }
-    }
-    const int64_t pg = __builtin_amdgcn_readlane(page, n & 63);
-    const int tk = __builtin_amdgcn_readlane(tok, n & 63), nk = __builtin_amdgcn_readlane(live, n & 63);
-    const int64_t at = pg * c.page_stride + (int64_t)kvh * c.head_stride + (int64_t)tk * c.pitch;
-    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(nk * c.pitch));
-    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(nk * c.pitch));
-    KRaw kw[KS];
-    VRaw vw[4][VN];
-    float kstep[KS], vstep[4];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) kw[s].load(kr, koff[s]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int u = 0; u < VN; ++u) vw[r][u].load(vr, voff[u] + r * c.pitch);
-    if constexpr (kQ8) {
-      const int64_t sat = pg * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tk) * spitch;
-      const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + sat, (uint32_t)(nk * spitch));
-      const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + sat, (uint32_t)(nk * spitch));
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        kstep[s] = (float)__builtin_bit_cast(
-            _Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + 2 * s : kPastEnd, 0, 0));
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        vstep[r] = (float)__builtin_bit_cast(
-            _Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vs, svoff + r * spitch, 0, 0));
-    } else {
-#pragma unroll
-      for (int s = 0; s < KS; ++s) kstep[s] = 1.0f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) vstep[r] = 1.0f;
-    }
+  auto step = [&](const Tile& x) {
     f32x4 sc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (T == T_F32) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kw[s].at(j, kstep[s]), q[s][j], sc, 0, 0, 0);
+        for (int j = 0; j < 8; ++j)
+          sc = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x.k[s].w[j]), q.v[s][j], sc, 0, 0, 0);
+      } else if constexpr (kQ8) {
+        // The piece is a block: its products are summed alone and then scaled, key by key.  The
+        // lane's registers are keys 4 g + r, whose scales the lanes col = 4 g + r loaded.
+        const f32x4 y = q.mul(s, attn_bytes(x.k[s].w), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        const float own = attn_half(x.kstep[s]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * g + r >= nk) sc[r] = -INFINITY;
-    const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        for (int r = 0; r < 4; ++r) sc[r] += y[r] * __shfl(own, 4 * g + r);
+      } else {
+        sc = q.mul(s, __builtin_bit_cast(typename AttnQuery<T, KS>::Key, x.k[s].w), sc);
+      }
+    }
+    if (x.live < kAttnTile) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * g + r >= x.live) sc[r] = -INFINITY;
+    }
+    const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
     if (__any(top > m + kSlack)) {  // m + slack is -inf at the start: any finite logit moves it
       float t = fmaxf(top, __shfl_xor(top, 16));
       t = fmaxf(t, __shfl_xor(t, 32));
@@ -239,16 +364,32 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attn_split(AttnCall c) {
     float p[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      p[r] = attn_pow2(sc[r] - ref);
+      p[r] = attn_pow2(__builtin_fmaf(sc[r], mul, -ref));
       l += p[r];
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
+      const float vs = kQ8 ? attn_half(x.vstep[kQ8 ? r : 0]) : 1.0f;
 #pragma unroll
       for (int u = 0; u < VN; ++u)
 #pragma unroll
         for (int j = 0; j < VU; ++j)
-          acc[u * VU + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], vw[r][u].at(j, vstep[r]), acc[u * VU + j], 0, 0, 0);
+          acc[u * VU + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], x.v[r][u].at(j, vs), acc[u * VU + j], 0, 0, 0);
+    }
+  };
+  if constexpr (Tile::kAhead) {
+    for (int n = 0; n < tiles; n += 2) {
+      load(odd, n + 1);
+      step(even);
+      if (n + 1 >= tiles) break;
+      load(even, n + 2);
+      step(odd);
+    }
+  } else {
+    for (int n = 0; n < tiles; ++n) {
+      if (n) load(even, n);
+      step(even);
+    }
   }
 
   // The lane groups hold sums over their own keys.
