@@ -4,6 +4,7 @@
 #include "qvx_kv.hpp"
 
 #include <cstdio>
+#include <cstdlib>
 
 namespace qvx {
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
@@ -66,18 +67,23 @@ int check_cache(const qvx_kv_cache* c, int64_t* stride) {
 // A chunk has at least 8 tiles (128 keys), two a wave: shorter ones are all launch and join.
 constexpr int kAttnWgs = 1024, kMinChunk = 8;
 
+// Rows of a row tile for sequences of `rows` rows.  Up to four rows run on a matrix instruction that computes
+// four, a quarter the time of sixteen; up to eight on two of those.
+int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+
 // False: the partition passes 31 bits.
 bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t tiles = (int64_t)c.max_len / c.page_size * c.page_tiles +
                         (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
   c.min_chunk = kMinChunk;
-  c.target = std::max(1, kAttnWgs / c.kv_heads);
+  static const int wgs = getenv("QVX_WGS") ? atoi(getenv("QVX_WGS")) : kAttnWgs;  // TUNE
+  c.target = std::max(1, wgs / c.kv_heads);
   *join = tiles > c.min_chunk;
   const int64_t items = std::min(row_tiles + c.target, row_tiles * std::max<int64_t>((tiles + kMinChunk - 1) / kMinChunk, 1));
   if (items > 0x7fffffffll || tiles > 0x7fffffffll) return false;
   c.items = (int)items;
   const int d16 = (c.head_dim + 15) / 16 * 16;
-  *ws_bytes = *join ? (size_t)attn_slots(c) * c.kv_heads * attn_part(c.lds_rows, d16) * sizeof(float) : 0;
+  *ws_bytes = *join ? (size_t)attn_slots(c) * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float) : 0;
   return true;
 }
 
@@ -104,8 +110,8 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   c.kv_heads = cache->kv_heads;
   c.group = q_heads / cache->kv_heads;
   c.head_dim = d;
-  c.lds_rows = std::min(kAttnRows, c.group);
-  const int64_t row_tiles = (int64_t)n_seqs * ((c.group + kAttnRows - 1) / kAttnRows);
+  c.tile_rows = tile_rows(c.group);
+  const int64_t row_tiles = (int64_t)n_seqs * ((c.group + c.tile_rows - 1) / c.tile_rows);
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
@@ -145,9 +151,10 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   c.group = q_heads / st->kv_heads;
   c.head_dim = st->head_dim;
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
-  if ((int64_t)n_q * c.group > 0x7fffffffll - kAttnRows) return QVX_E_RANGE;
-  c.lds_rows = (int)std::max<int64_t>(1, std::min<int64_t>(kAttnRows, rows));
-  const int64_t row_tiles = ragged ? (int64_t)n_q * c.group / kAttnRows + n_seqs : n_seqs * ((rows + kAttnRows - 1) / kAttnRows);
+  if ((int64_t)n_q * c.group > 0x7ffffff0ll) return QVX_E_RANGE;
+  c.tile_rows = tile_rows(ragged ? rows / n_seqs : rows);  // ragged: of a sequence in the mean
+  const int64_t row_tiles =
+      ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 

@@ -4,7 +4,7 @@
 //
 // A call attends rows of queries to the keys of their own sequence.  For one key / value head, the
 // query heads of its group at each query of a sequence are its rows, row = query * group + head in
-// the group, taken 16 at a time (the matrix instruction's width); the keys are taken in tiles of 16.
+// the group, taken R at a time; the keys are taken in tiles of 16.
 // A page of the paged cache holds whole tiles but for its last one, so tiles never cross a page.
 #pragma once
 
@@ -12,7 +12,6 @@
 
 namespace qvx {
 
-constexpr int kAttnRows = 16;   // query rows of a row tile
 constexpr int kAttnTile = 16;   // keys of a tile
 constexpr int kAttnWaves = 4;   // waves of a workgroup of the split kernel
 
@@ -37,7 +36,7 @@ struct AttnCall {
   int max_len;
   int n_seqs, kv_heads, group, head_dim;
   float scale2;     // scale * log2(e): the kernels work with powers of two
-  int lds_rows;     // rows of a row tile that can exist: min(16, queries of a sequence * group)
+  int tile_rows;    // query rows of a row tile of the split kernel: 4, 8 or 16
   int items;        // bound on the work items of a key / value head (grid x)
   int target, min_chunk;  // work items aimed at, fewest tiles of a chunk
   float* ws;        // partial results of split sequences
@@ -45,7 +44,7 @@ struct AttnCall {
 
 // Floats of the workspace per item of a split sequence and key / value head, head_dim rounded up to a
 // multiple of 16: the rows' values, maxima and sums.
-__host__ __device__ inline size_t attn_part(int rows, int d16) { return (size_t)rows * (d16 + 2); }
+__host__ __device__ inline size_t attn_part(int rows, int d16) { return (size_t)rows * (d16 + 4); }
 
 // The partition's bounds.  A chunk has C = max(min_chunk, sum / target) tiles, so sequences give at
 // most target items more than they have row tiles, and those of several chunks, each less than twice

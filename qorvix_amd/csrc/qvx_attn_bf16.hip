@@ -3,8 +3,8 @@
 
 namespace qvx {
 
-bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, size_t lds, hipStream_t s) {
-  return attn_split_dt<T_BF16>(c, grid, lds, s);
+bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, hipStream_t s) {
+  return attn_split_dt<T_BF16>(c, grid, s);
 }
 
 }  // namespace qvx

@@ -3,8 +3,8 @@
 
 namespace qvx {
 
-bool launch_attn_split_q8(const AttnCall& c, dim3 grid, size_t lds, hipStream_t s) {
-  return attn_split_dt<T_Q8_0>(c, grid, lds, s);
+bool launch_attn_split_q8(const AttnCall& c, dim3 grid, hipStream_t s) {
+  return attn_split_dt<T_Q8_0>(c, grid, s);
 }
 
 }  // namespace qvx

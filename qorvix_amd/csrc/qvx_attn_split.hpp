@@ -28,6 +28,8 @@
 
 #include "qvx_attn.hpp"
 
+#include <algorithm>
+
 namespace qvx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -113,14 +115,51 @@ __device__ __forceinline__ void attn_load8(float (&x)[8], const void* p, int64_t
                            : __builtin_bit_cast(float, (uint32_t)e.v[i] << 16);
   }
 }
-__device__ __forceinline__ void attn_store(void* p, int64_t i, uint32_t type, float x) {
+// Four consecutive elements of an output row, on any address of their type.
+__device__ __forceinline__ void attn_store4(void* p, int64_t at, uint32_t type, const float (&x)[4]) {
   if (type == T_F32) {
-    static_cast<float*>(p)[i] = x;
-  } else if (type == T_F16) {
-    static_cast<_Float16*>(p)[i] = (_Float16)x;
+    struct __attribute__((packed, aligned(4))) Four {
+      float v[4];
+    };
+    *reinterpret_cast<Four*>(static_cast<float*>(p) + at) = Four{{x[0], x[1], x[2], x[3]}};
   } else {
-    static_cast<__bf16*>(p)[i] = (__bf16)x;
+    struct __attribute__((packed, aligned(2))) Four {
+      uint16_t v[4];
+    };
+    Four f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f.v[i] = type == T_F16 ? __builtin_bit_cast(uint16_t, (_Float16)x[i]) : __builtin_bit_cast(uint16_t, (__bf16)x[i]);
+    *reinterpret_cast<Four*>(static_cast<uint16_t*>(p) + at) = f;
   }
+}
+
+// Lanes 4 r .. 4 r + 3 of each row of sixteen lanes: x of the lane `shift` to the left (to the right if
+// negative); the other lanes keep `old`.
+template <int r, int shift> __device__ __forceinline__ int attn_move(int old, float x) {
+  constexpr int ctrl = shift == 0 ? 0xe4 : shift > 0 ? 0x110 + shift : 0x100 - shift;
+  return __builtin_amdgcn_update_dpp(old, __builtin_bit_cast(int, x), ctrl, 0xf, 1 << r, false);
+}
+
+// Rows 4 t .. 4 t + 3 of the first product, key 4 g + r in register r of lanes 4 t .. 4 t + 3 of each sixteen, to
+// key 4 g + r in lanes 4 r .. 4 r + 3.
+template <int t> __device__ __forceinline__ float attn_gather(const f32x4& s) {
+  int z = attn_move<0, -4 * t>(0, s[0]);
+  z = attn_move<1, 4 - 4 * t>(z, s[1]);
+  z = attn_move<2, 8 - 4 * t>(z, s[2]);
+  z = attn_move<3, 12 - 4 * t>(z, s[3]);
+  return __builtin_bit_cast(float, z);
+}
+
+// a and b exchange halves between the lanes N apart and are added: the lanes with bit N clear get a + a',
+// the others b + b', the stroke marking the other lane's.
+template <int N> __device__ __forceinline__ float attn_swap_add(float a, float b) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  const u32x2 s = N == 32 ? __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(x, y, false, false))
+                          : __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, y, false, false));
+  // through scalars: a bit cast of a vector's element reads element 0 whichever it names
+  const uint32_t s0 = s[0], s1 = s[1];
+  return __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
 }
 
 // Element offset of a row's head in q (stride: q_stride) or out, and whether the row exists.
@@ -181,19 +220,36 @@ template <int KS> struct AttnQuery<T_F32, KS> {
 };
 
 // A tile of 16 keys and their values as loaded: lane (col, g) holds pieces 32 s + 8 g of key col, and
-// values col * VB .. of keys 4 g .. 4 g + 3.
-template <uint32_t T, int DT> struct AttnTile {
+// values col * VB .. of keys 4 g .. 4 g + 3; of Q8_0 also the scales of those four keys' blocks, and of
+// the values' block in each of them.  FULL: head_dim is DT, so a key's scales are one load.
+template <uint32_t T, int DT, bool FULL> struct AttnTile {
   static constexpr int KS = DT / 32, VB = DT / 16, VU = VB < 8 ? VB : 8, VN = VB / VU;
-  // The next tile is loaded during the present one where both fit the registers of two waves a SIMD
-  // (up to 8 KB a tile); larger tiles are loads enough by themselves.
-  static constexpr bool kAhead = DT * AttnRaw<T, 8>::kBytes * 4 <= 8192;
+  static constexpr bool kQ8 = T == T_Q8_0;
+  static constexpr int kRegs = 2 * DT * AttnRaw<T, 8>::kBytes / 32 / 4 + (kQ8 ? 2 * KS + 4 : 0);  // of a lane
   AttnRaw<T, 8> k[KS];
   AttnRaw<T, VU> v[4][VN];
-  uint16_t kstep[T == T_Q8_0 ? KS : 1], vstep[T == T_Q8_0 ? 4 : 1];
+  uint32_t kstep[kQ8 ? 4 : 1][kQ8 ? (KS + 1) / 2 : 1];  // [key r], two blocks' scales a word
+  uint16_t vstep[kQ8 ? 4 : 1];
   int live;
 };
 
 __device__ __forceinline__ float attn_half(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+
+// The second product for values 4 g + r of a tile, up to three sets of four rows: 16 blocks of 4 x 4 x 1, the four
+// of a lane group all taking the weights of block 4 g + r, that is of the group's key.
+template <int r, int NT, int VN, int VU, bool Q8, class Tile, int VB>
+__device__ __forceinline__ void attn_values(f32x4 (&acc)[NT][VB], const float (&p)[NT], const Tile& x) {
+  const float vs = Q8 ? attn_half(x.vstep[Q8 ? r : 0]) : 1.0f;
+#pragma unroll
+  for (int u = 0; u < VN; ++u)
+#pragma unroll
+    for (int j = 0; j < VU; ++j) {
+      const float v = x.v[r][u].at(j, vs);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        acc[t][u * VU + j] = __builtin_amdgcn_mfma_f32_4x4x1f32(p[t], v, acc[t][u * VU + j], 2, r, 0);
+    }
+}
 
 // Eight int8 as fp16: each byte b becomes the fp16 number 1024 + (b + 128), less 1152: exact.
 __device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&w)[2]) {
@@ -207,18 +263,19 @@ __device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&
   return __builtin_bit_cast(AttnQuery<T_F16, 1>::Key, u32x4{x[0], x[1], x[2], x[3]});
 }
 
-// DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.
-template <uint32_t T, int DT>
+// DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.  NS: sets of four
+// rows of a row tile, 1, 2 or 4.
+template <uint32_t T, int DT, bool FULL, int NS>
 __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_split(AttnCall c) {
-  using Tile = AttnTile<T, DT>;
-  constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN;
+  using Tile = AttnTile<T, DT, FULL>;
+  constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN, R = 4 * NS;
   constexpr int kKeyBytes = AttnRaw<T, 8>::kBytes, kValBytes = AttnRaw<T, VU>::kBytes / VU;
   constexpr bool kQ8 = T == T_Q8_0;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.y, d = c.head_dim;
-  const AttnItem it = attn_item<kAttnRows>(c, blockIdx.x, reinterpret_cast<int*>(lds));
+  const AttnItem it = attn_item<R>(c, blockIdx.x, reinterpret_cast<int*>(lds));
   if (!it.any) return;
 
   // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
@@ -248,12 +305,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   }
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   if constexpr (kQ8) {
-    soff = (uint32_t)(col * spitch);
+    soff = (uint32_t)(4 * g * spitch);
     svoff = col * VB < d ? (uint32_t)(4 * g * spitch + col * VB / 32 * 2) : kPastEnd;
   }
   // Tile n of the wave's, none (and no memory) past the last.
   auto load = [&](Tile& x, int n) {
-    if (n && (n & 63) == 0) look_up(n);
+    if (n && (n & 63) == 0 && n < tiles) look_up(n);
     const int64_t pg = __builtin_amdgcn_readlane(page, n & 63);
     const int tk = __builtin_amdgcn_readlane(tok, n & 63);
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
@@ -267,8 +324,21 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + sat, (uint32_t)(x.live * spitch));
       const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + sat, (uint32_t)(x.live * spitch));
 #pragma unroll
-      for (int s = 0; s < KS; ++s)  // the scales of the keys that this lane gets in the product: 4 g .. 4 g + 3
-        x.kstep[s] = __builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + 2 * s : kPastEnd, 0, 0);
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (FULL) {
+          AttnWords<(KS + 1) / 2> w;
+          w.load(ks, soff + r * spitch);
+#pragma unroll
+          for (int i = 0; i < (KS + 1) / 2; ++i) x.kstep[r][i] = w.w[i];
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const uint32_t h =
+                (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + r * spitch + 2 * s : kPastEnd, 0, 0);
+            x.kstep[r][s / 2] = s % 2 ? x.kstep[r][s / 2] | h << 16 : h;
+          }
+        }
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) x.vstep[r] = __builtin_amdgcn_raw_buffer_load_b16(vs, svoff + r * spitch, 0, 0);
     }
@@ -277,8 +347,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int u = 0; u < VN; ++u) x.v[r][u].load(vr, voff[u] + r * c.pitch);
   };
-  Tile even, odd;
-  load(even, 0);
+  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT == 128) ? 2 : 1;
+  Tile held[kHeld];
+  load(held[0], 0);
 
   // This lane's query values: row col, pieces 32 s + 8 g; rows and values that are not there are zeros.
   AttnQuery<T, KS> q;
@@ -292,7 +363,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       const int i = 32 * s + 8 * g;
       attn_load8(x[s], c.q, at + (i < d ? i : 0), c.q_type);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[s][j] = row < it.rows && i < d ? x[s][j] * c.scale2 : 0.0f;
+      for (int j = 0; j < 8; ++j) x[s][j] = col < R && row < it.rows && i < d ? x[s][j] * c.scale2 : 0.0f;
     }
     if constexpr (T != T_F32) {
       float top = 0.0f;
@@ -315,10 +386,20 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     for (int s = 0; s < KS; ++s) q.set(s, x[s]);
   }
 
-  float m = -INFINITY, l = 0.0f;
-  f32x4 acc[VB];
+  // Four sets of rows: a lane's weights are row col's for keys 4 g + r in register r.  Fewer: row
+  // 4 t + lane % 4's for key lane / 4 in register t.
+  constexpr bool kSets = NS < 4;
+  constexpr int NT = kSets ? NS : 1;
+  float m[NT], l[NT], muls[NT];
+  f32x4 acc[NT][VB];
 #pragma unroll
-  for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+    muls[t] = kSets ? __shfl(mul, 4 * t + (lane & 3)) : mul;
+#pragma unroll
+    for (int j = 0; j < VB; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
   auto step = [&](const Tile& x) {
     f32x4 sc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -329,129 +410,211 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         for (int j = 0; j < 8; ++j)
           sc = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x.k[s].w[j]), q.v[s][j], sc, 0, 0, 0);
       } else if constexpr (kQ8) {
-        // The piece is a block: its products are summed alone and then scaled, key by key.  The
-        // lane's registers are keys 4 g + r, whose scales the lanes col = 4 g + r loaded.
+        // The piece is a block: its products are summed alone and then scaled, key by key.
         const f32x4 y = q.mul(s, attn_bytes(x.k[s].w), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-        const float own = attn_half(x.kstep[s]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[r] += y[r] * __shfl(own, 4 * g + r);
+        for (int r = 0; r < 4; ++r) {
+          const f16x2 two = __builtin_bit_cast(f16x2, x.kstep[r][s / 2]);
+          sc[r] = __builtin_fmaf((float)(s % 2 ? two.y : two.x), y[r], sc[r]);
+        }
       } else {
         sc = q.mul(s, __builtin_bit_cast(typename AttnQuery<T, KS>::Key, x.k[s].w), sc);
       }
     }
-    if (x.live < kAttnTile) {
+    if constexpr (kSets) {
+      float top[NT], p[NT];
+      bool past = false;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (4 * g + r >= x.live) sc[r] = -INFINITY;
-    }
-    const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
-    if (__any(top > m + kSlack)) {  // m + slack is -inf at the start: any finite logit moves it
-      float t = fmaxf(top, __shfl_xor(top, 16));
-      t = fmaxf(t, __shfl_xor(t, 32));
-      const float now = fmaxf(m, t);
-      const float f = m == now ? 1.0f : attn_pow2(m - now);
-      m = now;
-      l *= f;
-      float fr[4];
+      for (int t = 0; t < NT; ++t) {
+        p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
+        if (x.live < kAttnTile && lane >> 2 >= x.live) p[t] = -INFINITY;
+        top[t] = p[t] * muls[t];
+        past |= top[t] > m[t] + kSlack;  // m + slack is -inf at the start: any finite logit moves it
+      }
+      if (__any(past)) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
+        for (int t = 0; t < NT; ++t) {
+          float now = top[t];
 #pragma unroll
-      for (int j = 0; j < VB; ++j)
+          for (int s = 4; s < 64; s *= 2) now = fmaxf(now, __shfl_xor(now, s));
+          now = fmaxf(m[t], now);
+          const float f = m[t] == now ? 1.0f : attn_pow2(m[t] - now);
+          m[t] = now;
+          l[t] *= f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][r] *= fr[r];
-    }
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float p[4];
+          for (int i = 0; i < 4; ++i) {
+            const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      p[r] = attn_pow2(__builtin_fmaf(sc[r], mul, -ref));
-      l += p[r];
-    }
+            for (int j = 0; j < VB; ++j) acc[t][j][i] *= fi;
+          }
+        }
+      }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float vs = kQ8 ? attn_half(x.vstep[kQ8 ? r : 0]) : 1.0f;
+      for (int t = 0; t < NT; ++t) {
+        p[t] = attn_pow2(__builtin_fmaf(p[t], muls[t], m[t] == -INFINITY ? 0.0f : -m[t]));
+        l[t] += p[t];
+      }
+      attn_values<0, NT, VN, VU, kQ8>(acc, p, x);
+      attn_values<1, NT, VN, VU, kQ8>(acc, p, x);
+      attn_values<2, NT, VN, VU, kQ8>(acc, p, x);
+      attn_values<3, NT, VN, VU, kQ8>(acc, p, x);
+    } else {
+      if (x.live < kAttnTile) {
 #pragma unroll
-      for (int u = 0; u < VN; ++u)
+        for (int r = 0; r < 4; ++r)
+          if (4 * g + r >= x.live) sc[r] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
+      if (__any(top > m[0] + kSlack)) {
+        float t = fmaxf(top, __shfl_xor(top, 16));
+        t = fmaxf(t, __shfl_xor(t, 32));
+        const float now = fmaxf(m[0], t);
+        const float f = m[0] == now ? 1.0f : attn_pow2(m[0] - now);
+        m[0] = now;
+        l[0] *= f;
+        float fr[4];
 #pragma unroll
-        for (int j = 0; j < VU; ++j)
-          acc[u * VU + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], x.v[r][u].at(j, vs), acc[u * VU + j], 0, 0, 0);
+        for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
+#pragma unroll
+        for (int j = 0; j < VB; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[0][j][r] *= fr[r];
+      }
+      const float ref = m[0] == -INFINITY ? 0.0f : m[0];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = attn_pow2(__builtin_fmaf(sc[r], mul, -ref));
+        l[0] += p;
+        const float vs = kQ8 ? attn_half(x.vstep[kQ8 ? r : 0]) : 1.0f;
+#pragma unroll
+        for (int u = 0; u < VN; ++u)
+#pragma unroll
+          for (int j = 0; j < VU; ++j)
+            acc[0][u * VU + j] =
+                __builtin_amdgcn_mfma_f32_16x16x4f32(p, x.v[r][u].at(j, vs), acc[0][u * VU + j], 0, 0, 0);
+      }
     }
   };
-  if constexpr (Tile::kAhead) {
-    for (int n = 0; n < tiles; n += 2) {
-      load(odd, n + 1);
-      step(even);
-      if (n + 1 >= tiles) break;
-      load(even, n + 2);
-      step(odd);
+  if constexpr (kHeld == 1) {
+    for (int n = 0; n < tiles; ++n) {
+      if (n) load(held[0], n);
+      step(held[0]);
     }
   } else {
-    for (int n = 0; n < tiles; ++n) {
-      if (n) load(even, n);
-      step(even);
+    for (int n = 0; n < tiles; n += kHeld) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (n + i >= tiles) break;
+        load(held[(i + kHeld - 1) % kHeld], n + i + kHeld - 1);
+        step(held[i]);
+      }
     }
   }
 
-  // The lane groups hold sums over their own keys.
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  // Join the waves: m, l and the values of the rows that exist, through LDS.
-  const int d16 = (d + 15) & ~15, nrow = min(kAttnRows, it.rows - it.row0);
-  float* lm = lds;                           // [wave][16]
-  float* ll = lds + kAttnWaves * kAttnRows;  // [wave][16]
-  float* lv = lds + 2 * kAttnWaves * kAttnRows + (size_t)wave * c.lds_rows * d16;
+  // Join the waves: m, l and the values of the rows, through LDS.
+  const int d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0);
+  float* lm = lds;                   // [wave][R]
+  float* ll = lds + kAttnWaves * R;  // [wave][R]
+  float* lv = lds + 2 * kAttnWaves * R + wave * R * d16;
   __syncthreads();  // attn_item's words have been read
-  if (lane < 16) {
-    lm[wave * kAttnRows + lane] = m;
-    ll[wave * kAttnRows + lane] = l;
+  if constexpr (kSets) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int s = 4; s < 64; s *= 2) l[t] += __shfl_xor(l[t], s);
+      if (lane < 4) {
+        lm[wave * R + 4 * t + lane] = m[t];
+        ll[wave * R + 4 * t + lane] = l[t];
+      }
+      // The lane groups hold sums over their own keys.  Halves of the values change places between the
+      // groups and are added, twice: group g ends with values VB / 4 * (2 (g / 2) + g % 2) .. of its VB.
+      constexpr int H = VB / 2, Q = VB / 4;
+      f32x4 half[H];
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) half[j][i] = attn_swap_add<32>(acc[t][j][i], acc[t][j + H][i]);
+#pragma unroll
+      for (int j = 0; j < Q; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = attn_swap_add<16>(half[j][i], half[j + Q][i]);
+          const int at = col * VB + (g >> 1) * H + (g & 1) * Q + j;
+          if (at < d) lv[(4 * t + i) * d16 + at] = v;
+        }
+    }
+  } else {
+    l[0] += __shfl_xor(l[0], 16);
+    l[0] += __shfl_xor(l[0], 32);
+    if (lane < 16) {
+      lm[wave * R + lane] = m[0];
+      ll[wave * R + lane] = l[0];
+    }
+#pragma unroll
+    for (int j = 0; j < VB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (col * VB + j < d) lv[(4 * g + r) * d16 + col * VB + j] = acc[0][j][r];
   }
-#pragma unroll
-  for (int j = 0; j < VB; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * g + r < nrow && col * VB + j < d) lv[(4 * g + r) * d16 + col * VB + j] = acc[j][r];
   __syncthreads();
-  const float* v0 = lds + 2 * kAttnWaves * kAttnRows;
-  const int vstride = c.lds_rows * d16;
-  float* part = it.chunks > 1 ? c.ws + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(c.lds_rows, d16) : nullptr;
-  for (int e = threadIdx.x; e < nrow * d; e += 64 * kAttnWaves) {
-    const int r = e / d, i = e - r * d;
+  const float* v0 = lds + 2 * kAttnWaves * R;
+  float* part = it.chunks > 1 ? c.ws + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16) : nullptr;
+  const int quads = d / 4;
+  for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
+    const int r = e / quads, i = 4 * (e - r * quads);
     float top = lm[r];
 #pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, lm[w * kAttnRows + r]);
+    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, lm[w * R + r]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, val = 0.0f;
+    float sum = 0.0f;
+    f32x4 val = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kAttnWaves; ++w) {
-      const float f = attn_pow2(lm[w * kAttnRows + r] - ref);
-      sum += ll[w * kAttnRows + r] * f;
-      val += v0[w * vstride + r * d16 + i] * f;
+      const float f = attn_pow2(lm[w * R + r] - ref);
+      sum += ll[w * R + r] * f;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(v0 + (w * R + r) * d16 + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) val[k] += x[k] * f;
     }
     if (it.chunks == 1) {
-      attn_store(c.out, attn_row(c, it, it.row0 + r, kvh, c.out_stride) + i, c.q_type, it.len ? val / sum : 0.0f);
+      float o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = it.len ? val[k] / sum : 0.0f;
+      attn_store4(c.out, attn_row(c, it, it.row0 + r, kvh, c.out_stride) + i, c.q_type, o);
     } else {
-      part[r * d16 + i] = val;
+      *reinterpret_cast<f32x4*>(part + r * d16 + i) = val;
       if (i == 0) {
-        part[c.lds_rows * d16 + r] = top;
-        part[c.lds_rows * (d16 + 1) + r] = sum;
+        part[R * d16 + r] = top;
+        part[R * (d16 + 1) + r] = sum;
       }
     }
   }
 }
 
-template <uint32_t T> bool attn_split_dt(const AttnCall& c, dim3 grid, size_t lds, hipStream_t s) {
-  static LdsLimit lim64, lim128, lim256;
-  if (c.head_dim <= 64) {
-    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 64>), lim64, lds)) return false;
-    k_attn_split<T, 64><<<grid, 64 * kAttnWaves, lds, s>>>(c);
-  } else if (c.head_dim <= 128) {
-    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 128>), lim128, lds)) return false;
-    k_attn_split<T, 128><<<grid, 64 * kAttnWaves, lds, s>>>(c);
-  } else {
-    if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, 256>), lim256, lds)) return false;
-    k_attn_split<T, 256><<<grid, 64 * kAttnWaves, lds, s>>>(c);
-  }
+// Rows of a row tile, 4, 8 or 16: as many as a call's row tiles hold (the launchers' and the join's R).
+template <uint32_t T, int DT, bool FULL, int NS> bool attn_split(const AttnCall& c, dim3 grid, hipStream_t s) {
+  static LdsLimit lim;
+  const size_t lds = (size_t)kAttnWaves * 4 * NS * (2 + (c.head_dim + 15) / 16 * 16) * sizeof(float);
+  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, DT, FULL, NS>), lim, lds)) return false;
+  k_attn_split<T, DT, FULL, NS><<<grid, 64 * kAttnWaves, lds, s>>>(c);
   return true;
+}
+
+template <uint32_t T, int DT, bool FULL> bool attn_split_rows(const AttnCall& c, dim3 grid, hipStream_t s) {
+  if (c.tile_rows == 4) return attn_split<T, DT, FULL, 1>(c, grid, s);
+  if (c.tile_rows == 8) return attn_split<T, DT, FULL, 2>(c, grid, s);
+  return attn_split<T, DT, FULL, 4>(c, grid, s);
+}
+
+template <uint32_t T> bool attn_split_dt(const AttnCall& c, dim3 grid, hipStream_t s) {
+  if constexpr (T == T_Q8_0) {
+    if (c.head_dim == 64) return attn_split_rows<T, 64, true>(c, grid, s);
+    if (c.head_dim == 128) return attn_split_rows<T, 128, true>(c, grid, s);
+    if (c.head_dim == 256) return attn_split_rows<T, 256, true>(c, grid, s);
+  }
+  if (c.head_dim <= 64) return attn_split_rows<T, 64, false>(c, grid, s);
+  if (c.head_dim <= 128) return attn_split_rows<T, 128, false>(c, grid, s);
+  return attn_split_rows<T, 256, false>(c, grid, s);
 }
 
 }  // namespace qvx
