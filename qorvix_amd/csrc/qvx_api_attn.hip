@@ -65,7 +65,7 @@ int check_cache(const qvx_kv_cache* c, int64_t* stride) {
 // The partition of a call whose heads, pages and sequences are filled in: how many work items are
 // aimed at, and the bounds that grid and workspace are sized by.  Workgroups to fill the chip: four a CU.
 // A chunk has at least 8 tiles (128 keys), two a wave: shorter ones are all launch and join.
-constexpr int kAttnWgs = 1024, kMinChunk = 8;
+constexpr int kAttnWgs = 512, kMinChunk = 8;
 
 // Rows of a row tile for sequences of `rows` rows.  Up to four rows run on a matrix instruction that computes
 // four, a quarter the time of sixteen; up to eight on two of those.
@@ -80,10 +80,13 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   c.target = std::max(1, wgs / c.kv_heads);
   *join = tiles > c.min_chunk;
   const int64_t items = std::min(row_tiles + c.target, row_tiles * std::max<int64_t>((tiles + kMinChunk - 1) / kMinChunk, 1));
-  if (items > 0x7fffffffll || tiles > 0x7fffffffll) return false;
+  if (items * c.kv_heads > 0x7fffffffll || tiles > 0x7fffffffll) return false;
   c.items = (int)items;
   const int d16 = (c.head_dim + 15) / 16 * 16;
-  *ws_bytes = *join ? (size_t)attn_slots(c) * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float) : 0;
+  c.small_sum = row_tiles * tiles <= 0x7fffffffll;
+  *ws_bytes = *join ? sizeof(AttnPiece) * (1 + (size_t)attn_slots(c)) +
+                          (size_t)attn_slots(c) * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float)
+                    : 0;
   return true;
 }
 
@@ -164,7 +167,7 @@ bool cross16(const AttnCall& c, uint32_t type, bool ragged, float scale, int* it
   if (c.q_type != type || type == T_F32 || !(scale >= 0.0f)) return false;
   const int64_t r = attn16_rows(), rows = (int64_t)(ragged ? c.n_q : c.q_each) * c.group;
   const int64_t tiles = ragged ? rows / r + c.n_seqs : c.n_seqs * ((rows + r - 1) / r);
-  if ((int64_t)c.n_q * c.group < 32 * (int64_t)c.n_seqs || tiles > 0x7fffffffll) return false;
+  if ((int64_t)c.n_q * c.group < 32 * (int64_t)c.n_seqs || tiles * c.kv_heads > 0x7fffffffll) return false;
   *items = (int)tiles;
   return true;
 }
@@ -296,7 +299,7 @@ int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q
   c.table = d_table;
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
-  c.ws = static_cast<float*>(d_ws);
+  c.ws = join ? static_cast<float*>(d_ws) : nullptr;
   return attn_status(launch_attn_split(c, cache->type, join, static_cast<hipStream_t>(stream)));
 }
 
@@ -334,7 +337,7 @@ int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_s
   c.q_offsets = d_offsets;
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
-  c.ws = static_cast<float*>(d_ws);
+  c.ws = join ? static_cast<float*>(d_ws) : nullptr;
   if (int items; cross16(c, states->type, d_offsets != nullptr, scale, &items)) {
     c.items = items;
     c.min_chunk = 0x7ffffff0;  // a row tile takes all keys

@@ -11,68 +11,81 @@ bool launch_attn_split_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 namespace {
 
 // The chunks of a split sequence's row tile joined: out = sum_j 2^(m_j - m) v_j / sum_j 2^(m_j - m) l_j,
-// m the largest m_j.  The grid is k_attn_split's; the workgroups of a row tile's chunks share its rows, one
-// at a time.  A row's factors are formed first, 256 chunks at a time, so that the loads of the values
-// depend on nothing and go out together: 4 values a lane, the lanes that a row leaves over on other
-// chunks.  Sums are taken in the same order in every run.
+// m the largest m_j.  A workgroup a piece and key / value head.  Up to kFewChunks chunks the workgroup of the
+// first takes all rows, else the row tile's workgroups share them, one row at a time.  Four values a
+// thread; the threads that the rows leave over take other chunks, each a running maximum over its own, eight
+// chunks' loads at a time; then the groups meet in LDS.  Latency bounds it: three dependent loads
+// (piece, partial results, store).  The order of the sums is the same in every run.
+constexpr int kFewChunks = 16;
+
 template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
-  __shared__ __attribute__((aligned(16))) float factor[256];
-  __shared__ __attribute__((aligned(16))) float4 sums[256];
-  __shared__ float red[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kvh = blockIdx.y;
-  const AttnItem it = attn_item<R>(c, blockIdx.x, reinterpret_cast<int*>(factor));
-  if (!it.any || it.chunks == 1) return;
-  const int d = c.head_dim, d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0);
+  __shared__ __attribute__((aligned(16))) float4 vals[256];
+  __shared__ float2 stats[256];
+  const int tid = threadIdx.x, kvh = blockIdx.y, slot = blockIdx.x;
+  const AttnPiece pc = attn_pieces(c.ws)[slot];  // of the workspace: may be read before it is known to be one
+  if (slot >= *reinterpret_cast<const int*>(c.ws)) return;
+  const bool few = pc.chunks <= kFewChunks;
+  if (few && pc.chunk != 0) return;
+  const int d = c.head_dim, d16 = (d + 15) & ~15, quads = d / 4, nrow = min(R, pc.rows - pc.row0);
   const size_t size = attn_part(R, d16), step = (size_t)c.kv_heads * size;
-  const float* first = c.ws + ((size_t)(it.slot - it.chunk) * c.kv_heads + kvh) * size;
-  const int quads = d / 4, groups = 256 / quads, mine = tid / quads, quad = tid - mine * quads;
-  for (int r = it.chunk; r < nrow; r += it.chunks) {
-    const float* ms = first + R * d16 + r;
-    float top = -INFINITY;
-    for (int j = tid; j < it.chunks; j += 256) top = fmaxf(top, ms[j * step]);
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    __syncthreads();
-    if (lane == 0) red[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
+  const float* first = attn_parts(c.ws, c.target) + ((size_t)(slot - pc.chunk) * c.kv_heads + kvh) * size;
+  const int wide = few ? min(R, 256 / quads) : 1;  // rows at a time
+  const int groups = 256 / (quads * wide), mine = tid / (quads * wide), rest = tid - mine * quads * wide;
+  const int row = rest / quads, quad = rest - row * quads;
+  for (int r0 = few ? 0 : pc.chunk; r0 < nrow; r0 += few ? wide : pc.chunks) {
+    const int r = r0 + row;
+    float m = -INFINITY, l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int j0 = 0; j0 < it.chunks; j0 += 256) {
-      const int n = min(256, it.chunks - j0);
-      if (j0) __syncthreads();
-      if (tid < n) {
-        const float* p = ms + (size_t)(j0 + tid) * step;
-        const float f = attn_pow2(p[0] - ref);
-        factor[tid] = f;
-        l += f * p[R];
-      }
-      __syncthreads();
-      if (mine < groups) {
-        const float* p = first + (size_t)j0 * step + r * d16 + 4 * quad;
-#pragma unroll 8
-        for (int j = mine; j < n; j += groups) {
-          const float4 x = *reinterpret_cast<const float4*>(p + (size_t)j * step);
-          const float f = factor[j];
-          v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+    if (mine < groups && r < nrow) {
+      for (int j0 = mine; j0 < pc.chunks; j0 += 8 * groups) {
+        float mj[8], lj[8];
+        float4 vj[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = j0 + i * groups;
+          const float* p = first + (size_t)min(j, pc.chunks - 1) * step;
+          mj[i] = p[R * d16 + r];
+          lj[i] = p[R * (d16 + 1) + r];
+          vj[i] = *reinterpret_cast<const float4*>(p + r * d16 + 4 * quad);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (j0 + i * groups >= pc.chunks) mj[i] = -INFINITY, lj[i] = 0.0f, vj[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          top = fmaxf(top, mj[i]);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top, f0 = attn_pow2(m - ref);
+        m = top;
+        l *= f0;
+        v.x *= f0, v.y *= f0, v.z *= f0, v.w *= f0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = attn_pow2(mj[i] - ref);
+          l += f * lj[i];
+          v.x += f * vj[i].x, v.y += f * vj[i].y, v.z += f * vj[i].z, v.w += f * vj[i].w;
         }
       }
     }
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-    if (lane == 0) red[4 + wave] = l;
-    sums[tid] = v;
+    __syncthreads();  // the round before has been read
+    vals[tid] = v;
+    stats[tid] = make_float2(m, l);
     __syncthreads();
-    if (mine == 0) {
+    if (mine == 0 && r < nrow) {
+      float top = m;
+      for (int i = 1; i < groups; ++i) top = fmaxf(top, stats[i * quads * wide + rest].x);
+      const float ref = top == -INFINITY ? 0.0f : top, f0 = attn_pow2(m - ref);
+      float sum = l * f0;
+      float o[4] = {v.x * f0, v.y * f0, v.z * f0, v.w * f0};
       for (int i = 1; i < groups; ++i) {
-        const float4 x = sums[i * quads + quad];
-        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        const float2 ml = stats[i * quads * wide + rest];
+        const float4 x = vals[i * quads * wide + rest];
+        const float f = attn_pow2(ml.x - ref);
+        sum += ml.y * f;
+        o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
       }
-      const float sum = red[4] + red[5] + red[6] + red[7];
-      const int64_t at = attn_row(c, it, it.row0 + r, kvh, c.out_stride) + 4 * quad;
-      const float o[4] = {v.x / sum, v.y / sum, v.z / sum, v.w / sum};
-      attn_store4(c.out, at, c.q_type, o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] /= sum;
+      attn_store4(c.out, attn_row(c, pc.q0, pc.row0 + r, kvh, c.out_stride) + 4 * quad, c.q_type, o);
     }
   }
 }
@@ -81,7 +94,7 @@ template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) 
 
 // The split kernel and, where the host's bound on the chunks allows a split, the join.
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s) {
-  const dim3 grid((unsigned)c.items, (unsigned)c.kv_heads);
+  const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
   bool ok = false;
   switch (type) {
     case T_F16: ok = launch_attn_split_f16(c, grid, s); break;
@@ -91,6 +104,7 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
     default: break;
   }
   if (ok && join) {
+    const dim3 grid((unsigned)std::min(c.items, attn_slots(c)), (unsigned)c.kv_heads);
     if (c.tile_rows == 4)
       k_attn_join<4><<<grid, 256, 0, s>>>(c);
     else if (c.tile_rows == 8)

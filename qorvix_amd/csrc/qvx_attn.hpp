@@ -37,9 +37,15 @@ struct AttnCall {
   int n_seqs, kv_heads, group, head_dim;
   float scale2;     // scale * log2(e): the kernels work with powers of two
   int tile_rows;    // query rows of a row tile of the split kernel: 4, 8 or 16
-  int items;        // bound on the work items of a key / value head (grid x)
+  int items;        // bound on the work items of a key / value head; the grid is items * kv_heads
   int target, min_chunk;  // work items aimed at, fewest tiles of a chunk
+  bool small_sum;         // the tiles of all row tiles stay below 2^31
   float* ws;        // partial results of split sequences
+};
+
+// What k_attn_join needs to know of a split sequence's item.
+struct AttnPiece {
+  int32_t q0, row0, rows, chunk, chunks, pad[3];
 };
 
 // Floats of the workspace per item of a split sequence and key / value head, head_dim rounded up to a
@@ -49,7 +55,12 @@ __host__ __device__ inline size_t attn_part(int rows, int d16) { return (size_t)
 // The partition's bounds.  A chunk has C = max(min_chunk, sum / target) tiles, so sequences give at
 // most target items more than they have row tiles, and those of several chunks, each less than twice
 // its share, at most 2 target in all: the workspace holds no more, however many sequences there are.
+// It begins with the number of those items and a piece for each.
 inline int attn_slots(const AttnCall& c) { return 2 * c.target; }
+__host__ __device__ inline AttnPiece* attn_pieces(float* ws) { return reinterpret_cast<AttnPiece*>(ws) + 1; }
+__host__ __device__ inline float* attn_parts(float* ws, int target) {
+  return reinterpret_cast<float*>(attn_pieces(ws) + 2 * target);
+}
 
 __device__ inline int attn_tiles(const AttnCall& c, int len) {
   const int full = len / c.page_size;
@@ -92,49 +103,73 @@ __device__ inline int attn_chunk(const AttnCall& c, long long total) {
   return (int)min(max((long long)c.min_chunk, (per + 3) / 4 * 4), 0x7ffffff0ll);
 }
 
+// A sequence's items: row_tiles times `full` chunks of C tiles, and row_tiles times `rest` (0 or 1) shorter
+// ones (an empty sequence has one, which writes zeros).  All sequences' full chunks come first, so that the
+// short ones fill the gaps at the end; `slots` is its share of the workspace.
+struct AttnCount {
+  int full, rest, slots;
+};
+__device__ inline AttnCount attn_count(const AttnSeq& s, int chunk) {
+  const int full = s.tiles / chunk, rest = s.tiles - full * chunk > 0 || s.tiles == 0 ? 1 : 0;
+  return {s.row_tiles * full, s.row_tiles * rest, full + rest > 1 ? s.row_tiles * (full + rest) : 0};
+}
+
+// Item i of sequence b's full (or else short) ones; slot0: its first slot.
 template <int R>
-__device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b, int chunk, int i, int slot0) {
+__device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b, int chunk, int i, bool full, int slot0) {
   AttnItem it;
   it.seq = b;
   it.len = s.len;
   it.q0 = s.q0;
   it.chunks = max((s.tiles + chunk - 1) / chunk, 1);
-  const int rt = i / it.chunks;
-  it.chunk = i - rt * it.chunks;
+  const int whole = s.tiles / chunk, rt = full ? i / max(whole, 1) : i;
+  it.chunk = full ? i - rt * whole : whole;
   it.rows = s.nq;
   it.row0 = rt * R;
   it.tile0 = it.chunk * chunk;
   it.tile1 = min(it.tile0 + chunk, s.tiles);
-  it.slot = slot0 + i;
+  it.slot = slot0 + rt * it.chunks + it.chunk;
   // Offsets that are no running sums can wrap the counts: nothing past the rows or the workspace then.
-  it.any = i >= 0 && it.row0 < it.rows && (it.chunks == 1 || (unsigned)it.slot < 2u * (unsigned)c.target);
+  it.any = i >= 0 && it.row0 >= 0 && it.row0 < it.rows && it.tile0 >= 0 &&
+           (it.chunks == 1 || (unsigned)it.slot < 2u * (unsigned)c.target);
   return it;
 }
 
+// Sum over the lanes up to this one (lane 63: of all).
+__device__ inline int attn_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes to the left in each sixteen
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the next sixteen, of each two
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
+}
+
 // The work item of number `item`, the same in every thread of the workgroup (256 threads); `lds`:
-// 20 words that the caller does not use across the call.  Sequences that fit a wave are looked
-// through by every wave for itself, more by the workgroup together.
-template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// 32 words that the caller does not use across the call; all_slots: the items of split sequences in all.
+// Sequences that fit a wave are looked through by every wave for itself, more by the workgroup together.
+template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, int& all_slots) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  AttnItem none{};
   if (c.n_seqs <= 64) {
     const AttnSeq s = attn_seq<R>(c, lane);
-    long long total = (long long)s.row_tiles * s.tiles;
+    long long total;
+    if (c.small_sum) {
+      total = __builtin_amdgcn_readlane(attn_scan(s.row_tiles * s.tiles), 63);
+    } else {
+      total = (long long)s.row_tiles * s.tiles;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      if (d < c.n_seqs) total += __shfl_xor(total, d);
-    total = __shfl(total, 0);
-    const int chunk = attn_chunk(c, total);
-    const int parts = (s.tiles + chunk - 1) / chunk;
-    const int mine = s.row_tiles * max(parts, 1), split = parts > 1 ? mine : 0;
-    int upto = mine, slots = split;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      if (d < c.n_seqs) {
-        const int o = __shfl_up(upto, d), p = __shfl_up(slots, d);
-        if (lane >= d) upto += o, slots += p;
-      }
-    const unsigned long long past = __ballot(upto > item);
-    AttnItem none{};
+      for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    }
+    const int chunk = __builtin_amdgcn_readfirstlane(attn_chunk(c, total));
+    const AttnCount n = attn_count(s, chunk);
+    const int full = attn_scan(n.full), rest = attn_scan(n.rest), slots = attn_scan(n.slots);
+    all_slots = __builtin_amdgcn_readlane(slots, 63);
+    const int fulls = __builtin_amdgcn_readlane(full, 63);
+    const bool first = item < fulls;
+    const int i = first ? item : item - fulls, upto = first ? full : rest;
+    const unsigned long long past = __ballot(upto > i);
     if (!past) return none;
     const int b = __builtin_ctzll(past);
     AttnSeq t;
@@ -142,8 +177,8 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
     t.q0 = __builtin_amdgcn_readlane(s.q0, b);
     t.nq = __builtin_amdgcn_readlane(s.nq, b) * c.group;
     t.tiles = __builtin_amdgcn_readlane(s.tiles, b);
-    return attn_take<R>(c, t, b, chunk, item - __builtin_amdgcn_readlane(upto - mine, b),
-                     __builtin_amdgcn_readlane(slots - split, b));
+    return attn_take<R>(c, t, b, chunk, i - __builtin_amdgcn_readlane(upto - (first ? n.full : n.rest), b), first,
+                        __builtin_amdgcn_readlane(slots - n.slots, b));
   }
   // Every thread takes a run of sequences; the runs' sums are scanned through LDS.
   const int per = (c.n_seqs + 255) / 256;
@@ -158,47 +193,43 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   long long* sums = reinterpret_cast<long long*>(lds);
   if (lane == 0) sums[wave] = total;
   __syncthreads();
-  const int chunk = attn_chunk(c, sums[0] + sums[1] + sums[2] + sums[3]);
-  int mine = 0, split = 0;
+  const int chunk = __builtin_amdgcn_readfirstlane(attn_chunk(c, sums[0] + sums[1] + sums[2] + sums[3]));
+  AttnCount n{0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    const AttnSeq s = attn_seq<R>(c, b);
-    const int parts = (s.tiles + chunk - 1) / chunk, n = s.row_tiles * max(parts, 1);
-    mine += n;
-    split += parts > 1 ? n : 0;
+    const AttnCount x = attn_count(attn_seq<R>(c, b), chunk);
+    n.full += x.full, n.rest += x.rest, n.slots += x.slots;
   }
-  int upto = mine, slots = split;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int o = __shfl_up(upto, d), p = __shfl_up(slots, d);
-    if (lane >= d) upto += o, slots += p;
-  }
-  if (lane == 63) lds[8 + wave] = upto, lds[12 + wave] = slots;
-  if (threadIdx.x == 0) lds[16] = -1;
+  int full = attn_scan(n.full), rest = attn_scan(n.rest), slots = attn_scan(n.slots);
+  if (lane == 63) lds[8 + wave] = full, lds[12 + wave] = rest, lds[16 + wave] = slots;
+  if (threadIdx.x == 0) lds[20] = -1;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += lds[8 + w], slots += lds[12 + w];
-  if (item >= upto - mine && item < upto) {
-    int first = upto - mine, slot0 = slots - split;
+  for (int w = 0; w < wave; ++w) full += lds[8 + w], rest += lds[12 + w], slots += lds[16 + w];
+  const int fulls = __builtin_amdgcn_readfirstlane(lds[8] + lds[9] + lds[10] + lds[11]);
+  all_slots = __builtin_amdgcn_readfirstlane(lds[16] + lds[17] + lds[18] + lds[19]);
+  const bool first = item < fulls;
+  const int i = first ? item : item - fulls, upto = first ? full : rest, mine = first ? n.full : n.rest;
+  if (i >= upto - mine && i < upto) {
+    int before = upto - mine, slot0 = slots - n.slots;
     for (int b = b0; b < b1; ++b) {
-      const AttnSeq s = attn_seq<R>(c, b);
-      const int parts = (s.tiles + chunk - 1) / chunk, n = s.row_tiles * max(parts, 1);
-      if (item < first + n) {
-        lds[16] = b;
-        lds[17] = item - first;
-        lds[18] = slot0;
+      const AttnCount x = attn_count(attn_seq<R>(c, b), chunk);
+      const int here = first ? x.full : x.rest;
+      if (i < before + here) {
+        lds[20] = b;
+        lds[21] = i - before;
+        lds[22] = slot0;
         break;
       }
-      first += n;
-      slot0 += parts > 1 ? n : 0;
+      before += here;
+      slot0 += x.slots;
     }
   }
   __syncthreads();
-  const int b = __builtin_amdgcn_readfirstlane(lds[16]), i = __builtin_amdgcn_readfirstlane(lds[17]);
-  const int slot0 = __builtin_amdgcn_readfirstlane(lds[18]);
-  AttnItem none{};
+  const int b = __builtin_amdgcn_readfirstlane(lds[20]), at = __builtin_amdgcn_readfirstlane(lds[21]);
+  const int slot0 = __builtin_amdgcn_readfirstlane(lds[22]);
   if (b < 0) return none;
   AttnSeq s = attn_seq<R>(c, b);
   s.nq *= c.group;
-  return attn_take<R>(c, s, b, chunk, i, slot0);
+  return attn_take<R>(c, s, b, chunk, at, first, slot0);
 }
 
 }  // namespace qvx

@@ -78,17 +78,18 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
   using L = Tile16<T, DP, KT>;
   constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds16[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const int kvh = blockIdx.y, d = c.head_dim;
-  const AttnItem it = attn_item<kRows16>(c, blockIdx.x, reinterpret_cast<int*>(lds16));
+  const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
+  int no_slots;
+  const AttnItem it = attn_item<kRows16>(c, item, reinterpret_cast<int*>(lds16), no_slots);
   if (!it.any) return;
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds16;
 
   const int row = it.row0 + 32 * wave + col;
   const bool live = row < it.rows;
-  const int64_t qat = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
+  const int64_t qat = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
   u32x4 q[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
@@ -169,6 +170,10 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
         const u32x4 a = *(__attribute__((address_space(3))) u32x4*)(kb + L::k_at(32 * b + col, 2 * i + h));
         s[b] = mma32<T>(a, q[i], s[b]);
       }
+    // The results of the matrix instructions are waited for here: on the path that skips the mask the
+    // compiler leaves too few slots between them and the first read.
+#pragma unroll
+    for (int b = 0; b < KB; ++b) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[b]));
     const int left = it.len - t * KT;
     if (left < KT) {
 #pragma unroll
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
   l += __shfl_xor(l, 32);
   if (!live) return;
   const float inv = it.len ? 1.0f / l : 0.0f;  // no keys: zeros (acc is zero)
-  uint16_t* o = static_cast<uint16_t*>(c.out) + attn_row(c, it, row, kvh, c.out_stride);
+  uint16_t* o = static_cast<uint16_t*>(c.out) + attn_row(c, it.q0, row, kvh, c.out_stride);
 #pragma unroll
   for (int e = 0; e < DB; ++e)
 #pragma unroll
@@ -266,7 +271,7 @@ template <uint32_t T> bool attn16_dp(const AttnCall& c, dim3 grid, hipStream_t s
 int attn16_rows() { return kRows16; }
 
 bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s) {
-  const dim3 grid((unsigned)c.items, (unsigned)c.kv_heads);
+  const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
   return type == T_F16 ? attn16_dp<T_F16>(c, grid, s) : attn16_dp<T_BF16>(c, grid, s);
 }
 

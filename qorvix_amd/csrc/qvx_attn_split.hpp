@@ -41,11 +41,9 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr float kSlack = 20.0f;
 constexpr uint32_t kPastEnd = 0x7fffff00u;  // an offset no descriptor reaches: the load gives zeros
 
+// A descriptor of `bytes` bytes from p (the same in all lanes): loads past them give zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const uint8_t* p, uint32_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
-  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
 }
 
 // N consecutive values of type T, N in 4, 8, 16: the raw words as loaded, and their fp32 values.
@@ -89,9 +87,7 @@ template <int N> struct AttnRaw<T_BF16, N> : AttnWords<N / 2> {
 template <int N> struct AttnRaw<T_Q8_0, N> : AttnWords<N / 4> {
   static constexpr int kBytes = N;
   __device__ __forceinline__ float at(int i, float step) const {
-    // the byte as b + 128, unsigned: one conversion and one multiply-add a value
-    const uint32_t u = this->w[i / 4] ^ 0x80808080u;
-    return __builtin_fmaf((float)(u >> (8 * (i % 4)) & 255u), step, -128.0f * step);
+    return (float)(int8_t)(this->w[i / 4] >> (8 * (i % 4))) * step;
   }
 };
 
@@ -163,9 +159,9 @@ template <int N> __device__ __forceinline__ float attn_swap_add(float a, float b
 }
 
 // Element offset of a row's head in q (stride: q_stride) or out, and whether the row exists.
-__device__ __forceinline__ int64_t attn_row(const AttnCall& c, const AttnItem& it, int row, int kvh, int64_t stride) {
+__device__ __forceinline__ int64_t attn_row(const AttnCall& c, int q0, int row, int kvh, int64_t stride) {
   const int query = row / c.group, head = row - query * c.group;
-  return (int64_t)(it.q0 + query) * stride + (int64_t)(kvh * c.group + head) * c.head_dim;
+  return (int64_t)(q0 + query) * stride + (int64_t)(kvh * c.group + head) * c.head_dim;
 }
 
 __device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -235,20 +231,45 @@ template <uint32_t T, int DT, bool FULL> struct AttnTile {
 
 __device__ __forceinline__ float attn_half(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
 
+// Values formed here, all of them, before anything that uses them.  Left to itself the compiler converts each
+// value right before the matrix instruction that reads it, in one register, and every pair then waits out
+// the hazard between the two: two idle slots a value.
+template <int N> __device__ __forceinline__ void attn_pin(float (&v)[N]) {
+  if constexpr (N == 8)
+    asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]));
+  else
+    asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+}
+
 // The second product for values 4 g + r of a tile, up to three sets of four rows: 16 blocks of 4 x 4 x 1, the four
-// of a lane group all taking the weights of block 4 g + r, that is of the group's key.
+// of a lane group all taking the weights of block 4 g + r, that is of the group's key.  Q8_0: the four
+// lanes of a block hold one 32-value block of the key, so its scale goes into the weights, which each
+// block then takes for itself, and the values are the integers.
 template <int r, int NT, int VN, int VU, bool Q8, class Tile, int VB>
 __device__ __forceinline__ void attn_values(f32x4 (&acc)[NT][VB], const float (&p)[NT], const Tile& x) {
-  const float vs = Q8 ? attn_half(x.vstep[Q8 ? r : 0]) : 1.0f;
+  constexpr bool kOwn = Q8 && VB == 8;  // DT = 128: a block of four lanes holds 32 values
+  float w[NT];
 #pragma unroll
-  for (int u = 0; u < VN; ++u)
+  for (int t = 0; t < NT; ++t) {
+    w[t] = p[t];
+    if constexpr (kOwn)  // lanes 4 r + lane % 4 of the sixteen
+      w[t] = __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, p[t]), 4 * r << 5 | 0x13)) *
+             attn_half(x.vstep[r]);
+  }
+  const float vs = Q8 && !kOwn ? attn_half(x.vstep[Q8 ? r : 0]) : 1.0f;
 #pragma unroll
-    for (int j = 0; j < VU; ++j) {
-      const float v = x.v[r][u].at(j, vs);
+  for (int u = 0; u < VN; ++u) {
+    float v[VU];
+#pragma unroll
+    for (int j = 0; j < VU; ++j) v[j] = x.v[r][u].at(j, vs);
+    attn_pin(v);
+#pragma unroll
+    for (int j = 0; j < VU; ++j)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        acc[t][u * VU + j] = __builtin_amdgcn_mfma_f32_4x4x1f32(p[t], v, acc[t][u * VU + j], 2, r, 0);
-    }
+        acc[t][u * VU + j] =
+            __builtin_amdgcn_mfma_f32_4x4x1f32(w[t], v[j], acc[t][u * VU + j], kOwn ? 0 : 2, kOwn ? 0 : r, 0);
+  }
 }
 
 // Eight int8 as fp16: each byte b becomes the fp16 number 1024 + (b + 128), less 1152: exact.
@@ -272,25 +293,38 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   constexpr int kKeyBytes = AttnRaw<T, 8>::kBytes, kValBytes = AttnRaw<T, VU>::kBytes / VU;
   constexpr bool kQ8 = T == T_Q8_0;
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, d = c.head_dim;
-  const AttnItem it = attn_item<R>(c, blockIdx.x, reinterpret_cast<int*>(lds));
+  const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
+  int all_slots = 0;
+  const AttnItem it = attn_item<R>(c, item, reinterpret_cast<int*>(lds), all_slots);
+  if (c.ws && kvh == 0 && threadIdx.x == 0) {
+    if (item == 0) *reinterpret_cast<int*>(c.ws) = min(all_slots, 2 * c.target);
+    if (it.any && it.chunks > 1) attn_pieces(c.ws)[it.slot] = AttnPiece{it.q0, it.row0, it.rows, it.chunk, it.chunks, {}};
+  }
   if (!it.any) return;
 
   // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
   const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
-  int page = 0, tok = 0, live = 0;
+  const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
+  int64_t at = 0, sat = 0;  // of the tile's keys (and values), and of their scales, from the cache's start
+  int live = 0;
   auto look_up = [&](int n) {
     const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
     live = 0;
     if (t < it.tile1) {
-      const int p = t / c.page_tiles;
-      tok = (t - p * c.page_tiles) * kAttnTile;
-      page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
+      const int p = t / c.page_tiles, tok = (t - p * c.page_tiles) * kAttnTile;
+      int page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
       live = min(min(kAttnTile, c.page_size - tok), it.len - p * c.page_size - tok);
       if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
+      at = page * c.page_stride + kvh * c.head_stride + (int64_t)tok * c.pitch;
+      if constexpr (kQ8) sat = page * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tok) * spitch;
     }
+  };
+  // A lane's 64-bit value in all of them.
+  auto of_lane = [](int64_t x, int i) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)x, i));
   };
   look_up(0);
 
@@ -303,7 +337,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     const int i = col * VB + u * VU;
     voff[u] = i < d ? (uint32_t)(4 * g * c.pitch + i * kValBytes) : kPastEnd;
   }
-  const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   if constexpr (kQ8) {
     soff = (uint32_t)(4 * g * spitch);
     svoff = col * VB < d ? (uint32_t)(4 * g * spitch + col * VB / 32 * 2) : kPastEnd;
@@ -311,18 +344,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   // Tile n of the wave's, none (and no memory) past the last.
   auto load = [&](Tile& x, int n) {
     if (n && (n & 63) == 0 && n < tiles) look_up(n);
-    const int64_t pg = __builtin_amdgcn_readlane(page, n & 63);
-    const int tk = __builtin_amdgcn_readlane(tok, n & 63);
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
-    const int64_t at = pg * c.page_stride + (int64_t)kvh * c.head_stride + (int64_t)tk * c.pitch;
-    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(x.live * c.pitch));
-    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(x.live * c.pitch));
+    const int64_t ta = of_lane(at, n & 63);
+    const uint32_t bytes = (uint32_t)(x.live * c.pitch);
+    const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + ta, bytes);
+    const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + ta, bytes);
 #pragma unroll
     for (int s = 0; s < KS; ++s) x.k[s].load(kr, koff[s]);
     if constexpr (kQ8) {
-      const int64_t sat = pg * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tk) * spitch;
-      const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + sat, (uint32_t)(x.live * spitch));
-      const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + sat, (uint32_t)(x.live * spitch));
+      const int64_t ts = of_lane(sat, n & 63);
+      const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + ts, (uint32_t)(x.live * spitch));
+      const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + ts, (uint32_t)(x.live * spitch));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (FULL) {
@@ -349,14 +381,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   };
   constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT == 128) ? 2 : 1;
   Tile held[kHeld];
-  load(held[0], 0);
+#pragma unroll
+  for (int i = 0; i < std::max(1, kHeld - 1); ++i) load(held[i], i);
 
   // This lane's query values: row col, pieces 32 s + 8 g; rows and values that are not there are zeros.
   AttnQuery<T, KS> q;
   float mul = 1.0f;
   {
     const int row = it.row0 + col;
-    const int64_t at = attn_row(c, it, min(row, it.rows - 1), kvh, c.q_stride);
+    const int64_t at = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
     float x[KS][8];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -427,7 +460,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
-        if (x.live < kAttnTile && lane >> 2 >= x.live) p[t] = -INFINITY;
+        if (lane >> 2 >= x.live) p[t] = -INFINITY;
         top[t] = p[t] * muls[t];
         past |= top[t] > m[t] + kSlack;  // m + slack is -inf at the start: any finite logit moves it
       }
@@ -459,11 +492,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       attn_values<2, NT, VN, VU, kQ8>(acc, p, x);
       attn_values<3, NT, VN, VU, kQ8>(acc, p, x);
     } else {
-      if (x.live < kAttnTile) {
+      // In every tile: a branch around it right behind the product would lead to reads of sc sooner than the
+      // matrix instruction's results are there, and the compiler counts the wait on the other path alone.
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (4 * g + r >= x.live) sc[r] = -INFINITY;
-      }
+      for (int r = 0; r < 4; ++r) sc[r] = 4 * g + r >= x.live ? -INFINITY : sc[r];
       const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
       if (__any(top > m[0] + kSlack)) {
         float t = fmaxf(top, __shfl_xor(top, 16));
@@ -487,11 +519,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         l[0] += p;
         const float vs = kQ8 ? attn_half(x.vstep[kQ8 ? r : 0]) : 1.0f;
 #pragma unroll
-        for (int u = 0; u < VN; ++u)
+        for (int u = 0; u < VN; ++u) {
+          float v[VU];
+#pragma unroll
+          for (int j = 0; j < VU; ++j) v[j] = x.v[r][u].at(j, vs);
+          attn_pin(v);
 #pragma unroll
           for (int j = 0; j < VU; ++j)
-            acc[0][u * VU + j] =
-                __builtin_amdgcn_mfma_f32_16x16x4f32(p, x.v[r][u].at(j, vs), acc[0][u * VU + j], 0, 0, 0);
+            acc[0][u * VU + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, v[j], acc[0][u * VU + j], 0, 0, 0);
+        }
       }
     }
   };
@@ -506,6 +542,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int i = 0; i < kHeld; ++i) {
         if (n + i >= tiles) break;
         load(held[(i + kHeld - 1) % kHeld], n + i + kHeld - 1);
+        __builtin_amdgcn_sched_barrier(0);  // the loads go out before the tile in work is waited for
         step(held[i]);
       }
     }
@@ -558,7 +595,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   }
   __syncthreads();
   const float* v0 = lds + 2 * kAttnWaves * R;
-  float* part = it.chunks > 1 ? c.ws + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16) : nullptr;
+  float* part = it.chunks > 1 ? attn_parts(c.ws, c.target) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
+                              : nullptr;
   const int quads = d / 4;
   for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
     const int r = e / quads, i = 4 * (e - r * quads);
@@ -580,7 +618,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       float o[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = it.len ? val[k] / sum : 0.0f;
-      attn_store4(c.out, attn_row(c, it, it.row0 + r, kvh, c.out_stride) + i, c.q_type, o);
+      attn_store4(c.out, attn_row(c, it.q0, it.row0 + r, kvh, c.out_stride) + i, c.q_type, o);
     } else {
       *reinterpret_cast<f32x4*>(part + r * d16 + i) = val;
       if (i == 0) {
