@@ -7,7 +7,7 @@
 //
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction, fp32 sums.  The weights are
 // rounded to the operands' type (to the nearest) before the second product: each by at most half a
-// step, and the denominator sums them unrounded in fp32.  The reference m follows the largest logit
+// step; the denominator sums them in fp32.  The reference m follows the largest logit
 // lazily, as in qvx_attn_split.hpp, at most 2^kSlack16 behind: weights to 2^8 are as exact in fp16 as
 // those to 1, and those of 2^-22 of the largest are still above its smallest normal number.
 //
@@ -55,6 +55,19 @@ template <uint32_t T> __device__ __forceinline__ uint32_t pack2(float x, float y
   }
 }
 
+// The denominator's sum with two more weights: bf16 as rounded (one instruction for both, and the rounding then
+// cancels where values are alike), fp16 unrounded (its dot instruction is not promised to keep subnormal
+// inputs, and many small weights may carry a row).
+template <uint32_t T> __device__ __forceinline__ float sum2(float l, float x, float y, uint32_t xy) {
+  if constexpr (T == T_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, xy), one, l, false);
+  } else {
+    return l + x + y;
+  }
+}
+
 // DP: head_dim rounded up to a multiple of 32; KT: keys of a tile.
 template <uint32_t T, int DP, int KT> struct Tile16 {
   static constexpr int kPitch = 2 * DP;       // bytes of a row
@@ -74,7 +87,7 @@ template <uint32_t T, int DP, int KT> struct Tile16 {
 };
 
 template <uint32_t T, int DP, int KT>
-__global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn16(AttnCall c) {
   using L = Tile16<T, DP, KT>;
   constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds16[];
@@ -154,10 +167,13 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
     fetch(0);
     stage(0);
   }
+  // Nothing is on its way when the loop starts: a query register that might be makes the compiler wait, in
+  // every tile, for the loads of the next one.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
-  for (int t = 0; t < tiles; ++t) {
-    if (t + 1 < tiles) fetch(t + 1);
-    const LdsPtr kb = lds + (t & 1) * 2 * L::kBytes, vb = kb + L::kBytes;
+  // One tile from buffer `buf`, a constant in the unrolled loop: the LDS addresses are then lane offsets and immediates.
+  auto tile = [&](int t, int buf) {
+    const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
     f32x16 s[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b)
@@ -172,8 +188,10 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
       }
     // The results of the matrix instructions are waited for here: on the path that skips the mask the
     // compiler leaves too few slots between them and the first read.
-#pragma unroll
-    for (int b = 0; b < KB; ++b) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[b]));
+    if constexpr (KB == 2)
+      asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[1]));
+    else
+      asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]));
     const int left = it.len - t * KT;
     if (left < KT) {
 #pragma unroll
@@ -206,9 +224,9 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
       for (int r = 0; r < 16; r += 2) {
         const float x = attn_pow2(__builtin_fmaf(s[b][r], c.scale2, -ref));
         const float y = attn_pow2(__builtin_fmaf(s[b][r + 1], c.scale2, -ref));
-        l += x;
-        l += y;
-        p[b][r / 8][r / 2 % 4] = pack2<T>(x, y);
+        const uint32_t xy = pack2<T>(x, y);
+        l = sum2<T>(l, x, y, xy);
+        p[b][r / 8][r / 2 % 4] = xy;
       }
 #pragma unroll
     for (int b = 0; b < KB; ++b)
@@ -224,9 +242,20 @@ __global__ __launch_bounds__(256) void k_attn16(AttnCall c) {
           const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
           acc[e] = mma32<T>(__builtin_bit_cast(u32x4, v), p[b][n], acc[e]);
         }
-    if (t + 1 < tiles) stage((t + 1) & 1);  // the buffer that everyone left a barrier ago
-    __syncthreads();
+  };
+  const bool any_row = it.row0 + 32 * wave < it.rows;  // a wave past the rows only stages
+  for (int t0 = 0; t0 < tiles; t0 += 2) {
+#pragma unroll
+    for (int buf = 0; buf < 2; ++buf) {
+      const int t = t0 + buf;
+      if (t >= tiles) break;
+      if (t + 1 < tiles) fetch(t + 1);
+      if (any_row) tile(t, buf);
+      if (t + 1 < tiles) stage(buf ^ 1);  // the buffer that everyone left a barrier ago
+      __syncthreads();
+    }
   }
+
 
   l += __shfl_xor(l, 32);
   if (!live) return;
