@@ -137,6 +137,12 @@ template <int r, int shift> __device__ __forceinline__ int attn_move(int old, fl
   return __builtin_amdgcn_update_dpp(old, __builtin_bit_cast(int, x), ctrl, 0xf, 1 << r, false);
 }
 
+// x of the lane N further to the right in its sixteen, around the end.
+template <int N> __device__ __forceinline__ float attn_rotate(float x) {
+  const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, false);
+  return __builtin_bit_cast(float, y);
+}
+
 // Rows 4 t .. 4 t + 3 of the first product, key 4 g + r in register r of lanes 4 t .. 4 t + 3 of each sixteen, to
 // key 4 g + r in lanes 4 r .. 4 r + 3.
 template <int t> __device__ __forceinline__ float attn_gather(const f32x4& s) {
@@ -218,13 +224,22 @@ template <int KS> struct AttnQuery<T_F32, KS> {
 // A tile of 16 keys and their values as loaded: lane (col, g) holds pieces 32 s + 8 g of key col, and
 // values col * VB .. of keys 4 g .. 4 g + 3; of Q8_0 also the scales of those four keys' blocks, and of
 // the values' block in each of them.  FULL: head_dim is DT, so a key's scales are one load.
-template <uint32_t T, int DT, bool FULL> struct AttnTile {
+//
+// Q8_0 for four rows (kGroup): the products of each block have to be summed alone, and sixteen lanes that each
+// fetch 8 bytes of another key keep the address units busier than the memory (4.4 TB/s where fp16 reaches
+// 5.6).  So a lane group takes whole blocks: NP of them at a time, one for 4 / NP groups, in 16-byte
+// loads, and the four rows stand NP times among the sixteen columns of the product, each time with the
+// values of one group's block and zeros for the others': one instruction chain sums NP blocks apart.
+template <uint32_t T, int DT, bool FULL, int NS> struct AttnTile {
   static constexpr int KS = DT / 32, VB = DT / 16, VU = VB < 8 ? VB : 8, VN = VB / VU;
-  static constexpr bool kQ8 = T == T_Q8_0;
-  static constexpr int kRegs = 2 * DT * AttnRaw<T, 8>::kBytes / 32 / 4 + (kQ8 ? 2 * KS + 4 : 0);  // of a lane
+  static constexpr bool kQ8 = T == T_Q8_0, kGroup = kQ8 && NS == 1;
+  static constexpr int NP = kGroup ? (KS < 4 ? KS : 4) : 1, U = KS / NP, J = KS / U, G4 = 4 / NP;
+  static constexpr int kRegs = 2 * DT * AttnRaw<T, 8>::kBytes / 32 / 4 +
+                               (kGroup ? 4 * U + 4 : kQ8 ? 2 * KS + 4 : 0);  // of a lane
   AttnRaw<T, 8> k[KS];
   AttnRaw<T, VU> v[4][VN];
-  uint32_t kstep[kQ8 ? 4 : 1][kQ8 ? (KS + 1) / 2 : 1];  // [key r], two blocks' scales a word
+  // [key r][two blocks' scales a word]; kGroup: [key r][this lane's block of round u]
+  uint32_t kstep[kQ8 ? 4 : 1][kGroup ? U : kQ8 ? (KS + 1) / 2 : 1];
   uint16_t vstep[kQ8 ? 4 : 1];
   int live;
 };
@@ -242,12 +257,12 @@ template <int N> __device__ __forceinline__ void attn_pin(float (&v)[N]) {
 }
 
 // The second product for values 4 g + r of a tile, up to three sets of four rows: 16 blocks of 4 x 4 x 1, the four
-// of a lane group all taking the weights of block 4 g + r, that is of the group's key.  Q8_0: the four
-// lanes of a block hold one 32-value block of the key, so its scale goes into the weights, which each
-// block then takes for itself, and the values are the integers.
+// of a lane group all taking the weights of block 4 g + r, that is of the group's key.  Q8_0 up to 128 values:
+// what the four lanes of a block hold has one scale, so that goes into the weights, which each block then
+// takes for itself, and the values are the integers.
 template <int r, int NT, int VN, int VU, bool Q8, class Tile, int VB>
 __device__ __forceinline__ void attn_values(f32x4 (&acc)[NT][VB], const float (&p)[NT], const Tile& x) {
-  constexpr bool kOwn = Q8 && VB == 8;  // DT = 128: a block of four lanes holds 32 values
+  constexpr bool kOwn = Q8 && VB <= 8;  // the values of a block of four lanes, 16 or 32, lie in one 32-value block
   float w[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -288,10 +303,11 @@ __device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&
 // rows of a row tile, 1, 2 or 4.
 template <uint32_t T, int DT, bool FULL, int NS>
 __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_split(AttnCall c) {
-  using Tile = AttnTile<T, DT, FULL>;
+  using Tile = AttnTile<T, DT, FULL, NS>;
   constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN, R = 4 * NS;
   constexpr int kKeyBytes = AttnRaw<T, 8>::kBytes, kValBytes = AttnRaw<T, VU>::kBytes / VU;
-  constexpr bool kQ8 = T == T_Q8_0;
+  constexpr bool kQ8 = T == T_Q8_0, kGroup = Tile::kGroup;
+  constexpr int NP = Tile::NP, U = Tile::U, J = Tile::J, G4 = Tile::G4;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -328,10 +344,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   };
   look_up(0);
 
+  // The first of the eight values that this lane's piece s of a key stands for.
+  auto piece = [&](int s) {
+    return kGroup ? (s / J * NP + g / G4) * 32 + g % G4 * (32 / G4) + 8 * (s % J) : 32 * s + 8 * g;
+  };
   uint32_t koff[KS], voff[VN], soff = 0, svoff = 0;
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    koff[s] = 32 * s + 8 * g < d ? (uint32_t)(col * c.pitch + (4 * s + g) * kKeyBytes) : kPastEnd;
+    koff[s] = piece(s) < d ? (uint32_t)(col * c.pitch + piece(s) * kKeyBytes / 8) : kPastEnd;
 #pragma unroll
   for (int u = 0; u < VN; ++u) {
     const int i = col * VB + u * VU;
@@ -349,15 +369,32 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     const uint32_t bytes = (uint32_t)(x.live * c.pitch);
     const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + ta, bytes);
     const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + ta, bytes);
+    if constexpr (kGroup) {  // a round's pieces lie side by side
 #pragma unroll
-    for (int s = 0; s < KS; ++s) x.k[s].load(kr, koff[s]);
+      for (int u = 0; u < U; ++u) {
+        AttnWords<2 * J> w;
+        w.load(kr, koff[u * J]);
+#pragma unroll
+        for (int i = 0; i < 2 * J; ++i) x.k[u * J + i / 2].w[i % 2] = w.w[i];
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x.k[s].load(kr, koff[s]);
+    }
     if constexpr (kQ8) {
       const int64_t ts = of_lane(sat, n & 63);
       const __amdgpu_buffer_rsrc_t ks = attn_rsrc(c.k + ts, (uint32_t)(x.live * spitch));
       const __amdgpu_buffer_rsrc_t vs = attn_rsrc(c.v + ts, (uint32_t)(x.live * spitch));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if constexpr (FULL) {
+        if constexpr (kGroup) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int block = u * NP + col / 4;
+            x.kstep[r][u] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                ks, col / 4 < NP && 32 * block < d ? soff + r * spitch + 2 * block : kPastEnd, 0, 0);
+          }
+        } else if constexpr (FULL) {
           AttnWords<(KS + 1) / 2> w;
           w.load(ks, soff + r * spitch);
 #pragma unroll
@@ -388,15 +425,16 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   AttnQuery<T, KS> q;
   float mul = 1.0f;
   {
-    const int row = it.row0 + col;
+    const int row = it.row0 + (kGroup ? col & 3 : col);
+    const bool mine = row < it.rows && (kGroup ? col / 4 == g / G4 : col < R);
     const int64_t at = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
     float x[KS][8];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int i = 32 * s + 8 * g;
+      const int i = piece(s);
       attn_load8(x[s], c.q, at + (i < d ? i : 0), c.q_type);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[s][j] = col < R && row < it.rows && i < d ? x[s][j] * c.scale2 : 0.0f;
+      for (int j = 0; j < 8; ++j) x[s][j] = mine && i < d ? x[s][j] * c.scale2 : 0.0f;
     }
     if constexpr (T != T_F32) {
       float top = 0.0f;
@@ -404,8 +442,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+#pragma unroll
+      for (int o = kGroup ? 4 : 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
       // 2^e <= top < 2^(e + 1) to 2^14; a row with an infinite value as it is
       const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
       const int up = e < 128 ? 14 - e : 0;
@@ -436,8 +474,24 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 
   auto step = [&](const Tile& x) {
     f32x4 sc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (kGroup) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+      for (int u = 0; u < U; ++u) {
+        f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) y = q.mul(u * J + j, attn_bytes(x.k[u * J + j].w), y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] = __builtin_fmaf(attn_half((uint16_t)x.kstep[r][u]), y[r], sc[r]);
+      }
+      // The blocks of a row stand in four columns each (zeros where there are fewer groups): their sum, in all four.
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[r] += attn_rotate<4>(sc[r]);
+        sc[r] += attn_rotate<8>(sc[r]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < (kGroup ? 0 : KS); ++s) {
       if constexpr (T == T_F32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
