@@ -84,6 +84,7 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   c.items = (int)items;
   const int d16 = (c.head_dim + 15) / 16 * 16;
   c.small_sum = row_tiles * tiles <= 0x7fffffffll;
+  c.read_once = row_tiles <= c.n_seqs;
   *ws_bytes = *join ? sizeof(AttnPiece) * (1 + (size_t)attn_slots(c)) +
                           (size_t)attn_slots(c) * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float)
                     : 0;

@@ -39,6 +39,7 @@ struct AttnCall {
   int tile_rows;    // query rows of a row tile of the split kernel: 4, 8 or 16
   int items;        // bound on the work items of a key / value head; the grid is items * kv_heads
   int target, min_chunk;  // work items aimed at, fewest tiles of a chunk
+  bool read_once;         // no two row tiles read the same keys
   bool small_sum;         // the tiles of all row tiles stay below 2^31
   float* ws;        // partial results of split sequences
 };
@@ -146,10 +147,22 @@ __device__ inline int attn_scan(int x) {
   return x;
 }
 
+// A value that is the same in all lanes, as one that the compiler knows to be.
+__device__ inline long long attn_uniform(long long x) {
+  return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+
+// Of the whole call: items of split sequences, and tiles (a row tile's each).
+struct AttnSums {
+  int slots;
+  long long tiles;
+};
+
 // The work item of number `item`, the same in every thread of the workgroup (256 threads); `lds`:
-// 32 words that the caller does not use across the call; all_slots: the items of split sequences in all.
+// 32 words that the caller does not use across the call.
 // Sequences that fit a wave are looked through by every wave for itself, more by the workgroup together.
-template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, int& all_slots) {
+template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, AttnSums& sums) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   AttnItem none{};
   if (c.n_seqs <= 64) {
@@ -162,10 +175,11 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
     }
-    const int chunk = __builtin_amdgcn_readfirstlane(attn_chunk(c, total));
+    sums.tiles = attn_uniform(total);
+    const int chunk = attn_chunk(c, sums.tiles);
     const AttnCount n = attn_count(s, chunk);
     const int full = attn_scan(n.full), rest = attn_scan(n.rest), slots = attn_scan(n.slots);
-    all_slots = __builtin_amdgcn_readlane(slots, 63);
+    sums.slots = __builtin_amdgcn_readlane(slots, 63);
     const int fulls = __builtin_amdgcn_readlane(full, 63);
     const bool first = item < fulls;
     const int i = first ? item : item - fulls, upto = first ? full : rest;
@@ -190,10 +204,11 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
-  long long* sums = reinterpret_cast<long long*>(lds);
-  if (lane == 0) sums[wave] = total;
+  long long* parts = reinterpret_cast<long long*>(lds);
+  if (lane == 0) parts[wave] = total;
   __syncthreads();
-  const int chunk = __builtin_amdgcn_readfirstlane(attn_chunk(c, sums[0] + sums[1] + sums[2] + sums[3]));
+  sums.tiles = attn_uniform(parts[0] + parts[1] + parts[2] + parts[3]);
+  const int chunk = attn_chunk(c, sums.tiles);
   AttnCount n{0, 0, 0};
   for (int b = b0; b < b1; ++b) {
     const AttnCount x = attn_count(attn_seq<R>(c, b), chunk);
@@ -205,7 +220,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   __syncthreads();
   for (int w = 0; w < wave; ++w) full += lds[8 + w], rest += lds[12 + w], slots += lds[16 + w];
   const int fulls = __builtin_amdgcn_readfirstlane(lds[8] + lds[9] + lds[10] + lds[11]);
-  all_slots = __builtin_amdgcn_readfirstlane(lds[16] + lds[17] + lds[18] + lds[19]);
+  sums.slots = __builtin_amdgcn_readfirstlane(lds[16] + lds[17] + lds[18] + lds[19]);
   const bool first = item < fulls;
   const int i = first ? item : item - fulls, upto = first ? full : rest, mine = first ? n.full : n.rest;
   if (i >= upto - mine && i < upto) {

@@ -94,8 +94,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
-  int no_slots;
-  const AttnItem it = attn_item<kRows16>(c, item, reinterpret_cast<int*>(lds16), no_slots);
+  AttnSums sums;
+  const AttnItem it = attn_item<kRows16>(c, item, reinterpret_cast<int*>(lds16), sums);
   if (!it.any) return;
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds16;
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   }
   const int64_t base = (int64_t)it.seq * c.page_stride + (int64_t)kvh * c.head_stride;
   u32x4 kreg[L::kLoads], vreg[L::kLoads];
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t) __attribute__((always_inline)) {
     const int n = min(KT, it.len - t * KT);
     const int64_t at = base + (int64_t)t * KT * c.pitch;
     const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(n * c.pitch));
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, goff[i], 0, 0);
   };
-  auto stage = [&](int buf) {
+  auto stage = [&](int buf) __attribute__((always_inline)) {
     const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i)
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   // One tile from buffer `buf`, a constant in the unrolled loop: the LDS addresses are then lane offsets and immediates.
-  auto tile = [&](int t, int buf) {
+  auto tile = [&](int t, int buf) __attribute__((always_inline)) {
     const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
     f32x16 s[KB];
 #pragma unroll

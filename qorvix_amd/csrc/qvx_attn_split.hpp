@@ -49,18 +49,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const uint8_t* p, ui
 // N consecutive values of type T, N in 4, 8, 16: the raw words as loaded, and their fp32 values.
 template <uint32_t T, int N> struct AttnRaw;
 
+// AUX: the load's cache policy, 0 or kOnce.
+constexpr int kOnce = 2;  // non-temporal: will not be read again
 template <int W> struct AttnWords {
   uint32_t w[W];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  template <int AUX = 0> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     if constexpr (W == 1) {
-      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, AUX);
     } else if constexpr (W == 2) {
-      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, AUX);
       w[0] = x[0], w[1] = x[1];
     } else {
 #pragma unroll
       for (int i = 0; i < W; i += 4) {
-        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0);
+        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, AUX);
         w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
       }
     }
@@ -91,26 +93,35 @@ template <int N> struct AttnRaw<T_Q8_0, N> : AttnWords<N / 4> {
   }
 };
 
-// Eight consecutive elements of a query row, on any address of their type.
-__device__ __forceinline__ void attn_load8(float (&x)[8], const void* p, int64_t at, uint32_t type) {
+// Eight consecutive elements of a query row at each of N places, on any address of their type.  One branch
+// for all of them: a branch a place would wait for each before the next.
+template <int N>
+__device__ __forceinline__ void attn_load8(float (&x)[N][8], const void* p, const int64_t (&at)[N], uint32_t type) {
   if (type == T_F32) {
     struct __attribute__((packed, aligned(4))) Eight {
       float v[8];
-    };
-    const Eight e = *reinterpret_cast<const Eight*>(static_cast<const float*>(p) + at);
+    } e[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = e.v[i];
+    for (int s = 0; s < N; ++s) e[s] = *reinterpret_cast<const Eight*>(static_cast<const float*>(p) + at[s]);
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = e[s].v[i];
   } else {
     struct __attribute__((packed, aligned(2))) Eight {
       uint16_t v[8];
-    };
-    const Eight e = *reinterpret_cast<const Eight*>(static_cast<const uint16_t*>(p) + at);
+    } e[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = type == T_F16 ? (float)__builtin_bit_cast(_Float16, e.v[i])
-                           : __builtin_bit_cast(float, (uint32_t)e.v[i] << 16);
+    for (int s = 0; s < N; ++s) e[s] = *reinterpret_cast<const Eight*>(static_cast<const uint16_t*>(p) + at[s]);
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[s][i] = type == T_F16 ? (float)__builtin_bit_cast(_Float16, e[s].v[i])
+                                : __builtin_bit_cast(float, (uint32_t)e[s].v[i] << 16);
   }
 }
+
 // Four consecutive elements of an output row, on any address of their type.
 __device__ __forceinline__ void attn_store4(void* p, int64_t at, uint32_t type, const float (&x)[4]) {
   if (type == T_F32) {
@@ -312,20 +323,24 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
-  int all_slots = 0;
-  const AttnItem it = attn_item<R>(c, item, reinterpret_cast<int*>(lds), all_slots);
+  AttnSums sums;
+  const AttnItem it = attn_item<R>(c, item, reinterpret_cast<int*>(lds), sums);
   if (c.ws && kvh == 0 && threadIdx.x == 0) {
-    if (item == 0) *reinterpret_cast<int*>(c.ws) = min(all_slots, 2 * c.target);
+    if (item == 0) *reinterpret_cast<int*>(c.ws) = min(sums.slots, 2 * c.target);
     if (it.any && it.chunks > 1) attn_pieces(c.ws)[it.slot] = AttnPiece{it.q0, it.row0, it.rows, it.chunk, it.chunks, {}};
   }
   if (!it.any) return;
+  // A call that reads more than half the 256 MB memory-side cache finds nothing of it there again, and its
+  // loads are marked so: fp16 of 131071 tokens 102 -> 90 us, 128 x 4096 tokens 377 -> 345.  Smaller calls
+  // keep the ordinary policy: 47 MB of fp32 in turn with two others like it 17.5 us against 19.3.
+  const bool once = c.read_once && sums.tiles * (long long)(2 * kAttnTile) * c.pitch * c.kv_heads > (128ll << 20);
 
   // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
   const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   int64_t at = 0, sat = 0;  // of the tile's keys (and values), and of their scales, from the cache's start
   int live = 0;
-  auto look_up = [&](int n) {
+  auto look_up = [&](int n) __attribute__((always_inline)) {
     const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
     live = 0;
     if (t < it.tile1) {
@@ -338,14 +353,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     }
   };
   // A lane's 64-bit value in all of them.
-  auto of_lane = [](int64_t x, int i) {
+  auto of_lane = [](int64_t x, int i) __attribute__((always_inline)) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 |
                      (uint32_t)__builtin_amdgcn_readlane((int)x, i));
   };
   look_up(0);
 
   // The first of the eight values that this lane's piece s of a key stands for.
-  auto piece = [&](int s) {
+  auto piece = [&](int s) __attribute__((always_inline)) {
     return kGroup ? (s / J * NP + g / G4) * 32 + g % G4 * (32 / G4) + 8 * (s % J) : 32 * s + 8 * g;
   };
   uint32_t koff[KS], voff[VN], soff = 0, svoff = 0;
@@ -362,7 +377,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     svoff = col * VB < d ? (uint32_t)(4 * g * spitch + col * VB / 32 * 2) : kPastEnd;
   }
   // Tile n of the wave's, none (and no memory) past the last.
-  auto load = [&](Tile& x, int n) {
+  auto load = [&]<int AUX>(Tile& x, int n) __attribute__((always_inline)) {
     if (n && (n & 63) == 0 && n < tiles) look_up(n);
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
     const int64_t ta = of_lane(at, n & 63);
@@ -373,13 +388,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         AttnWords<2 * J> w;
-        w.load(kr, koff[u * J]);
+        w.template load<AUX>(kr, koff[u * J]);
 #pragma unroll
         for (int i = 0; i < 2 * J; ++i) x.k[u * J + i / 2].w[i % 2] = w.w[i];
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[s].load(kr, koff[s]);
+      for (int s = 0; s < KS; ++s) x.k[s].template load<AUX>(kr, koff[s]);
     }
     if constexpr (kQ8) {
       const int64_t ts = of_lane(sat, n & 63);
@@ -414,28 +429,40 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int u = 0; u < VN; ++u) x.v[r][u].load(vr, voff[u] + r * c.pitch);
+      for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, voff[u] + r * c.pitch);
   };
-  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT == 128) ? 2 : 1;
+  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT >= 128) ? 2 : 1;
   Tile held[kHeld];
-#pragma unroll
-  for (int i = 0; i < std::max(1, kHeld - 1); ++i) load(held[i], i);
-
-  // This lane's query values: row col, pieces 32 s + 8 g; rows and values that are not there are zeros.
   AttnQuery<T, KS> q;
   float mul = 1.0f;
-  {
+  // Four sets of rows: a lane's weights are row col's for keys 4 g + r in register r.  Fewer: row
+  // 4 t + lane % 4's for key lane / 4 in register t.
+  constexpr bool kSets = NS < 4;
+  constexpr int NT = kSets ? NS : 1;
+  float m[NT], l[NT], muls[NT];
+  f32x4 acc[NT][VB];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VB; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // This lane's query values: row col's pieces; rows and values that are not there are zeros.
+  auto set_query = [&]() __attribute__((always_inline)) {
     const int row = it.row0 + (kGroup ? col & 3 : col);
     const bool mine = row < it.rows && (kGroup ? col / 4 == g / G4 : col < R);
-    const int64_t at = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
+    const int64_t first = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
+    int64_t from[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) from[s] = first + (piece(s) < d ? piece(s) : 0);
     float x[KS][8];
+    attn_load8(x, c.q, from, c.q_type);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int i = piece(s);
-      attn_load8(x[s], c.q, at + (i < d ? i : 0), c.q_type);
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[s][j] = mine && i < d ? x[s][j] * c.scale2 : 0.0f;
-    }
+      for (int j = 0; j < 8; ++j) x[s][j] = mine && piece(s) < d ? x[s][j] * c.scale2 : 0.0f;
     if constexpr (T != T_F32) {
       float top = 0.0f;
 #pragma unroll
@@ -455,24 +482,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) q.set(s, x[s]);
-  }
-
-  // Four sets of rows: a lane's weights are row col's for keys 4 g + r in register r.  Fewer: row
-  // 4 t + lane % 4's for key lane / 4 in register t.
-  constexpr bool kSets = NS < 4;
-  constexpr int NT = kSets ? NS : 1;
-  float m[NT], l[NT], muls[NT];
-  f32x4 acc[NT][VB];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.0f;
-    muls[t] = kSets ? __shfl(mul, 4 * t + (lane & 3)) : mul;
-#pragma unroll
-    for (int j = 0; j < VB; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+    for (int t = 0; t < NT; ++t) muls[t] = kSets ? __shfl(mul, 4 * t + (lane & 3)) : mul;
+  };
 
-  auto step = [&](const Tile& x) {
+  auto step = [&](const Tile& x) __attribute__((always_inline)) {
     f32x4 sc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (kGroup) {
 #pragma unroll
@@ -585,22 +599,28 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       }
     }
   };
-  if constexpr (kHeld == 1) {
-    for (int n = 0; n < tiles; ++n) {
-      if (n) load(held[0], n);
-      step(held[0]);
-    }
-  } else {
+  auto run = [&]<int AUX>() __attribute__((always_inline)) {
+    load.template operator()<AUX>(held[0], 0);
+    set_query();
     for (int n = 0; n < tiles; n += kHeld) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         if (n + i >= tiles) break;
-        load(held[(i + kHeld - 1) % kHeld], n + i + kHeld - 1);
-        __builtin_amdgcn_sched_barrier(0);  // the loads go out before the tile in work is waited for
+        if constexpr (kHeld == 2) {
+          load.template operator()<AUX>(held[i ^ 1], n + i + 1);
+          __builtin_amdgcn_sched_barrier(0);  // the loads go out before the tile in work is waited for
+        } else if (n) {
+          load.template operator()<AUX>(held[0], n);
+        }
         step(held[i]);
       }
     }
-  }
+  };
+  // The two loops apart: loads of one kind or the other inside one loop would blur what is on its way.
+  if (once)
+    run.template operator()<kOnce>();
+  else
+    run.template operator()<0>();
 
   // Join the waves: m, l and the values of the rows, through LDS.
   const int d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0);
