@@ -20,13 +20,17 @@ attn_norm), o on the attention output, gate|up on rmsnorm(x, ffn_norm) with the 
 down on that SwiGLU output, and the LM head on rmsnorm(x, output_norm) -- 5 launches a layer.  RoPE,
 attention and the residual adds stay outside, so the hidden state x and the attention output are
 stand-ins; the FFN's SwiGLU activation is the engine's own.
+
+``PagedDecodeStep`` is the whole layer: the fused projections with rotary positions, a paged key / value
+cache and its attention between them (``qvx_kv_map``, ``qvx_rope_kv``, ``qvx_attn_paged``), for M
+sequences that each get one token a step.
 """
 from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass, field
 
-from . import (F32, GEMM_F16, OK, Q4_K, Q6_K, QvxError, empty_weight, fill_normal_t, fill_synthetic_t, lib,
+from . import (F16, F32, GEMM_F16, OK, Q4_K, Q6_K, QvxError, empty_weight, fill_normal_t, fill_synthetic_t, lib,
                weight_bytes)
 
 
@@ -499,6 +503,105 @@ class OpsDecodeStep:
             self.run(torch.cuda.current_stream().cuda_stream)
 
     def replay(self, stream: int = 0) -> None:
+        self.graph.replay()
+
+
+class PagedDecodeStep:
+    """One whole decode step of ``m`` sequences over a paged key / value cache (text_model.cpp:139-177), on a
+    ``Model.fused_ops()`` model: ``qvx_kv_map`` once, then per layer q|k and v on rmsnorm(x), ``qvx_rope_kv``
+    (rotary positions, append), ``qvx_attn_paged``, x += Wo . attn, the SwiGLU FFN on rmsnorm(x), x += its
+    down projection; logits = Wlm . rmsnorm(x).  The caller writes the new tokens' embeddings into ``x``
+    [m, d] and runs the step; ``lens`` [m] are the tokens that each sequence holds (0 at the start),
+    ``table`` and ``taken`` its page table and the pages of ``free`` handed out, all on the device and all
+    carried on by the step itself, so a captured step replays as it is.  ``taken[1]`` is qvx_kv_map's status: not 0 once
+    pages or columns run out, from when on the steps store and attend nothing new.
+
+    heads x head_dim is wo's row length; the cache is ``n_pages`` pages of ``page_size`` tokens a layer, of
+    a type of ``KvCache``; the rotation turns halves with the given base (and per-pair factors)."""
+
+    def __init__(self, model: Model, m: int, heads: int, kv_heads: int, n_pages: int, max_pages: int,
+                 page_size: int = 16, cache_type: int = F16, rope_base: float = 500000.0, rope_factors=None,
+                 device="cuda"):
+        import torch
+        from . import KvCache, Rope, attn_paged_ws, kv_page_bytes
+        l0 = model.layers[0]
+        d, width = l0["wo"].rows, l0["wo"].cols
+        if width % heads or heads % kv_heads or l0["wv"].rows != width // heads * kv_heads:
+            raise ValueError("PagedDecodeStep: the projections do not fit the heads")
+        for l, layer in enumerate(model.layers):
+            if any(k not in layer for k in ("wqk", "wv", "wo", "ffn_gateup", "ffn_down")):
+                raise ValueError("PagedDecodeStep needs a Model.fused_ops() model with q and k stacked")
+            if any(model.norms[l].get(k) is None for k in ("attn_norm", "ffn_norm")):
+                raise ValueError(f"PagedDecodeStep needs the norms of layer {l}; the model lacks some")
+        self.model, self.m, self.heads, self.kv_heads, self.page_size = model, m, heads, kv_heads, page_size
+        self.head_dim = hd = width // heads
+        size = kv_page_bytes(cache_type, kv_heads, page_size, hd)
+        if size == 0:
+            raise ValueError("PagedDecodeStep: the cache does not take this type or head size")
+        f32, i32 = dict(dtype=torch.float32, device=device), dict(dtype=torch.int32, device=device)
+        self.x = torch.zeros((m, d), **f32)
+        self.qk, self.v = torch.empty((m, l0["wqk"].rows), **f32), torch.empty((m, l0["wv"].rows), **f32)
+        self.attn, self.o = torch.empty((m, width), **f32), torch.empty((m, d), **f32)
+        self.h = torch.empty((m, l0["ffn_gateup"].rows // 2), **f32)
+        self.logits = torch.empty((m, model.lm_head.rows), **f32) if model.lm_head is not None else None
+        # K and V pages of a layer side by side: one allocation a layer
+        self.pages = [torch.zeros((n_pages, 2 * size), dtype=torch.uint8, device=device) for _ in model.layers]
+        self.caches = [KvCache.of(p[:, :size], p[:, size:], cache_type, page_size, kv_heads, hd) for p in self.pages]
+        self.lens, self.new = torch.zeros(m, **i32), torch.ones(m, **i32)
+        self.table = torch.full((m, max_pages), -1, **i32)
+        self.free = torch.arange(n_pages, **i32)
+        self.taken = torch.zeros(2, **i32)
+        self.offsets, self.slots, self.pos = (torch.zeros(n, **i32) for n in (m + 1, m, m))
+        freq = rope_base ** (-torch.arange(hd // 2, dtype=torch.float64, device=device) * 2 / hd)
+        if rope_factors is not None:
+            freq = freq / rope_factors.to(freq)
+        self.rope = Rope.of(freq)
+        self.ws = torch.empty(attn_paged_ws(self.caches[0], heads, m, max_pages), dtype=torch.uint8, device=device)
+        self.graph = None
+
+    def run(self, stream: int) -> None:
+        """The step on ``stream``, which is torch's current one (the residual adds are torch's)."""
+        from . import _check, attn_paged, kv_map, rope_kv
+        so, m, hd, model = lib(), self.m, self.head_dim, self.model
+        d, q_row, width = self.x.shape[1], self.heads * self.head_dim, self.qk.shape[1]
+        x, qk, v, attn, o = (t.data_ptr() for t in (self.x, self.qk, self.v, self.attn, self.o))
+        _check(kv_map(self.lens.data_ptr(), self.new.data_ptr(), m, self.table.data_ptr(), self.table.shape[1],
+                      self.page_size, self.free.data_ptr(), self.free.shape[0], self.taken.data_ptr(),
+                      self.taken.data_ptr(), self.lens.data_ptr(), self.offsets.data_ptr(), self.slots.data_ptr(),
+                      self.pos.data_ptr(), 0, m, stream), "qvx_kv_map")
+
+        def normed(out, w, norm):
+            _check(so.qvx_qmatmul_n_rmsnorm(out, w.data.data_ptr(), w.type, x, norm.data_ptr(), model.eps, m, w.rows,
+                                            w.cols, stream), "qvx_qmatmul_n_rmsnorm")
+
+        for l, layer in enumerate(model.layers):
+            normed(qk, layer["wqk"], model.norms[l]["attn_norm"])
+            normed(v, layer["wv"], model.norms[l]["attn_norm"])
+            _check(rope_kv(qk, width, qk, width, self.heads, qk + 4 * q_row, width, v, self.v.shape[1], m, hd, self.rope,
+                           self.pos.data_ptr(), m, self.caches[l], self.slots.data_ptr(), stream), "qvx_rope_kv")
+            _check(attn_paged(attn, q_row, qk, width, self.heads, self.caches[l], self.table.data_ptr(),
+                              self.table.shape[1], self.lens.data_ptr(), m, hd ** -0.5, self.ws.data_ptr(),
+                              self.ws.numel(), stream), "qvx_attn_paged")
+            wmatmul_n(self.o, layer["wo"], self.attn, m, stream)
+            self.x.add_(self.o)
+            gu = layer["ffn_gateup"]
+            _check(so.qvx_qmatmul_swiglu(self.h.data_ptr(), gu.data.data_ptr(), gu.type, x,
+                                         model.norms[l]["ffn_norm"].data_ptr(), model.eps, m, gu.rows // 2, gu.cols,
+                                         stream), "qvx_qmatmul_swiglu")
+            wmatmul_n(self.o, layer["ffn_down"], self.h, m, stream)
+            self.x.add_(self.o)
+        if model.lm_head is not None:
+            normed(self.logits.data_ptr(), model.lm_head, model.output_norm)
+
+    def capture(self) -> None:
+        """Record the step into one graph.  Nothing runs and no state moves on; run the step eagerly at
+        least once before."""
+        import torch
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.run(torch.cuda.current_stream().cuda_stream)
+
+    def replay(self) -> None:
         self.graph.replay()
 
 
