@@ -8,7 +8,7 @@
 
 namespace qvx {
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
-int attn16_rows();
+void launch_attn_join(const AttnCall& c, hipStream_t s);
 bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s);
 bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s);
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s);
@@ -71,24 +71,41 @@ constexpr int kAttnWgs = 512, kMinChunk = 8;
 // four, a quarter the time of sixteen; up to eight on two of those.
 int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
-// False: the partition passes 31 bits.
-bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
+// The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
+// False: it passes 31 bits.
+bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t tiles = (int64_t)c.max_len / c.page_size * c.page_tiles +
                         (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
-  c.min_chunk = kMinChunk;
-  static const int wgs = getenv("QVX_WGS") ? atoi(getenv("QVX_WGS")) : kAttnWgs;  // TUNE
-  c.target = std::max(1, wgs / c.kv_heads);
-  *join = tiles > c.min_chunk;
-  const int64_t items = std::min(row_tiles + c.target, row_tiles * std::max<int64_t>((tiles + kMinChunk - 1) / kMinChunk, 1));
+  *join = c.min_chunk && tiles > c.min_chunk;
+  const int64_t most = *join ? (tiles + c.min_chunk - 1) / c.min_chunk : 1;  // chunks of a row tile
+  const int64_t items = std::min(row_tiles + c.target, row_tiles * most);
   if (items * c.kv_heads > 0x7fffffffll || tiles > 0x7fffffffll) return false;
+  if (!*join) c.min_chunk = 0x7ffffff0;
   c.items = (int)items;
   const int d16 = (c.head_dim + 15) / 16 * 16;
   c.small_sum = row_tiles * tiles <= 0x7fffffffll;
   c.read_once = row_tiles <= c.n_seqs;
-  *ws_bytes = *join ? sizeof(AttnPiece) * (1 + (size_t)attn_slots(c)) +
-                          (size_t)attn_slots(c) * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float)
+  c.slots = (int)std::min<int64_t>(2 * (int64_t)c.target, row_tiles * most);
+  *ws_bytes = *join ? sizeof(AttnPiece) * (1 + (size_t)c.slots) +
+                          (size_t)c.slots * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float)
                     : 0;
   return true;
+}
+
+bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
+  c.min_chunk = kMinChunk;
+  c.target = std::max(1, kAttnWgs / c.kv_heads);
+  return plan_items(c, row_tiles, join, ws_bytes);
+}
+
+// The 16-bit kernel's: row tiles of 128 rows.  They are split only where they are fewer than two workgroups a CU,
+// into chunks of 256 keys at least: 64 queries on 1500 states, 20 heads of 64, 26 -> XX us.
+bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
+  c.tile_rows = kAttnRows16;
+  const bool split = row_tiles * c.kv_heads < kAttnWgs;
+  c.min_chunk = split ? 16 : 0;
+  c.target = std::max(1, kAttnWgs / c.kv_heads);
+  return plan_items(c, row_tiles, join, ws_bytes);
 }
 
 int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width, AttnCall& c, bool* join,
@@ -119,8 +136,10 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
-int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, AttnCall& c,
-                bool* join, size_t* ws_bytes) {
+// wide: the call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a 16-bit type, the scale is not
+// negative (the kernel takes the largest product for the largest logit), and sequences have 32 rows or more in the mean.
+int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, float scale,
+                AttnCall& c, bool* wide, bool* join, size_t* ws_bytes) {
   if (!st) return QVX_E_NULL;
   if (n_seqs <= 0) return QVX_E_NVEC;
   if ((q_type != T_F32 && q_type != T_F16 && q_type != T_BF16) ||
@@ -156,21 +175,11 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   c.head_dim = st->head_dim;
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
   if ((int64_t)n_q * c.group > 0x7ffffff0ll) return QVX_E_RANGE;
-  c.tile_rows = tile_rows(ragged ? rows / n_seqs : rows);  // ragged: of a sequence in the mean
+  *wide = q_type == st->type && q_type != T_F32 && scale >= 0.0f && (int64_t)n_q * c.group >= 32 * (int64_t)n_seqs;
+  c.tile_rows = *wide ? kAttnRows16 : tile_rows(ragged ? rows / n_seqs : rows);  // ragged: of a sequence in the mean
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
-  return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
-}
-
-// Whether a checked cross call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a
-// 16-bit type and there are row tiles enough.
-bool cross16(const AttnCall& c, uint32_t type, bool ragged, float scale, int* items) {
-  if (c.q_type != type || type == T_F32 || !(scale >= 0.0f)) return false;
-  const int64_t r = attn16_rows(), rows = (int64_t)(ragged ? c.n_q : c.q_each) * c.group;
-  const int64_t tiles = ragged ? rows / r + c.n_seqs : c.n_seqs * ((rows + r - 1) / r);
-  if ((int64_t)c.n_q * c.group < 32 * (int64_t)c.n_seqs || tiles * c.kv_heads > 0x7fffffffll) return false;
-  *items = (int)tiles;
-  return true;
+  return (*wide ? plan16 : plan_split)(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -305,13 +314,13 @@ int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q
 }
 
 size_t qvx_attn_cross_ws(const qvx_kv_states* states, uint32_t q_type, int q_heads, int n_q, int n_seqs) {
-  // Ragged and equal queries differ in their bounds: the larger need serves both.
+  // Ragged and equal queries differ in their bounds, scales of either sign in their kernel: the largest need serves all.
   size_t most = 0;
-  for (int ragged = 0; ragged < 2; ++ragged) {
+  for (int i = 0; i < 4; ++i) {
     AttnCall c{};
-    bool join = false;
+    bool wide = false, join = false;
     size_t bytes = 0;
-    if (check_cross(states, q_type, q_heads, ragged != 0, n_q, n_seqs, c, &join, &bytes) == QVX_OK)
+    if (check_cross(states, q_type, q_heads, i & 1, n_q, n_seqs, i & 2 ? 1.0f : -1.0f, c, &wide, &join, &bytes) == QVX_OK)
       most = std::max(most, bytes);
   }
   return most;
@@ -321,9 +330,10 @@ int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_s
                    const int32_t* d_offsets, int n_q, const qvx_kv_states* states, const int32_t* d_lens, int n_seqs,
                    float scale, void* d_ws, size_t ws_bytes, void* stream) {
   AttnCall c{};
-  bool join = false;
+  bool wide = false, join = false;
   size_t need = 0;
-  if (int rc = check_cross(states, q_type, q_heads, d_offsets != nullptr, n_q, n_seqs, c, &join, &need); rc != QVX_OK)
+  if (int rc = check_cross(states, q_type, q_heads, d_offsets != nullptr, n_q, n_seqs, scale, c, &wide, &join, &need);
+      rc != QVX_OK)
     return rc;
   if (q_stride < 0 || out_stride < (int64_t)q_heads * states->head_dim) return QVX_E_SHAPE;
   if (n_q == 0) return QVX_OK;
@@ -339,14 +349,13 @@ int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_s
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
   c.ws = join ? static_cast<float*>(d_ws) : nullptr;
-  if (int items; cross16(c, states->type, d_offsets != nullptr, scale, &items)) {
-    c.items = items;
-    c.min_chunk = 0x7ffffff0;  // a row tile takes all keys
-    c.q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
-    c.out_wide = aligned(d_out, 8) && out_stride % 4 == 0;
-    return attn_status(launch_attn16(c, states->type, static_cast<hipStream_t>(stream)));
-  }
-  return attn_status(launch_attn_split(c, states->type, join, static_cast<hipStream_t>(stream)));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!wide) return attn_status(launch_attn_split(c, states->type, join, s));
+  c.q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
+  c.out_wide = aligned(d_out, 8) && out_stride % 4 == 0;
+  const bool ok = launch_attn16(c, states->type, s);
+  if (ok && join) launch_attn_join(c, s);
+  return attn_status(ok);
 }
 
 }  // extern "C"

@@ -8,11 +8,13 @@ bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_f32(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 
+void launch_attn_join(const AttnCall& c, hipStream_t s);
+
 namespace {
 
 // The chunks of a split sequence's row tile joined: out = sum_j 2^(m_j - m) v_j / sum_j 2^(m_j - m) l_j,
-// m the largest m_j.  A workgroup a piece and key / value head.  Up to kFewChunks chunks the workgroup of the
-// first takes all rows, else the row tile's workgroups share them, one row at a time.  Four values a
+// m the largest m_j.  A workgroup a piece and key / value head; the workgroups of a row tile share its rows, as
+// many at a time as fill the threads up to kFewChunks chunks, else one at a time.  Four values a
 // thread; the threads that the rows leave over take other chunks, each a running maximum over its own, eight
 // chunks' loads at a time; then the groups meet in LDS.  Latency bounds it: three dependent loads
 // (piece, partial results, store).  The order of the sums is the same in every run.
@@ -25,14 +27,13 @@ template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) 
   const AttnPiece pc = attn_pieces(c.ws)[slot];  // of the workspace: may be read before it is known to be one
   if (slot >= *reinterpret_cast<const int*>(c.ws)) return;
   const bool few = pc.chunks <= kFewChunks;
-  if (few && pc.chunk != 0) return;
   const int d = c.head_dim, d16 = (d + 15) & ~15, quads = d / 4, nrow = min(R, pc.rows - pc.row0);
   const size_t size = attn_part(R, d16), step = (size_t)c.kv_heads * size;
-  const float* first = attn_parts(c.ws, c.target) + ((size_t)(slot - pc.chunk) * c.kv_heads + kvh) * size;
+  const float* first = attn_parts(c.ws, c.slots) + ((size_t)(slot - pc.chunk) * c.kv_heads + kvh) * size;
   const int wide = few ? min(R, 256 / quads) : 1;  // rows at a time
   const int groups = 256 / (quads * wide), mine = tid / (quads * wide), rest = tid - mine * quads * wide;
   const int row = rest / quads, quad = rest - row * quads;
-  for (int r0 = few ? 0 : pc.chunk; r0 < nrow; r0 += few ? wide : pc.chunks) {
+  for (int r0 = pc.chunk * wide; r0 < nrow; r0 += pc.chunks * wide) {
     const int r = r0 + row;
     float m = -INFINITY, l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -103,16 +104,18 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
     case T_Q8_0: ok = launch_attn_split_q8(c, grid, s); break;
     default: break;
   }
-  if (ok && join) {
-    const dim3 grid((unsigned)std::min(c.items, attn_slots(c)), (unsigned)c.kv_heads);
-    if (c.tile_rows == 4)
-      k_attn_join<4><<<grid, 256, 0, s>>>(c);
-    else if (c.tile_rows == 8)
-      k_attn_join<8><<<grid, 256, 0, s>>>(c);
-    else
-      k_attn_join<16><<<grid, 256, 0, s>>>(c);
-  }
+  if (ok && join) launch_attn_join(c, s);
   return ok;
+}
+
+void launch_attn_join(const AttnCall& c, hipStream_t s) {
+  const dim3 grid((unsigned)c.slots, (unsigned)c.kv_heads);
+  switch (c.tile_rows) {
+    case 4: k_attn_join<4><<<grid, 256, 0, s>>>(c); break;
+    case 8: k_attn_join<8><<<grid, 256, 0, s>>>(c); break;
+    case 16: k_attn_join<16><<<grid, 256, 0, s>>>(c); break;
+    default: k_attn_join<kAttnRows16><<<grid, 256, 0, s>>>(c); break;
+  }
 }
 
 }  // namespace qvx

@@ -13,6 +13,7 @@
 namespace qvx {
 
 constexpr int kAttnTile = 16;   // keys of a tile
+constexpr int kAttnRows16 = 128;  // query rows of a workgroup of the 16-bit kernel
 constexpr int kAttnWaves = 4;   // waves of a workgroup of the split kernel
 
 struct AttnCall {
@@ -36,9 +37,10 @@ struct AttnCall {
   int max_len;
   int n_seqs, kv_heads, group, head_dim;
   float scale2;     // scale * log2(e): the kernels work with powers of two
-  int tile_rows;    // query rows of a row tile of the split kernel: 4, 8 or 16
+  int tile_rows;    // query rows of a row tile: 4, 8 or 16 in the split kernel, 128 in the 16-bit one
   int items;        // bound on the work items of a key / value head; the grid is items * kv_heads
   int target, min_chunk;  // work items aimed at, fewest tiles of a chunk
+  int slots;              // bound on the items of split sequences: the workspace's parts
   bool read_once;         // no two row tiles read the same keys
   bool small_sum;         // the tiles of all row tiles stay below 2^31
   float* ws;        // partial results of split sequences
@@ -57,10 +59,9 @@ __host__ __device__ inline size_t attn_part(int rows, int d16) { return (size_t)
 // most target items more than they have row tiles, and those of several chunks, each less than twice
 // its share, at most 2 target in all: the workspace holds no more, however many sequences there are.
 // It begins with the number of those items and a piece for each.
-inline int attn_slots(const AttnCall& c) { return 2 * c.target; }
 __host__ __device__ inline AttnPiece* attn_pieces(float* ws) { return reinterpret_cast<AttnPiece*>(ws) + 1; }
-__host__ __device__ inline float* attn_parts(float* ws, int target) {
-  return reinterpret_cast<float*>(attn_pieces(ws) + 2 * target);
+__host__ __device__ inline float* attn_parts(float* ws, int slots) {
+  return reinterpret_cast<float*>(attn_pieces(ws) + slots);
 }
 
 __device__ inline int attn_tiles(const AttnCall& c, int len) {
@@ -132,7 +133,7 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   it.slot = slot0 + rt * it.chunks + it.chunk;
   // Offsets that are no running sums can wrap the counts: nothing past the rows or the workspace then.
   it.any = i >= 0 && it.row0 >= 0 && it.row0 < it.rows && it.tile0 >= 0 &&
-           (it.chunks == 1 || (unsigned)it.slot < 2u * (unsigned)c.target);
+           (it.chunks == 1 || (unsigned)it.slot < (unsigned)c.slots);
   return it;
 }
 
@@ -245,6 +246,14 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   AttnSeq s = attn_seq<R>(c, b);
   s.nq *= c.group;
   return attn_take<R>(c, s, b, chunk, at, first, slot0);
+}
+
+// Leaves the join what it needs: the number of pieces, and this item's if it is one (of one head, as all
+// heads' are alike).
+__device__ inline void attn_note(const AttnCall& c, const AttnItem& it, int item, int kvh, const AttnSums& sums) {
+  if (!c.ws || kvh != 0 || threadIdx.x != 0) return;
+  if (item == 0) *reinterpret_cast<int*>(c.ws) = min(sums.slots, c.slots);
+  if (it.any && it.chunks > 1) attn_pieces(c.ws)[it.slot] = AttnPiece{it.q0, it.row0, it.rows, it.chunk, it.chunks, {}};
 }
 
 }  // namespace qvx

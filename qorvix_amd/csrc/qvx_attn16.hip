@@ -32,7 +32,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kRows16 = 128;  // query rows of a workgroup
+constexpr int kRows16 = kAttnRows16;
 constexpr float kSlack16 = 8.0f;
 
 typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
@@ -96,6 +96,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
   const AttnItem it = attn_item<kRows16>(c, item, reinterpret_cast<int*>(lds16), sums);
+  attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds16;
@@ -129,10 +130,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
     kst[i] = L::k_at(r, u);
     vst[i] = L::v_at(r, u);
   }
-  const int64_t base = (int64_t)it.seq * c.page_stride + (int64_t)kvh * c.head_stride;
   u32x4 kreg[L::kLoads], vreg[L::kLoads];
+  const int key0 = it.tile0 * kAttnTile, keys = min(it.tile1 * kAttnTile, it.len) - key0;  // of this chunk
+  const int64_t base = (int64_t)it.seq * c.page_stride + (int64_t)kvh * c.head_stride + (int64_t)key0 * c.pitch;
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int n = min(KT, it.len - t * KT);
+    const int n = min(KT, keys - t * KT);
     const int64_t at = base + (int64_t)t * KT * c.pitch;
     const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + at, (uint32_t)(n * c.pitch));
     const __amdgpu_buffer_rsrc_t vr = attn_rsrc(c.v + at, (uint32_t)(n * c.pitch));
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
 
-  const int tiles = (it.len + KT - 1) / KT;
+  const int tiles = (keys + KT - 1) / KT;
   if (tiles > 0) {
     fetch(0);
     stage(0);
@@ -172,37 +174,38 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   // One tile from buffer `buf`, a constant in the unrolled loop: the LDS addresses are then lane offsets and immediates.
-  auto tile = [&](int t, int buf) __attribute__((always_inline)) {
+  // With its first BN blocks of 32 keys alone where the rest holds none.
+  auto tile = [&]<int BN>(int t, int buf) __attribute__((always_inline)) {
     const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
-    f32x16 s[KB];
+    f32x16 s[BN];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < BN; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
+      for (int b = 0; b < BN; ++b) {
         const u32x4 a = *(__attribute__((address_space(3))) u32x4*)(kb + L::k_at(32 * b + col, 2 * i + h));
         s[b] = mma32<T>(a, q[i], s[b]);
       }
     // The results of the matrix instructions are waited for here: on the path that skips the mask the
     // compiler leaves too few slots between them and the first read.
-    if constexpr (KB == 2)
+    if constexpr (BN == 2)
       asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[1]));
     else
       asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]));
-    const int left = it.len - t * KT;
-    if (left < KT) {
+    const int left = keys - t * KT;
+    if (left < 32 * BN) {
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
+      for (int b = 0; b < BN; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * b + 8 * (r / 4) + 4 * h + r % 4 >= left) s[b][r] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < BN; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top *= c.scale2;  // scale2 >= 0: the order stays
@@ -217,9 +220,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
         for (int r = 0; r < 16; ++r) acc[b][r] *= f;
     }
     const float ref = m == -INFINITY ? 0.0f : m;
-    u32x4 p[KB][2];
+    u32x4 p[BN][2];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < BN; ++b)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const float x = attn_pow2(__builtin_fmaf(s[b][r], c.scale2, -ref));
@@ -229,7 +232,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
         p[b][r / 8][r / 2 % 4] = xy;
       }
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < BN; ++b)
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -250,7 +253,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
       const int t = t0 + buf;
       if (t >= tiles) break;
       if (t + 1 < tiles) fetch(t + 1);
-      if (any_row) tile(t, buf);
+      if (any_row) {
+        if (KB == 1 || keys - t * KT > 32)
+          tile.template operator()<KB>(t, buf);
+        else
+          tile.template operator()<1>(t, buf);
+      }
       if (t + 1 < tiles) stage(buf ^ 1);  // the buffer that everyone left a barrier ago
       __syncthreads();
     }
@@ -259,6 +267,23 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
 
   l += __shfl_xor(l, 32);
   if (!live) return;
+  if (it.chunks > 1) {  // a part of the keys: for k_attn_join
+    const int d16 = (d + 15) & ~15, r16 = row - it.row0;
+    float* part = attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(kRows16, d16);
+#pragma unroll
+    for (int e = 0; e < DB; ++e)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int i = 32 * e + 8 * (r / 4) + 4 * h;
+        if (i < d)
+          *reinterpret_cast<f32x4*>(part + r16 * d16 + i) = f32x4{acc[e][r], acc[e][r + 1], acc[e][r + 2], acc[e][r + 3]};
+      }
+    if (h == 0) {
+      part[kRows16 * d16 + r16] = m;
+      part[kRows16 * (d16 + 1) + r16] = l;
+    }
+    return;
+  }
   const float inv = it.len ? 1.0f / l : 0.0f;  // no keys: zeros (acc is zero)
   uint16_t* o = static_cast<uint16_t*>(c.out) + attn_row(c, it.q0, row, kvh, c.out_stride);
 #pragma unroll
@@ -296,8 +321,6 @@ template <uint32_t T> bool attn16_dp(const AttnCall& c, dim3 grid, hipStream_t s
 }
 
 }  // namespace
-
-int attn16_rows() { return kRows16; }
 
 bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s) {
   const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);

@@ -325,10 +325,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
   const AttnItem it = attn_item<R>(c, item, reinterpret_cast<int*>(lds), sums);
-  if (c.ws && kvh == 0 && threadIdx.x == 0) {
-    if (item == 0) *reinterpret_cast<int*>(c.ws) = min(sums.slots, 2 * c.target);
-    if (it.any && it.chunks > 1) attn_pieces(c.ws)[it.slot] = AttnPiece{it.q0, it.row0, it.rows, it.chunk, it.chunks, {}};
-  }
+  attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
   // A call that reads more than half the 256 MB memory-side cache finds nothing of it there again, and its
   // loads are marked so: fp16 of 131071 tokens 102 -> 90 us, 128 x 4096 tokens 377 -> 345.  Smaller calls
@@ -669,7 +666,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   }
   __syncthreads();
   const float* v0 = lds + 2 * kAttnWaves * R;
-  float* part = it.chunks > 1 ? attn_parts(c.ws, c.target) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
+  float* part = it.chunks > 1 ? attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
                               : nullptr;
   const int quads = d / 4;
   for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
