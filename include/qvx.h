@@ -304,10 +304,11 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
  * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head
  * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and
  * out_stride elements apart; out may be q.  Long sequences are split over workgroups and joined in a
- * second launch, in the same order in every run: equal inputs give equal bits.  A length of 0 gives zeros; lengths
- * are cut to table_width * page_size; tokens on page ids outside the cache do not count; rows of the
- * cache behind a sequence's last token are not read.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less -> QVX_E_RANGE; its
- * contents need not be kept or cleared). */
+ * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
+ * 0 .. table_width * page_size; tokens on page ids outside the cache do not count; a row without any key gets
+ * zeros; rows of the cache behind a sequence's last token are not read.  Keys are finite: an infinite one of a 16-bit
+ * cache makes its rows NaN, as NaN does.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less ->
+ * QVX_E_RANGE; its contents need not be kept or cleared). */
 int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q_stride, int q_heads,
                    const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens,
                    int n_seqs, float scale, void* d_ws, size_t ws_bytes, void* stream);
@@ -331,9 +332,10 @@ typedef struct qvx_kv_states {
  * first d_lens[b] states of sequence b (0: zeros; NULL: all max_len), none masked by position.
  * d_offsets NULL: n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  Rows behind the last
  * sequence's are left as they were.  q and out share q_type: F32, F16 or BF16, rows and heads as in
- * qvx_attn_paged.  Where q and the states share a 16-bit type and there are many queries, both
+ * qvx_attn_paged; out may be q.  Where q and the states share a 16-bit type, the rows of a sequence and head (queries times heads
+ * a group) are 32 or more in the mean, scale is at least 1e-30 and the row stride at most 16 Mi bytes, both
  * products run on the 16-bit matrix cores and the softmax weights are rounded to that type (sums
- * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout. */
+ * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout.  d_ws as there. */
 int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
                    const int32_t* d_offsets, int n_q, const qvx_kv_states* states, const int32_t* d_lens, int n_seqs,
                    float scale, void* d_ws, size_t ws_bytes, void* stream);

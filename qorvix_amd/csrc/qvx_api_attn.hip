@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kAttnMaxSeqs = 65536, kMapMaxSeqs = 16384;
 constexpr int64_t kMaxPitch = 64ll << 20;  // sixteen rows stay far inside 32-bit offsets
+constexpr float kLeastScale = 1e-30f;       // far above the subnormal numbers
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -135,8 +136,9 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
-// wide: the call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a 16-bit type, the scale is not
-// negative (the kernel takes the largest product for the largest logit), and sequences have 32 rows or more in the mean.
+// wide: the call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a 16-bit type, the scale is
+// positive (the kernel takes the largest product for the largest logit, and -inf times the scale for a masked one),
+// sequences have 32 rows or more in the mean, and its tiles of 64 states stay inside 32-bit offsets.
 int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, float scale,
                 AttnCall& c, bool* wide, bool* join, size_t* ws_bytes) {
   if (!st) return QVX_E_NULL;
@@ -174,7 +176,8 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   c.head_dim = st->head_dim;
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
   if ((int64_t)n_q * c.group > 0x7fffff00ll) return QVX_E_RANGE;
-  *wide = q_type == st->type && q_type != T_F32 && scale >= 0.0f && (int64_t)n_q * c.group >= 32 * (int64_t)n_seqs;
+  *wide = q_type == st->type && q_type != T_F32 && scale >= kLeastScale && c.pitch <= kMaxPitch / 4 &&
+          (int64_t)n_q * c.group >= 32 * (int64_t)n_seqs;
   c.tile_rows = *wide ? kAttnRows16 : tile_rows(ragged ? rows / n_seqs : rows);  // ragged: of a sequence in the mean
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);

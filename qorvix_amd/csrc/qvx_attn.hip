@@ -85,7 +85,7 @@ template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) 
         o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] /= sum;
+      for (int k = 0; k < 4; ++k) o[k] = top == -INFINITY ? 0.0f : o[k] / sum;
       attn_store4(c.out, attn_row(c, pc.q0, pc.row0 + r, kvh, c.out_stride) + 4 * quad, c.q_type, o);
     }
   }

@@ -8,8 +8,8 @@
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction, fp32 sums.  The weights are
 // rounded to the operands' type (to the nearest) before the second product: each by at most half a
 // step; the denominator sums them in fp32.  The reference m follows the largest logit
-// lazily, as in qvx_attn_split.hpp, at most 2^kSlack16 behind: weights to 2^8 are as exact in fp16 as
-// those to 1, and those of 2^-22 of the largest are still above its smallest normal number.
+// lazily, as in qvx_attn_split.hpp, at most 2^kSlack16 behind.  In fp16 all weights are 2^kUp16 larger than that:
+// up to 2^15 they stay in range, and down to 2^-21 of the largest above its smallest normal number.
 //
 // Layout.  In S^T a lane holds query row lane % 32 and, with h = lane / 32, the keys 8 (r / 4) + 4 h + r % 4
 // in registers r = 0 .. 15.  The second product's right operand wants, for 16 keys, eight of them in
@@ -34,6 +34,7 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRows16 = kAttnRows16;
 constexpr float kSlack16 = 8.0f;
+template <uint32_t T> constexpr float kUp16 = T == T_F16 ? 7.0f : 0.0f;
 
 typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
 
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[b][r] *= f;
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = m == -INFINITY ? 0.0f : m - kUp16<T>;
     u32x4 p[BN][2];
 #pragma unroll
     for (int b = 0; b < BN; ++b)
@@ -264,7 +265,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
     }
   }
 
-
   l += __shfl_xor(l, 32);
   if (!live) return;
   if (it.chunks > 1) {  // a part of the keys: for k_attn_join
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
           *reinterpret_cast<f32x4*>(part + r16 * d16 + i) = f32x4{acc[e][r], acc[e][r + 1], acc[e][r + 2], acc[e][r + 3]};
       }
     if (h == 0) {
-      part[kRows16 * d16 + r16] = m;
+      part[kRows16 * d16 + r16] = fmaxf(m, kAttnLow);  // a chunk has keys
       part[kRows16 * (d16 + 1) + r16] = l;
     }
     return;

@@ -336,7 +336,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   int64_t at = 0, sat = 0;  // of the tile's keys (and values), and of their scales, from the cache's start
-  int live = 0;
+  int live = 0, seen = 0;  // seen: keys that count
   auto look_up = [&](int n) __attribute__((always_inline)) {
     const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
     live = 0;
@@ -377,6 +377,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   auto load = [&]<int AUX>(Tile& x, int n) __attribute__((always_inline)) {
     if (n && (n & 63) == 0 && n < tiles) look_up(n);
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
+    seen |= x.live;
     const int64_t ta = of_lane(at, n & 63);
     const uint32_t bytes = (uint32_t)(x.live * c.pitch);
     const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + ta, bytes);
@@ -619,6 +620,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   else
     run.template operator()<0>();
 
+  // Weightless keys, all at -inf, are keys all the same: their row is 0 / 0, a row without keys zeros.
+  if (seen) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) m[t] = fmaxf(m[t], kAttnLow);
+  }
+
   // Join the waves: m, l and the values of the rows, through LDS.
   const int d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0);
   float* lm = lds;                   // [wave][R]
@@ -688,7 +695,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     if (it.chunks == 1) {
       float o[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = it.len ? val[k] / sum : 0.0f;
+      for (int k = 0; k < 4; ++k) o[k] = top == -INFINITY ? 0.0f : val[k] / sum;
       attn_store4(c.out, attn_row(c, it.q0, it.row0 + r, kvh, c.out_stride) + i, c.q_type, o);
     } else {
       *reinterpret_cast<f32x4*>(part + r * d16 + i) = val;

@@ -227,7 +227,47 @@ def test_paged_missing_pages_do_not_count(cuda):
     keep = np.r_[0:16, 32:64, 80:96]
     want, s = _attend(q[0].cpu().double().numpy(), k[0][keep], v[0][keep], 64 ** -0.5)
     assert np.abs(out[0].cpu().double().numpy() - want).max() <= 2 * U * (67 * s + 104) * np.abs(v).max()
-    assert bool(torch.isnan(out[1]).all())  # no key left of a sequence that has some: 0 / 0
+    assert bool((out[1] == 0).all())  # none is left: as for a sequence without any
+
+
+@pytest.mark.parametrize("t", (qvx.F16, qvx.F32))
+@pytest.mark.parametrize("n", [20, 2000])
+@pytest.mark.parametrize("group", [1, 6, 16])
+def test_paged_keys_without_weight(cuda, t, n, group):
+    """Logits of -inf weigh nothing; where a row has no other it is 0 / 0, unless its pages are missing: then zeros."""
+    torch = cuda
+    c = Cache(torch, t, (n, n, n), 16, 1, 64, seed=15)
+    k = c.desc.tensors[0].view(_torch_type(torch, t)).view(c.n_pages, 16, 64)
+    pages = torch.from_numpy(c.table).cuda().long()
+    full = n // 16
+    k[pages[0, : full - 1], :, 3] = float("-inf")   # all but the last pages' keys of sequence 0
+    k[pages[1, : c.width - 1], :, 3] = float("-inf")  # all of sequence 1
+    c.dev_table[2] = -1
+    q = torch.randn((3, group, 64), device="cuda")
+    q[:, :, 3] = 1.0
+    out = qvx.attn_paged_t(q, c.desc, c.dev_table, c.dev_lens)
+    kept = np.arange(16 * (full - 1), n)
+    kk, vv = c.rows(0, 0)[0][kept], c.rows(0, 1)[0][kept]
+    want, s = _attend(q[0].cpu().double().numpy(), kk, vv, 64 ** -0.5)
+    if t == qvx.F32:  # of a 16-bit cache the query is multiplied in parts, 0 times an infinite key among them
+        assert np.abs(out[0].cpu().double().numpy() - want).max() <= 2 * U * (67 * s + n + 8) * np.abs(c.rows(0, 1)).max()
+    assert bool(torch.isnan(out[1]).all()) and bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("t", CACHE_TYPES)
+@pytest.mark.parametrize("group", [1, 8, 16])
+def test_paged_scale_of_zero_and_below(cuda, t, group):
+    """Equal weights, whatever the masked tail of a tile holds; and the smallest key the heaviest."""
+    for scale in (0.0, -0.3):
+        c = Cache(cuda, t, (37, 1, 500), 24, 1, 64, seed=16)
+        _check_paged(cuda, c, group, scale=scale)
+
+
+@pytest.mark.parametrize("t,n", [(qvx.F16, 8), (qvx.Q8_0, 16)])
+def test_paged_past_half_the_memory_side_cache(cuda, t, n):
+    """More than 128 MiB of keys and values (their loads are marked as read once), the smallest sequences beside them."""
+    c = Cache(cuda, t, (8191,) * n + (1, 0), 32, 8, 64 if t == qvx.F16 else 64, seed=17)
+    _check_paged(cuda, c, 8)
 
 
 def test_paged_lengths_past_the_table(cuda):
@@ -298,7 +338,8 @@ def test_paged_on_another_stream(cuda):
 
 # ---- cross attention --------------------------------------------------------------------------------------
 
-def _check_cross(torch, q_type, kv_type, nq, ns, hq, hk, d, seed=0, stacked=True, equal=False, tail=3):
+def _check_cross(torch, q_type, kv_type, nq, ns, hq, hk, d, seed=0, stacked=True, equal=False, tail=3, scale=None, pads=None):
+    """pads: elements before q's and out's first row, and behind each of their rows."""
     r = np.random.default_rng(seed)
     qt, kt = _torch_type(torch, q_type), _torch_type(torch, kv_type)
     n, most = len(nq), max(max(ns), 1)
@@ -312,14 +353,19 @@ def _check_cross(torch, q_type, kv_type, nq, ns, hq, hk, d, seed=0, stacked=True
         k, v = dev[:, :, 0], dev[:, :, 1]
     else:  # head by head
         k, v = (dev[:, :, i].transpose(1, 2).contiguous().transpose(1, 2) for i in range(2))
+    place = lambda x, pad, gap: torch.cat([x.flatten(1), torch.full((rows, gap), 5.0, dtype=qt)], 1).flatten()  # noqa: E731
+    view = lambda x, pad, gap: x[pad:].view(rows, -1)[:, : hq * d].unflatten(1, (hq, d))  # noqa: E731
     out = torch.full((rows, hq, d), 3.0, dtype=qt, device="cuda")
+    qdev = q.cuda()
+    if pads:
+        qdev, out = (view(torch.nn.functional.pad(place(x.cpu(), *p), (p[0], 0)).cuda(), *p) for x, p in zip((q, out), pads))
     offsets = None if equal else torch.tensor(np.r_[0, np.cumsum(nq)], dtype=torch.int32, device="cuda")
     lens = None if equal and len(set(ns)) == 1 else torch.tensor(ns, dtype=torch.int32, device="cuda")
-    qvx.attn_cross_t(q.cuda(), qvx.KvStates.of(k, v), lens=lens, offsets=offsets, out=out)
+    qvx.attn_cross_t(qdev, qvx.KvStates.of(k, v), lens=lens, offsets=offsets, out=out, scale=scale)
     torch.cuda.synchronize()
     got = out.cpu().double().numpy()
     qn, kvn = q.double().numpy(), kv.double().numpy()
-    g, at, scale = hq // hk, 0, d ** -0.5
+    g, at, scale = hq // hk, 0, d ** -0.5 if scale is None else scale
     half = {qvx.F32: 0.0, qvx.F16: 2.0 ** -11, qvx.BF16: 2.0 ** -8}[q_type]
     for b in range(n):
         mine = got[at:at + nq[b]]
@@ -369,3 +415,122 @@ def test_cross_many_sequences(cuda, q_type, kv_type):
     r = np.random.default_rng(3)
     nq, ns = [int(x) for x in r.integers(0, 40, 90)], [int(x) for x in r.integers(0, 60, 90)]
     _check_cross(cuda, q_type, kv_type, nq, ns, 2, 2, 64, seed=5)
+
+
+# ---- cross attention on the 16-bit matrix cores: its split, its fallbacks and its callers ------------------
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16)
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("nq,ns", [((40,), (1500,)), ((129, 33, 0, 32), (700, 255, 90, 0)), ((64, 200), (257, 4100))])
+def test_cross_few_rows_on_many_states(cuda, q_type, kv_type, d, nq, ns):
+    """Too few row tiles for the card: their states are split over workgroups."""
+    _check_cross(cuda, q_type, kv_type, nq, ns, 2, 1, d, seed=d + len(nq))
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16)
+def test_cross_split_of_many_sequences(cuda, q_type, kv_type):
+    """More sequences than a wave has lanes, some long enough for a split."""
+    r = np.random.default_rng(18)
+    nq = [int(x) for x in r.integers(20, 60, 70)]
+    ns = [int(x) for x in r.integers(0, 40, 70)]
+    ns[3], ns[68] = 1300, 900
+    _check_cross(cuda, q_type, kv_type, nq, ns, 1, 1, 40, seed=6)
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED[:1])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 2e-30, -0.2, 1.0])
+def test_cross_scales(cuda, q_type, kv_type, scale):
+    """Odd states in the last tile: masked ones stay masked at every scale."""
+    _check_cross(cuda, q_type, kv_type, (50, 33), (45, 70), 2, 2, 64, seed=7, scale=scale)
+    _check_cross(cuda, q_type, kv_type, (40,), (800,), 1, 1, 64, seed=8, scale=scale)
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED)
+@pytest.mark.parametrize("pads", [((8, 8), (4, 4)), ((1, 0), (0, 3)), ((0, 5), (1, 8)), ((3, 7), (2, 2))])
+def test_cross_alignment(cuda, q_type, kv_type, pads):
+    """Rows of q and out on any element."""
+    _check_cross(cuda, q_type, kv_type, (50, 33), (45, 70), 2, 2, 40, seed=9, pads=pads)
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16)
+def test_cross_wide_pitch(cuda, q_type, kv_type):
+    """States 20 MiB apart: a tile of 64 would pass 32-bit offsets."""
+    torch = cuda
+    pitch, d = 10 << 20, 64
+    kt = _torch_type(torch, kv_type)
+    held = torch.zeros(3 * pitch, dtype=kt, device="cuda")
+    k, v = (held[i * 64:].as_strided((1, 3, 1, d), (0, pitch, 0, 1)) for i in (0, 1))
+    k.copy_(torch.randn((1, 3, 1, d), device="cuda"))
+    v.copy_(torch.randn((1, 3, 1, d), device="cuda"))
+    q = torch.randn((40, 1, d), device="cuda").to(kt)
+    got = qvx.attn_cross_t(q, qvx.KvStates.of(k, v))
+    packed = qvx.attn_cross_t(q.float(), qvx.KvStates.of(k.contiguous(), v.contiguous()))
+    half = 2.0 ** -11 if kv_type == qvx.F16 else 2.0 ** -8
+    s = float((q.float()[:, 0].abs() @ k.float()[0, :, 0].abs().T).max()) / 8
+    tol = 2 * 2 * U * ((d + 3) * s + 11) * float(v.abs().max()) + half * packed.abs()
+    assert bool(((got.float() - packed).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED[:1])
+def test_cross_in_place_and_repeatable(cuda, q_type, kv_type):
+    torch = cuda
+    q = torch.randn((60, 2, 64), device="cuda").to(_torch_type(torch, q_type))
+    k, v = (torch.randn((2, 1100, 2, 64), device="cuda").to(_torch_type(torch, kv_type)) for _ in range(2))
+    offsets = torch.tensor([0, 50, 58], dtype=torch.int32, device="cuda")
+    st = qvx.KvStates.of(k, v)
+    first = qvx.attn_cross_t(q, st, offsets=offsets)
+    assert torch.equal(first[:58], qvx.attn_cross_t(q, st, offsets=offsets)[:58])
+    behind = q[58:].clone()
+    qvx.attn_cross_t(q, st, offsets=offsets, out=q)
+    assert torch.equal(first[:58], q[:58]) and torch.equal(behind, q[58:])
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED[:1])
+def test_cross_captured_replays_follow_the_lengths(cuda, q_type, kv_type):
+    """Lengths and offsets change between replays, in two graphs with workspaces of their own."""
+    torch = cuda
+    kt = _torch_type(torch, kv_type)
+    k, v = (torch.randn((3, 1500, 2, 64), device="cuda").to(kt) for _ in range(2))
+    st = qvx.KvStates.of(k, v)
+    qs = [torch.randn((120, 2, 64), device="cuda").to(_torch_type(torch, q_type)) for _ in range(2)]
+    lens = torch.tensor([1500, 3, 700], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, 40, 41, 120], dtype=torch.int32, device="cuda")
+    qvx.attn_cross_t(qs[0], st, lens=lens, offsets=offsets)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        out = torch.empty_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            qvx.attn_cross_t(q, st, lens=lens, offsets=offsets, out=out)
+        graphs.append(g)
+        outs.append(out)
+    for n, o in (([1500, 3, 700], [0, 40, 41, 120]), ([0, 1500, 1], [0, 1, 119, 120]), ([17, 16, 15], [0, 0, 0, 120]),
+                 ([1500, 1500, 1500], [0, 100, 110, 120])):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        offsets.copy_(torch.tensor(o, dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        for q, out in zip(qs, outs):
+            assert torch.equal(out, qvx.attn_cross_t(q, st, lens=lens, offsets=offsets))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16)
+def test_cross_many_small_weights(cuda, q_type, kv_type):
+    """One heavy state and thousands whose weights lie among fp16's subnormal numbers, which together weigh as much."""
+    torch = cuda
+    n, d = 4096, 64
+    kt = _torch_type(torch, kv_type)
+    k = torch.zeros((1, n, 1, d), device="cuda")
+    k[0, 5, 0, 0] = 8.0  # logit 64 / 8 = 8: the others weigh e^-8 of it, and 4095 e^-8 = 1.37 of it in all
+    v = torch.ones((1, n, 1, d), device="cuda")
+    v[0, 5] = 0.0
+    q = torch.zeros((64, 1, d), device="cuda")
+    q[:, 0, 0] = 8.0
+    got = qvx.attn_cross_t(q.to(kt), qvx.KvStates.of(k.to(kt), v.to(kt)), scale=0.125).float()
+    rest = (n - 1) * np.exp(-8.0)
+    want = rest / (1 + rest)
+    # Two roundings to 16 bits (the weights', the output's) of half a step each; the power of two and the sums as ever.
+    half = 2.0 ** -11 if kv_type == qvx.F16 else 2.0 ** -8
+    assert float((got - want).abs().max()) <= (2 * half + 2 * U * (67 * 8 + n + 8)) * 1.0
