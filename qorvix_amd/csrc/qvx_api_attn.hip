@@ -73,9 +73,12 @@ int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
 // The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
 // False: it passes 31 bits.
+int64_t most_tiles(const AttnCall& c) {
+  return (int64_t)c.max_len / c.page_size * c.page_tiles + (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
+}
+
 bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
-  const int64_t tiles = (int64_t)c.max_len / c.page_size * c.page_tiles +
-                        (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
+  const int64_t tiles = most_tiles(c);
   *join = c.min_chunk && tiles > c.min_chunk;
   const int64_t most = *join ? (tiles + c.min_chunk - 1) / c.min_chunk : 1;  // chunks of a row tile
   const int64_t items = std::min(row_tiles + c.target, row_tiles * most);
@@ -92,8 +95,15 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   return true;
 }
 
+// One workgroup reads some 45 GB/s, a split costs a launch of its own and the workspace's traffic, together 4 to 5 us.
+// So sequences that cannot pass 320 KB of keys and values a head are left whole, and up to 640 KB those of calls that
+// occupy a good part of the card all the same.  Head size 128, fp16, split against whole: 256 keys 11.3 and 8.3 us
+// at 40 items, 21.4 and 13.5 at 320; 512 keys 12.2 and 11.1, 26.6 and 20.2; 1024 keys 14.5 and 15.7 at 40,
+// 20.7 and 15.7 at 96, 25.7 and 17.7 at 160, 44.3 and 41.3 at 320; 2048 keys 16.0 and 24.2, 74.3 and 76.0.
 bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
-  c.min_chunk = kMinChunk;
+  const int64_t bytes = most_tiles(c) * 2 * kAttnTile * c.pitch;
+  const bool whole = bytes <= 320 << 10 || (bytes <= 640 << 10 && row_tiles * c.kv_heads >= 96);
+  c.min_chunk = whole ? 0 : kMinChunk;
   c.target = std::max(1, kAttnWgs / c.kv_heads);
   return plan_items(c, row_tiles, join, ws_bytes);
 }
