@@ -101,7 +101,7 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 // at 40 items, 21.4 and 13.5 at 320; 512 keys 12.2 and 11.1, 26.6 and 20.2; 1024 keys 14.5 and 15.7 at 40,
 // 20.7 and 15.7 at 96, 25.7 and 17.7 at 160, 44.3 and 41.3 at 320; 2048 keys 16.0 and 24.2, 74.3 and 76.0.
 bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
-  const int64_t bytes = most_tiles(c) * 2 * kAttnTile * c.pitch;
+  const int64_t bytes = most_tiles(c) * 2 * kAttnTile * c.key_bytes;
   const bool whole = bytes <= 320 << 10 || (bytes <= 640 << 10 && row_tiles * c.kv_heads >= 96);
   c.min_chunk = whole ? 0 : kMinChunk;
   c.target = std::max(1, kAttnWgs / c.kv_heads);
@@ -129,6 +129,7 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   c.k = static_cast<const uint8_t*>(cache->d_k);
   c.v = static_cast<const uint8_t*>(cache->d_v);
   c.pitch = cache->type == T_Q8_0 ? d : (int)value_bytes(cache->type, d);
+  c.key_bytes = (int)value_bytes(cache->type, d);
   c.head_stride = (int64_t)cache->page_size * c.pitch;
   c.scale_off = (int64_t)cache->kv_heads * c.head_stride;
   c.table_width = table_width;
@@ -174,6 +175,7 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   c.page_stride = st->batch_stride * es;
   c.head_stride = st->head_stride * es;
   c.pitch = (int)(st->row_stride * es);
+  c.key_bytes = (int)(st->head_dim * es);
   c.n_pages = n_seqs;
   c.page_tiles = std::max(1, st->max_len / kAttnTile + (st->max_len % kAttnTile != 0));
   c.page_size = std::max(1, st->max_len);

@@ -30,6 +30,7 @@ struct AttnCall {
   int64_t head_stride;  // bytes from a head to the next within it
   int64_t scale_off;    // Q8_0: bytes from a page's quants to its scales
   int pitch;            // bytes from a token's values of one head to the next token's
+  int key_bytes;        // bytes of those values
   const int32_t* table;  // paged: [n_seqs, table_width]; null: sequence b is "page" b
   int table_width, n_pages;
   int page_size;       // tokens of a page (states: the longest sequence)

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   // A call that reads more than half the 256 MB memory-side cache finds nothing of it there again, and its
   // loads are marked so: fp16 of 131071 tokens 102 -> 90 us, 128 x 4096 tokens 377 -> 345.  Smaller calls
   // keep the ordinary policy: 47 MB of fp32 in turn with two others like it 17.5 us against 19.3.
-  const bool once = c.read_once && sums.tiles * (long long)(2 * kAttnTile) * c.pitch * c.kv_heads > (128ll << 20);
+  const bool once = c.read_once && sums.tiles * (long long)(2 * kAttnTile) * c.key_bytes * c.kv_heads > (128ll << 20);
 
   // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
   const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;

@@ -16,7 +16,7 @@ namespace {
 // share of the tokens up by bisection.  A token at the start of a page stores the page's table entry:
 // new pages all have one.  Bound by latency: for 256 sequences a few KB are touched.
 
-constexpr int kMapThreads = 1024, kMapWgs = 256;
+constexpr int kMapThreads = 1024;
 
 struct MapSums {
   long long tokens, pages;
@@ -45,21 +45,8 @@ __device__ inline MapSums map_scan(MapSums mine, MapSums* wave_sums, MapSums& to
   return MapSums{before.tokens + x.tokens - mine.tokens, before.pages + x.pages - mine.pages};
 }
 
-// PER values of an output at t, as many as it has.
-template <int PER> __device__ inline void map_store(int32_t* out, int64_t t, int max_tokens, const int (&x)[PER]) {
-  if constexpr (PER == 4) {
-    if (t + 4 <= max_tokens && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-      *reinterpret_cast<int4*>(out + t) = make_int4(x[0], x[1], x[2], x[3]);
-      return;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (t + j < max_tokens) out[t + j] = x[j];
-}
-
 // `write`: which outputs the launch stores: the tokens' (kMapTokens), the sequences' (kMapSeqs) or both.
-template <int PER> __global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCall c, int write) {
+__global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCall c, int write) {
   __shared__ MapSums wave_sums[kMapThreads / 64];
   __shared__ int bad;
   extern __shared__ int32_t sums[];  // [n_seqs] rows behind each sequence, [n_seqs] its first new page
@@ -111,49 +98,30 @@ template <int PER> __global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCa
     }
   }
   if (!(write & kMapTokens)) return;
-  // PER tokens in a row a thread: one bisection, then a step at the sequences' ends; their loads go out together.
   const int tokens = ok ? (int)all.tokens : 0;
-  const int64_t stride = (int64_t)gridDim.x * kMapThreads * PER;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kMapThreads + tid) * PER; t0 < c.max_tokens; t0 += stride) {
-    int slot[PER], pos[PER], seq[PER];
-    int lo = 0, hi = n - 1;  // the first sequence whose rows end past t0
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (sums[mid] > t0) hi = mid; else lo = mid + 1;
+  const int stride = (int)gridDim.x * kMapThreads;
+  for (int t = (int)blockIdx.x * kMapThreads + tid; t < c.max_tokens; t += stride) {
+    int slot = -1, pos = 0, seq = -1;
+    if (t < tokens) {
+      int lo = 0, hi = n - 1;  // the first sequence whose rows end past t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > t) hi = mid; else lo = mid + 1;
+      }
+      seq = lo;
+      const int held = c.held[seq];
+      pos = held + t - (seq ? sums[seq - 1] : 0);
+      const int column = pos / page, off = pos - column * page, first = (int)(((long long)held + page - 1) / page);
+      int32_t* entry = c.table + (int64_t)seq * c.table_width + column;
+      const int id = column < first ? *entry : c.free_list[taken + sums[n + seq] + column - first];
+      if (off == 0) *entry = id;  // a page starts here, so it is new (or was left empty: its own id again)
+      const long long s = (long long)id * page + off;
+      slot = id < 0 || s > 0x7fffffffll ? -1 : (int)s;
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (j && t0 + j < tokens)
-        while (sums[lo] <= t0 + j) ++lo;  // ends: the last sum is `tokens`
-      seq[j] = lo;
-    }
-    int held[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) held[j] = c.held[seq[j]];
-    const int32_t* from[PER];
-    int32_t* entry[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      pos[j] = held[j] + (int)(t0 + j) - (seq[j] ? sums[seq[j] - 1] : 0);
-      const int column = pos[j] / page, first = (int)(((long long)held[j] + page - 1) / page);
-      entry[j] = c.table + (int64_t)seq[j] * c.table_width + column;
-      from[j] = column < first ? entry[j] : c.free_list + (taken + sums[n + seq[j]] + column - first);
-    }
-    int id[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) id[j] = t0 + j < tokens ? *from[j] : -1;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const bool real = t0 + j < tokens;
-      const int off = pos[j] % page;
-      if (real && off == 0) *entry[j] = id[j];  // a page starts here, so it is new (or was left empty: its own id again)
-      const long long s = (long long)id[j] * page + off;
-      slot[j] = !real || id[j] < 0 || s > 0x7fffffffll ? -1 : (int)s;
-      if (!real) pos[j] = 0, seq[j] = -1;
-    }
-    map_store(c.slots, t0, c.max_tokens, slot);
-    if (c.pos) map_store(c.pos, t0, c.max_tokens, pos);
-    if (c.seq) map_store(c.seq, t0, c.max_tokens, seq);
+    c.slots[t] = slot;
+    if (c.pos) c.pos[t] = pos;
+    if (c.seq) c.seq[t] = seq;
+    if (t > 0x7fffffff - stride) break;
   }
 }
 
@@ -347,21 +315,18 @@ template <uint32_t T> void rope_launch(const RopeCall& c, bool vec, dim3 grid, h
 
 }  // namespace
 
-template <int PER> bool map_launch(const MapCall& c, bool alias, hipStream_t s) {
+bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s) {
   static LdsLimit lim;
   const size_t lds = 2 * (size_t)c.n_seqs * sizeof(int32_t);
-  if (!lds_ready(reinterpret_cast<const void*>(&k_kv_map<PER>), lim, lds)) return false;
-  const int wgs = std::min(kMapWgs, c.max_tokens / (PER * kMapThreads) + 1);
+  if (!lds_ready(reinterpret_cast<const void*>(&k_kv_map), lim, lds)) return false;
+  // A token a thread up to a workgroup a CU; more only repeat the sums (506196 rows 9.0 us, with 512 workgroups 11.2).
+  // With four tokens a thread, which share a bisection and load together, 151640 rows took 8.7 us against 6.5 and 506196
+  // 9.4: neighbours are then different sequences or pages.
+  const int wgs = std::min(256, c.max_tokens / kMapThreads + 1);
   // Outputs that lie on inputs are stored by a launch of one workgroup, behind the one that reads them.
-  k_kv_map<PER><<<wgs, kMapThreads, lds, s>>>(c, alias ? kMapTokens : kMapTokens | kMapSeqs);
-  if (alias) k_kv_map<PER><<<1, kMapThreads, lds, s>>>(c, kMapSeqs);
+  k_kv_map<<<wgs, kMapThreads, lds, s>>>(c, alias ? kMapTokens : kMapTokens | kMapSeqs);
+  if (alias) k_kv_map<<<1, kMapThreads, lds, s>>>(c, kMapSeqs);
   return true;
-}
-
-// Four tokens a thread where one would take more than a round: a million rows 10.7 -> 9.0 us, but the 256 of a
-// decode step 5.1 -> 7.0, as neighbours are then different sequences.
-bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s) {
-  return c.max_tokens > kMapWgs * kMapThreads ? map_launch<4>(c, alias, s) : map_launch<1>(c, alias, s);
 }
 
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s) {
