@@ -286,7 +286,7 @@ typedef struct qvx_rope {
 } qvx_rope;
 
 /* Rotary positions with several axes, and the append to the cache, in one launch (rope and the cache
- * store of cuda/src/cuda_backend.cu:249-272, 274-346).  q_out[t] = rotated q[t]; rotated k[t] and v[t] are
+ * store of cuda/src/cuda_backend.cu:249-272, 325-340).  q_out[t] = rotated q[t]; rotated k[t] and v[t] are
  * stored in the cache at d_slots[t], rounded once to its type (Q8_0: scale = max|x| / 127 of a block in
  * fp16, quants to the nearest of x / scale).  Token t's heads lie side by side at d_q + t * q_stride
  * (elements; likewise q_out, k, v), so parts of one stacked product can be passed.  d_pos [n_axes]
@@ -299,7 +299,7 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
                 const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
                 const int32_t* d_slots, void* stream);
 
-/* Attention of one new token a sequence over the paged cache (attentionDecodeKernel,
+/* Attention of one new token a sequence over the paged cache (the reference's over one sequence,
  * cuda/src/cuda_backend.cu:347-409): out[b, h] = softmax(scale q[b, h] . K)  V over the first d_lens[b] tokens
  * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head
  * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and

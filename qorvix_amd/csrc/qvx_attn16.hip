@@ -20,6 +20,11 @@
 //
 // LDS rows are swizzled: 16-byte units of K by the row, so that sixteen rows' equal units cover the
 // banks, 64-byte runs of V by the row, so that the four rows of a transposing read do.
+//
+// Bound by the vector instructions beside the matrix ones: per weight an fma, a power of two, half a maximum, half a
+// pack and half a sum.  Measured, 2048 queries on 2048 states, 16 heads, 16 sequences, bf16: head size 64 800 TFLOP/s,
+// 96 855, 128 905, 256 730, where a library product of 8192 cubed reaches 1264.  Three workgroups a CU up to a head size
+// of 64 (with four, one register spills: 47.8 us against 46.4 for the ragged prompts below), two up to 160.
 #include "qvx_attn_split.hpp"
 
 namespace qvx {

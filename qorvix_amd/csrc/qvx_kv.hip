@@ -14,7 +14,8 @@ namespace {
 // tokens' rows and the pages are prefix sums over the sequences.  Every workgroup forms both sums for
 // itself in LDS (a few loads a thread: less than a launch of their own would take) and then looks its
 // share of the tokens up by bisection.  A token at the start of a page stores the page's table entry:
-// new pages all have one.  Bound by latency: for 256 sequences a few KB are touched.
+// new pages all have one.  Bound by latency: for 256 sequences a few KB are touched (4.4 us captured; 1024 with
+// 151640 new tokens 5.9).
 
 constexpr int kMapThreads = 1024;
 
@@ -129,7 +130,8 @@ __global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCall c, int write) {
 //
 // Pair i of a head is turned by pos[axis[i]] * inv_freq[i]; the angle's whole turns are taken off in
 // 64 bits (at position 10^6 an fp32 product is off by 0.06), the rest is an fp32 number of half turns.
-// One pass over q, k and v; the bytes bound it.  A workgroup takes `tokens_wg` tokens and a range of
+// One pass over q, k and v; the bytes bound it: 8192 tokens of 32 + 2 x 8 heads of 128 into a bf16 cache 77.7 us,
+// 4.7 TB/s where a copy of 2 GiB reaches 4.9; one token 3.5 us.  A workgroup takes `tokens_wg` tokens and a range of
 // their heads: its threads first form the cosines and sines of the tokens' pairs in LDS, each once, and
 // then take 8 values of a head at a time.
 
