@@ -303,7 +303,7 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
  * cuda/src/cuda_backend.cu:347-409): out[b, h] = softmax(scale q[b, h] . K)  V over the first d_lens[b] tokens
  * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head
  * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and
- * out_stride elements apart; out may be q.  Long sequences are split over workgroups and joined in a
+ * out_stride elements apart; out may be q (the same stride), else they do not overlap.  Long sequences are split over workgroups and joined in a
  * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
  * 0 .. table_width * page_size; tokens on page ids outside the cache do not count; a row without any key gets
  * zeros; rows of the cache behind a sequence's last token are not read.  Keys are finite: an infinite one of a 16-bit
@@ -317,7 +317,8 @@ size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int
 
 /* An encoder's keys and values: value i of head h of state j of sequence b at d_k[b * batch_stride +
  * j * row_stride + h * head_stride + i] (elements; d_v alike), F32, F16 or BF16, max_len states a sequence at most.
- * Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and under 64 Mi bytes.  head_dim: a multiple of 8
+ * Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and at most 64 Mi bytes; with
+ * max_len 0 the addresses may be NULL.  head_dim: a multiple of 8
  * up to 256. */
 typedef struct qvx_kv_states {
   const void* d_k;
@@ -332,7 +333,7 @@ typedef struct qvx_kv_states {
  * first d_lens[b] states of sequence b (0: zeros; NULL: all max_len), none masked by position.
  * d_offsets NULL: n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  Rows behind the last
  * sequence's are left as they were.  q and out share q_type: F32, F16 or BF16, rows and heads as in
- * qvx_attn_paged; out may be q.  Where q and the states share a 16-bit type, the rows of a sequence and head (queries times heads
+ * qvx_attn_paged.  Where q and the states share a 16-bit type, the rows of a sequence and head (queries times heads
  * a group) are 32 or more in the mean, scale is at least 1e-30 and the row stride at most 16 Mi bytes, both
  * products run on the 16-bit matrix cores and the softmax weights are rounded to that type (sums
  * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout.  d_ws as there. */

@@ -541,10 +541,17 @@ def qmatmul_swiglu_t(w_gu, ggml_type: int, x, ffn: int, cols: int, norm_w=None, 
 def _rows(x, what: str):
     """(address, elements from row to row) of a device tensor [rows, heads, head_dim] or [rows, heads *
     head_dim] whose rows are contiguous."""
-    width = x[0].numel() if x.shape[0] else 0
+    width = x.shape[1:].numel()
     if not x.is_cuda or (x.shape[0] and not x[0].is_contiguous()):
         raise ValueError(f"{what}: device rows with their heads side by side")
     return x.data_ptr(), (x.stride(0) if x.shape[0] > 1 else width)
+
+
+def _beside(x, device, what: str):
+    """The tensors of a description, or a workspace, lie on the call's device."""
+    for t in getattr(x, "tensors", (x,)):
+        if t is not None and hasattr(t, "device") and t.device != device:
+            raise ValueError(f"{what}: on {t.device}, the call's tensors on {device}")
 
 
 def _int32(x, shape, device, what: str):
@@ -576,6 +583,9 @@ def rope_kv_t(q, k, v, pos, rope: Rope, cache: KvCache | None = None, slots=None
     head_dim] (None without a cache), pos [tokens] or [axes, tokens] int32, slots [tokens] int32.  Returns q_out."""
     import torch
     n, heads, d = q.shape
+    _beside(rope, q.device, "rope")
+    if cache is not None:
+        _beside(cache, q.device, "cache")
     if out is None:
         out = torch.empty((n, heads, d), dtype=torch.float32, device=q.device)
     for x, what, h in ((q, "q", heads), (out, "out", heads), (k, "k", cache.kv_heads if cache is not None else 0),
@@ -603,6 +613,7 @@ def attn_paged_t(q, cache: KvCache, table, lens, scale: float | None = None, out
     n, heads, d = q.shape
     if q.dtype != torch.float32 or d != cache.head_dim:
         raise ValueError("attn_paged_t: q is float32 [n, heads, the cache's head_dim]")
+    _beside(cache, q.device, "cache")
     if out is None:
         out = torch.empty((n, heads, d), dtype=torch.float32, device=q.device)
     elif out.dtype != torch.float32 or out.shape != q.shape or out.device != q.device:
@@ -612,6 +623,7 @@ def attn_paged_t(q, cache: KvCache, table, lens, scale: float | None = None, out
     with torch.cuda.device(q.device):
         if ws is None:
             ws = torch.empty(attn_paged_ws(cache, heads, n, width), dtype=torch.uint8, device=q.device)
+        _beside(ws, q.device, "ws")
         _check(attn_paged(*_rows(out, "out"), *_rows(q, "q"), heads, cache, tp, width, lp, n,
                           d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(),
                           _stream()), "qvx_attn_paged")
@@ -625,6 +637,7 @@ def attn_cross_t(q, states: KvStates, lens=None, offsets=None, scale: float | No
     n_q, heads, d = q.shape
     if q.dtype not in _torch_types() or d != states.head_dim:
         raise ValueError("attn_cross_t: q is float32, float16 or bfloat16 [rows, heads, the states' head_dim]")
+    _beside(states, q.device, "states")
     if out is None:
         out = torch.zeros((n_q, heads, d), dtype=q.dtype, device=q.device) if offsets is not None else \
             torch.empty((n_q, heads, d), dtype=q.dtype, device=q.device)
@@ -637,6 +650,7 @@ def attn_cross_t(q, states: KvStates, lens=None, offsets=None, scale: float | No
     with torch.cuda.device(q.device):
         if ws is None:
             ws = torch.empty(attn_cross_ws(states, t, heads, n_q, n), dtype=torch.uint8, device=q.device)
+        _beside(ws, q.device, "ws")
         _check(attn_cross(*_rows(out, "out"), *_rows(q, "q"), t, heads, op, n_q, states, lp, n,
                           d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(),
                           _stream()), "qvx_attn_cross")

@@ -167,7 +167,7 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
       st->row_stride > kMaxPitch / es || (st->row_stride * es) % 16 || (st->batch_stride * es) % 16 ||
       (st->head_stride * es) % 16)
     return QVX_E_RANGE;
-  if (!st->d_k || !st->d_v) return QVX_E_NULL;
+  if (st->max_len && (!st->d_k || !st->d_v)) return QVX_E_NULL;
   if (!aligned(st->d_k, 16) || !aligned(st->d_v, 16)) return QVX_E_RANGE;
   c.q_type = q_type;
   c.k = static_cast<const uint8_t*>(st->d_k);

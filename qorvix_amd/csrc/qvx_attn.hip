@@ -27,6 +27,11 @@ template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) 
   const int tid = threadIdx.x, kvh = blockIdx.y, slot = blockIdx.x;
   const AttnPiece pc = attn_pieces(c.ws)[slot];  // of the workspace: may be read before it is known to be one
   if (slot >= *reinterpret_cast<const int*>(c.ws)) return;
+  // Offsets that are no running sums can name more pieces than there are workgroups to leave them: what stands there
+  // instead is used only as far as it stays inside the call's rows and parts.
+  if (pc.q0 < 0 || pc.row0 < 0 || pc.row0 >= pc.rows || pc.chunk < 0 || pc.chunk >= pc.chunks || pc.chunk > slot ||
+      pc.chunks > c.slots - (slot - pc.chunk) || (int64_t)pc.q0 * c.group + pc.rows > (int64_t)c.n_q * c.group)
+    return;
   const bool few = pc.chunks <= kFewChunks;
   const int d = c.head_dim, d16 = (d + 15) & ~15, quads = d / 4, nrow = min(R, pc.rows - pc.row0);
   const size_t size = attn_part(R, d16), step = (size_t)c.kv_heads * size;

@@ -91,7 +91,7 @@ template <int R> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
   s.len = min(max(len, 0), c.max_len);
   if (c.q_offsets) {  // clamped to the rows that the host vouches for
     s.q0 = min(max(c.q_offsets[b], 0), c.n_q);
-    s.nq = max(min(c.q_offsets[b + 1], c.n_q) - s.q0, 0);
+    s.nq = max(min(max(c.q_offsets[b + 1], 0), c.n_q) - s.q0, 0);
   } else {
     s.q0 = b * c.q_each;
     s.nq = c.q_each;

@@ -98,6 +98,7 @@ def test_cross_refusals():
     assert cross(offsets=0, n_q=7) == qvx.E_SHAPE  # 7 queries are no three equal parts
     assert cross(out_stride=255) == qvx.E_SHAPE and cross(q_stride=-256) == qvx.E_SHAPE
     assert cross(n_q=0) == qvx.OK  # nothing to do
+    assert cross(states(d_k=0, d_v=0, max_len=0), n_q=0) == qvx.OK  # no states: no addresses
     assert cross(out=0) == qvx.E_NULL and cross(q=0) == qvx.E_NULL
     assert cross(out=P + 2) == qvx.E_RANGE and cross(q=P + 1, q_type=qvx.F16) == qvx.E_RANGE
     assert cross(out=P, q=P, q_stride=300) == qvx.E_RANGE
@@ -162,6 +163,23 @@ def test_descriptions_of_tensors_are_checked():
         qvx.Rope.of(torch.zeros(32))
     with pytest.raises(ValueError):
         qvx.KvStates.of(torch.zeros((1, 4, 2, 64)), torch.zeros((1, 4, 2, 64)))
+
+
+def test_descriptions_and_workspaces_lie_beside_the_tensors():
+    import torch
+    far = torch.empty(1, device="meta")
+    q, ints = torch.zeros((3, 4, 64)), torch.zeros(3, dtype=torch.int32)
+    c, st, r = cache(), states(), qvx.Rope(P, None, 64, 1, 0, 1.0)
+    c.tensors = st.tensors = r.tensors = (far, far)
+    with pytest.raises(ValueError, match="cache: on meta"):
+        qvx.attn_paged_t(q, c, ints, ints)
+    with pytest.raises(ValueError, match="states: on meta"):
+        qvx.attn_cross_t(q, st)
+    with pytest.raises(ValueError, match="rope: on meta"):
+        qvx.rope_kv_t(q, None, None, ints, r)
+    r.tensors = (q, None)
+    with pytest.raises(ValueError, match="cache: on meta"):
+        qvx.rope_kv_t(q, q, q, ints, r, cache=c, slots=ints)
 
 
 def test_structures_match_the_header():

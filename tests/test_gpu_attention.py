@@ -534,3 +534,62 @@ def test_cross_many_small_weights(cuda, q_type, kv_type):
     # Two roundings to 16 bits (the weights', the output's) of half a step each; the power of two and the sums as ever.
     half = 2.0 ** -11 if kv_type == qvx.F16 else 2.0 ** -8
     assert float((got - want).abs().max()) <= (2 * half + 2 * U * (67 * 8 + n + 8)) * 1.0
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED[:1])
+def test_cross_without_queries_or_states(cuda, q_type, kv_type):
+    torch = cuda
+    qt, kt = _torch_type(torch, q_type), _torch_type(torch, kv_type)
+    k = torch.randn((2, 9, 2, 64), device="cuda").to(kt)
+    none = qvx.attn_cross_t(torch.empty((0, 2, 64), dtype=qt, device="cuda"), qvx.KvStates.of(k, k))
+    assert none.shape == (0, 2, 64)
+    empty = torch.empty((2, 0, 2, 64), dtype=kt, device="cuda")
+    for rows in (2, 80):
+        out = qvx.attn_cross_t(torch.randn((rows, 2, 64), device="cuda").to(qt), qvx.KvStates.of(empty, empty))
+        assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES16 + MIXED[:1])
+def test_cross_offsets_that_are_no_running_sums(cuda, q_type, kv_type):
+    """Decreasing and far offsets: nothing outside the rows is written, whatever the workspace holds, and the next call
+    with good ones is right."""
+    torch = cuda
+    qt, kt = _torch_type(torch, q_type), _torch_type(torch, kv_type)
+    k, v = (torch.randn((6, 1400, 2, 64), device="cuda").to(kt) for _ in range(2))
+    st = qvx.KvStates.of(k, v)
+    q = torch.randn((40, 2, 64), device="cuda").to(qt)
+    whole = torch.full((60, 2, 64), 5.0, dtype=qt, device="cuda")
+    good = torch.tensor([0, 3, 3, 10, 20, 38, 40], dtype=torch.int32, device="cuda")
+    ws = torch.full((qvx.attn_cross_ws(st, q.dtype, 2, 40, 6),), 255, dtype=torch.uint8, device="cuda")
+    want = qvx.attn_cross_t(q, st, offsets=good)
+    for bad in ([40, 0, 40, 0, 40, 0, 40], [0, 40, 0, 40, 0, 40, 0], [-7, 1 << 30, -(1 << 31), 5, 2000000000, 1, 40]):
+        qvx.attn_cross_t(q, st, offsets=torch.tensor(bad, dtype=torch.int32, device="cuda"), out=whole[10:50], ws=ws)
+        torch.cuda.synchronize()
+        assert bool((whole[:10] == 5.0).all()) and bool((whole[50:] == 5.0).all())
+        assert torch.equal(qvx.attn_cross_t(q, st, offsets=good, ws=ws), want)
+
+
+@pytest.mark.parametrize("t", (qvx.BF16, qvx.Q8_0))
+def test_pages_past_four_gib(cuda, t):
+    """Append and attention on pages whose byte offsets pass 32 bits, beside one at the start."""
+    torch = cuda
+    page, hk, d, n = 128, 8, 128, 1000
+    size = qvx.kv_page_bytes(t, hk, page, d)
+    n_pages = (5 << 30) // size
+    k, v = (torch.empty((n_pages, size), dtype=torch.uint8, device="cuda") for _ in range(2))
+    far = qvx.KvCache.of(k, v, t, page, hk, d)
+    near_k, near_v = (torch.empty((9, size), dtype=torch.uint8, device="cuda") for _ in range(2))
+    near = qvx.KvCache.of(near_k, near_v, t, page, hk, d)
+    ids = torch.tensor([0, n_pages - 1, n_pages - 5, 3, n_pages - 9, n_pages // 2, n_pages - 2, n_pages - 3], dtype=torch.int32,
+                       device="cuda")
+    here = torch.tensor([8, 1, 2, 3, 4, 5, 6, 7], dtype=torch.int32, device="cuda")
+    at = torch.arange(n, dtype=torch.int32, device="cuda")
+    q, kk, vv = (torch.randn((n, h, d), device="cuda") for h in (16, hk, hk))
+    rope = qvx.Rope.of(10000.0 ** -(torch.arange(64, dtype=torch.float64, device="cuda") / 64))
+    outs = []
+    for c, p in ((far, ids), (near, here)):
+        turned = qvx.rope_kv_t(q, kk, vv, at, rope, cache=c, slots=p[(at // page).long()] * page + at % page)
+        lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+        outs.append((turned, qvx.attn_paged_t(turned[-1:], c, p[None], lens)))
+    assert torch.equal(k[ids.long()][:, :64], near_k[here.long()][:, :64])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

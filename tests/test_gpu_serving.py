@@ -91,8 +91,7 @@ def _near(got, want, tol):
     assert float((got - want).abs().max() / want.abs().max()) <= tol
 
 
-@pytest.mark.parametrize("m", [1, 3])
-@pytest.mark.parametrize("t", [qvx.F16, qvx.F32])
+@pytest.mark.parametrize("m,t", [(1, qvx.F16), (3, qvx.F16), (1, qvx.F32), (3, qvx.F32), (20, qvx.F16)])
 def test_paged_decode_steps(cuda, m, t):
     """Twelve eager steps, then as many replays of the captured step, pages filling up one after another."""
     torch = cuda
