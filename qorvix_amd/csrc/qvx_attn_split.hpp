@@ -241,15 +241,15 @@ template <int KS> struct AttnQuery<T_F32, KS> {
 // values col * VB .. of keys 4 g .. 4 g + 3; of Q8_0 also the scales of those four keys' blocks, and of
 // the values' block in each of them.  FULL: head_dim is DT, so a key's scales are one load.
 //
-// Q8_0 for four rows (kGroup): the products of each block have to be summed alone, and sixteen lanes that each
+// Q8_0 for four rows or eight (kGroup): the products of each block have to be summed alone, and sixteen lanes that each
 // fetch 8 bytes of another key keep the address units busier than the memory (4.4 TB/s where fp16 reaches
 // 5.6).  So a lane group takes whole blocks: NP of them at a time, one for 4 / NP groups, in 16-byte
-// loads, and the four rows stand NP times among the sixteen columns of the product, each time with the
+// loads, and the rows stand NP times among the sixteen columns of the product, each time with the
 // values of one group's block and zeros for the others': one instruction chain sums NP blocks apart.
 template <uint32_t T, int DT, bool FULL, int NS> struct AttnTile {
   static constexpr int KS = DT / 32, VB = DT / 16, VU = VB < 8 ? VB : 8, VN = VB / VU;
-  static constexpr bool kQ8 = T == T_Q8_0, kGroup = kQ8 && NS == 1;
-  static constexpr int NP = kGroup ? (KS < 4 ? KS : 4) : 1, U = KS / NP, J = KS / U, G4 = 4 / NP;
+  static constexpr bool kQ8 = T == T_Q8_0, kGroup = kQ8 && NS <= 2;
+  static constexpr int kMostNP = 4 / NS, NP = kGroup ? (KS < kMostNP ? KS : kMostNP) : 1, U = KS / NP, J = KS / U, G4 = 4 / NP;
   static constexpr int kRegs = 2 * DT * AttnRaw<T, 8>::kBytes / 32 / 4 +
                                (kGroup ? 4 * U + 4 : kQ8 ? 2 * KS + 4 : 0);  // of a lane
   AttnRaw<T, 8> k[KS];
@@ -408,9 +408,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         if constexpr (kGroup) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int block = u * NP + col / 4;
+            const int block = u * NP + col / R;
             x.kstep[r][u] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
-                ks, col / 4 < NP && 32 * block < d ? soff + r * spitch + 2 * block : kPastEnd, 0, 0);
+                ks, col / R < NP && 32 * block < d ? soff + r * spitch + 2 * block : kPastEnd, 0, 0);
           }
         } else if constexpr (FULL) {
           AttnWords<(KS + 1) / 2> w;
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, voff[u] + r * c.pitch);
   };
   // Tiles in registers, one in work and one on its way where they fit: 131071 tokens in bf16 103 us against 111 with one.
-  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT >= 128) ? 2 : 1;
+  // For eight rows of 128 values they fit over Q8_0 alone, less six registers (64 x 4096 tokens 139 us against 145).
+  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT >= (kGroup ? 256 : 128)) ? 2 : 1;
   Tile held[kHeld];
   AttnQuery<T, KS> q;
   float mul = 1.0f;
@@ -455,8 +456,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 
   // This lane's query values: row col's pieces; rows and values that are not there are zeros.
   auto set_query = [&]() __attribute__((always_inline)) {
-    const int row = it.row0 + (kGroup ? col & 3 : col);
-    const bool mine = row < it.rows && (kGroup ? col / 4 == g / G4 : col < R);
+    const int row = it.row0 + (kGroup ? col % R : col);
+    const bool mine = row < it.rows && (kGroup ? col / R == g / G4 : col < R);
     const int64_t first = attn_row(c, it.q0, min(row, it.rows - 1), kvh, c.q_stride);
     int64_t from[KS];
 #pragma unroll
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
 #pragma unroll
-      for (int o = kGroup ? 4 : 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+      for (int o = kGroup ? R : 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
       // 2^e <= top < 2^(e + 1) to 2^14; a row with an infinite value as it is
       const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
       const int up = e < 128 ? 14 - e : 0;
@@ -501,10 +502,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
         for (int r = 0; r < 4; ++r) sc[r] = __builtin_fmaf(attn_half((uint16_t)x.kstep[r][u]), y[r], sc[r]);
       }
-      // The blocks of a row stand in four columns each (zeros where there are fewer groups): their sum, in all four.
+      // The blocks of a row stand in four columns, or two (zeros where there are fewer groups): their sum, in all of them.
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[r] += attn_rotate<4>(sc[r]);
+        if constexpr (NS == 1) sc[r] += attn_rotate<4>(sc[r]);
         sc[r] += attn_rotate<8>(sc[r]);
       }
     }
