@@ -85,6 +85,8 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   if (items * c.kv_heads > 0x7fffffffll || tiles > 0x7fffffffll) return false;
   if (!*join) c.min_chunk = 0x7ffffff0;
   c.items = (int)items;
+  c.most_tiles = (int)tiles;
+  c.by_length = items * c.kv_heads > kAttnWgs;
   const int d16 = (c.head_dim + 15) / 16 * 16;
   c.small_sum = row_tiles * tiles <= 0x7fffffffll;
   c.read_once = row_tiles <= c.n_seqs;

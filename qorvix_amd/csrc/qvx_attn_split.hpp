@@ -27,7 +27,7 @@
 //
 // Measured, 32 query and 8 key / value heads of 128, where a read of 2 GiB reaches 6.8 TB/s: one sequence of 131071
 // tokens in bf16 92 us (5.8 TB/s, the join's 6 in it), 64 of 4096 in Q8_0 104 us (5.5), 128 of 4096 in fp16 345 us (6.2);
-// 48 of 1 to 8192 tokens in fp16 51 us (3.8: uneven chunks, and the join).  Calls that do not fill the card are
+// 48 of 1 to 8192 tokens in fp16 47 us (4.2: uneven chunks, and the join).  Calls that do not fill the card are
 // bound by latency and by what one CU reads, about 45 GB/s, with four waves as with eight.
 #pragma once
 
