@@ -161,6 +161,16 @@ def test_paged_many_sequences(cuda, n):
     _check_paged(cuda, Cache(cuda, qvx.F16, lens, 16, 1, 64, seed=n), 2)
 
 
+@pytest.mark.parametrize("n,longest", [(60, 3000), (64, 200), (150, 2500)])
+@pytest.mark.parametrize("t", (qvx.F16, qvx.Q8_0))
+def test_paged_lengths_of_every_kind(cuda, t, n, longest):
+    """More chunks and rests than the card has places, of all lengths, in no order, empty sequences among them."""
+    r = np.random.default_rng(n)
+    lens = [int(x) for x in np.exp(r.uniform(0, np.log(longest), n))]
+    lens[n // 2], lens[n // 3], lens[7] = longest, 0, longest // 2 + 1
+    _check_paged(cuda, Cache(cuda, t, lens, 16, 8, 32, seed=n), 16)
+
+
 def test_paged_long_sequence(cuda):
     """Many chunks a sequence, several tiles a wave: lengths around 40000 tokens."""
     _check_paged(cuda, Cache(cuda, qvx.BF16, (40007, 39999), 64, 2, 64, seed=4), 4)
