@@ -130,8 +130,8 @@ __global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCall c, int write) {
 //
 // Pair i of a head is turned by pos[axis[i]] * inv_freq[i]; the angle's whole turns are taken off in
 // 64 bits (at position 10^6 an fp32 product is off by 0.06), the rest is an fp32 number of half turns.
-// One pass over q, k and v; the bytes bound it: 8192 tokens of 32 + 2 x 8 heads of 128 into a bf16 cache 77.7 us,
-// 4.7 TB/s where a copy of 2 GiB reaches 4.9; one token 3.5 us.  A workgroup takes `tokens_wg` tokens and a range of
+// One pass over q, k and v; the bytes bound it: 8192 tokens of 32 + 2 x 8 heads of 128 into a bf16 cache 70.7 us,
+// 5.2 TB/s where a copy of 2 GiB reaches 4.9; one token 3.5 us.  A workgroup takes `tokens_wg` tokens and a range of
 // their heads: its threads first form the cosines and sines of the tokens' pairs in LDS, each once, and
 // then take 8 values of a head at a time.
 
@@ -333,14 +333,15 @@ bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s) {
 
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s) {
   const int rows = c.q_heads + 2 * c.kv_heads, half = c.rot_dim / 2;
-  // Tokens a workgroup takes together: enough pairs for its threads.  Few tokens spread their heads
-  // over workgroups instead, until there are two of them a CU.
-  c.tokens_wg = std::max(1, std::min(kRopeMaxTokens, half ? kRopeThreads / half : kRopeMaxTokens));
+  // A workgroup takes one token, or several whose rows together occupy its threads once.  (As many as their pairs
+  // occupied it, four of 64 pairs: 8192 tokens 78.7 us against 71.5, 2048 29.4 against 19.2.)  Few tokens spread their
+  // heads over workgroups, until there are two of them a CU: 8 tokens 4.2 us, 12.5 with each on one.
+  const int units = c.head_dim / 8, least = std::max(1, kRopeThreads / units);  // rows that occupy the threads once
+  const int most = std::max(1, std::min(kRopeMaxTokens, half ? kRopeThreads / half : kRopeMaxTokens));
+  c.tokens_wg = std::max(1, std::min({most, kRopeThreads / (rows * units), c.n_tokens / 512}));
   c.rows_wg = rows;
-  if (c.n_tokens / c.tokens_wg < 512) {
-    c.tokens_wg = 1;
-    const int least = std::max(1, kRopeThreads / (c.head_dim / 8));  // rows that occupy the threads once
-    const int parts = std::max(1, std::min((rows + least - 1) / least, 512 / std::max(c.n_tokens, 1)));
+  if (c.n_tokens < 512) {
+    const int parts = std::max(1, std::min((rows + least - 1) / least, 512 / c.n_tokens));
     c.rows_wg = (rows + parts - 1) / parts;
   }
   const dim3 grid((unsigned)((c.n_tokens + c.tokens_wg - 1) / c.tokens_wg), (unsigned)((rows + c.rows_wg - 1) / c.rows_wg));
