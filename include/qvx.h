@@ -334,7 +334,7 @@ typedef struct qvx_kv_states {
  * d_offsets NULL: n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  Rows behind the last
  * sequence's are left as they were.  q and out share q_type: F32, F16 or BF16, rows and heads as in
  * qvx_attn_paged.  Where q and the states share a 16-bit type, the rows of a sequence and head (queries times heads
- * a group) are 32 or more in the mean, scale is at least 1e-30 and the row stride at most 16 Mi bytes, both
+ * a group) are more than 16 in the mean, scale is at least 1e-30 and the row stride at most 16 Mi bytes, both
  * products run on the 16-bit matrix cores and the softmax weights are rounded to that type (sums
  * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout.  d_ws as there. */
 int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,

@@ -64,11 +64,13 @@ int check_cache(const qvx_kv_cache* c, int64_t* stride) {
 
 // The partition of a call whose heads, pages and sequences are filled in: how many work items are
 // aimed at, and the bounds that grid and workspace are sized by.  Workgroups to fill the chip: two a CU.
-// A chunk has at least 8 tiles (128 keys), two a wave: shorter ones are all launch and join.
+// A chunk has at least 8 tiles (128 keys), two a wave: 2048 tokens of 8 heads of 128 11.3 us, with 4 tiles 12.0 and with 16
+// 12.3; 8192 tokens 16.2, 17.7 and 16.1.
 constexpr int kAttnWgs = 512, kMinChunk = 8;
 
 // Rows of a row tile for sequences of `rows` rows.  Up to four rows run on a matrix instruction that computes
-// four, a quarter the time of sixteen; up to eight on two of those.
+// four, a quarter the time of sixteen; up to eight on two of those: 2048 tokens, 4 heads a group, 11.2 us against 12.7 as 16
+// rows, 8 heads 12.9 against 13.3.
 int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
 // The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
@@ -151,7 +153,9 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
 
 // wide: the call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a 16-bit type, the scale is
 // positive (the kernel takes the largest product for the largest logit, and -inf times the scale for a masked one),
-// sequences have 32 rows or more in the mean, and its tiles of 64 states stay inside 32-bit offsets.
+// sequences have more than 16 rows in the mean, and its tiles of 64 states stay inside 32-bit offsets.  20 heads of 64 on
+// 1500 states, one sequence and eight, there against the split kernel: 16 queries 12.0 and 20.1 us against 12.9 and 19.4, 24
+// 12.3 and 20.3 against 14.8 and 29.2, 128 16.2 and 31.6 against 19.3 and 59.3.
 int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, float scale,
                 AttnCall& c, bool* wide, bool* join, size_t* ws_bytes) {
   if (!st) return QVX_E_NULL;
@@ -191,7 +195,7 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
   if ((int64_t)n_q * c.group > 0x7fffff00ll) return QVX_E_RANGE;
   *wide = q_type == st->type && q_type != T_F32 && scale >= kLeastScale && c.pitch <= kMaxPitch / 4 &&
-          (int64_t)n_q * c.group >= 32 * (int64_t)n_seqs;
+          (int64_t)n_q * c.group > 16 * (int64_t)n_seqs;
   c.tile_rows = *wide ? kAttnRows16 : tile_rows(ragged ? rows / n_seqs : rows);  // ragged: of a sequence in the mean
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);

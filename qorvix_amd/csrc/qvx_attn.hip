@@ -19,6 +19,7 @@ namespace {
 // chunks' loads at a time; then the groups meet in LDS.  Latency bounds it: three dependent loads
 // (piece, partial results, store): 4.3 us for a hundred pieces, 6.0 for 512 of one sequence, 4.8 where there are none.
 // The order of the sums is the same in every run.
+// One row at a time throughout took 2048 tokens from 11.3 to 12.0 us, rows together throughout 65536 from 54.4 to 58.0.
 constexpr int kFewChunks = 16;
 
 template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
