@@ -112,13 +112,19 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   return plan_items(c, row_tiles, join, ws_bytes);
 }
 
-// The 16-bit kernel's: row tiles of 128 rows.  They are split only where they are fewer than two workgroups a CU,
-// into chunks of 256 keys at least: 64 queries on 1500 states, 20 heads of 64, 26.3 -> 13.4 us.
+// The 16-bit kernel's: row tiles of 128 rows.  Partial results of so many rows are dear, so they are split only where they
+// leave half the CUs idle or more and the states are the longer the more of them there are; into chunks of 256 keys at
+// least, one a CU (two, where row tiles are half empty in the mean).  Head size 64 and 128, whole against split: 8 row tiles on 800 states 15.8 and 22.5 us against 13.2 and
+// 17.0, on 300 9.4 and 12.9 against 12.8 and 17.7; 64 on 1500 25.4 and 37.9 against 18.9 and 25.2, on 700 14.7 and 21.5 against
+// 16.9 and 23.1; 192 on 4000 59.0 and 88.1 against 54.8 and 94.4.  Chunks for two workgroups a CU: 32 on 4000 27.6 and 35.1
+// against 21.8 and 28.5; but 4 sequences of 32 rows on 1500, 20 heads of 64, 15.5 against 17.3.
 bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   c.tile_rows = kAttnRows16;
-  const bool split = row_tiles * c.kv_heads < kAttnWgs;
+  const int64_t whole = row_tiles * c.kv_heads;
+  const bool split = whole < kAttnWgs / 2 && most_tiles(c) > 40 + whole / 2;
   c.min_chunk = split ? 16 : 0;
-  c.target = std::max(1, kAttnWgs / c.kv_heads);
+  const bool sparse = 2 * (int64_t)c.n_q * c.group <= kAttnRows16 * row_tiles;
+  c.target = std::max(1, (sparse ? kAttnWgs : kAttnWgs / 2) / c.kv_heads);
   return plan_items(c, row_tiles, join, ws_bytes);
 }
 

@@ -21,6 +21,8 @@ namespace {
 // The order of the sums is the same in every run.
 // One row at a time throughout took 2048 tokens from 11.3 to 12.0 us, rows together throughout 65536 from 54.4 to 58.0.
 constexpr int kFewChunks = 16;
+constexpr int kJoinShares = 4;  // workgroups a piece of 128 rows: with one 32 row tiles on 700 states 26.4 us against 21.1, with 8 20.0,
+                                // but on 4000 then 44.3 against 35.9
 
 template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
   __shared__ __attribute__((aligned(16))) float4 vals[256];
@@ -40,7 +42,8 @@ template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) 
   const int wide = few ? min(R, 256 / quads) : 1;  // rows at a time
   const int groups = 256 / (quads * wide), mine = tid / (quads * wide), rest = tid - mine * quads * wide;
   const int row = rest / quads, quad = rest - row * quads;
-  for (int r0 = pc.chunk * wide; r0 < nrow; r0 += pc.chunks * wide) {
+  const int share = pc.chunk * (int)gridDim.z + (int)blockIdx.z, shares = pc.chunks * (int)gridDim.z;
+  for (int r0 = share * wide; r0 < nrow; r0 += shares * wide) {
     const int r = r0 + row;
     float m = -INFINITY, l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -121,7 +124,7 @@ void launch_attn_join(const AttnCall& c, hipStream_t s) {
     case 4: k_attn_join<4><<<grid, 256, 0, s>>>(c); break;
     case 8: k_attn_join<8><<<grid, 256, 0, s>>>(c); break;
     case 16: k_attn_join<16><<<grid, 256, 0, s>>>(c); break;
-    default: k_attn_join<kAttnRows16><<<grid, 256, 0, s>>>(c); break;
+    default: k_attn_join<kAttnRows16><<<dim3(grid.x, grid.y, kJoinShares), 256, 0, s>>>(c); break;
   }
 }
 
