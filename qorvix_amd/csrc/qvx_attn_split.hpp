@@ -435,8 +435,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, voff[u] + r * c.pitch);
   };
   // Tiles in registers, one in work and one on its way where they fit: 131071 tokens in bf16 103 us against 111 with one.
-  // For eight rows of 128 values they fit over Q8_0 alone, less six registers (64 x 4096 tokens 139 us against 145).
-  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && DT >= (kGroup ? 256 : 128)) ? 2 : 1;
+  // For eight rows of 128 values they do but for 1 to 22 registers (32 x 2000 tokens in bf16, 7 heads of 80 a group, 45 us
+  // against 77; 64 x 4096 in Q8_0 139 against 145), but not fp32 (8 heads of 128 a group 175 against 128) or 256 values.
+  constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && (DT == 256 || (DT == 128 && T == T_F32))) ? 2 : 1;
   Tile held[kHeld];
   AttnQuery<T, KS> q;
   float mul = 1.0f;
@@ -616,6 +617,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
           __builtin_amdgcn_sched_barrier(0);  // the loads go out before the tile in work is waited for
         } else if (n) {
           load.template operator()<AUX>(held[0], n);
+          // Both loads before the first product: the compiler would have the values' wait behind it (fp32, 32 x 2000
+          // tokens, heads of 256: 405 us against 263).
+          __builtin_amdgcn_sched_barrier(0);
         }
         step(held[i]);
       }
