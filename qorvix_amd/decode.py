@@ -525,14 +525,29 @@ class PagedDecodeStep:
         import torch
         from . import KvCache, Rope, attn_paged_ws, kv_page_bytes
         l0 = model.layers[0]
+        if any(k not in l0 for k in ("wo", "ffn_gateup")):
+            raise ValueError("PagedDecodeStep needs a Model.fused_ops() model")
         d, width = l0["wo"].rows, l0["wo"].cols
-        if width % heads or heads % kv_heads or l0["wv"].rows != width // heads * kv_heads:
+        if min(m, heads, kv_heads, n_pages, max_pages, page_size) < 1:
+            raise ValueError("PagedDecodeStep: sequences, heads and pages are at least one")
+        if width % heads or heads % kv_heads:
             raise ValueError("PagedDecodeStep: the projections do not fit the heads")
+        # one set of buffers serves every layer, so every layer has to have their sizes
+        kv, ffn = width // heads * kv_heads, l0["ffn_gateup"].rows // 2
+        sizes = {"wqk": (width + kv, d), "wv": (kv, d), "wo": (d, width), "ffn_gateup": (2 * ffn, d),
+                 "ffn_down": (d, ffn)}
         for l, layer in enumerate(model.layers):
-            if any(k not in layer for k in ("wqk", "wv", "wo", "ffn_gateup", "ffn_down")):
+            if any(k not in layer for k in sizes):
                 raise ValueError("PagedDecodeStep needs a Model.fused_ops() model with q and k stacked")
-            if any(model.norms[l].get(k) is None for k in ("attn_norm", "ffn_norm")):
-                raise ValueError(f"PagedDecodeStep needs the norms of layer {l}; the model lacks some")
+            for k, size in sizes.items():
+                if (layer[k].rows, layer[k].cols) != size:
+                    raise ValueError(f"PagedDecodeStep: {k} of layer {l} is {layer[k].rows} x {layer[k].cols}, "
+                                     f"not {size[0]} x {size[1]}")
+            norms = model.norms[l] if l < len(model.norms) else {}
+            if any(norms.get(k) is None or norms[k].numel() != d for k in ("attn_norm", "ffn_norm")):
+                raise ValueError(f"PagedDecodeStep needs the norms of layer {l}, of {d} values; the model lacks some")
+        if model.lm_head is not None and model.lm_head.cols != d:
+            raise ValueError(f"PagedDecodeStep: the LM head takes {model.lm_head.cols} values, the layers give {d}")
         self.model, self.m, self.heads, self.kv_heads, self.page_size = model, m, heads, kv_heads, page_size
         self.head_dim = hd = width // heads
         size = kv_page_bytes(cache_type, kv_heads, page_size, hd)

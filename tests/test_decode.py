@@ -101,3 +101,55 @@ def test_fused_step_refuses_a_model_without_norms():
     m.lm_head = object()
     with pytest.raises(ValueError, match="output_norm"):
         decode.FusedDecodeStep(m, 1)
+
+
+def _paged_model(layers=2, d=512, heads=8, kv_heads=2, hd=64, ffn=1024, vocab=256):
+    """A Model.fused_ops() model of the given sizes without any weights: the checks read the sizes alone."""
+    import torch
+    w = lambda t, rows, cols: decode.DevWeight(None, t, rows, cols)  # noqa: E731
+    m = decode.Model(lm_head=w(qvx.Q6_K, vocab, d), output_norm=torch.ones(d))
+    for _ in range(layers):
+        m.layers.append({"wqk": w(qvx.Q4_K, (heads + kv_heads) * hd, d), "wv": w(qvx.Q6_K, kv_heads * hd, d),
+                         "wo": w(qvx.Q4_K, d, heads * hd), "ffn_gateup": w(qvx.Q4_K, 2 * ffn, d),
+                         "ffn_down": w(qvx.Q6_K, d, ffn)})
+        m.norms.append({"attn_norm": torch.ones(d), "ffn_norm": torch.ones(d)})
+    return m
+
+
+def _paged_step(model, **kw):
+    a = dict(m=1, heads=8, kv_heads=2, n_pages=4, max_pages=2, device="meta")
+    a.update(kw)
+    return decode.PagedDecodeStep(model, **a)
+
+
+def test_paged_step_refuses_projections_that_do_not_fit():
+    """The step's buffers are sized once: a projection of any layer that would write or read past them, or whose heads
+    are not where the rotation looks for them, is refused before anything is allocated."""
+    import pytest
+
+    with pytest.raises(ValueError, match="KvCache.of"):  # the sizes fit: it comes as far as the device's memory
+        _paged_step(_paged_model())
+    for layer in (0, 1):
+        for key, rows, cols in (("wqk", 8 * 64, 512), ("wqk", 11 * 64, 512), ("wqk", 10 * 64, 256), ("wv", 4 * 64, 512),
+                                ("wv", 2 * 64, 768), ("wo", 768, 512), ("wo", 512, 768), ("ffn_gateup", 4096, 512),
+                                ("ffn_gateup", 2048, 768), ("ffn_down", 512, 2048), ("ffn_down", 768, 1024)):
+            m = _paged_model()
+            m.layers[layer][key] = decode.DevWeight(None, m.layers[layer][key].type, rows, cols)
+            with pytest.raises(ValueError, match="PagedDecodeStep"):
+                _paged_step(m)
+        m = _paged_model()
+        m.norms[layer]["attn_norm"] = m.norms[layer]["attn_norm"][:256]
+        with pytest.raises(ValueError, match="PagedDecodeStep"):
+            _paged_step(m)
+    m = _paged_model()
+    m.lm_head = decode.DevWeight(None, qvx.Q6_K, 256, 768)
+    with pytest.raises(ValueError, match="PagedDecodeStep"):
+        _paged_step(m)
+    m = _paged_model()
+    m.norms.pop()
+    with pytest.raises(ValueError, match="norms of layer 1"):
+        _paged_step(m)
+    for kw in (dict(m=0), dict(heads=0), dict(kv_heads=0), dict(kv_heads=-2), dict(n_pages=0), dict(max_pages=0),
+               dict(page_size=0)):
+        with pytest.raises(ValueError, match="PagedDecodeStep"):
+            _paged_step(_paged_model(), **kw)
