@@ -548,6 +548,8 @@ class PagedDecodeStep:
                 raise ValueError(f"PagedDecodeStep needs the norms of layer {l}, of {d} values; the model lacks some")
         if model.lm_head is not None and model.lm_head.cols != d:
             raise ValueError(f"PagedDecodeStep: the LM head takes {model.lm_head.cols} values, the layers give {d}")
+        if model.lm_head is not None and (model.output_norm is None or model.output_norm.numel() != d):
+            raise ValueError(f"PagedDecodeStep needs output_norm, of {d} values, for the LM head")
         self.model, self.m, self.heads, self.kv_heads, self.page_size = model, m, heads, kv_heads, page_size
         self.head_dim = hd = width // heads
         size = kv_page_bytes(cache_type, kv_heads, page_size, hd)

@@ -153,3 +153,13 @@ def test_paged_step_refuses_projections_that_do_not_fit():
                dict(page_size=0)):
         with pytest.raises(ValueError, match="PagedDecodeStep"):
             _paged_step(_paged_model(), **kw)
+
+
+def test_paged_step_refuses_a_head_without_its_norm():
+    import pytest
+
+    for norm in (None, "short"):
+        m = _paged_model()
+        m.output_norm = None if norm is None else m.output_norm[:256]
+        with pytest.raises(ValueError, match="output_norm"):
+            _paged_step(m)
