@@ -281,6 +281,8 @@ class KvCache(C.Structure):
         need = kv_page_bytes(ggml_type, kv_heads, page_size, head_dim)
         strides = []
         for x in (k, v):
+            if x.shape[0] > 1 and x.stride(0) * x.element_size() < need:
+                raise ValueError("KvCache.of: pages overlap")
             held = x.element_size() * (x.numel() // max(x.shape[0], 1))
             inner = x[0] if x.shape[0] else x
             if need == 0 or held < need or not inner.is_contiguous() or not x.is_cuda:

@@ -205,3 +205,13 @@ def test_structures_match_the_header():
         cls = names[name]
         assert C.sizeof(cls) == int(size)
         assert [getattr(cls, f[0]).offset for f in cls._fields_] == [int(o) for o in offsets]
+
+
+def test_cache_pages_that_overlap_are_refused():
+    """An expanded page has a stride of 0, which a description reads as pages side by side: past the one that there is."""
+    import torch
+    size = qvx.kv_page_bytes(qvx.F16, 2, 16, 64)
+    one = torch.zeros((1, size), dtype=torch.uint8)
+    for pages in (one.expand(4, size), torch.zeros(4 * size, dtype=torch.uint8).as_strided((4, size), (16, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            qvx.KvCache.of(pages, pages, qvx.F16, 16, 2, 64)
