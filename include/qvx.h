@@ -305,7 +305,7 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
  * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and
  * out_stride elements apart; out may be q (the same stride), else they do not overlap.  Long sequences are split over workgroups and joined in a
  * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
- * 0 .. table_width * page_size; tokens on page ids outside the cache do not count; a row without any key gets
+ * 0 .. table_width * page_size (at most 2^31 - 16, on pages of one token 2^30 - 1; more -> QVX_E_RANGE); tokens on page ids outside the cache do not count; a row without any key gets
  * zeros; rows of the cache behind a sequence's last token are not read.  Keys are finite: an infinite one of a 16-bit
  * cache makes its rows NaN, as NaN does.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less ->
  * QVX_E_RANGE; its contents need not be kept or cleared). */
@@ -316,8 +316,8 @@ int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q
 size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width);
 
 /* An encoder's keys and values: value i of head h of state j of sequence b at d_k[b * batch_stride +
- * j * row_stride + h * head_stride + i] (elements; d_v alike), F32, F16 or BF16, max_len states a sequence at most.
- * Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and at most 64 Mi bytes; with
+ * j * row_stride + h * head_stride + i] (elements; d_v alike), F32, F16 or BF16, max_len states a sequence at most
+ * (up to 2^31 - 16).  Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and at most 64 Mi bytes; with
  * max_len 0 the addresses may be NULL.  head_dim: a multiple of 8
  * up to 256. */
 typedef struct qvx_kv_states {

@@ -18,6 +18,8 @@ using namespace qvx;
 namespace {
 
 constexpr int kAttnMaxSeqs = 65536, kMapMaxSeqs = 16384;
+constexpr int kMaxLen = 0x7ffffff0;  // the kernels round lengths up to whole tiles
+constexpr int kMaxTiles = 0x3fffffff;  // and add a chunk's first tile and length, each at most this
 constexpr int64_t kMaxPitch = 64ll << 20;  // sixteen rows stay far inside 32-bit offsets
 constexpr float kLeastScale = 1e-30f;       // far above the subnormal numbers
 
@@ -84,7 +86,7 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   *join = c.min_chunk && tiles > c.min_chunk;
   const int64_t most = *join ? (tiles + c.min_chunk - 1) / c.min_chunk : 1;  // chunks of a row tile
   const int64_t items = std::min(row_tiles + c.target, row_tiles * most);
-  if (items * c.kv_heads > 0x7fffffffll || tiles > 0x7fffffffll) return false;
+  if (items * c.kv_heads > 0x7fffffffll || tiles > kMaxTiles) return false;
   if (!*join) c.min_chunk = 0x7ffffff0;
   c.items = (int)items;
   c.most_tiles = (int)tiles;
@@ -133,7 +135,7 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   if (n_seqs <= 0) return QVX_E_NVEC;
   if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
   if (q_heads <= 0 || q_heads % cache->kv_heads || table_width <= 0) return QVX_E_SHAPE;
-  if (n_seqs > kAttnMaxSeqs || cache->kv_heads > 65535 || (int64_t)table_width * cache->page_size > 0x7fffffffll)
+  if (n_seqs > kAttnMaxSeqs || cache->kv_heads > 65535 || (int64_t)table_width * cache->page_size > kMaxLen)
     return QVX_E_RANGE;
   const int d = cache->head_dim;
   c.k = static_cast<const uint8_t*>(cache->d_k);
@@ -175,7 +177,7 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
     return QVX_E_SHAPE;
   const int64_t es = value_bytes(st->type, 1);
   constexpr int64_t kMost = 1ll << 56;
-  if (n_seqs > kAttnMaxSeqs || st->kv_heads > 65535 || st->batch_stride > kMost || st->head_stride > kMost ||
+  if (n_seqs > kAttnMaxSeqs || st->max_len > kMaxLen || st->kv_heads > 65535 || st->batch_stride > kMost || st->head_stride > kMost ||
       st->row_stride > kMaxPitch / es || (st->row_stride * es) % 16 || (st->batch_stride * es) % 16 ||
       (st->head_stride * es) % 16)
     return QVX_E_RANGE;

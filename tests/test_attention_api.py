@@ -215,3 +215,17 @@ def test_cache_pages_that_overlap_are_refused():
     for pages in (one.expand(4, size), torch.zeros(4 * size, dtype=torch.uint8).as_strided((4, size), (16, 1))):
         with pytest.raises(ValueError, match="overlap"):
             qvx.KvCache.of(pages, pages, qvx.F16, 16, 2, 64)
+
+
+def test_lengths_whose_tiles_pass_31_bits_are_refused():
+    """A length is rounded up to whole tiles of 16 keys, and a chunk's first tile and length are added, in 32 bits."""
+    for n in (0x7ffffff1, 0x7fffffff):
+        long = states(max_len=n, batch_stride=1 << 40)
+        assert cross(long) == qvx.E_RANGE and qvx.attn_cross_ws(long, qvx.F32, 4, 6, 3) == 0
+        one = cache(n_pages=1, page_size=n)
+        assert paged(one, width=1, ws_bytes=1 << 40) == qvx.E_RANGE and qvx.attn_paged_ws(one, 4, 3, 1) == 0
+    assert qvx.attn_cross_ws(states(max_len=0x7ffffff0, batch_stride=1 << 40), qvx.F32, 4, 6, 3) > 0
+    assert qvx.attn_paged_ws(cache(n_pages=1, page_size=0x7ffffff0), 4, 3, 1) > 0
+    small = cache(n_pages=0x7fffffff, page_size=1)
+    assert paged(small, width=0x7fffffff, ws_bytes=1 << 40) == qvx.E_RANGE
+    assert qvx.attn_paged_ws(small, 4, 1, 0x40000000) == 0 and qvx.attn_paged_ws(small, 4, 1, 0x3fffffff) > 0
