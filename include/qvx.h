@@ -223,7 +223,8 @@ int qvx_interleave_rows16(void* d_dst, const void* d_a, const void* d_b, uint32_
  * and a decoder's attention to an encoder's states.  Activations are fp32, softmax statistics and sums
  * at least that.  All four calls are asynchronous on `stream`, allocate nothing and keep nothing between
  * calls, so they can be captured into a graph and replayed while the device data they read changes;
- * calls that may overlap need workspaces of their own (two graphs too).  Row lengths, page ids, slots
+ * calls that may overlap need workspaces of their own (two graphs too).  Sizes whose launch would pass 2^24 - 1 workgroups
+ * (sequences, row tiles and chunks times key heads) -> QVX_E_RANGE.  Row lengths, page ids, slots
  * and positions are read on the device and checked there: what lies outside is left out as described,
  * never read or written. */
 
@@ -292,7 +293,8 @@ typedef struct qvx_rope {
  * (elements; likewise q_out, k, v), so parts of one stacked product can be passed.  d_pos [n_axes]
  * [pos_stride] int32; angles are formed in 64 bits.  A token whose slot is negative or past the cache
  * is padding: none of its rows is written, q_out's neither.  q_out may be q itself (the same stride);
- * slots of one call are distinct, else which token's values a row holds is not specified.
+ * slots of one call are distinct, else which token's values a row holds is not specified.  At most
+ * 134217720 tokens a call (more -> QVX_E_RANGE).
  * cache NULL: q alone is rotated (d_k, d_v, d_slots are not read), as an image encoder's q and k. */
 int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t q_stride, int q_heads,
                 const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens, int head_dim,

@@ -86,7 +86,7 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   *join = c.min_chunk && tiles > c.min_chunk;
   const int64_t most = *join ? (tiles + c.min_chunk - 1) / c.min_chunk : 1;  // chunks of a row tile
   const int64_t items = std::min(row_tiles + c.target, row_tiles * most);
-  if (items * c.kv_heads > 0x7fffffffll || tiles > kMaxTiles) return false;
+  if (items * c.kv_heads > kMostWgs || tiles > kMaxTiles) return false;
   if (!*join) c.min_chunk = 0x7ffffff0;
   c.items = (int)items;
   c.most_tiles = (int)tiles;
@@ -279,7 +279,8 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
   if (q_stride < 0 || q_out_stride < q_row || (cache && (k_stride < 0 || v_stride < 0)) || pos_stride < 0 ||
       (rope->n_axes > 1 && pos_stride < n_tokens))
     return QVX_E_SHAPE;
-  if (q_row > 0x7fffffffll / 16 || kv_row > 0x7fffffffll / 16) return QVX_E_RANGE;
+  if (q_row > 0x7fffffffll / 16 || kv_row > 0x7fffffffll / 16 || n_tokens > kRopeMaxTokens * kMostWgs)
+    return QVX_E_RANGE;
   if ((q_heads && (!d_q || !d_q_out)) || (cache && (!d_k || !d_v || !d_slots)) ||
       (rope->rot_dim && (!rope->d_inv_freq || !d_pos)))
     return QVX_E_NULL;

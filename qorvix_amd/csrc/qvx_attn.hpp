@@ -14,6 +14,7 @@ namespace qvx {
 
 constexpr int kAttnTile = 16;   // keys of a tile
 constexpr int kAttnRows16 = 128;  // query rows of a workgroup of the 16-bit kernel
+constexpr int kMostWgs = (1 << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32 of them
 constexpr int kAttnWaves = 4;   // waves of a workgroup of the split kernel
 constexpr float kAttnLow = -3.4028235e38f;  // stands for the maximum of keys that are all at -inf; -inf: of no keys
 

@@ -339,6 +339,7 @@ void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s) {
   const int units = c.head_dim / 8, least = std::max(1, kRopeThreads / units);  // rows that occupy the threads once
   const int most = std::max(1, std::min(kRopeMaxTokens, half ? kRopeThreads / half : kRopeMaxTokens));
   c.tokens_wg = std::max(1, std::min({most, kRopeThreads / (rows * units), c.n_tokens / 512}));
+  c.tokens_wg = std::max(c.tokens_wg, (c.n_tokens + kMostWgs - 1) / kMostWgs);  // at most kRopeMaxTokens: checked
   c.rows_wg = rows;
   if (c.n_tokens < 512) {
     const int parts = std::max(1, std::min((rows + least - 1) / least, 512 / c.n_tokens));

@@ -10,7 +10,7 @@
 namespace qvx {
 
 enum { kMapTokens = 1, kMapSeqs = 2 };
-constexpr int kRopeMaxPairs = 128, kRopeMaxTokens = 8;
+constexpr int kRopeMaxPairs = 128, kRopeMaxTokens = 8;  // of a workgroup's table of cosines and sines
 
 struct MapCall {
   const int32_t *held, *added;

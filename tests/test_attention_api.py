@@ -229,3 +229,14 @@ def test_lengths_whose_tiles_pass_31_bits_are_refused():
     small = cache(n_pages=0x7fffffff, page_size=1)
     assert paged(small, width=0x7fffffff, ws_bytes=1 << 40) == qvx.E_RANGE
     assert qvx.attn_paged_ws(small, 4, 1, 0x40000000) == 0 and qvx.attn_paged_ws(small, 4, 1, 0x3fffffff) > 0
+
+
+def test_launches_past_32_bits_of_threads_are_refused():
+    """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256."""
+    many = cache(kv_heads=256)
+    assert paged(many, heads=256, out_stride=256 * 64, q_stride=256 * 64, n=65536, ws_bytes=1 << 40) == qvx.E_RANGE
+    assert paged(cache(kv_heads=255), heads=256 * 255, n=65536, ws_bytes=1 << 40) == qvx.E_RANGE  # row tiles count too
+    wide = states(kv_heads=256, row_stride=256 * 64, batch_stride=0)
+    assert cross(wide, heads=256, out_stride=256 * 64, q_stride=256 * 64, n_q=65536, n=65536) == qvx.E_RANGE
+    for c in (True, None):
+        assert rope(c=c, n=8 * 0xffffff + 1, ps=1 << 28) == qvx.E_RANGE
