@@ -192,8 +192,11 @@ __device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_ex
 // values a lane for eight 16x16x4 instructions a piece.  Otherwise 16-bit parts that add up to the fp32
 // value, each multiplied by the keys in its own 16x16x32 instruction: fp16 twice (11 + 11 bits), bf16
 // three times (8 + 8 + 8); products of 16-bit values are exact in the instruction's fp32 sums.  The
-// row is first brought to a largest magnitude of 2^14 (a power of two, undone in the exponent), so
-// that no part overflows fp16 and the small part of every value that matters stays normal.
+// row is first multiplied by a power of two, undone in the exponent.  For fp16 (and Q8_0's integers) to a largest
+// magnitude of 2^14, so that no part overflows and the small part of every value that matters stays normal.  bf16
+// keys reach as far as fp32: there rows below 2^-10 are brought to that, where 256 products with keys of any size stay
+// below 2^127 and the small parts far above 2^-126, and rows above 2^60 to that, where no part rounds to infinity and
+// products that matter to a logit stay normal; those between are as they are, and their sums as large as their logits.
 template <uint32_t T, int KS> struct AttnQuery {
   typedef _Float16 Key __attribute__((ext_vector_type(8)));
   Key hi[KS], lo[KS];
@@ -477,9 +480,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
 #pragma unroll
       for (int o = kGroup ? R : 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
-      // 2^e <= top < 2^(e + 1) to 2^14; a row with an infinite value as it is
+      // 2^e <= top < 2^(e + 1) to 2^14, for bf16 into 2^-10 .. 2^60; a row with an infinite value as it is
       const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-      const int up = e < 128 ? 14 - e : 0;
+      const int up = e == 128 ? 0 : (T == T_BF16 ? min(max(e, -10), 60) : 14) - e;
       mul = __builtin_ldexpf(1.0f, -up);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
