@@ -309,7 +309,7 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
  * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
  * 0 .. table_width * page_size (at most 2^31 - 16, on pages of one token 2^30 - 1; more -> QVX_E_RANGE); tokens on page ids outside the cache do not count; a row without any key gets
  * zeros; rows of the cache behind a sequence's last token are not read.  Keys are finite: an infinite one of a 16-bit
- * cache makes its rows NaN, as NaN does.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less ->
+ * cache makes its rows NaN, as NaN does.  Values times the number of keys stay below fp32's largest number.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less ->
  * QVX_E_RANGE; its contents need not be kept or cleared). */
 int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q_stride, int q_heads,
                    const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens,

@@ -7,9 +7,9 @@
 //
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction, fp32 sums.  The weights are
 // rounded to the operands' type (to the nearest) before the second product: each by at most half a
-// step; the denominator sums them in fp32.  The reference m follows the largest logit
-// lazily, as in qvx_attn_split.hpp, at most 2^kSlack16 behind.  In fp16 all weights are 2^kUp16 larger than that:
-// up to 2^15 they stay in range, and down to 2^-21 of the largest above its smallest normal number.
+// step; the denominator sums them in fp32.  The reference m follows the largest logit lazily, as in
+// qvx_attn_split.hpp, kSlack16 above it when it is set, so bf16 weights lie at 2^-kSlack16 to 1.  In fp16 all weights are
+// 2^kUp16 larger than that: up to 2^15 they stay in range, and down to 2^-21 of the largest above its smallest normal number.
 //
 // Layout.  In S^T a lane holds query row lane % 32 and, with h = lane / 32, the keys 8 (r / 4) + 4 h + r % 4
 // in registers r = 0 .. 15.  The second product's right operand wants, for 16 keys, eight of them in
@@ -39,7 +39,7 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRows16 = kAttnRows16;
 constexpr float kSlack16 = 8.0f;
-template <uint32_t T> constexpr float kUp16 = T == T_F16 ? 7.0f : 0.0f;
+template <uint32_t T> constexpr float kUp16 = T == T_F16 ? 15.0f : 0.0f;
 
 typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
 
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top *= c.scale2;  // scale2 >= 0: the order stays
-    if (__any(top > m + kSlack16)) {
-      const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    if (__any(top > m)) {
+      const float both = fmaxf(top, __shfl_xor(top, 32)), now = both > m ? both + kSlack16 : m;
       const float f = m == now ? 1.0f : attn_pow2(m - now);
       m = now;
       l *= f;

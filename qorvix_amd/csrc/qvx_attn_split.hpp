@@ -16,10 +16,11 @@
 // product to the next in place, without a lane exchange or LDS, when the values of key 4 g + r are
 // loaded by the lanes of group g: 16 lanes cover a token's values in consecutive pieces.
 //
-// The reference m.  A row's weights may use any common m; m moves only when a logit exceeds it by
-// more than 2^kSlack, which after the first tiles is rare, so a step costs a compare and a wave vote
-// instead of a lane reduction and a rescale.  Weights reach at most 2^kSlack, sums of 2^20 of them
-// 2^40: far from fp32's range, and the relative error of each stays that of fp32.
+// The reference m.  A row's weights may use any common m.  It stands kSlack above the row's largest logit (in powers of
+// two) when it is set, and is set again only when a logit passes it, which after the first tiles is rare, so a step costs
+// a compare and a wave vote instead of a lane reduction and a rescale.  Weights are therefore never above 1 and the row's
+// largest never below 2^-kSlack: their sums stay finite for values of up to fp32's largest number over the number of keys,
+// and weights of 2^-100 of the largest are still normal numbers; the relative error of each stays that of fp32.
 //
 // Split.  A work item is a chunk of a sequence's tiles (qvx_attn.hpp); its four waves take tiles in
 // turn and join through LDS.  Items of a sequence that has several leave their sums, their maxima
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
         if (lane >> 2 >= x.live) p[t] = -INFINITY;
         top[t] = p[t] * muls[t];
-        past |= top[t] > m[t] + kSlack;  // m + slack is -inf at the start: any finite logit moves it
+        past |= top[t] > m[t];  // m is -inf at the start: any finite logit moves it
       }
       if (__any(past)) {
 #pragma unroll
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
           float now = top[t];
 #pragma unroll
           for (int s = 4; s < 64; s *= 2) now = fmaxf(now, __shfl_xor(now, s));
-          now = fmaxf(m[t], now);
+          now = now > m[t] ? now + kSlack : m[t];
           const float f = m[t] == now ? 1.0f : attn_pow2(m[t] - now);
           m[t] = now;
           l[t] *= f;
@@ -574,10 +575,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int r = 0; r < 4; ++r) sc[r] = 4 * g + r >= x.live ? -INFINITY : sc[r];
       const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
-      if (__any(top > m[0] + kSlack)) {
+      if (__any(top > m[0])) {
         float t = fmaxf(top, __shfl_xor(top, 16));
         t = fmaxf(t, __shfl_xor(t, 32));
-        const float now = fmaxf(m[0], t);
+        const float now = t > m[0] ? t + kSlack : m[0];
         const float f = m[0] == now ? 1.0f : attn_pow2(m[0] - now);
         m[0] = now;
         l[0] *= f;

@@ -1,9 +1,12 @@
-"""The attention calls at the ends of fp32's and bf16's range: keys and queries of far exponents whose logits are ordinary.
+"""The attention calls at the ends of fp32's and bf16's range: keys and queries of far exponents whose logits are
+ordinary, and values so large that only weights of at most 1 keep their sums finite.
 
 Tolerances as in test_gpu_attention.py: powers of two move nothing but the exponents.  A query below 2^-126 loses
 half of 2^-149 to its scale, which its key (2^123 at most) and d = 256 of them make 2^-19 of a logit: the (d + 3) u S of
 those tests is at least 2^-24 * 67 * 1 = 2^-17.9 for the sums S >= 1 here."""
 from __future__ import annotations
+
+import math
 
 import numpy as np
 import pytest
@@ -81,3 +84,39 @@ def test_cross_far_exponents(cuda, q_type, kv_type, rows):
     top = float(v.double().abs().max())
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= 2 * U * ((d + 3) * s + n + 8) * top + half * (np.abs(want) + top)).all()
+
+
+@pytest.mark.parametrize("t", (qvx.BF16, qvx.F32))
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 6, 16])
+def test_paged_large_values(cuda, t, d, group):
+    """Logits that rise by 2^19 behind the first tiles, values of 2^115: their products with weights above 1 overflow."""
+    torch = cuda
+    n = 150
+    c = Cache(torch, t, (n,), 16, 1, d, seed=d)
+    c.host[1] = np.ldexp(c.host[1], 115)
+    for p, o, j in _each_key(c):
+        c.host[0][p, :, o, 0] = 0.0 if j < 64 else 19.0
+    _upload(torch, c, 0)
+    _upload(torch, c, 1)
+    q = torch.zeros((1, group, d))
+    q[:, :, 0] = 1.0
+    _compare(torch, c, q, math.log(2.0))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_cross_large_values(cuda, d):
+    """As above on the 16-bit matrix cores: logits that rise by 2^7, values of 2^122."""
+    torch = cuda
+    n, rows = 200, 40
+    r = np.random.default_rng(d)
+    k = torch.zeros((1, n, 1, d), dtype=torch.bfloat16)
+    k[0, 64:, 0, 0] = 7.0
+    v = torch.from_numpy(np.ldexp(r.standard_normal((1, n, 1, d)), 122).astype(np.float32)).to(torch.bfloat16)
+    q = torch.zeros((rows, 1, d), dtype=torch.bfloat16)
+    q[:, 0, 0] = 1.0
+    got = qvx.attn_cross_t(q.cuda(), qvx.KvStates.of(k.cuda(), v.cuda()), scale=math.log(2.0)).cpu().double().numpy()[:, 0]
+    want, s = _attend(q.double().numpy()[:, 0], k.double().numpy()[0, :, 0], v.double().numpy()[0, :, 0], math.log(2.0))
+    top = float(v.double().abs().max())
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= 2 * U * ((d + 3) * s + n + 8) * top + 2.0 ** -8 * (np.abs(want) + top)).all()
