@@ -28,10 +28,10 @@ sequences that each get one token a step.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
-from . import (F16, F32, GEMM_F16, OK, Q4_K, Q6_K, QvxError, empty_weight, fill_normal_t, fill_synthetic_t, lib,
-               weight_bytes)
+from . import (F16, F32, GEMM_F16, OK, Q4_K, Q6_K, ROPE_HALVES, ROPE_PAIRS, QvxError, empty_weight, fill_normal_t,
+               fill_synthetic_t, lib, weight_bytes)
 
 
 @dataclass
@@ -99,6 +99,54 @@ NORM_EPS = 1e-5  # Llama-3 rms_norm_eps (the GGUF key llama.attention.layer_norm
 
 
 @dataclass
+class Rotation:
+    """How a model's q and k heads turn: pair i of the first ``dim`` values (None: all) by position *
+    base^(-2 i / dim) / (scaling * factors[i]), cosine and sine times ``magnitude``; ``pairing`` ROPE_HALVES
+    (ropeNeoxKernel, cuda_backend.cu:249-272) or ROPE_PAIRS.  A pairing or scaling of None stands for one that a file
+    leaves open, or that this rotation does not express: a step asks its caller for a Rotation then."""
+    base: float = 500000.0
+    pairing: int | None = ROPE_HALVES
+    dim: int | None = None
+    scaling: float | None = 1.0
+    factors: object = None  # tensor [dim / 2]
+    magnitude: float = 1.0
+
+    @staticmethod
+    def of_gguf(f, device="cuda") -> "Rotation":
+        """A file's rotation, by the format's public keys: <arch>.rope.freq_base, .dimension_count, .scaling.type and
+        .scaling.factor (or the older .scale_linear), and the divisors in rope_freqs.weight.  Files of the architecture
+        "llama" hold their q and k rows so that neighbours form a pair; for another architecture the file does not say."""
+        key = f.architecture + ".rope."
+        base, linear = f.get_f64(key + "freq_base"), f.get_f64(key + "scale_linear")
+        kind, factor = f.get_string(key + "scaling.type"), f.get_f64(key + "scaling.factor")
+        r = Rotation(base=10000.0 if base is None else base, dim=f.arch_u64("rope.dimension_count"),
+                     pairing=ROPE_PAIRS if f.architecture == "llama" else None)
+        if kind in (None, "none", "linear"):
+            r.scaling = 1.0 if kind == "none" else (factor if kind == "linear" else None) or linear or 1.0
+        else:
+            r.scaling = None
+        t = f.tensor("rope_freqs.weight")
+        if t is not None:
+            if t.type_raw != F32:
+                raise ValueError("rope_freqs.weight must be F32")
+            import torch
+            r.factors = f.upload("rope_freqs.weight", device).data.view(torch.float32)
+        return r
+
+    def frequencies(self, head_dim: int, device):
+        """The pairs' inverse frequencies in 64 bits."""
+        import torch
+        dim = head_dim if self.dim is None else self.dim
+        if self.pairing is None or self.scaling is None:
+            raise ValueError("the file does not say how its q and k rows pair, or scales positions in a way of its own: "
+                             "pass a Rotation")
+        if dim < 0 or dim > head_dim or dim % 8 or (self.factors is not None and tuple(self.factors.shape) != (dim // 2,)):
+            raise ValueError(f"Rotation: {dim} values of a head of {head_dim}, in eights, with a factor a pair")
+        freq = self.base ** (-torch.arange(dim // 2, dtype=torch.float64, device=device) * 2 / max(dim, 1)) / self.scaling
+        return freq if self.factors is None else freq / self.factors.to(freq)
+
+
+@dataclass
 class Model:
     """Synthetic Llama-3-8B Q4_K_M weights on the device (``layers[l][name]``, ``lm_head``) and the
     RMSNorm weights (``norms[l]`` = {"attn_norm", "ffn_norm"} fp32 [d], ``output_norm``)."""
@@ -109,12 +157,14 @@ class Model:
     norms: list = field(default_factory=list)
     output_norm: object = None
     eps: float = NORM_EPS
+    rotation: Rotation = field(default_factory=Rotation)
 
     def fused(self) -> "Model":
         """The same weights with each FUSED pair of a layer stacked into one device weight when the
         two share type and row length (the other projections are shared, not copied)."""
         import torch
-        m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps)
+        m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
+                  rotation=self.rotation)
         for layer in self.layers:
             out, used = {}, set()
             for name, (a, b) in FUSED:
@@ -134,7 +184,8 @@ class Model:
         the rest shared."""
         import torch
         from . import interleave_rows16_t
-        m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps)
+        m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
+                  rotation=self.rotation)
         for layer in self.layers:
             out = {k: w for k, w in layer.items() if k not in ("wq", "wk", "ffn_gate", "ffn_up")}
             wq, wk, wg, wu = layer["wq"], layer["wk"], layer["ffn_gate"], layer["ffn_up"]
@@ -189,7 +240,7 @@ class Model:
         runtime/include/qorvix/runtime/tensor_load.hpp:51-63): each projection must exist, hold
         rows x cols elements and have a type the engine computes; the LM head is output.weight, or
         token_embd.weight when the file ties them (weights.hpp:119, lmHead()).  The raw blocks are
-        uploaded once and kept quantized."""
+        uploaded once and kept quantized; ``rotation`` is the file's."""
         from . import supports
         from .gguf import GgufFile
         f = file if isinstance(file, GgufFile) else GgufFile.open(file)
@@ -236,6 +287,7 @@ class Model:
         m.output_norm = load_norm("output_norm.weight")
         eps = f.get_f64(f"{f.architecture}.attention.layer_norm_rms_epsilon") if f.architecture else None
         m.eps = float(eps) if eps is not None else NORM_EPS
+        m.rotation = Rotation.of_gguf(f, device)
         return m
 
     @property
@@ -517,11 +569,12 @@ class PagedDecodeStep:
     pages or columns run out, from when on the steps store and attend nothing new.
 
     heads x head_dim is wo's row length; the cache is ``n_pages`` pages of ``page_size`` tokens a layer, of
-    a type of ``KvCache``; the rotation turns halves with the given base (and per-pair factors)."""
+    a type of ``KvCache``; the rotation is the model's unless one is given, ``rope_base`` and ``rope_factors`` in
+    place of its base and factors."""
 
     def __init__(self, model: Model, m: int, heads: int, kv_heads: int, n_pages: int, max_pages: int,
-                 page_size: int = 16, cache_type: int = F16, rope_base: float = 500000.0, rope_factors=None,
-                 device="cuda"):
+                 page_size: int = 16, cache_type: int = F16, rope_base: float | None = None, rope_factors=None,
+                 device="cuda", rotation: Rotation | None = None):
         import torch
         from . import KvCache, Rope, attn_paged_ws, kv_page_bytes
         l0 = model.layers[0]
@@ -555,6 +608,10 @@ class PagedDecodeStep:
         size = kv_page_bytes(cache_type, kv_heads, page_size, hd)
         if size == 0:
             raise ValueError("PagedDecodeStep: the cache does not take this type or head size")
+        turn = replace(rotation or model.rotation)
+        turn.base = turn.base if rope_base is None else rope_base
+        turn.factors = turn.factors if rope_factors is None else rope_factors
+        freq = turn.frequencies(hd, device)
         f32, i32 = dict(dtype=torch.float32, device=device), dict(dtype=torch.int32, device=device)
         self.x = torch.zeros((m, d), **f32)
         self.qk, self.v = torch.empty((m, l0["wqk"].rows), **f32), torch.empty((m, l0["wv"].rows), **f32)
@@ -569,10 +626,7 @@ class PagedDecodeStep:
         self.free = torch.arange(n_pages, **i32)
         self.taken = torch.zeros(2, **i32)
         self.offsets, self.slots, self.pos = (torch.zeros(n, **i32) for n in (m + 1, m, m))
-        freq = rope_base ** (-torch.arange(hd // 2, dtype=torch.float64, device=device) * 2 / hd)
-        if rope_factors is not None:
-            freq = freq / rope_factors.to(freq)
-        self.rope = Rope.of(freq)
+        self.rope = Rope.of(freq, pairing=turn.pairing, scale=turn.magnitude)
         self.ws = torch.empty(attn_paged_ws(self.caches[0], heads, m, max_pages), dtype=torch.uint8, device=device)
         self.graph = None
 

@@ -163,3 +163,51 @@ def test_paged_step_refuses_a_head_without_its_norm():
         m.output_norm = None if norm is None else m.output_norm[:256]
         with pytest.raises(ValueError, match="output_norm"):
             _paged_step(m)
+
+
+def _gguf(arch="llama", **keys):
+    from gguf_build import GgufBuilder
+    from qorvix_amd.gguf import GgufFile
+    b = GgufBuilder(3).str("general.architecture", arch)
+    for key, value in keys.items():
+        key = f"{arch}.rope.{key.replace('__', '.')}"
+        b = b.str(key, value) if isinstance(value, str) else b.u32(key, value) if isinstance(value, int) else b.f32(key, value)
+    return GgufFile.parse(b.build(32))
+
+
+def test_rotation_of_a_file():
+    """The pairing, base and scaling that the file's q and k rows were laid out for, not the synthetic model's."""
+    r = decode.Rotation.of_gguf(_gguf(freq_base=500000.0, dimension_count=64))
+    assert (r.base, r.dim, r.pairing, r.scaling, r.factors, r.magnitude) == (500000.0, 64, qvx.ROPE_PAIRS, 1.0, None, 1.0)
+    assert decode.Rotation.of_gguf(_gguf()) == decode.Rotation(10000.0, qvx.ROPE_PAIRS)
+    assert decode.Rotation.of_gguf(_gguf(scaling__type="linear", scaling__factor=4.0)).scaling == 4.0
+    assert decode.Rotation.of_gguf(_gguf(scaling__type="none", scaling__factor=4.0)).scaling == 1.0
+    assert decode.Rotation.of_gguf(_gguf(scale_linear=2.0)).scaling == 2.0
+    assert decode.Rotation.of_gguf(_gguf(scaling__type="yarn", scaling__factor=4.0)).scaling is None
+    assert decode.Rotation.of_gguf(_gguf("other")).pairing is None
+
+
+def test_paged_step_takes_the_models_rotation():
+    """Fused forms carry the rotation; one that a file leaves open, or that does not fit the heads, is refused unless the
+    caller gives one."""
+    import pytest
+
+    def layers():
+        m = decode.Model(rotation=decode.Rotation(pairing=qvx.ROPE_PAIRS))
+        return m
+    assert layers().fused().rotation.pairing == layers().fused_ops().rotation.pairing == qvx.ROPE_PAIRS
+    for bad in (decode.Rotation(pairing=None), decode.Rotation(scaling=None), decode.Rotation(dim=72), decode.Rotation(dim=12)):
+        m = _paged_model()
+        m.rotation = bad
+        with pytest.raises(ValueError, match="[Rr]otation"):
+            _paged_step(m)
+        with pytest.raises(ValueError, match="KvCache.of"):
+            _paged_step(m, rotation=decode.Rotation(dim=32))
+
+
+def test_rotation_frequencies():
+    import torch
+    r = decode.Rotation(base=100.0, dim=16, scaling=2.0, factors=torch.arange(1.0, 9.0))
+    want = torch.tensor([100.0 ** (-i / 8) / 2 / (i + 1) for i in range(8)], dtype=torch.float64)
+    assert torch.allclose(r.frequencies(32, "cpu"), want, rtol=1e-14, atol=0)
+    assert decode.Rotation().frequencies(64, "cpu").shape == (32,) and decode.Rotation(dim=0).frequencies(64, "cpu").shape == (0,)

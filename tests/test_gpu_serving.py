@@ -194,3 +194,51 @@ def test_speech_decoder_layer(cuda):
             _near(ca[b], (p.unsqueeze(1) @ vv).squeeze(1), 2e-5)
         assert bool((y + product("co", ca.view(n, d))).isfinite().all())
     assert taken.tolist() == [9, 0]
+
+
+def test_paged_decode_step_of_a_file(cuda, tmp_path):
+    """A file's own rotation: neighbours form the pairs, half of a head turns, base and divisors as the file gives them.
+    What the step leaves in q and stores in the fp32 cache is the projections' outputs turned in 64 bits; the bar is the
+    rotation's own (32 u of the largest value) and what a projection of the same activations repeats bit by bit."""
+    from gguf_build import GgufBuilder
+    torch = cuda
+    rng = np.random.default_rng(8)
+    d, heads, kv_heads, hd, rot, ffn, base = 512, 8, 2, 64, 32, 512, 700.0
+    b = (GgufBuilder(3).str("general.architecture", "llama").u32("general.alignment", 32).u32("llama.block_count", 1)
+         .u32("llama.embedding_length", d).u32("llama.feed_forward_length", ffn).u32("llama.attention.head_count", heads)
+         .u32("llama.attention.head_count_kv", kv_heads).f32("llama.rope.freq_base", base)
+         .u32("llama.rope.dimension_count", rot).str("llama.rope.scaling.type", "linear").f32("llama.rope.scaling.factor", 2.0))
+    factors = (1.0 + rng.random(rot // 2)).astype(np.float32)
+    tensors = [("rope_freqs.weight", [rot // 2], factors)]
+    tensors += [(n, [d], (1.0 + 0.1 * rng.standard_normal(d)).astype(np.float32)) for n in
+                ("blk.0.attn_norm.weight", "blk.0.ffn_norm.weight", "output_norm.weight")]
+    tensors += [(f"blk.0.{n}.weight", [cols, rows], (rng.standard_normal((rows, cols)) * cols ** -0.5).astype(np.float32))
+                for n, rows, cols in (("attn_q", d, d), ("attn_k", kv_heads * hd, d), ("attn_v", kv_heads * hd, d),
+                                      ("attn_output", d, d), ("ffn_gate", ffn, d), ("ffn_up", ffn, d), ("ffn_down", d, ffn))]
+    tensors.append(("token_embd.weight", [d, 64], rng.standard_normal((64, d)).astype(np.float32)))
+    data = bytearray()
+    for name, dims, x in tensors:
+        b.tensor(name, dims, qvx.F32, len(data))
+        data += x.tobytes()
+    path = tmp_path / "model.gguf"
+    path.write_bytes(b.build(32, data=bytes(data)))
+    step = decode.PagedDecodeStep(decode.Model.from_gguf(path).fused_ops(), 2, heads, kv_heads, n_pages=8, max_pages=3,
+                                  page_size=4, cache_type=qvx.F32)
+    layer, norms = step.model.layers[0], step.model.norms[0]
+    for t in range(6):
+        x = torch.randn((2, d), device="cuda")
+        step.x.copy_(x)
+        step.run(torch.cuda.current_stream().cuda_stream)
+        w = layer["wqk"]
+        qk = qvx.qmatmul_rmsnorm_t(w.data, w.type, x, norms["attn_norm"], step.model.eps, w.rows, w.cols)
+        qk = qk.cpu().double().numpy().reshape(2, heads + kv_heads, hd)
+        angle = t * base ** (-np.arange(rot // 2) * 2 / rot) / 2.0 / factors.astype(np.float64)
+        a, c = qk[..., 0:rot:2].copy(), qk[..., 1:rot:2].copy()
+        qk[..., 0:rot:2], qk[..., 1:rot:2] = a * np.cos(angle) - c * np.sin(angle), a * np.sin(angle) + c * np.cos(angle)
+        bar = 32 * 2.0 ** -24 * np.abs(qk).max()
+        got = step.qk.cpu().double().numpy().reshape(2, heads + kv_heads, hd)[:, :heads]
+        assert np.abs(got - qk[:, :heads]).max() <= bar
+        page = step.table.cpu().numpy()[:, t // 4]
+        stored = step.caches[0].tensors[0].cpu().contiguous().view(torch.float32).view(8, kv_heads, 4, hd)
+        assert np.abs(stored[page, :, t % 4].double().numpy() - qk[:, heads:]).max() <= bar
+    assert step.taken.tolist() == [4, 0] and bool(step.logits.isfinite().all())
