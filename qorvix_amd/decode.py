@@ -158,13 +158,14 @@ class Model:
     output_norm: object = None
     eps: float = NORM_EPS
     rotation: Rotation = field(default_factory=Rotation)
+    left_out: list = field(default_factory=list)  # the file's layer tensors that none of these weights stands for
 
     def fused(self) -> "Model":
         """The same weights with each FUSED pair of a layer stacked into one device weight when the
         two share type and row length (the other projections are shared, not copied)."""
         import torch
         m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
-                  rotation=self.rotation)
+                  rotation=self.rotation, left_out=self.left_out)
         for layer in self.layers:
             out, used = {}, set()
             for name, (a, b) in FUSED:
@@ -185,7 +186,7 @@ class Model:
         import torch
         from . import interleave_rows16_t
         m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
-                  rotation=self.rotation)
+                  rotation=self.rotation, left_out=self.left_out)
         for layer in self.layers:
             out = {k: w for k, w in layer.items() if k not in ("wq", "wk", "ffn_gate", "ffn_up")}
             wq, wk, wg, wu = layer["wq"], layer["wk"], layer["ffn_gate"], layer["ffn_up"]
@@ -288,7 +289,15 @@ class Model:
         eps = f.get_f64(f"{f.architecture}.attention.layer_norm_rms_epsilon") if f.architecture else None
         m.eps = float(eps) if eps is not None else NORM_EPS
         m.rotation = Rotation.of_gguf(f, device)
+        m.left_out = Model.not_computed(f)
         return m
+
+    @staticmethod
+    def not_computed(f) -> list:
+        """Names of a file's layer tensors ("blk.<layer>.<name>") beside the seven projections and two norms."""
+        known = {f"{k}.weight" for k in ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down",
+                                         "attn_norm", "ffn_norm")}
+        return [t.name for t in f.tensors if t.name.startswith("blk.") and t.name.split(".", 2)[-1] not in known]
 
     @property
     def nbytes(self) -> int:
@@ -599,6 +608,9 @@ class PagedDecodeStep:
             norms = model.norms[l] if l < len(model.norms) else {}
             if any(norms.get(k) is None or norms[k].numel() != d for k in ("attn_norm", "ffn_norm")):
                 raise ValueError(f"PagedDecodeStep needs the norms of layer {l}, of {d} values; the model lacks some")
+        if model.left_out:
+            raise ValueError("PagedDecodeStep: the file's layers hold more than the step computes: "
+                             + ", ".join(model.left_out[:4]))
         if model.lm_head is not None and model.lm_head.cols != d:
             raise ValueError(f"PagedDecodeStep: the LM head takes {model.lm_head.cols} values, the layers give {d}")
         if model.lm_head is not None and (model.output_norm is None or model.output_norm.numel() != d):

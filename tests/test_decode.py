@@ -211,3 +211,19 @@ def test_rotation_frequencies():
     want = torch.tensor([100.0 ** (-i / 8) / 2 / (i + 1) for i in range(8)], dtype=torch.float64)
     assert torch.allclose(r.frequencies(32, "cpu"), want, rtol=1e-14, atol=0)
     assert decode.Rotation().frequencies(64, "cpu").shape == (32,) and decode.Rotation(dim=0).frequencies(64, "cpu").shape == (0,)
+
+
+def test_paged_step_refuses_layers_with_more_than_it_computes():
+    """A bias, a norm of q and k, another layer form in the file: the projections alone serve it, the whole step does not."""
+    import pytest
+
+    class File:
+        tensors = [type("T", (), dict(name=n)) for n in (
+            "token_embd.weight", "output.weight", "rope_freqs.weight", "blk.0.attn_q.weight", "blk.0.attn_q.bias",
+            "blk.1.ffn_norm.weight", "blk.1.attn_q_norm.weight", "blk.0.ffn_down.weight", "position_embd.weight")]
+    assert decode.Model.not_computed(File) == ["blk.0.attn_q.bias", "blk.1.attn_q_norm.weight"]
+    m = _paged_model()
+    m.left_out = decode.Model.not_computed(File)
+    with pytest.raises(ValueError, match="blk.0.attn_q.bias"):
+        _paged_step(m)
+    assert decode.Model(left_out=["a"]).fused().left_out == decode.Model(left_out=["a"]).fused_ops().left_out == ["a"]
