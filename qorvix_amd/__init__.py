@@ -582,14 +582,15 @@ def kv_map_t(held, new, table, page_size: int, free, taken, max_tokens: int):
 
 def rope_kv_t(q, k, v, pos, rope: Rope, cache: KvCache | None = None, slots=None, out=None):
     """rope_kv on device tensors: q [tokens, heads, head_dim] fp32 (rows of any stride), k and v [tokens, kv_heads,
-    head_dim] (None without a cache), pos [tokens] or [axes, tokens] int32, slots [tokens] int32.  Returns q_out."""
+    head_dim] (None without a cache), pos [tokens] or [axes, tokens] int32, slots [tokens] int32.  Returns q_out;
+    rows of tokens without a slot keep out's values, zeros where none is given."""
     import torch
     n, heads, d = q.shape
     _beside(rope, q.device, "rope")
     if cache is not None:
         _beside(cache, q.device, "cache")
-    if out is None:
-        out = torch.empty((n, heads, d), dtype=torch.float32, device=q.device)
+    if out is None:  # with a cache, rows of padding are not written
+        out = (torch.empty if cache is None else torch.zeros)((n, heads, d), dtype=torch.float32, device=q.device)
     for x, what, h in ((q, "q", heads), (out, "out", heads), (k, "k", cache.kv_heads if cache is not None else 0),
                        (v, "v", cache.kv_heads if cache is not None else 0)):
         if (cache is None and what in "kv") or (what in ("q", "out") and x is None):

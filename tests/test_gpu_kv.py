@@ -333,3 +333,23 @@ def test_rope_captured(cuda):
         got, kept = out.clone(), [c.clone() for c in caches]
         want = qvx.rope_kv_t(q, k, v, pos, rope, desc, slots)
         assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(kept, caches))
+
+
+def test_rope_leaves_zeros_in_padding_rows_of_its_own_output(cuda):
+    """Rows of a token without a slot in the tensor that the call makes: zeros, not what its memory held before."""
+    torch = cuda
+    n, hq, hk, d = 6, 4, 2, 64
+    q, k, v = (torch.randn((n, h, d), device="cuda") for h in (hq, hk, hk))
+    caches = [torch.zeros((4, qvx.kv_page_bytes(qvx.F16, hk, 16, d)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    desc = qvx.KvCache.of(*caches, qvx.F16, 16, hk, d)
+    rope = qvx.Rope.of(torch.ones(32, dtype=torch.float64, device="cuda"))
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots = torch.tensor([3, -1, 64, 5, -1, 0], dtype=torch.int32, device="cuda")
+    held = [torch.full((n, hq, d), float("nan"), device="cuda") for _ in range(8)]
+    del held
+    got = qvx.rope_kv_t(q, k, v, pos, rope, desc, slots)
+    dead = torch.tensor([1, 2, 4], device="cuda")
+    assert bool((got[dead] == 0).all())
+    want = qvx.rope_kv_t(q, k, v, pos, rope, desc, slots, out=torch.full_like(q, 2.0))
+    live = torch.tensor([0, 3, 5], device="cuda")
+    assert torch.equal(got[live], want[live]) and bool((want[dead] == 2.0).all())
