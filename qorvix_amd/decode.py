@@ -575,7 +575,8 @@ class PagedDecodeStep:
     [m, d] and runs the step; ``lens`` [m] are the tokens that each sequence holds (0 at the start),
     ``table`` and ``taken`` its page table and the pages of ``free`` handed out, all on the device and all
     carried on by the step itself, so a captured step replays as it is.  ``taken[1]`` is qvx_kv_map's status: not 0 once
-    pages or columns run out, from when on the steps store and attend nothing new.
+    pages or columns run out.  Such a step changes neither lengths, table nor cache, and what it leaves in ``x`` and
+    ``logits`` means nothing (its queries are not rotated and attend the older tokens alone): read the status with them.
 
     heads x head_dim is wo's row length; the cache is ``n_pages`` pages of ``page_size`` tokens a layer, of
     a type of ``KvCache``; the rotation is the model's unless one is given, ``rope_base`` and ``rope_factors`` in

@@ -242,3 +242,28 @@ def test_paged_decode_step_of_a_file(cuda, tmp_path):
         stored = step.caches[0].tensors[0].cpu().contiguous().view(torch.float32).view(8, kv_heads, 4, hd)
         assert np.abs(stored[page, :, t % 4].double().numpy() - qk[:, heads:]).max() <= bar
     assert step.taken.tolist() == [4, 0] and bool(step.logits.isfinite().all())
+
+
+def test_paged_decode_step_without_pages_left_changes_nothing(cuda):
+    """Lengths, table and every byte of the cache stand still, eager and replayed, and the step goes on once the caller has
+    handed pages back."""
+    torch = cuda
+    step = decode.PagedDecodeStep(_model(torch, layers=1), 2, heads=8, kv_heads=2, n_pages=3, max_pages=4, page_size=2)
+    for _ in range(2):
+        step.x.normal_()
+        step.run(torch.cuda.current_stream().cuda_stream)
+    step.capture()
+    before = [x.clone() for x in (step.table, step.lens, *step.pages)]
+    for replay in (False, True, True):
+        step.x.normal_()
+        step.replay() if replay else step.run(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert step.taken.tolist() == [2, qvx.MAP_PAGES]
+        assert all(torch.equal(a, b) for a, b in zip(before, (step.table, step.lens, *step.pages)))
+    step.lens.zero_()  # both requests end: their pages go back
+    step.table.fill_(-1)
+    step.taken.zero_()
+    step.x.normal_()
+    step.replay()
+    torch.cuda.synchronize()
+    assert step.taken.tolist() == [2, 0] and step.lens.tolist() == [1, 1] and bool(step.logits.isfinite().all())
