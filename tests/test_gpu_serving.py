@@ -267,3 +267,48 @@ def test_paged_decode_step_without_pages_left_changes_nothing(cuda):
     step.replay()
     torch.cuda.synchronize()
     assert step.taken.tolist() == [2, 0] and step.lens.tolist() == [1, 1] and bool(step.logits.isfinite().all())
+
+
+@pytest.mark.parametrize("t", (qvx.F16, qvx.F32, qvx.Q8_0))
+@pytest.mark.parametrize("scale_mul", (2.4e-4, 1e-4))
+def test_paged_decode_step_weighs_its_tokens(cuda, t, scale_mul):
+    """The step's attention by itself, on logits that leave weight to several tokens: what it leaves in `attn` against the
+    softmax in 64 bits of its rotated queries on the keys and values that its cache holds.  Bar: that of the attention's
+    own tests; a scale a tenth off, put into the reference, passes it in some row of every step from two tokens on."""
+    torch = cuda
+    torch.manual_seed(3)
+    heads, hk, hd, m, page, u = 8, 2, 64, 3, 3, 2.0 ** -24
+    model = _model(torch, layers=1)
+    w = model.layers[0]["wqk"]
+    qvx.fill_synthetic_t(w.data, w.type, w.rows, w.cols, seed=77, scale_mul=scale_mul)
+    step = decode.PagedDecodeStep(model, m, heads=heads, kv_heads=hk, n_pages=8 * m + 1, max_pages=9, page_size=page, cache_type=t)
+    for i in range(20):
+        visible = []
+        step.x.normal_()
+        step.run(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        q = step.qk[:, : heads * hd].cpu().double().view(m, heads, hd).numpy()
+        got, table = step.attn.cpu().double().view(m, heads, hd).numpy(), step.table.cpu().long()
+        for b in range(m):
+            kv = []
+            for x in step.caches[0].tensors:
+                raw = x[table[b, : i // page + 1].cuda()].cpu().contiguous()
+                if t == qvx.Q8_0:
+                    cut = hk * page * hd
+                    x = raw[:, :cut].contiguous().view(torch.int8).double().view(-1, hk, page, hd // 32, 32)
+                    x = x * raw[:, cut: cut + cut // 16].contiguous().view(torch.float16).double().view(-1, hk, page, hd // 32, 1)
+                else:
+                    used = hk * page * hd * (2 if t == qvx.F16 else 4)
+                    x = raw[:, :used].contiguous().view(torch.float16 if t == qvx.F16 else torch.float32).double()
+                kv.append(x.reshape(-1, hk, page, hd).transpose(1, 2).reshape(-1, hk, hd)[: i + 1].numpy())
+            for h in range(heads):
+                k, v = kv[0][:, h // 4], kv[1][:, h // 4]
+                s = k @ q[b, h] * hd ** -0.5
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                size = (np.abs(k) @ np.abs(q[b, h])).max() * hd ** -0.5
+                bar = 2 * u * ((hd + 3) * size + i + 9) * np.abs(v).max()
+                assert np.abs(got[b, h] - p @ v).max() <= bar
+                wrong = np.exp(1.1 * (s - s.max()))
+                visible.append(bool(np.abs(wrong @ v / wrong.sum() - p @ v).max() > 2 * bar))
+        assert i < 1 or any(visible)
