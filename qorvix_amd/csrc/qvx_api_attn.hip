@@ -102,15 +102,13 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 }
 
 // One workgroup reads some 45 GB/s, a split costs a launch of its own and the workspace's traffic, together 4 to 5 us.
-// So sequences that cannot pass 320 KB of keys and values a head are left whole, and up to 640 KB those of calls with an
-// item for each 8 KB.  Head size 128, fp16, whole against split: 672 keys (344 KB) at 16 items 11.9 and 11.5 us, at 40
-// 13.0 and 13.2, at 88 13.1 and 19.3; 800 keys at 40 14.0 and 14.5, at 64 14.1 and 15.4; 1024 keys at 16 14.7 and 11.4,
-// at 56 15.8 and 15.5, at 72 16.1 and 16.6, at 96 16.0 and 21.5; 1264 keys at 16 17.3 and 12.5, at 64 18.0 and 16.8,
-// at 80 18.0 and 18.6, at 160 24.9 and 29.6.  20 heads of 64 on 1500 states, 384 KB: 40 items 14.4 and 12.9, 60 14.5 and 14.2, 100 14.6
-// and 16.0; on 2400, 614 KB, 80 19.3 and 18.0, 160 28.3 and 27.6.  2048 keys of 128: 24.2 and 16.0 at 40, 76.0 and 74.3 at 320.
+// So sequences that cannot pass 320 KB of keys and values a head are left whole, and up to 640 KB those of calls that
+// occupy a good part of the card all the same.  Head size 128, fp16, split against whole: 256 keys 11.3 and 8.3 us
+// at 40 items, 21.4 and 13.5 at 320; 512 keys 12.2 and 11.1, 26.6 and 20.2; 1024 keys 14.5 and 15.7 at 40,
+// 20.7 and 15.7 at 96, 25.7 and 17.7 at 160, 44.3 and 41.3 at 320; 2048 keys 16.0 and 24.2, 74.3 and 76.0.
 bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t bytes = most_tiles(c) * 2 * kAttnTile * c.key_bytes;
-  const bool whole = bytes <= 320 << 10 || (bytes <= 640 << 10 && row_tiles * c.kv_heads >= bytes >> 13);
+  const bool whole = bytes <= 320 << 10 || (bytes <= 640 << 10 && row_tiles * c.kv_heads >= 96);
   c.min_chunk = whole ? 0 : kMinChunk;
   c.target = std::max(1, kAttnWgs / c.kv_heads);
   return plan_items(c, row_tiles, join, ws_bytes);

@@ -240,14 +240,3 @@ def test_launches_past_32_bits_of_threads_are_refused():
     assert cross(wide, heads=256, out_stride=256 * 64, q_stride=256 * 64, n_q=65536, n=65536) == qvx.E_RANGE
     for c in (True, None):
         assert rope(c=c, n=8 * 0xffffff + 1, ps=1 << 28) == qvx.E_RANGE
-
-
-def test_short_sequences_of_many_items_are_left_whole():
-    """A split of up to 640 KB of keys and values a head pays while there are fewer items than one for each 8 KB."""
-    def ws(keys, items, type=qvx.F16, d=128):
-        return qvx.attn_paged_ws(cache(kv_heads=8, head_dim=d, type=type, n_pages=4000), 32, items // 8, keys // 16)
-    for keys, items in ((672, 48), (672, 88), (800, 56), (1024, 72), (1024, 88), (1264, 80), (1264, 96)):
-        assert ws(keys, items) == 0, (keys, items)
-    for keys, items in ((672, 16), (800, 40), (1024, 40), (1264, 72), (1296, 96), (4096, 320)):
-        assert ws(keys, items) > 0, (keys, items)
-    assert ws(640, 8) == 0 and ws(1264, 64, qvx.F32, 64) > 0 and ws(1264, 80, qvx.F32, 64) == 0
