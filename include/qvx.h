@@ -289,7 +289,7 @@ typedef struct qvx_rope {
 /* Rotary positions with several axes, and the append to the cache, in one launch (rope and the cache
  * store of cuda/src/cuda_backend.cu:249-272, 325-340).  q_out[t] = rotated q[t]; rotated k[t] and v[t] are
  * stored in the cache at d_slots[t], rounded once to its type (Q8_0: scale = max|x| / 127 of a block in
- * fp16, quants to the nearest of x / scale).  Token t's heads lie side by side at d_q + t * q_stride
+ * fp16, quants to the nearest of x / scale, -127 to 127; a block past 8.3e6 has an infinite scale and stands for NaN).  Token t's heads lie side by side at d_q + t * q_stride
  * (elements; likewise q_out, k, v), so parts of one stacked product can be passed.  d_pos [n_axes]
  * [pos_stride] int32; angles are formed in 64 bits.  A token whose slot is negative or past the cache
  * is padding: none of its rows is written, q_out's neither.  q_out may be q itself (the same stride);
@@ -304,7 +304,8 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
 /* Attention of one new token a sequence over the paged cache (the reference's over one sequence,
  * cuda/src/cuda_backend.cu:347-409): out[b, h] = softmax(scale q[b, h] . K)  V over the first d_lens[b] tokens
  * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head
- * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  q and out fp32, heads side by side, rows q_stride and
+ * (q_heads % kv_heads != 0 -> QVX_E_SHAPE).  Products, weights and sums in fp32, a query value on F16 or Q8_0 keys to
+ * 2^-23 of itself.  q and out fp32, heads side by side, rows q_stride and
  * out_stride elements apart; out may be q (the same stride), else they do not overlap.  Long sequences are split over workgroups and joined in a
  * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
  * 0 .. table_width * page_size (at most 2^31 - 16, on pages of one token 2^30 - 1; more -> QVX_E_RANGE); tokens on page ids outside the cache do not count; a row without any key gets
@@ -338,7 +339,8 @@ typedef struct qvx_kv_states {
  * qvx_attn_paged.  Where q and the states share a 16-bit type, the rows of a sequence and head (queries times heads
  * a group) are more than 16 in the mean, scale is at least 1e-30 and the row stride at most 16 Mi bytes, both
  * products run on the 16-bit matrix cores and the softmax weights are rounded to that type (sums
- * stay fp32); all else computes as qvx_attn_paged, in fp32 throughout.  d_ws as there. */
+ * stay fp32; the mean is of the call, so a sequence's last bits may depend on those beside it); all else computes as
+ * qvx_attn_paged, which fp32 queries always do.  d_ws as there. */
 int qvx_attn_cross(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
                    const int32_t* d_offsets, int n_q, const qvx_kv_states* states, const int32_t* d_lens, int n_seqs,
                    float scale, void* d_ws, size_t ws_bytes, void* stream);

@@ -75,12 +75,13 @@ constexpr int kAttnWgs = 512, kMinChunk = 8;
 // rows, 8 heads 12.9 against 13.3.
 int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
-// The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
-// False: it passes 31 bits.
+// Tiles of the longest sequence that the call allows.
 int64_t most_tiles(const AttnCall& c) {
   return (int64_t)c.max_len / c.page_size * c.page_tiles + (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
 }
 
+// The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
+// False: it passes what a launch or 32 bits hold.
 bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t tiles = most_tiles(c);
   *join = c.min_chunk && tiles > c.min_chunk;
@@ -104,8 +105,11 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 // One workgroup reads some 45 GB/s, a split costs a launch of its own and the workspace's traffic, together 4 to 5 us.
 // So sequences that cannot pass 320 KB of keys and values a head are left whole, and up to 640 KB those of calls that
 // occupy a good part of the card all the same.  Head size 128, fp16, split against whole: 256 keys 11.3 and 8.3 us
-// at 40 items, 21.4 and 13.5 at 320; 512 keys 12.2 and 11.1, 26.6 and 20.2; 1024 keys 14.5 and 15.7 at 40,
-// 20.7 and 15.7 at 96, 25.7 and 17.7 at 160, 44.3 and 41.3 at 320; 2048 keys 16.0 and 24.2, 74.3 and 76.0.
+// at 40 items, 21.4 and 13.5 at 320; 512 keys 12.2 and 11.1, 26.6 and 20.2; 1024 keys 15.0 and 15.8 at 40,
+// 21.5 and 16.0 at 96, 27.5 and 20.6 at 160, 44.6 and 41.3 at 320; 2048 keys 16.0 and 24.2, 74.3 and 76.0.
+// Between 40 and 96 items sequences of equal length would be faster whole from an item for each 8 KB on (672 keys at 88 items
+// 19.3 and 13.1, 800 at 64 15.4 and 14.1, 1024 at 72 16.6 and 16.1), but mixed lengths split, the longest setting the time:
+// up to 800 keys at 80 items 11.7 and 12.9, up to 1264 12.9 and 17.2, up to 2000 in Q8_0 15.9 and 27.9.  They lose more.
 bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t bytes = most_tiles(c) * 2 * kAttnTile * c.key_bytes;
   const bool whole = bytes <= 320 << 10 || (bytes <= 640 << 10 && row_tiles * c.kv_heads >= 96);
@@ -114,12 +118,15 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   return plan_items(c, row_tiles, join, ws_bytes);
 }
 
-// The 16-bit kernel's: row tiles of 128 rows.  Partial results of so many rows are dear, so they are split only where they
-// leave half the CUs idle or more and the states are the longer the more of them there are; into chunks of 256 keys at
-// least, one a CU (two, where row tiles are half empty in the mean).  Head size 64 and 128, whole against split: 8 row tiles on 800 states 15.8 and 22.5 us against 13.2 and
-// 17.0, on 300 9.4 and 12.9 against 12.8 and 17.7; 64 on 1500 25.4 and 37.9 against 18.9 and 25.2, on 700 14.7 and 21.5 against
-// 16.9 and 23.1; 192 on 4000 59.0 and 88.1 against 54.8 and 94.4.  Chunks for two workgroups a CU: 32 on 4000 27.6 and 35.1
-// against 21.8 and 28.5; but 4 sequences of 32 rows on 1500, 20 heads of 64, 15.5 against 17.3.
+// The 16-bit kernel's: row tiles of 128 rows.  Partial results of so many rows are dear, so they are split only where all of
+// them find a place at once, one a CU, and the states are the longer the more of them there are; into chunks of 256 keys at
+// least, one a CU (two, where row tiles are half empty in the mean).  Whole against split, a sequence a row tile of each of 8
+// heads, head size 64 and 128: 8 row tiles on 700 states 14.4 and 20.3 us against 12.9 and 17.4, on 300 9.4 and 12.8 against 12.9
+// and 17.6; 64 on 1500 25.9 and 37.5 against 22.3 and 30.7, on 700 15.2 and 21.9 against 16.3 and 23.4; 128 on 2500 39.2 and
+// 61.9 against 36.7 and 60.6.  Above half the CUs lengths decide: 192 of equal length on 4000 states 62.5 and 103 against 67.9 and
+// 114 (of one sequence 57.7 and 86.5 against 57.6 and 87.1), but seven ragged ones of 450 queries at most 57.3 and 85.3 against
+// 45.3 and 68.2.  Chunks for two workgroups a CU: 32 on 4000 27.6 and 35.1 against 21.8 and 28.5; but 4 sequences of 32 rows on
+// 1500, 20 heads of 64, 15.5 against 17.3.
 bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   c.tile_rows = kAttnRows16;
   const int64_t whole = row_tiles * c.kv_heads;

@@ -6,8 +6,8 @@
 // for any m, here a running reference that follows the largest s_j seen (below).  The sum is one pass
 // over the keys, so the cache is read once and that read bounds the kernel.
 //
-// Arithmetic: fp32 throughout, whatever the cache holds.  The first product takes 16-bit keys as they are
-// and the queries in 16-bit parts that add up to the fp32 values (below); fp32 keys, and the values of
+// Arithmetic: fp32 sums and weights, whatever the cache holds.  The first product takes 16-bit keys as they are
+// and the queries in 16-bit parts (below); fp32 keys, and the values of
 // every type widened in registers, run on the fp32 matrix instructions (16x16x4, and 4x4x1 for up to eight rows), so
 // the weights are never rounded.
 //
@@ -181,7 +181,7 @@ template <int N> __device__ __forceinline__ float attn_swap_add(float a, float b
   return __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
 }
 
-// Element offset of a row's head in q (stride: q_stride) or out, and whether the row exists.
+// Element offset of a row's head in q (stride: q_stride) or out.
 __device__ __forceinline__ int64_t attn_row(const AttnCall& c, int q0, int row, int kvh, int64_t stride) {
   const int query = row / c.group, head = row - query * c.group;
   return (int64_t)(q0 + query) * stride + (int64_t)(kvh * c.group + head) * c.head_dim;
@@ -190,9 +190,10 @@ __device__ __forceinline__ int64_t attn_row(const AttnCall& c, int q0, int row, 
 __device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The queries as the first product's right operand, KS pieces of 32 values.  F32: fp32 itself, eight
-// values a lane for eight 16x16x4 instructions a piece.  Otherwise 16-bit parts that add up to the fp32
-// value, each multiplied by the keys in its own 16x16x32 instruction: fp16 twice (11 + 11 bits), bf16
-// three times (8 + 8 + 8); products of 16-bit values are exact in the instruction's fp32 sums.  The
+// values a lane for eight 16x16x4 instructions a piece.  Otherwise 16-bit parts, each multiplied by the keys in its
+// own 16x16x32 instruction: bf16 three times (8 + 8 + 8 bits), which add up to the fp32 value; fp16 twice (11 + 11), which
+// leave at most 2^-23 of it, as much as the products' own rounding in fp32 and the scale's before them add: a third
+// instruction a piece would be a half more of them for less than either.  Products of 16-bit values are exact.  The
 // row is first multiplied by a power of two, undone in the exponent.  For fp16 (and Q8_0's integers) to a largest
 // magnitude of 2^14, so that no part overflows and the small part of every value that matters stays normal.  bf16
 // keys reach as far as fp32: there rows below 2^-10 are brought to that, where 256 products with keys of any size stay

@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kMapThreads) void k_kv_map(MapCall c, int write) {
 // Pair i of a head is turned by pos[axis[i]] * inv_freq[i]; the angle's whole turns are taken off in
 // 64 bits (at position 10^6 an fp32 product is off by 0.06), the rest is an fp32 number of half turns.
 // One pass over q, k and v; the bytes bound it: 8192 tokens of 32 + 2 x 8 heads of 128 into a bf16 cache 70.7 us,
-// 5.2 TB/s where a copy of 2 GiB reaches 4.9; one token 3.5 us.  A workgroup takes `tokens_wg` tokens and a range of
+// 5.2 TB/s where an elementwise pass over as many bytes reaches 5.9, into a Q8_0 one 70.3 (5.0); one token 3.5 us.  A workgroup takes `tokens_wg` tokens and a range of
 // their heads: its threads first form the cosines and sines of the tokens' pairs in LDS, each once, and
 // then take 8 values of a head at a time.
 
@@ -185,8 +185,10 @@ __device__ __forceinline__ void cache_store(const RopeCall& c, uint8_t* pages, i
     }
     *reinterpret_cast<uint4*>(page + (row * c.head_dim + i) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    // scale = max|x| / 127 rounded to fp16, quants to the nearest (ties to even) of x / that scale:
-    // dividing by the rounded scale keeps each value within half a step of what is stored.
+    // scale = max|x| / 127 rounded to fp16, quants to the nearest (ties to even) of x / that scale, -127 to 127:
+    // dividing by the rounded scale keeps each value within half a step of what is stored, but for what a scale rounded
+    // down leaves of the block's largest: 127 times fp16's half step, which counts where the scale is subnormal (max|x|
+    // below 2^-14 * 127; below 2^-25 * 127 the block is zeros).  Past 65504 * 127 the scale is infinite, the block NaN.
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(a.v[j]), fabsf(b.v[j])));

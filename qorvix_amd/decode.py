@@ -706,7 +706,7 @@ class PrefillStep:
     positions at once as one GEMM (``qvx_qgemm_f16``: Q4_K on the engine's raw-block MFMA kernels,
     the Q6_K tensors on its dequantising MFMA kernel), and the LM head runs on the last position
     only, as the reference keeps only the logits after the last prompt token.  Activations are
-    seeded fp16 stand-ins (norms, RoPE, attention and SwiGLU are outside the engine); one output
+    seeded fp16 stand-ins (this step has the projections alone, no norm, rotation, attention or SwiGLU); one output
     buffer per projection name is reused across layers.  ``run`` issues the calls eagerly;
     ``capture`` records them into one graph through the no-allocation entry point and ``replay``
     launches it."""
