@@ -126,9 +126,9 @@ class Rotation:
         else:
             r.scaling = None
         t = f.tensor("rope_freqs.weight")
-        if t is not None:
-            if t.type_raw != F32:
-                raise ValueError("rope_freqs.weight must be F32")
+        if t is not None and t.type_raw != F32:
+            r.scaling = None
+        elif t is not None:
             import torch
             r.factors = f.upload("rope_freqs.weight", device).data.view(torch.float32)
         return r
@@ -140,6 +140,8 @@ class Rotation:
         if self.pairing is None or self.scaling is None:
             raise ValueError("the file does not say how its q and k rows pair, or scales positions in a way of its own: "
                              "pass a Rotation")
+        if not (self.base > 0 and self.scaling > 0):
+            raise ValueError("Rotation: base and scaling are positive")
         if dim < 0 or dim > head_dim or dim % 8 or (self.factors is not None and tuple(self.factors.shape) != (dim // 2,)):
             raise ValueError(f"Rotation: {dim} values of a head of {head_dim}, in eights, with a factor a pair")
         freq = self.base ** (-torch.arange(dim // 2, dtype=torch.float64, device=device) * 2 / max(dim, 1)) / self.scaling

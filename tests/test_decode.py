@@ -227,3 +227,17 @@ def test_paged_step_refuses_layers_with_more_than_it_computes():
     with pytest.raises(ValueError, match="blk.0.attn_q.bias"):
         _paged_step(m)
     assert decode.Model(left_out=["a"]).fused().left_out == decode.Model(left_out=["a"]).fused_ops().left_out == ["a"]
+
+
+def test_a_files_rotation_never_keeps_its_weights_from_loading():
+    """Divisors of another type than F32 leave the rotation open, for the step alone to refuse."""
+    import pytest
+    from gguf_build import GgufBuilder
+    from qorvix_amd.gguf import GgufFile
+    b = GgufBuilder(3).str("general.architecture", "llama")
+    b.tensor("rope_freqs.weight", [8], qvx.F16, 0)
+    r = decode.Rotation.of_gguf(GgufFile.parse(b.build(32, data=bytes(32))))
+    assert r.scaling is None and r.factors is None
+    for bad in (r, decode.Rotation(base=0.0), decode.Rotation(base=-1.0), decode.Rotation(scaling=0.0)):
+        with pytest.raises(ValueError):
+            bad.frequencies(64, "cpu")
