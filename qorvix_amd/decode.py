@@ -648,6 +648,7 @@ class PagedDecodeStep:
     def run(self, stream: int) -> None:
         """The step on ``stream``, which is torch's current one (the residual adds are torch's)."""
         from . import _check, attn_paged, kv_map, rope_kv
+        self._on_device()
         so, m, hd, model = lib(), self.m, self.head_dim, self.model
         d, q_row, width = self.x.shape[1], self.heads * self.head_dim, self.qk.shape[1]
         x, qk, v, attn, o = (t.data_ptr() for t in (self.x, self.qk, self.v, self.attn, self.o))
@@ -683,9 +684,16 @@ class PagedDecodeStep:
         """Record the step into one graph.  Nothing runs and no state moves on; run the step eagerly at
         least once before."""
         import torch
+        self._on_device()
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.run(torch.cuda.current_stream().cuda_stream)
+
+    def _on_device(self) -> None:
+        """The launches go to the current device, which has to be the buffers'."""
+        import torch
+        if torch.cuda.current_device() != self.x.device.index:
+            raise ValueError(f"PagedDecodeStep: made on {self.x.device}, the current device is {torch.cuda.current_device()}")
 
     def replay(self) -> None:
         self.graph.replay()

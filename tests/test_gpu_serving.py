@@ -312,3 +312,22 @@ def test_paged_decode_step_weighs_its_tokens(cuda, t, scale_mul):
                 wrong = np.exp(1.1 * (s - s.max()))
                 visible.append(bool(np.abs(wrong @ v / wrong.sum() - p @ v).max() > 2 * bar))
         assert i < 1 or any(visible)
+
+
+def test_paged_decode_step_stays_on_its_device(cuda, monkeypatch):
+    """The step's launches go to the current device: with another one current it is refused, eager and in a capture."""
+    torch = cuda
+    step = decode.PagedDecodeStep(_model(torch, layers=1), 1, heads=8, kv_heads=2, n_pages=4, max_pages=2)
+    step.run(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "current_device", lambda: step.x.device.index + 1)
+        with pytest.raises(ValueError, match="device"):
+            step.run(stream)
+        with pytest.raises(ValueError, match="device"):
+            step.capture()
+    step.capture()
+    step.replay()
+    torch.cuda.synchronize()
+    assert step.lens.tolist() == [2]
