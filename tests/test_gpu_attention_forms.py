@@ -268,3 +268,29 @@ def test_cross_few_rows_at_every_head_size(cuda, q_type, kv_type, d, nq):
     _sharp_cross(cuda, q_type, kv_type, nq, (300, 41, 77), 2, 2, d, seed=d)
     _sharp_cross(cuda, q_type, kv_type, nq, (300, 3000, 1), 1, 1, d, seed=d)
     _check_cross(cuda, q_type, kv_type, nq, (300, 0, 77), 2, 2, d, seed=d)
+
+
+# ---- counts at the ends of what the calls take --------------------------------------------------------------------
+
+def test_paged_thousands_of_sequences(cuda):
+    """Threads that each look through many sequences, one of them split."""
+    r = np.random.default_rng(2)
+    lens = [int(x) for x in r.integers(0, 4, 9000)]
+    lens[8191], lens[4000] = 4200, 33
+    c = Cache(cuda, qvx.F16, lens, 16, 1, 64, seed=2)
+    assert qvx.attn_paged_ws(c.desc, 2, len(lens), c.width) > 0
+    _sharp_paged(cuda, c, 2)
+
+
+def test_paged_as_many_sequences_as_a_call_takes(cuda):
+    """65536 sequences of no key or one: the key's value, or zeros."""
+    torch = cuda
+    n, d = 65536, 32
+    size = qvx.kv_page_bytes(qvx.F32, 1, 1, d)
+    k, v = (torch.randn((n, size // 4), device="cuda") for _ in range(2))
+    cache = qvx.KvCache.of(k, v, qvx.F32, 1, 1, d)
+    table = torch.randperm(n, device="cuda").to(torch.int32).view(n, 1)
+    lens = (torch.arange(n, device="cuda") % 3 != 1).to(torch.int32)
+    out = qvx.attn_paged_t(torch.randn((n, 1, d), device="cuda"), cache, table, lens)
+    want = v[table[:, 0].long()] * lens[:, None]
+    assert bool(((out[:, 0] - want).abs() <= 4 * U * want.abs()).all())

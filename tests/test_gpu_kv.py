@@ -353,3 +353,9 @@ def test_rope_leaves_zeros_in_padding_rows_of_its_own_output(cuda):
     want = qvx.rope_kv_t(q, k, v, pos, rope, desc, slots, out=torch.full_like(q, 2.0))
     live = torch.tensor([0, 3, 5], device="cuda")
     assert torch.equal(got[live], want[live]) and bool((want[dead] == 2.0).all())
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_map_of_as_many_sequences_as_a_call_takes(cuda, in_place):
+    held, new, table, free, need = _map_case(3, 16384, 30, 4, 8)
+    _check_map(cuda, held, new, table, 8, free, 2, sum(new) + 3, in_place)
