@@ -8,7 +8,8 @@
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction, fp32 sums.  The weights are
 // rounded to the operands' type (to the nearest) before the second product: each by at most half a
 // step; the denominator sums them in fp32.  The reference m follows the largest logit lazily, as in
-// qvx_attn_split.hpp, kSlack16 above it when it is set, so bf16 weights lie at 2^-kSlack16 to 1.  In fp16 all weights are
+// qvx_attn_split.hpp, kSlack16 above it when it is set (which moves a weight by 2^-21 of itself at most), so the largest
+// bf16 weight lies at 2^-kSlack16 to 1.  In fp16 all weights are
 // 2^kUp16 larger than that: up to 2^15 they stay in range, and down to 2^-21 of the largest above its smallest normal number.
 //
 // Layout.  In S^T a lane holds query row lane % 32 and, with h = lane / 32, the keys 8 (r / 4) + 4 h + r % 4

@@ -16,11 +16,12 @@
 // product to the next in place, without a lane exchange or LDS, when the values of key 4 g + r are
 // loaded by the lanes of group g: 16 lanes cover a token's values in consecutive pieces.
 //
-// The reference m.  A row's weights may use any common m.  It stands kSlack above the row's largest logit (in powers of
-// two) when it is set, and is set again only when a logit passes it, which after the first tiles is rare, so a step costs
-// a compare and a wave vote instead of a lane reduction and a rescale.  Weights are therefore never above 1 and the row's
-// largest never below 2^-kSlack: their sums stay finite for values of up to fp32's largest number over the number of keys,
-// and weights of 2^-100 of the largest are still normal numbers; the relative error of each stays that of fp32.
+// The reference m.  A row's weights may use any common m; it is the row's largest logit (in powers of two) when it is set,
+// and set again only when a logit passes it by more than kSlack, which after the first tiles is rare, so a step costs
+// a compare and a wave vote instead of a lane reduction and a rescale.  All weights are 2^kSlack smaller than 2^(s_j - m): never
+// above 1, the row's largest never below 2^-kSlack.  So their sums stay finite for values of up to fp32's largest number over
+// the number of keys, and weights of 2^-100 of the largest are still normal numbers.  The factor follows the power of
+// two: taken into m it would cost the exponents near 0 their last five bits (33 keys, an error of 4.3e-7 against 2.1e-7).
 //
 // Split.  A work item is a chunk of a sequence's tiles (qvx_attn.hpp); its four waves take tiles in
 // turn and join through LDS.  Items of a sequence that has several leave their sums, their maxima
@@ -44,7 +45,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kSlack = 20.0f;
+constexpr float kSlack = 20.0f, kWeight = 0x1p-20f;  // 2^-kSlack
 constexpr uint32_t kPastEnd = 0x7fffff00u;  // an offset no descriptor reaches: the load gives zeros
 
 // A descriptor of `bytes` bytes from p (the same in all lanes): loads past them give zeros.
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
         if (lane >> 2 >= x.live) p[t] = -INFINITY;
         top[t] = p[t] * muls[t];
-        past |= top[t] > m[t];  // m is -inf at the start: any finite logit moves it
+        past |= top[t] > m[t] + kSlack;  // m + slack is -inf at the start: any finite logit moves it
       }
       if (__any(past)) {
 #pragma unroll
@@ -549,7 +550,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
           float now = top[t];
 #pragma unroll
           for (int s = 4; s < 64; s *= 2) now = fmaxf(now, __shfl_xor(now, s));
-          now = now > m[t] ? now + kSlack : m[t];
+          now = fmaxf(m[t], now);
           const float f = m[t] == now ? 1.0f : attn_pow2(m[t] - now);
           m[t] = now;
           l[t] *= f;
@@ -563,7 +564,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        p[t] = attn_pow2(__builtin_fmaf(p[t], muls[t], m[t] == -INFINITY ? 0.0f : -m[t]));
+        p[t] = attn_pow2(__builtin_fmaf(p[t], muls[t], m[t] == -INFINITY ? 0.0f : -m[t])) * kWeight;
         l[t] += p[t];
       }
       attn_values<0, NT, VN, VU, kQ8>(acc, p, x);
@@ -576,10 +577,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int r = 0; r < 4; ++r) sc[r] = 4 * g + r >= x.live ? -INFINITY : sc[r];
       const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
-      if (__any(top > m[0])) {
+      if (__any(top > m[0] + kSlack)) {
         float t = fmaxf(top, __shfl_xor(top, 16));
         t = fmaxf(t, __shfl_xor(t, 32));
-        const float now = t > m[0] ? t + kSlack : m[0];
+        const float now = fmaxf(m[0], t);
         const float f = m[0] == now ? 1.0f : attn_pow2(m[0] - now);
         m[0] = now;
         l[0] *= f;
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       const float ref = m[0] == -INFINITY ? 0.0f : m[0];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = attn_pow2(__builtin_fmaf(sc[r], mul, -ref));
+        const float p = attn_pow2(__builtin_fmaf(sc[r], mul, -ref)) * kWeight;
         l[0] += p;
         const float vs = kQ8 ? attn_half(x.vstep[kQ8 ? r : 0]) : 1.0f;
 #pragma unroll
