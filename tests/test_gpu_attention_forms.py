@@ -6,11 +6,12 @@ Queries.  A row is zero or has one value, so its logits are zeros or single prod
 zeros weighs all keys alike and exactly, so its output is their mean value, and a key that is lost or counted twice
 moves it by what it is: each check also leaves one tile of 16 keys out of the reference and asks that the bar sees it.
 
-Bars.  u = 2^-24.  Weights: 8 u (S + 20), the reference standing 20 above the largest logit, and nothing where S = 0; the
-hardware's power of two and the factors of the joins 8 u in all.  Sums: `depth` additions on any path, at most
+Bars.  u = 2^-24.  Weights: 8 u S (above, and the exponent's own rounding: at most S log2(e) from the reference on
+either side), nothing where S = 0; the hardware's power of two and the factors of the joins 8 u in all.  Sums: `depth` additions on any path, at most
 16 a tile for the tiles of a chunk that a wave takes (every fourth), four waves and the chunks of the sequence; so
-|error| <= 2 u (8 (S + 20) + depth + 8) max |v|, numerator and denominator both.  On the 16-bit matrix cores the
-logits are whole powers of two, so the weights are 16-bit numbers and only the output is rounded: half a step more."""
+|error| <= 2 u (8 S + depth + 8) max |v|, numerator and denominator both.  On the 16-bit matrix cores the
+weights are powers of two from 1 to 2^-7 of the largest, so rounding them changes nothing and only the output is rounded: half
+a step more."""
 from __future__ import annotations
 
 import math
@@ -52,7 +53,7 @@ def _mean(q, k, v, scale):
 
 
 def _bar(s, depth, top):
-    return 2 * U * (np.where(s > 0, 8 * (s + 20), 0) + depth + 8) * top
+    return 2 * U * (8 * s + depth + 8) * top
 
 
 def _sharp_queries(n, heads, d, value, seed):
@@ -193,7 +194,7 @@ def test_paged_graphs_with_workspaces_of_their_own(cuda):
 # ---- cross attention ------------------------------------------------------------------------------------------
 
 def _sharp_cross(torch, q_type, kv_type, nq, ns, hq, hk, d, seed=0):
-    """Ragged queries and states; logits are whole powers of two from 2^-7 up to 1 (scale ln 2, keys of 0 to -7)."""
+    """Ragged queries and states; weights are powers of two (scale ln 2, keys of 0 to -7)."""
     r = np.random.default_rng(seed)
     n, most, rows, group = len(nq), max(ns), sum(nq), hq // hk
     q = _sharp_queries(rows, hq, d, 1.0, seed)
