@@ -108,7 +108,7 @@ class Rotation:
     pairing: int | None = ROPE_HALVES
     dim: int | None = None
     scaling: float | None = 1.0
-    factors: object = None  # tensor [dim / 2]
+    factors: object = None  # tensor of dim / 2 values, or of one
     magnitude: float = 1.0
 
     @staticmethod
@@ -142,10 +142,10 @@ class Rotation:
                              "pass a Rotation")
         if not (self.base > 0 and self.scaling > 0):
             raise ValueError("Rotation: base and scaling are positive")
-        if dim < 0 or dim > head_dim or dim % 8 or (self.factors is not None and tuple(self.factors.shape) != (dim // 2,)):
-            raise ValueError(f"Rotation: {dim} values of a head of {head_dim}, in eights, with a factor a pair")
+        if dim < 0 or dim > head_dim or dim % 8 or (self.factors is not None and self.factors.numel() not in (1, dim // 2)):
+            raise ValueError(f"Rotation: {dim} values of a head of {head_dim}, in eights, with a factor a pair or one")
         freq = self.base ** (-torch.arange(dim // 2, dtype=torch.float64, device=device) * 2 / max(dim, 1)) / self.scaling
-        return freq if self.factors is None else freq / self.factors.to(freq)
+        return freq if self.factors is None else freq / self.factors.to(freq).reshape(-1)
 
 
 @dataclass

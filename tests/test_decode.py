@@ -241,3 +241,12 @@ def test_a_files_rotation_never_keeps_its_weights_from_loading():
     for bad in (r, decode.Rotation(base=0.0), decode.Rotation(base=-1.0), decode.Rotation(scaling=0.0)):
         with pytest.raises(ValueError):
             bad.frequencies(64, "cpu")
+
+
+def test_rotation_takes_one_divisor_for_all_pairs():
+    """A caller's `rope_factors` of one value divide every pair, as they did before files had their own."""
+    import torch
+    want = decode.Rotation().frequencies(64, "cpu") / 4
+    for factors in (torch.tensor(4.0), torch.tensor([4.0]), torch.full((32,), 4.0)):
+        got = decode.Rotation(factors=factors).frequencies(64, "cpu")
+        assert got.shape == (32,) and torch.equal(got, want)
