@@ -289,7 +289,8 @@ typedef struct qvx_rope {
 /* Rotary positions with several axes, and the append to the cache, in one launch (rope and the cache
  * store of cuda/src/cuda_backend.cu:249-272, 325-340).  q_out[t] = rotated q[t]; rotated k[t] and v[t] are
  * stored in the cache at d_slots[t], rounded once to its type (Q8_0: scale = max|x| / 127 of a block in
- * fp16, quants to the nearest of x / scale, -127 to 127; a block past 8.3e6 has an infinite scale and stands for NaN).  Token t's heads lie side by side at d_q + t * q_stride
+ * fp16, quants to the nearest of x / scale, -127 to 127; a block past 8.3e6 has an infinite scale and
+ * stands for NaN).  Token t's heads lie side by side at d_q + t * q_stride
  * (elements; likewise q_out, k, v), so parts of one stacked product can be passed.  d_pos [n_axes]
  * [pos_stride] int32; angles are formed in 64 bits.  A token whose slot is negative or past the cache
  * is padding: none of its rows is written, q_out's neither.  q_out may be q itself (the same stride);
@@ -308,10 +309,11 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
  * 2^-23 of itself.  q and out fp32, heads side by side, rows q_stride and
  * out_stride elements apart; out may be q (the same stride), else they do not overlap.  Long sequences are split over workgroups and joined in a
  * second launch, in the same order in every run: equal inputs give equal bits.  Lengths are cut to
- * 0 .. table_width * page_size (at most 2^31 - 16, on pages of one token 2^30 - 1; more -> QVX_E_RANGE); tokens on page ids outside the cache do not count; a row without any key gets
+ * 0 .. table_width * page_size (at most 2^31 - 16, on pages of one token 2^30 - 1; more -> QVX_E_RANGE);
+ * tokens on page ids outside the cache do not count; a row without any key gets
  * zeros; rows of the cache behind a sequence's last token are not read.  Keys are finite: an infinite one of a 16-bit
- * cache makes its rows NaN, as NaN does.  Values times the number of keys stay below fp32's largest number.  d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less ->
- * QVX_E_RANGE; its contents need not be kept or cleared). */
+ * cache makes its rows NaN, as NaN does.  Values times the number of keys stay below fp32's largest number.
+ * d_ws: qvx_attn_paged_ws bytes, 16-byte aligned (less -> QVX_E_RANGE; its contents need not be kept or cleared). */
 int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q_stride, int q_heads,
                    const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens,
                    int n_seqs, float scale, void* d_ws, size_t ws_bytes, void* stream);

@@ -184,8 +184,8 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
     return QVX_E_SHAPE;
   const int64_t es = value_bytes(st->type, 1);
   constexpr int64_t kMost = 1ll << 56;
-  if (n_seqs > kAttnMaxSeqs || st->max_len > kMaxLen || st->kv_heads > 65535 || st->batch_stride > kMost || st->head_stride > kMost ||
-      st->row_stride > kMaxPitch / es || (st->row_stride * es) % 16 || (st->batch_stride * es) % 16 ||
+  if (n_seqs > kAttnMaxSeqs || st->max_len > kMaxLen || st->kv_heads > 65535 || st->batch_stride > kMost ||
+      st->head_stride > kMost || st->row_stride > kMaxPitch / es || (st->row_stride * es) % 16 || (st->batch_stride * es) % 16 ||
       (st->head_stride * es) % 16)
     return QVX_E_RANGE;
   if (st->max_len && (!st->d_k || !st->d_v)) return QVX_E_NULL;

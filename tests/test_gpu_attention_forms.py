@@ -7,8 +7,8 @@ zeros weighs all keys alike and exactly, so its output is their mean value, and 
 moves it by what it is: each check also leaves one tile of 16 keys out of the reference and asks that the bar sees it.
 
 Bars.  u = 2^-24.  Weights: 8 u S (above, and the exponent's own rounding: at most S log2(e) from the reference on
-either side), nothing where S = 0; the hardware's power of two and the factors of the joins 8 u in all.  Sums: `depth` additions on any path, at most
-16 a tile for the tiles of a chunk that a wave takes (every fourth), four waves and the chunks of the sequence; so
+either side), nothing where S = 0; the hardware's power of two and the factors of the joins 8 u in all.  Sums: `depth`
+additions on any path, at most 16 a tile for the tiles of a chunk that a wave takes (every fourth), four waves and the chunks of the sequence; so
 |error| <= 2 u (8 S + depth + 8) max |v|, numerator and denominator both.  On the 16-bit matrix cores the
 weights are powers of two from 1 to 2^-7 of the largest, so rounding them changes nothing and only the output is rounded: half
 a step more."""
