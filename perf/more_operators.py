@@ -308,7 +308,7 @@ def _prepare_compact(s, c, g):
     s.extra = torch.zeros(pages, dtype=torch.int32, device=DEVICE)
     s.extra[ids[:used].long()] = torch.randint(0, 5, (used,), generator=g, device=DEVICE, dtype=torch.int32)
     s.k, s.v = _layers(c, pages, g)
-    s.pairs, s.n_pairs = torch.full((max(1, pages // 2), 2), -1, dtype=torch.int32, device=DEVICE), _ints([0])
+    s.pairs, s.moved = torch.full((max(1, pages // 2), 2), -1, dtype=torch.int32, device=DEVICE), _ints([0, 0])
 
 
 def _own_handles(s, c):
@@ -332,7 +332,7 @@ def _own_handles(s, c):
         pages = s.extra.shape[0]
         s.caches = qvx.kv_caches([qvx.KvCache.of(k, v, TYPES[c["type"]], c["page"], c["kv_heads"], c["d"])
                                   for k, v in zip(s.k, s.v)])
-        s.ws = torch.empty(max(qvx.kv_free_ws(pages), qvx.kv_compact_ws(pages)), dtype=torch.uint8, device=DEVICE)
+        s.ws = torch.empty(qvx.kv_free_ws(pages), dtype=torch.uint8, device=DEVICE)
     if op == "compact":
         s.table_out, s.extra_out, s.free_out = (torch.empty_like(x) for x in (s.table, s.extra, s.free))
 
@@ -489,7 +489,8 @@ def _plain_compact(s):
     extra[dst], extra[src] = s.extra[src], 0
     free = torch.where(listed_free, n + torch.arange(s.free.shape[0], device=DEVICE) - s.taken[0], s.free).to(torch.int32)
     s.k[:, dst], s.v[:, dst] = s.k[:, src], s.v[:, src]
-    return [table, extra, free, torch.full((1,), src.shape[0], dtype=torch.int32, device=DEVICE), s.k, s.v]
+    moved = torch.stack([torch.full_like(n, src.shape[0]), n]).to(torch.int32)  # pages moved, pages in use
+    return [table, extra, free, moved, s.k, s.v]
 
 
 # ---- the framework's kernels ---------------------------------------------------------------------------------
@@ -532,10 +533,9 @@ def _own(s):
         pages = s.extra.shape[0]
         rc = qvx.kv_compact(s.table.data_ptr(), s.table_out.data_ptr(), s.table.shape[0], s.table.shape[1],
                             s.extra.data_ptr(), s.extra_out.data_ptr(), pages, s.free.data_ptr(), s.free_out.data_ptr(),
-                            s.free.shape[0], s.taken.data_ptr(), s.pairs.data_ptr(), s.n_pairs.data_ptr(),
-                            s.ws.data_ptr(), s.ws.numel(), stream)
-        rc = rc or qvx.kv_copy(s.caches, s.pairs.data_ptr(), s.n_pairs.data_ptr(), s.pairs.shape[0], stream)
-        out = [s.table_out, s.extra_out, s.free_out, s.n_pairs, s.k, s.v]
+                            s.free.shape[0], s.taken.data_ptr(), s.pairs.data_ptr(), s.moved.data_ptr(), stream)
+        rc = rc or qvx.kv_copy(s.caches, s.pairs.data_ptr(), s.moved.data_ptr(), s.pairs.shape[0], stream)
+        out = [s.table_out, s.extra_out, s.free_out, s.moved, s.k, s.v]
     if rc != qvx.OK:
         raise qvx.QvxError(rc, op)
     return out
