@@ -302,6 +302,73 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
                 const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
                 const int32_t* d_slots, void* stream);
 
+/* Norms of each q and k head before the rotation: y = x * w / sqrt(mean of x^2 + eps) over the head's values, the squares
+ * summed in 64 bits.  d_q_w, d_k_w: fp32 weights, head_dim of them for all heads (head_stride 0) or head_stride values (at
+ * least head_dim) from a head's to the next; NULL: q, or k, is not normed.  eps not below 0. */
+typedef struct qvx_qk_norm {
+  const float* d_q_w;
+  const float* d_k_w;
+  int32_t head_stride;
+  float eps;
+} qvx_qk_norm;
+
+/* qvx_rope_kv with those norms in the same pass: norm, rotation, append.  q_out is of q_out_type, F32, F16 or BF16 (rounded
+ * once; what qvx_attn_window and qvx_attn_shared take for their 16-bit products), its stride in those elements; in place
+ * (q_out = q) in F32 alone.  All else as in qvx_rope_kv, cache NULL too. */
+int qvx_norm_rope_kv(void* d_q_out, int64_t q_out_stride, uint32_t q_out_type, const float* d_q, int64_t q_stride,
+                     int q_heads, const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens,
+                     int head_dim, const qvx_qk_norm* norm, const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride,
+                     const qvx_kv_cache* cache, const int32_t* d_slots, void* stream);
+
+/* Pages that several sequences hold.  d_extra [n_pages] counts for each page the rows of the table that hold it beside the
+ * first: 0 for a page of one row and for a free one.  Pages of qvx_kv_map are of one row; qvx_kv_fork shares them and
+ * qvx_kv_free gives them back, both on the free list and the count of qvx_kv_map (d_free [n_free], the first d_taken_in[0]
+ * of it handed out).  The four calls are asynchronous and allocate nothing, and their results do not depend on the order in
+ * which workgroups run.  A table's rows have up to 2^24 columns (more -> QVX_E_RANGE), a call up to 16384 forks or
+ * rows; rows, lengths and ids are read on the device and checked there. */
+#define QVX_MAP_SEQUENCE 16 /* a row that the table does not have, or a fork onto itself */
+
+/* Forks: row d_to[i] of the table [n_rows, table_width] becomes a copy of row d_from[i], i < n, its sequence as long
+ * (d_lens).  The full pages are shared (d_extra + 1); where the last page is not full the fork gets the next page of the
+ * free list, and the pair of both ids is left in d_pairs [n][2], d_n_pairs[0] of them side by side in the order of the
+ * forks, for qvx_kv_copy to fill it: no shared page is appended to.  Columns behind the sequence's are -1.  The rows
+ * d_to are distinct, none of them a d_from, and hold no pages (they would be lost); several forks of one row are fine.
+ * d_taken_out[0] = pages taken so far, [1] = status (QVX_MAP_*; 0: done); it may be d_taken_in (then a second launch stores
+ * it).  All or nothing: unless the status is 0, table, lengths and counts stay and d_n_pairs[0] = 0.  Other overlaps of
+ * the arrays -> QVX_E_RANGE. */
+int qvx_kv_fork(const int32_t* d_from, const int32_t* d_to, int n, int32_t* d_table, int n_rows, int table_width,
+                int page_size, int32_t* d_lens, int32_t* d_extra, int n_pages, const int32_t* d_free, int n_free,
+                const int32_t* d_taken_in, int32_t* d_taken_out, int32_t* d_pairs, int32_t* d_n_pairs, void* stream);
+
+/* Releases: the rows d_rows[i] of the table give their pages back, all of them (d_begin, d_end NULL; d_lens is 0 then), or
+ * those of columns d_begin[i] .. d_end[i] - 1, as behind a window (lengths stay; d_lens may be NULL).  Entries become -1; a
+ * page that other rows hold loses one holder (d_extra - 1), the others return to the free list, in ascending order in
+ * front of what is free, d_taken_out[0] being less by their number.  An entry that is listed twice is released once.
+ * Status in d_taken_out[1]: QVX_MAP_SEQUENCE: rows that do not exist were passed over; QVX_MAP_PAGES: more pages came
+ * back than the list handed out, the first of them are lost (the count is 0 then).  d_taken_out may be d_taken_in; d_ws:
+ * qvx_kv_free_ws bytes, 4-byte aligned.  Other overlaps -> QVX_E_RANGE. */
+int qvx_kv_free(const int32_t* d_rows, const int32_t* d_begin, const int32_t* d_end, int n, int32_t* d_table, int n_rows,
+                int table_width, int32_t* d_lens, int32_t* d_extra, int n_pages, int32_t* d_free, int n_free,
+                const int32_t* d_taken_in, int32_t* d_taken_out, void* d_ws, size_t ws_bytes, void* stream);
+/* Workspace of that call, 0 for up to 16384 pages. */
+size_t qvx_kv_free_ws(int n_pages);
+
+/* Compaction: with u pages in use (all of 0 .. n_pages - 1 that d_free[d_taken[0] ..] does not name; u = d_moved[1]), those
+ * of ids from u on move to the unused ids below, both in ascending order: d_moved[0] of them, their pairs (from, to) in
+ * d_pairs [n_pages / 2][2] for qvx_kv_copy.  Table, counts and free list (u, u + 1, .. behind the handed out; -1 where a list
+ * named an id twice) are written as they are afterwards, each onto itself or elsewhere; other overlaps -> QVX_E_RANGE.
+ * Table entries that are no page, or a free one, stay.  Up to 2^20 pages (more -> QVX_E_RANGE). */
+int qvx_kv_compact(const int32_t* d_table, int32_t* d_table_out, int n_rows, int table_width, const int32_t* d_extra,
+                   int32_t* d_extra_out, int n_pages, const int32_t* d_free, int32_t* d_free_out, int n_free,
+                   const int32_t* d_taken, int32_t* d_pairs, int32_t* d_moved, void* stream);
+
+/* Copies whole pages, K and V, of n_caches caches (the layers; alike in type, shape and number of pages, else
+ * QVX_E_SHAPE; a launch for each 64): page d_pairs[2 i] to page d_pairs[2 i + 1], i < d_n_pairs[0] (NULL, or more:
+ * most_pairs).  Pairs with an id that is no page are passed over.  No page is written twice, nor read by another pair, else
+ * what it holds is not specified. */
+int qvx_kv_copy(const qvx_kv_cache* caches, int n_caches, const int32_t* d_pairs, const int32_t* d_n_pairs, int most_pairs,
+                void* stream);
+
 /* Attention of one new token a sequence over the paged cache (the reference's over one sequence,
  * cuda/src/cuda_backend.cu:347-409): out[b, h] = softmax(scale q[b, h] . K)  V over the first d_lens[b] tokens
  * of the sequence's pages d_table[b], the query heads in groups of q_heads / kv_heads per cache head

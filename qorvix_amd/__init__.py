@@ -36,7 +36,7 @@ GEMM_BF16, GEMM_I8, GEMM_F16 = 0, 1, 2
 
 # pairings of a rotation, and the status bits of kv_map
 ROPE_HALVES, ROPE_PAIRS = 0, 1
-MAP_PAGES, MAP_COLUMNS, MAP_ROWS, MAP_NEGATIVE = 1, 2, 4, 8
+MAP_PAGES, MAP_COLUMNS, MAP_ROWS, MAP_NEGATIVE, MAP_SEQUENCE = 1, 2, 4, 8, 16
 
 # The C ABI: name -> (argtypes, restype).  tests/test_capi.py checks this table against qvx.h.
 _vp, _u32, _i32, _sz, _u64, _f32 = C.c_void_p, C.c_uint32, C.c_int, C.c_size_t, C.c_uint64, C.c_float
@@ -63,6 +63,13 @@ SIGNATURES = {
     "qvx_kv_page_bytes": ([_u32, _i32, _i32, _i32], _sz),
     "qvx_kv_map": ([_vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
     "qvx_rope_kv": ([_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _vp], _i32),
+    "qvx_norm_rope_kv": ([_vp, _i64, _u32, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _vp,
+                          _vp], _i32),
+    "qvx_kv_fork": ([_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp], _i32),
+    "qvx_kv_free": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _sz, _vp], _i32),
+    "qvx_kv_free_ws": ([_i32], _sz),
+    "qvx_kv_compact": ([_vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp], _i32),
+    "qvx_kv_copy": ([_vp, _i32, _vp, _vp, _i32, _vp], _i32),
     "qvx_attn_paged": ([_vp, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
     "qvx_attn_paged_ws": ([_vp, _i32, _i32, _i32], _sz),
     "qvx_attn_cross": ([_vp, _i64, _vp, _i64, _u32, _i32, _vp, _i32, _vp, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
@@ -316,6 +323,27 @@ class Rope(C.Structure):
         return c
 
 
+class QkNorm(C.Structure):
+    """Norms of each q and k head (qvx_qk_norm)."""
+
+    _fields_ = [("d_q_w", _vp), ("d_k_w", _vp), ("head_stride", _i32), ("eps", _f32)]
+
+    @classmethod
+    def of(cls, q_w=None, k_w=None, eps: float = 1e-6) -> "QkNorm":
+        """Weights in float32 device tensors: [head_dim] for all heads, or [heads, head_dim] each their own; None: not
+        normed."""
+        import torch
+        given = [w for w in (q_w, k_w) if w is not None]
+        for w in given:
+            if w.dtype != torch.float32 or w.dim() not in (1, 2) or not w.is_contiguous() or not w.is_cuda \
+                    or w.dim() != given[0].dim() or w.shape[-1] != given[0].shape[-1] or w.device != given[0].device:
+                raise ValueError("QkNorm.of: contiguous float32 device weights, of both alike [head_dim] or [heads, head_dim]")
+        stride = given[0].shape[-1] if given and given[0].dim() == 2 else 0
+        c = cls(q_w.data_ptr() if q_w is not None else None, k_w.data_ptr() if k_w is not None else None, stride, eps)
+        c.tensors = (q_w, k_w)
+        return c
+
+
 class KvStates(C.Structure):
     """An encoder's keys and values (qvx_kv_states)."""
 
@@ -357,6 +385,55 @@ def rope_kv(q_out: int, q_out_stride: int, q: int, q_stride: int, q_heads: int, 
     return lib().qvx_rope_kv(q_out, q_out_stride, q, q_stride, q_heads, k, k_stride, v, v_stride, n_tokens, head_dim,
                              C.byref(rope), pos, pos_stride, C.byref(cache) if cache is not None else None, slots,
                              stream)
+
+
+def norm_rope_kv(q_out: int, q_out_stride: int, q_out_type: int, q: int, q_stride: int, q_heads: int, k: int, k_stride: int,
+                 v: int, v_stride: int, n_tokens: int, head_dim: int, norm: QkNorm, rope: Rope, pos: int, pos_stride: int,
+                 cache: KvCache | None, slots: int, stream: int = 0) -> int:
+    """Norms of each q and k head, rotary positions and the append to the paged cache, q_out of q_out_type. Status."""
+    return lib().qvx_norm_rope_kv(q_out, q_out_stride, q_out_type, q, q_stride, q_heads, k, k_stride, v, v_stride, n_tokens,
+                                  head_dim, C.byref(norm), C.byref(rope), pos, pos_stride,
+                                  C.byref(cache) if cache is not None else None, slots, stream)
+
+
+def kv_fork(from_rows: int, to_rows: int, n: int, table: int, n_rows: int, table_width: int, page_size: int, lens: int,
+            extra: int, n_pages: int, free: int, n_free: int, taken_in: int, taken_out: int, pairs: int, n_pairs: int,
+            stream: int = 0) -> int:
+    """Forks of rows of the page table: full pages shared, last ones paired with fresh pages for kv_copy. Status."""
+    return lib().qvx_kv_fork(from_rows, to_rows, n, table, n_rows, table_width, page_size, lens, extra, n_pages, free,
+                             n_free, taken_in, taken_out, pairs, n_pairs, stream)
+
+
+def kv_free(rows: int, begin: int, end: int, n: int, table: int, n_rows: int, table_width: int, lens: int, extra: int,
+            n_pages: int, free: int, n_free: int, taken_in: int, taken_out: int, ws: int, ws_bytes: int,
+            stream: int = 0) -> int:
+    """Releases of rows (begin, end 0), or of columns begin[i] .. end[i] - 1 of them. Status."""
+    return lib().qvx_kv_free(rows, begin or None, end or None, n, table, n_rows, table_width, lens or None, extra, n_pages,
+                             free, n_free, taken_in, taken_out, ws or None, ws_bytes, stream)
+
+
+def kv_free_ws(n_pages: int) -> int:
+    """Bytes of kv_free's workspace."""
+    return lib().qvx_kv_free_ws(n_pages)
+
+
+def kv_compact(table: int, table_out: int, n_rows: int, table_width: int, extra: int, extra_out: int, n_pages: int,
+               free: int, free_out: int, n_free: int, taken: int, pairs: int, moved: int, stream: int = 0) -> int:
+    """Ids of the pages in use brought to the front; pairs and moved[0] for kv_copy, moved[1] pages in use. Status."""
+    return lib().qvx_kv_compact(table, table_out, n_rows, table_width, extra, extra_out, n_pages, free, free_out, n_free,
+                                taken, pairs, moved, stream)
+
+
+def kv_caches(caches):
+    """The array of several layers' caches that kv_copy takes."""
+    a = (KvCache * len(caches))(*caches)
+    a.caches = list(caches)
+    return a
+
+
+def kv_copy(caches, pairs: int, n_pairs: int, most_pairs: int, stream: int = 0) -> int:
+    """Copies of whole pages of all caches (kv_caches(...)), n_pairs 0: most_pairs of them. Status."""
+    return lib().qvx_kv_copy(caches, len(caches), pairs, n_pairs or None, most_pairs, stream)
 
 
 def attn_paged(out: int, out_stride: int, q: int, q_stride: int, q_heads: int, cache: KvCache, table: int,
@@ -607,6 +684,96 @@ def rope_kv_t(q, k, v, pos, rope: Rope, cache: KvCache | None = None, slots=None
         _check(rope_kv(*_rows(out, "out"), *_rows(q, "q"), heads, *kv, n, d, rope, pp, n, cache, sl, _stream()),
                "qvx_rope_kv")
     return out
+
+
+def norm_rope_kv_t(q, k, v, pos, norm: QkNorm, rope: Rope, cache: KvCache | None = None, slots=None, out=None, dtype=None):
+    """norm_rope_kv on device tensors, as rope_kv_t's; out (or dtype) in float32, float16 or bfloat16.  Returns q_out."""
+    import torch
+    n, heads, d = q.shape
+    _beside(rope, q.device, "rope")
+    _beside(norm, q.device, "norm")
+    for w, h in zip(norm.tensors, (heads, cache.kv_heads if cache is not None else None)):
+        if w is not None and (w.shape[-1] != d or (w.dim() == 2 and h is not None and w.shape[0] != h)):
+            raise ValueError(f"norm_rope_kv_t: weights of {d} values a head")
+    if cache is not None:
+        _beside(cache, q.device, "cache")
+    if out is None:  # with a cache, rows of padding are not written
+        out = (torch.empty if cache is None else torch.zeros)((n, heads, d), dtype=dtype or torch.float32, device=q.device)
+    if out.dtype not in _torch_types() or tuple(out.shape) != (n, heads, d) or out.device != q.device:
+        raise ValueError(f"norm_rope_kv_t: out is float32, float16 or bfloat16 [{n}, {heads}, {d}] on {q.device}")
+    if q.dtype != torch.float32:
+        raise ValueError("norm_rope_kv_t: q is float32")
+    for x, what in ((k, "k"), (v, "v")) if cache is not None else ():
+        if x is None or x.dtype != torch.float32 or tuple(x.shape) != (n, cache.kv_heads, d) or x.device != q.device:
+            raise ValueError(f"norm_rope_kv_t: {what} is float32 [{n}, {cache.kv_heads}, {d}] on {q.device}")
+    if cache is not None and slots is None:
+        raise ValueError("norm_rope_kv_t: a cache needs slots")
+    pp = _int32(pos.reshape(-1, n), (rope.n_axes, n), q.device, "pos")
+    kv = (*_rows(k, "k"), *_rows(v, "v")) if cache is not None else (0, 0, 0, 0)
+    sl = _int32(slots, (n,), q.device, "slots") if cache is not None else 0
+    with torch.cuda.device(q.device):
+        _check(norm_rope_kv(*_rows(out, "out"), _torch_types()[out.dtype], *_rows(q, "q"), heads, *kv, n, d, norm, rope, pp, n,
+                            cache, sl, _stream()), "qvx_norm_rope_kv")
+    return out
+
+
+def kv_fork_t(from_rows, to_rows, table, page_size: int, lens, extra, free, taken):
+    """kv_fork on int32 device tensors: table [rows, width], lens [rows], extra [pages] and taken [2] are written in place.
+    Returns (pairs [n, 2], n_pairs [1]) for kv_copy_t."""
+    import torch
+    n, dev = from_rows.shape[0], table.device
+    rows, width = table.shape
+    pairs = torch.full((n, 2), -1, dtype=torch.int32, device=dev)
+    n_pairs = torch.zeros(1, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _check(kv_fork(_int32(from_rows, (n,), dev, "from_rows"), _int32(to_rows, (n,), dev, "to_rows"), n,
+                       _int32(table, (rows, width), dev, "table"), rows, width, page_size, _int32(lens, (rows,), dev, "lens"),
+                       _int32(extra, extra.shape[:1], dev, "extra"), extra.shape[0], _int32(free, free.shape[:1], dev, "free"),
+                       free.shape[0], _int32(taken, (2,), dev, "taken"), taken.data_ptr(), pairs.data_ptr(),
+                       n_pairs.data_ptr(), _stream()), "qvx_kv_fork")
+    return pairs, n_pairs
+
+
+def kv_free_t(rows, table, lens, extra, free, taken, begin=None, end=None):
+    """kv_free on int32 device tensors, all of table [rows, width], lens, extra, free and taken [2] written in place."""
+    import torch
+    n, dev = rows.shape[0], table.device
+    (n_rows, width), pages = table.shape, extra.shape[0]
+    part = [_int32(x, (n,), dev, what) if x is not None else 0 for x, what in ((begin, "begin"), (end, "end"))]
+    with torch.cuda.device(dev):
+        ws = torch.empty(kv_free_ws(pages), dtype=torch.uint8, device=dev)
+        _check(kv_free(_int32(rows, (n,), dev, "rows"), *part, n, _int32(table, (n_rows, width), dev, "table"), n_rows, width,
+                       _int32(lens, (n_rows,), dev, "lens"), _int32(extra, (pages,), dev, "extra"), pages,
+                       _int32(free, free.shape[:1], dev, "free"), free.shape[0], _int32(taken, (2,), dev, "taken"),
+                       taken.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "qvx_kv_free")
+
+
+def kv_compact_t(table, extra, free, taken):
+    """kv_compact on int32 device tensors, table, extra and free written in place.  Returns (pairs, moved [2]) for kv_copy_t:
+    pages that move, and pages in use."""
+    import torch
+    dev = table.device
+    (rows, width), pages = table.shape, extra.shape[0]
+    pairs = torch.full((max(pages // 2, 1), 2), -1, dtype=torch.int32, device=dev)
+    moved = torch.zeros(2, dtype=torch.int32, device=dev)
+    tp, ep, fp = (_int32(x, shape, dev, what) for x, shape, what in
+                  ((table, (rows, width), "table"), (extra, (pages,), "extra"), (free, free.shape[:1], "free")))
+    with torch.cuda.device(dev):
+        _check(kv_compact(tp, tp, rows, width, ep, ep, pages, fp, fp, free.shape[0], _int32(taken, (2,), dev, "taken"),
+                          pairs.data_ptr(), moved.data_ptr(), _stream()), "qvx_kv_compact")
+    return pairs, moved
+
+
+def kv_copy_t(caches, pairs, n_pairs=None):
+    """kv_copy of a list of KvCache on pairs [n, 2] int32, the first n_pairs[0] of them."""
+    import torch
+    dev = pairs.device
+    for c in caches:
+        _beside(c, dev, "cache")
+    count = _int32(n_pairs, n_pairs.shape[:1], dev, "n_pairs") if n_pairs is not None else 0
+    with torch.cuda.device(dev):
+        _check(kv_copy(kv_caches(caches), _int32(pairs, (pairs.shape[0], 2), dev, "pairs"), count, pairs.shape[0], _stream()),
+               "qvx_kv_copy")
 
 
 def attn_paged_t(q, cache: KvCache, table, lens, scale: float | None = None, out=None, ws=None):

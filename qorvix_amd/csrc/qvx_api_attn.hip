@@ -1,9 +1,8 @@
 // qvx_api_attn.hip -- the extern "C" boundary of the attention calls (include/qvx.h): argument checks,
 // which run before any device work, and the bounds that the kernels' partition of the work needs.
+#include "qvx_api_kv.hpp"
 #include "qvx_attn.hpp"
 #include "qvx_kv.hpp"
-
-#include <cstdio>
 
 namespace qvx {
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
@@ -11,6 +10,7 @@ void launch_attn_join(const AttnCall& c, hipStream_t s);
 bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s);
 bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s);
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s);
+void launch_norm_rope(NormRopeCall c, uint32_t type, uint32_t q_type, bool vec, hipStream_t s);
 }  // namespace qvx
 
 using namespace qvx;
@@ -22,47 +22,6 @@ constexpr int kMaxLen = 0x7ffffff0;  // the kernels round lengths up to whole ti
 constexpr int kMaxTiles = 0x3fffffff;  // and add a chunk's first tile and length, each at most this
 constexpr int64_t kMaxPitch = 64ll << 20;  // sixteen rows stay far inside 32-bit offsets
 constexpr float kLeastScale = 1e-30f;       // far above the subnormal numbers
-
-inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-int attn_status(bool launched) {
-  const hipError_t e = hipGetLastError();
-  if (launched && e == hipSuccess) return QVX_OK;
-  std::fprintf(stderr, "qvx: HIP error %d (%s)\n", (int)e, hipGetErrorString(e));
-  return QVX_E_HIP;
-}
-
-// Bytes of n values of a cache or states type; 0 for another type.
-int64_t value_bytes(uint32_t type, int64_t n) {
-  switch (type) {
-    case T_F32: return 4 * n;
-    case T_F16: case T_BF16: return 2 * n;
-    case T_Q8_0: return n + n / 16;
-    default: return 0;
-  }
-}
-
-bool head_dim_ok(uint32_t type, int d) { return d > 0 && d <= 256 && d % (type == T_Q8_0 ? 32 : 8) == 0; }
-
-int64_t page_bytes(uint32_t type, int kv_heads, int page_size, int head_dim) {
-  if (!value_bytes(type, 1) || kv_heads <= 0 || page_size <= 0 || !head_dim_ok(type, head_dim)) return 0;
-  const int64_t rows = (int64_t)kv_heads * page_size;
-  if (rows > (1ll << 40)) return 0;
-  return (value_bytes(type, rows * head_dim) + 15) / 16 * 16;
-}
-
-int check_cache(const qvx_kv_cache* c, int64_t* stride) {
-  if (!c) return QVX_E_NULL;
-  if (!value_bytes(c->type, 1)) return QVX_E_TYPE;
-  const int64_t packed = page_bytes(c->type, c->kv_heads, c->page_size, c->head_dim);
-  if (!packed || c->n_pages <= 0) return QVX_E_SHAPE;
-  if ((int64_t)c->n_pages * c->page_size > 0x7fffffffll) return QVX_E_RANGE;
-  if (c->page_stride && (c->page_stride < packed || c->page_stride % 16)) return QVX_E_RANGE;
-  if (!c->d_k || !c->d_v) return QVX_E_NULL;
-  if (!aligned(c->d_k, 16) || !aligned(c->d_v, 16)) return QVX_E_RANGE;
-  *stride = c->page_stride ? c->page_stride : packed;
-  return QVX_OK;
-}
 
 // The partition of a call whose heads, pages and sequences are filled in: how many work items are
 // aimed at, and the bounds that grid and workspace are sized by.  Workgroups to fill the chip: two a CU.
@@ -217,6 +176,68 @@ int check_cross(const qvx_kv_states* st, uint32_t q_type, int q_heads, bool ragg
   return (*wide ? plan16 : plan_split)(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
+// What qvx_rope_kv and qvx_norm_rope_kv check alike.  vec: rows on 16-byte addresses (q_out's of 16 bits on 8-byte ones).
+int check_rope(void* d_q_out, int64_t q_out_stride, uint32_t q_out_type, const float* d_q, int64_t q_stride, int q_heads,
+               const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens, int head_dim,
+               const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
+               const int32_t* d_slots, RopeCall& c, uint32_t* type, bool* vec) {
+  if (n_tokens <= 0) return QVX_E_NVEC;
+  if (!rope) return QVX_E_NULL;
+  *type = T_F32;
+  if (cache) {
+    if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
+    if (cache->head_dim != head_dim) return QVX_E_SHAPE;
+    *type = cache->type;
+    c.kv_heads = cache->kv_heads;
+    c.k_pages = static_cast<uint8_t*>(cache->d_k);
+    c.v_pages = static_cast<uint8_t*>(cache->d_v);
+    c.scale_off = (int64_t)cache->kv_heads * cache->page_size * head_dim;
+    c.page_size = cache->page_size;
+    c.n_slots = (int64_t)cache->n_pages * cache->page_size;
+  }
+  if (rope->pairing != QVX_ROPE_HALVES && rope->pairing != QVX_ROPE_PAIRS) return QVX_E_VARIANT;
+  if (q_heads < 0 || q_heads + c.kv_heads <= 0 || !head_dim_ok(T_F32, head_dim) || rope->rot_dim < 0 ||
+      rope->rot_dim > head_dim || rope->rot_dim % 8 || rope->n_axes < 1 || rope->n_axes > 4)
+    return QVX_E_SHAPE;
+  const int64_t q_row = (int64_t)q_heads * head_dim, kv_row = (int64_t)c.kv_heads * head_dim;
+  if (q_stride < 0 || q_out_stride < q_row || (cache && (k_stride < 0 || v_stride < 0)) || pos_stride < 0 ||
+      (rope->n_axes > 1 && pos_stride < n_tokens))
+    return QVX_E_SHAPE;
+  if (q_row > 0x7fffffffll / 16 || kv_row > 0x7fffffffll / 16 || n_tokens > kRopeMaxTokens * kMostWgs)
+    return QVX_E_RANGE;
+  if ((q_heads && (!d_q || !d_q_out)) || (cache && (!d_k || !d_v || !d_slots)) ||
+      (rope->rot_dim && (!rope->d_inv_freq || !d_pos)))
+    return QVX_E_NULL;
+  if (d_q == d_q_out && (q_stride != q_out_stride || q_out_type != T_F32)) return QVX_E_RANGE;
+  const uintptr_t size = q_out_type == T_F32 ? 4 : 2;
+  if (q_out_type != T_F32 && !aligned(d_q_out, 2)) return QVX_E_RANGE;
+  c.q_out = static_cast<float*>(d_q_out);
+  c.q = d_q;
+  c.q_out_stride = q_out_stride;
+  c.q_stride = q_stride;
+  c.q_heads = q_heads;
+  c.head_dim = head_dim;
+  c.n_tokens = n_tokens;
+  c.inv_freq = rope->d_inv_freq;
+  c.axis = rope->d_axis;
+  c.rot_dim = rope->rot_dim;
+  c.n_axes = rope->n_axes;
+  c.halves = rope->pairing == QVX_ROPE_HALVES;
+  c.scale = rope->scale;
+  c.pos = d_pos;
+  c.pos_stride = pos_stride;
+  *vec = q_stride % 4 == 0 && q_out_stride % 4 == 0 && aligned(d_q, 16) && aligned(d_q_out, 4 * size);
+  if (cache) {
+    c.k = d_k;
+    c.v = d_v;
+    c.k_stride = k_stride;
+    c.v_stride = v_stride;
+    c.slots = d_slots;
+    *vec = *vec && k_stride % 4 == 0 && v_stride % 4 == 0 && aligned(d_k, 16) && aligned(d_v, 16);
+  }
+  return QVX_OK;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 }  // namespace
@@ -263,60 +284,39 @@ int qvx_rope_kv(float* d_q_out, int64_t q_out_stride, const float* d_q, int64_t 
                 const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens, int head_dim,
                 const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride, const qvx_kv_cache* cache,
                 const int32_t* d_slots, void* stream) {
-  if (n_tokens <= 0) return QVX_E_NVEC;
-  if (!rope) return QVX_E_NULL;
   RopeCall c{};
-  uint32_t type = T_F32;
-  if (cache) {
-    if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
-    if (cache->head_dim != head_dim) return QVX_E_SHAPE;
-    type = cache->type;
-    c.kv_heads = cache->kv_heads;
-    c.k_pages = static_cast<uint8_t*>(cache->d_k);
-    c.v_pages = static_cast<uint8_t*>(cache->d_v);
-    c.scale_off = (int64_t)cache->kv_heads * cache->page_size * head_dim;
-    c.page_size = cache->page_size;
-    c.n_slots = (int64_t)cache->n_pages * cache->page_size;
-  }
-  if (rope->pairing != QVX_ROPE_HALVES && rope->pairing != QVX_ROPE_PAIRS) return QVX_E_VARIANT;
-  if (q_heads < 0 || q_heads + c.kv_heads <= 0 || !head_dim_ok(T_F32, head_dim) || rope->rot_dim < 0 ||
-      rope->rot_dim > head_dim || rope->rot_dim % 8 || rope->n_axes < 1 || rope->n_axes > 4)
-    return QVX_E_SHAPE;
-  const int64_t q_row = (int64_t)q_heads * head_dim, kv_row = (int64_t)c.kv_heads * head_dim;
-  if (q_stride < 0 || q_out_stride < q_row || (cache && (k_stride < 0 || v_stride < 0)) || pos_stride < 0 ||
-      (rope->n_axes > 1 && pos_stride < n_tokens))
-    return QVX_E_SHAPE;
-  if (q_row > 0x7fffffffll / 16 || kv_row > 0x7fffffffll / 16 || n_tokens > kRopeMaxTokens * kMostWgs)
-    return QVX_E_RANGE;
-  if ((q_heads && (!d_q || !d_q_out)) || (cache && (!d_k || !d_v || !d_slots)) ||
-      (rope->rot_dim && (!rope->d_inv_freq || !d_pos)))
-    return QVX_E_NULL;
-  if (d_q == d_q_out && q_stride != q_out_stride) return QVX_E_RANGE;
-  c.q_out = d_q_out;
-  c.q = d_q;
-  c.q_out_stride = q_out_stride;
-  c.q_stride = q_stride;
-  c.q_heads = q_heads;
-  c.head_dim = head_dim;
-  c.n_tokens = n_tokens;
-  c.inv_freq = rope->d_inv_freq;
-  c.axis = rope->d_axis;
-  c.rot_dim = rope->rot_dim;
-  c.n_axes = rope->n_axes;
-  c.halves = rope->pairing == QVX_ROPE_HALVES;
-  c.scale = rope->scale;
-  c.pos = d_pos;
-  c.pos_stride = pos_stride;
-  bool vec = q_stride % 4 == 0 && q_out_stride % 4 == 0 && aligned(d_q, 16) && aligned(d_q_out, 16);
-  if (cache) {
-    c.k = d_k;
-    c.v = d_v;
-    c.k_stride = k_stride;
-    c.v_stride = v_stride;
-    c.slots = d_slots;
-    vec = vec && k_stride % 4 == 0 && v_stride % 4 == 0 && aligned(d_k, 16) && aligned(d_v, 16);
-  }
+  uint32_t type = 0;
+  bool vec = false;
+  if (int rc = check_rope(d_q_out, q_out_stride, T_F32, d_q, q_stride, q_heads, d_k, k_stride, d_v, v_stride, n_tokens,
+                          head_dim, rope, d_pos, pos_stride, cache, d_slots, c, &type, &vec);
+      rc != QVX_OK)
+    return rc;
   launch_rope_kv(c, type, vec, static_cast<hipStream_t>(stream));
+  return attn_status(true);
+}
+
+int qvx_norm_rope_kv(void* d_q_out, int64_t q_out_stride, uint32_t q_out_type, const float* d_q, int64_t q_stride,
+                     int q_heads, const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride, int n_tokens,
+                     int head_dim, const qvx_qk_norm* norm, const qvx_rope* rope, const int32_t* d_pos, int64_t pos_stride,
+                     const qvx_kv_cache* cache, const int32_t* d_slots, void* stream) {
+  NormRopeCall c{};
+  uint32_t type = 0;
+  bool vec = false;
+  if (!norm) return QVX_E_NULL;
+  if (q_out_type != T_F32 && q_out_type != T_F16 && q_out_type != T_BF16) return QVX_E_TYPE;
+  if (int rc = check_rope(d_q_out, q_out_stride, q_out_type, d_q, q_stride, q_heads, d_k, k_stride, d_v, v_stride, n_tokens,
+                          head_dim, rope, d_pos, pos_stride, cache, d_slots, c, &type, &vec);
+      rc != QVX_OK)
+    return rc;
+  if (norm->head_stride != 0 && norm->head_stride < head_dim) return QVX_E_SHAPE;
+  if (!(norm->eps >= 0.0f)) return QVX_E_RANGE;
+  c.q_typed = d_q_out;
+  c.q_w = norm->d_q_w;
+  c.k_w = norm->d_k_w;
+  c.w_stride = norm->head_stride;
+  c.eps = norm->eps;
+  c.inv_dim = 1.0 / head_dim;
+  launch_norm_rope(c, type, q_out_type, vec, static_cast<hipStream_t>(stream));
   return attn_status(true);
 }
 

@@ -43,4 +43,13 @@ struct RopeCall {
   int tokens_wg, rows_wg;
 };
 
+// With norms: the weights of a head are w_stride values from the last one's (0: all heads' alike), null: no norm.
+struct NormRopeCall : RopeCall {
+  void* q_typed;  // in place of q_out
+  const float *q_w, *k_w;
+  int w_stride, lanes_log;
+  float eps;
+  double inv_dim;
+};
+
 }  // namespace qvx

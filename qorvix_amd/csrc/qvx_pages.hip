@@ -1,0 +1,391 @@
+// qvx_pages.hip -- pages of a cache that several sequences hold, on gfx950: forks, copies, releases, compaction.
+//
+// extra[p] counts the rows that hold page p beside the first, so a page of one owner needs no upkeep.  A fork shares a
+// sequence's full pages (extra + 1 each) and takes a fresh page for its last one where that is not full, which a copy then
+// fills: no shared page is ever appended to.  A release takes one holder from each page; pages without any go back to the
+// free list.  All results are whole numbers and the same in every run: counts meet in integer atomics, whose order does
+// not matter, and pages return in the order of their ids, not of their release.
+//
+// Bound by latency but for the copy and the compaction's copy, which the bytes bound.
+#include "qvx_pages.hpp"
+
+namespace qvx {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ bool page_ok(int id, int n_pages) { return (unsigned)id < (unsigned)n_pages; }
+
+// Sum over the workgroup, in every thread; `part`: LDS of a word a wave, free again at return.
+template <int THREADS> __device__ __forceinline__ int block_sum(int x, int* part) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) sum += part[w];
+  __syncthreads();
+  return sum;
+}
+
+// Sum over the threads before this one.
+template <int THREADS> __device__ __forceinline__ int block_before(int x, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int upto = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(upto, d);
+    if (lane >= d) upto += y;
+  }
+  if (lane == 63) part[wave] = upto;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w == wave) before = total;
+    total += part[w];
+  }
+  __syncthreads();
+  return before + upto - x;
+}
+
+// ---- fork --------------------------------------------------------------------------------------------
+//
+// Every workgroup looks all forks through for itself (a few loads a thread): how many want a fresh page before its own,
+// whether the free list reaches, whether any is wrong.  Then it takes forks blockIdx.x, + gridDim.x, ...
+
+// What fork i wants: 1 where its sequence's last page is not full; `bad` gets status bits.
+__device__ __forceinline__ int fork_wants(const ForkCall& c, int i, int& bad) {
+  const int from = c.from[i], to = c.to[i];
+  if ((unsigned)from >= (unsigned)c.n_rows || (unsigned)to >= (unsigned)c.n_rows || from == to) {
+    bad |= QVX_MAP_SEQUENCE;
+    return 0;
+  }
+  const int len = c.lens[from];
+  if (len < 0) bad |= QVX_MAP_NEGATIVE;
+  if (len > (long long)c.table_width * c.page_size) bad |= QVX_MAP_COLUMNS;
+  return len > 0 && len % c.page_size != 0;
+}
+
+__global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
+  extern __shared__ int32_t rank[];  // [n] fresh pages of the forks before
+  __shared__ int part[kThreads / 64];
+  const int tid = threadIdx.x, taken = c.taken_in[0];
+  int bad = taken < 0 ? QVX_MAP_NEGATIVE : 0, all = 0;
+  for (int i0 = 0; i0 < c.n; i0 += kThreads) {
+    const int i = i0 + tid;
+    const int wants = i < c.n ? fork_wants(c, i, bad) : 0;
+    int total;
+    const int before = block_before<kThreads>(wants, part, total);
+    if (i < c.n) rank[i] = all + before;
+    all += total;
+  }
+  int status = 0;
+#pragma unroll
+  for (int b = 1; b <= QVX_MAP_SEQUENCE; b *= 2) status |= __syncthreads_or(bad & b) ? b : 0;
+  if (taken >= 0 && (long long)taken + all > c.n_free) status |= QVX_MAP_PAGES;
+  if ((write & kForkTotals) && blockIdx.x == 0 && tid == 0) {
+    c.taken_out[0] = status ? taken : taken + all;
+    c.taken_out[1] = status;
+    *c.n_pairs = status ? 0 : all;
+  }
+  if (!(write & kForkRows) || status) return;
+  for (int i = blockIdx.x; i < c.n; i += gridDim.x) {
+    const int from = c.from[i], to = c.to[i], len = c.lens[from];
+    const int full = len / c.page_size, left = len - full * c.page_size;
+    const int32_t* old = c.table + (int64_t)from * c.table_width;
+    int32_t* row = c.table + (int64_t)to * c.table_width;
+    for (int col = tid; col < c.table_width; col += kThreads) {
+      int id = -1;
+      if (col < full) {
+        id = old[col];
+        if (page_ok(id, c.n_pages)) atomicAdd(&c.extra[id], 1);
+      } else if (col == full && left) {
+        id = taken + rank[i] < c.n_free ? c.free_list[taken + rank[i]] : -1;  // lengths that another fork changes: no place
+        c.pairs[2 * rank[i]] = old[col];
+        c.pairs[2 * rank[i] + 1] = id;
+      }
+      row[col] = id;
+    }
+    if (tid == 0) c.lens[to] = len;
+  }
+}
+
+// ---- release -----------------------------------------------------------------------------------------
+//
+// First every entry is taken out of the table and one holder from its page, which leaves -1 in extra where there was
+// none beside.  Then those are counted, range by range of ids, and stored in front of what is free.
+
+// Entries of row i, by the threads `at`, at + step, ...
+__device__ __forceinline__ void free_row(const FreeCall& c, int i, int at, int step) {
+  const int row = c.rows[i];
+  if ((unsigned)row >= (unsigned)c.n_rows) return;
+  const int begin = c.begin ? min(max(c.begin[i], 0), c.table_width) : 0, end = c.end ? min(c.end[i], c.table_width) : c.table_width;
+  int32_t* entry = c.table + (int64_t)row * c.table_width;
+  for (int col = begin + at; col < end; col += step) {
+    // by exchange: a row that is listed twice is released once
+    const int id = entry[col] < 0 ? -1 : atomicExch(&entry[col], -1);
+    if (page_ok(id, c.n_pages)) atomicSub(&c.extra[id], 1);
+  }
+  if (at == 0 && !c.begin && !c.end) c.lens[row] = 0;
+}
+
+__global__ __launch_bounds__(kThreads) void k_free_mark(FreeCall c) {
+  for (int i = blockIdx.x; i < c.n; i += gridDim.x)
+    free_row(c, i, (int)blockIdx.y * kThreads + threadIdx.x, (int)gridDim.y * kThreads);
+}
+
+// Pages freed in each range of kFreePages.
+__global__ __launch_bounds__(1024) void k_free_count(FreeCall c) {
+  __shared__ int part[16];
+  const int p0 = (int)blockIdx.x * kFreePages;
+  int mine = 0;
+  for (int p = p0 + threadIdx.x; p < min(p0 + kFreePages, c.n_pages); p += 1024) mine += c.extra[p] < 0;
+  mine = block_sum<1024>(mine, part);
+  if (threadIdx.x == 0) c.counts[blockIdx.x] = mine;
+  // the count taken so far, as the next launch's first workgroup may overwrite it before the others read it
+  if (threadIdx.x == 0 && blockIdx.x == 0) c.counts[gridDim.x] = c.taken_in[0];
+}
+
+// The free list's front and the totals.  ONE: this workgroup is the only one and counts for itself; MARK: it also takes the
+// entries out.
+template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_store(FreeCall c) {
+  __shared__ int part[16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  constexpr int kEach = kFreePages / 1024;
+  if constexpr (MARK) {
+    for (int i = tid >> 6; i < c.n; i += 16) free_row(c, i, lane, 64);
+    __threadfence();  // the counts are taken where the atomics of all waves have arrived
+    __syncthreads();
+  }
+  auto gone = [&](int p) {
+    return MARK ? __hip_atomic_load(&c.extra[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0 : c.extra[p] < 0;
+  };
+  const int p0 = (int)blockIdx.x * kFreePages, end = ONE ? c.n_pages : min(p0 + kFreePages, c.n_pages);
+  int before = 0, all = 0;
+  if constexpr (ONE) {
+    int mine = 0;
+    for (int p = tid; p < end; p += 1024) mine += gone(p);
+    all = block_sum<1024>(mine, part);
+  } else {
+    const int blocks = (c.n_pages + kFreePages - 1) / kFreePages;
+    int mine = 0, past = 0;
+    for (int b = tid; b < blocks; b += 1024) {
+      const int x = c.counts[b];
+      mine += x;
+      past += b < (int)blockIdx.x ? x : 0;
+    }
+    all = block_sum<1024>(mine, part);
+    before = block_sum<1024>(past, part);
+  }
+  int bad = 0;
+  if (blockIdx.x == 0)
+    for (int i = tid; i < c.n; i += 1024) bad |= (unsigned)c.rows[i] >= (unsigned)c.n_rows;
+  const int bad_row = __syncthreads_or(bad);
+  const int taken = ONE ? c.taken_in[0] : c.counts[gridDim.x], first = taken - all;  // may be negative: ids without a place are lost, and said so
+  for (int q = p0; q < end; q += 1024 * kEach) {
+    // a thread takes kEach pages in a row: one scan for all of them
+    int flags = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = q + tid * kEach + j;
+      if (p < end && gone(p)) flags |= 1 << j;
+    }
+    int total, at = first + before + block_before<1024>(__builtin_popcount(flags), part, total);
+    before += total;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (!(flags >> j & 1)) continue;
+      const int p = q + tid * kEach + j;
+      c.extra[p] = 0;
+      if (at >= 0 && at < c.n_free) c.free_list[at] = p;
+      ++at;
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    c.taken_out[0] = max(first, 0);
+    c.taken_out[1] = (bad_row ? QVX_MAP_SEQUENCE : 0) | (taken < 0 ? QVX_MAP_NEGATIVE : 0) |
+                     (first < 0 || taken > c.n_free ? QVX_MAP_PAGES : 0);
+  }
+}
+
+// ---- compaction --------------------------------------------------------------------------------------
+//
+// Pages in use are those that the free list does not name.  With n of them, each of id n or above moves to an unused id
+// below n, the r-th to the r-th in ascending order.  Every workgroup sets the free pages' bits in LDS for itself (one bit a page) and
+// sums them up by words of kRun bits, so that any page's rank is a few population counts; then it takes its share of the
+// outputs.  One launch; a second where the free list is rewritten in place, which the others read.
+
+constexpr int kCompactThreads = 1024, kRun = 256;  // bits of a run
+
+struct FreeBits {
+  const uint32_t* bits;
+  const int* runs;  // free pages before each run
+  int n_pages;
+  __device__ bool is_free(int p) const { return bits[p >> 5] >> (p & 31) & 1; }
+  __device__ int free_before(int p) const {  // p up to n_pages
+    int n = runs[p / kRun];
+    for (int w = p / kRun * (kRun / 32); w < p >> 5; ++w) n += __builtin_popcount(bits[w]);
+    return p & 31 ? n + __builtin_popcount(bits[p >> 5] & ((1u << (p & 31)) - 1)) : n;
+  }
+};
+
+// The r-th free page (r below the free pages' number): bisection over the runs, then its words.
+__device__ inline int free_at(const FreeBits& f, int r, int n_runs) {
+  int lo = 0, hi = n_runs - 1;  // the last run with at most r free pages before it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (f.runs[mid] <= r) lo = mid; else hi = mid - 1;
+  }
+  int left = r - f.runs[lo], w = lo * (kRun / 32);
+  for (int n; left >= (n = __builtin_popcount(f.bits[w])); ++w) left -= n;
+  uint32_t b = f.bits[w];
+  for (; left; --left) b &= b - 1;
+  return 32 * w + __builtin_ctz(b);
+}
+
+__global__ __launch_bounds__(kCompactThreads) void k_kv_compact(CompactCall c, bool in_place) {
+  extern __shared__ uint32_t lds[];
+  __shared__ int part[kCompactThreads / 64];
+  const int tid = threadIdx.x, runs = c.n_pages / kRun + 1;
+  const int whole = runs * (kRun / 32);  // words of whole runs
+  int* sums = reinterpret_cast<int*>(lds + whole);
+  for (int w = tid; w < whole; w += kCompactThreads) lds[w] = 0;
+  __syncthreads();
+  const int taken = min(max(c.taken[0], 0), c.n_free);
+  for (int i = taken + tid; i < c.n_free; i += kCompactThreads) {
+    const int id = c.free_list[i];
+    if (page_ok(id, c.n_pages)) atomicOr(&lds[id >> 5], 1u << (id & 31));
+  }
+  __syncthreads();
+  int free_pages = 0;
+  for (int r0 = 0; r0 < runs; r0 += kCompactThreads) {
+    const int r = r0 + tid;
+    int n = 0;
+    if (r < runs)
+      for (int w = 0; w < kRun / 32; ++w) n += __builtin_popcount(lds[r * (kRun / 32) + w]);
+    int total;
+    const int before = block_before<kCompactThreads>(n, part, total);
+    if (r < runs) sums[r] = free_pages + before;
+    free_pages += total;
+  }
+  __syncthreads();
+  const FreeBits f{lds, sums, c.n_pages};
+  const int used = c.n_pages - free_pages;  // ids below it are in use afterwards
+  const int moves = f.free_before(used);    // as many free ids below as used ones from it on
+  const int used_low = used - moves;
+  // Where page p, in use, lies afterwards.
+  auto place = [&](int p) { return p < used ? p : free_at(f, p - f.free_before(p) - used_low, runs); };
+  const int64_t step = (int64_t)gridDim.x * kCompactThreads, me = (int64_t)blockIdx.x * kCompactThreads + tid;
+  for (int64_t i = me; i < c.entries; i += step) {
+    const int id = c.table[i];
+    c.table_out[i] = page_ok(id, c.n_pages) && !f.is_free(id) ? place(id) : id;
+  }
+  for (int64_t p = me; p < c.n_pages; p += step) {
+    const bool gone = f.is_free((int)p);
+    if (gone && p < used) continue;  // the page that moves here brings its count
+    const int x = gone ? 0 : c.extra[p];
+    if (!gone && p >= used) {
+      const int to = place((int)p), r = (int)p - f.free_before((int)p) - used_low;
+      c.extra_out[to] = x;
+      c.pairs[2 * r] = (int)p;
+      c.pairs[2 * r + 1] = to;
+    }
+    c.extra_out[p] = gone || p >= used ? 0 : x;
+  }
+  if (!in_place)
+    for (int64_t i = me; i < c.n_free; i += step) {
+      const int64_t id = used + (i - taken);
+      c.free_out[i] = i < taken ? c.free_list[i] : id < c.n_pages ? (int)id : -1;
+    }
+  if (me == 0) {
+    c.moved[0] = moves;
+    c.moved[1] = used;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_compact_list(CompactCall c) {
+  const int taken = min(max(c.taken[0], 0), c.n_free), used = c.moved[1];
+  for (int64_t i = taken + (int64_t)blockIdx.x * kThreads + threadIdx.x; i < c.n_free; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t id = used + (i - taken);
+    c.free_out[i] = id < c.n_pages ? (int)id : -1;
+  }
+}
+
+// ---- copies ------------------------------------------------------------------------------------------
+//
+// Units of 16 KB (64 bytes a thread in four loads that go out together) of a pair's page of K or V of a cache, taken in
+// turn by as many workgroups as the card holds: the number of pairs is the device's.
+
+constexpr int kCopyUnit = 16 << 10, kCopyWgs = 2048;
+
+__global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c) {
+  const int parts = (int)((c.page_bytes + kCopyUnit - 1) / kCopyUnit), each = c.n_caches * 2 * parts;
+  const int count = c.count ? min(max(*c.count, 0), c.most) : c.most;
+  for (int64_t u = blockIdx.x; u < (int64_t)count * each; u += gridDim.x) {
+    const int pair = (int)(u / each), rest = (int)(u - (int64_t)pair * each), plane = rest / parts, part = rest - plane * parts;
+    const int src = c.pairs[2 * pair], dst = c.pairs[2 * pair + 1];
+    if (!page_ok(src, c.n_pages) || !page_ok(dst, c.n_pages) || src == dst) continue;
+    const auto& x = c.cache[plane >> 1];
+    uint8_t* base = plane & 1 ? x.v : x.k;
+    const int64_t at = (int64_t)part * kCopyUnit + 16 * threadIdx.x;
+    const uint8_t* from = base + src * x.stride;
+    uint8_t* to = base + dst * x.stride;
+    uint4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at + j * 16 * kThreads < c.page_bytes) w[j] = *reinterpret_cast<const uint4*>(from + at + j * 16 * kThreads);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at + j * 16 * kThreads < c.page_bytes) *reinterpret_cast<uint4*>(to + at + j * 16 * kThreads) = w[j];
+  }
+}
+
+}  // namespace
+
+void launch_kv_fork(const ForkCall& c, bool alias, hipStream_t s) {
+  const size_t lds = (size_t)c.n * sizeof(int32_t);  // at most 64 KB
+  // Totals that lie on what the others read are stored by a launch behind them.
+  k_kv_fork<<<std::min(c.n, 1024), kThreads, lds, s>>>(c, alias ? kForkRows : kForkRows | kForkTotals);
+  if (alias) k_kv_fork<<<1, kThreads, lds, s>>>(c, kForkTotals);
+}
+
+void launch_kv_free(const FreeCall& c, hipStream_t s) {
+  const bool one = c.n_pages <= 2 * kFreePages;
+  const int64_t entries = (int64_t)c.n * ((c.table_width + 63) / 64 * 64);
+  if (one && entries <= 8192) {
+    k_free_store<true, true><<<1, 1024, 0, s>>>(c);
+    return;
+  }
+  const int cols = std::min((c.table_width + kThreads - 1) / kThreads, 64);
+  k_free_mark<<<dim3(std::min(c.n, 4096), cols), kThreads, 0, s>>>(c);
+  if (one) {
+    k_free_store<true, false><<<1, 1024, 0, s>>>(c);
+    return;
+  }
+  const int blocks = (c.n_pages + kFreePages - 1) / kFreePages;
+  k_free_count<<<blocks, 1024, 0, s>>>(c);
+  k_free_store<false, false><<<blocks, 1024, 0, s>>>(c);
+}
+
+bool launch_kv_compact(const CompactCall& c, bool in_place, hipStream_t s) {
+  static LdsLimit lim;
+  const int runs = c.n_pages / kRun + 1;
+  const size_t lds = (size_t)runs * (kRun / 32) * 4 + (size_t)runs * 4;
+  if (!lds_ready(reinterpret_cast<const void*>(&k_kv_compact), lim, lds)) return false;
+  const int64_t most = std::max<int64_t>(std::max<int64_t>(c.entries, c.n_pages), c.n_free);
+  const int wgs = (int)std::min<int64_t>(256, (most + kCompactThreads - 1) / kCompactThreads);
+  k_kv_compact<<<wgs, kCompactThreads, lds, s>>>(c, in_place);
+  if (in_place) k_compact_list<<<std::max(1, std::min(256, (c.n_free + kThreads - 1) / kThreads)), kThreads, 0, s>>>(c);
+  return true;
+}
+
+void launch_kv_copy(const CopyCall& c, hipStream_t s) {
+  const int64_t units = (int64_t)c.most * c.n_caches * 2 * ((c.page_bytes + kCopyUnit - 1) / kCopyUnit);
+  k_kv_copy<<<(unsigned)std::min<int64_t>(units, kCopyWgs), kThreads, 0, s>>>(c);
+}
+
+}  // namespace qvx
