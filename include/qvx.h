@@ -387,6 +387,38 @@ int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q
 /* Workspace of that call; 0 also where it needs none, or would be refused. */
 size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width);
 
+/* Attention of each sequence's last tokens over the paged cache, with a window and a few first tokens that stay visible
+ * (sinks): the queries d_offsets[b] .. d_offsets[b + 1] - 1 of n_q are the last tokens of sequence b's d_lens[b] (as
+ * qvx_kv_map leaves offsets and lengths), so of one token (a decode step) or of a prompt's piece, and the one at position p sees
+ * the keys j <= p with j > p - window or j < sinks; with a window of at least the length all of its past.  d_offsets NULL:
+ * n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  window and sinks not below 0 (else QVX_E_SHAPE).  q and out
+ * share q_type: F32, F16 or BF16; rows behind the last sequence's are left as they were.  A row that sees no key (positions
+ * below 0, a window of 0 without sinks, pages outside the cache, which need not be held behind the window) gets zeros.
+ * Keys that no query of the sequence sees are not read.  All else, q = out, lengths, workspace, is as in
+ * qvx_attn_paged. */
+int qvx_attn_window(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                    const int32_t* d_offsets, int n_q, const qvx_kv_cache* cache, const int32_t* d_table, int table_width,
+                    const int32_t* d_lens, int n_seqs, int window, int sinks, float scale, void* d_ws, size_t ws_bytes,
+                    void* stream);
+/* Workspace of that call; 0 also where it needs none, or would be refused. */
+size_t qvx_attn_window_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_q, int n_seqs, int table_width,
+                          int window, int sinks);
+
+/* Attention of one new token a sequence, as qvx_attn_paged, for batches that share long prefixes (forks, or a server's
+ * common instructions): group g is the sequences d_groups[g] .. d_groups[g + 1] - 1 (the first begins at 0 and the last ends at
+ * n_seqs, whatever the ends hold; d_groups NULL: one group; at most n_seqs of them, more -> QVX_E_RANGE), whose first d_shared[g] tokens
+ * are those on the pages of the group's first sequence, and are read once for all of them; the tokens behind are each
+ * sequence's own.  The result is that of the whole rows: joined from the two parts' maxima and sums.  A sequence shorter
+ * than d_shared[g] attends the first d_lens[b] of the shared tokens.  q and out share q_type: F32, F16 or BF16.  All else is
+ * as in qvx_attn_paged; d_ws is always needed. */
+int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                    const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens, int n_seqs,
+                    const int32_t* d_groups, const int32_t* d_shared, int n_groups, float scale, void* d_ws,
+                    size_t ws_bytes, void* stream);
+/* Workspace of that call; 0 where it would be refused. */
+size_t qvx_attn_shared_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_seqs, int table_width,
+                          int n_groups);
+
 /* An encoder's keys and values: value i of head h of state j of sequence b at d_k[b * batch_stride +
  * j * row_stride + h * head_stride + i] (elements; d_v alike), F32, F16 or BF16, max_len states a sequence at most
  * (up to 2^31 - 16).  Strides and addresses in multiples of 16 bytes, row_stride at least head_dim and at most 64 Mi bytes; with

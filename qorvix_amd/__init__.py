@@ -72,6 +72,12 @@ SIGNATURES = {
     "qvx_kv_copy": ([_vp, _i32, _vp, _vp, _i32, _vp], _i32),
     "qvx_attn_paged": ([_vp, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
     "qvx_attn_paged_ws": ([_vp, _i32, _i32, _i32], _sz),
+    "qvx_attn_window": ([_vp, _i64, _vp, _i64, _u32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _sz,
+                         _vp], _i32),
+    "qvx_attn_window_ws": ([_vp, _u32, _i32, _i32, _i32, _i32, _i32, _i32], _sz),
+    "qvx_attn_shared": ([_vp, _i64, _vp, _i64, _u32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _f32, _vp, _sz, _vp],
+                        _i32),
+    "qvx_attn_shared_ws": ([_vp, _u32, _i32, _i32, _i32, _i32], _sz),
     "qvx_attn_cross": ([_vp, _i64, _vp, _i64, _u32, _i32, _vp, _i32, _vp, _vp, _i32, _f32, _vp, _sz, _vp], _i32),
     "qvx_attn_cross_ws": ([_vp, _u32, _i32, _i32, _i32], _sz),
     "qvx_qgemm_f16": ([_vp, _vp, _u32, _vp, _i32, _i32, _i32, _i32, _vp], _i32),
@@ -448,6 +454,38 @@ def attn_paged_ws(cache: KvCache, q_heads: int, n_seqs: int, table_width: int) -
     return lib().qvx_attn_paged_ws(C.byref(cache), q_heads, n_seqs, table_width)
 
 
+def attn_window(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, offsets: int, n_q: int,
+                cache: KvCache, table: int, table_width: int, lens: int, n_seqs: int, window: int, sinks: int, scale: float,
+                ws: int, ws_bytes: int, stream: int = 0) -> int:
+    """Attention of each sequence's last tokens over the paged cache, with a window and first tokens that stay visible.
+    Status."""
+    return lib().qvx_attn_window(out, out_stride, q, q_stride, q_type, q_heads, offsets or None, n_q, C.byref(cache), table,
+                                 table_width, lens, n_seqs, window, sinks, scale, ws or None, ws_bytes, stream)
+
+
+def attn_window_ws(cache: KvCache, q_type, q_heads: int, n_q: int, n_seqs: int, table_width: int, window: int,
+                   sinks: int) -> int:
+    """Bytes of attn_window's workspace; q_type a ggml type id or a torch dtype."""
+    if not isinstance(q_type, int):
+        q_type = _torch_types()[q_type]
+    return lib().qvx_attn_window_ws(C.byref(cache), q_type, q_heads, n_q, n_seqs, table_width, window, sinks)
+
+
+def attn_shared(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, cache: KvCache, table: int,
+                table_width: int, lens: int, n_seqs: int, groups: int, shared: int, n_groups: int, scale: float, ws: int,
+                ws_bytes: int, stream: int = 0) -> int:
+    """Attention of one new token a sequence where groups of sequences share their first tokens. Status."""
+    return lib().qvx_attn_shared(out, out_stride, q, q_stride, q_type, q_heads, C.byref(cache), table, table_width, lens,
+                                 n_seqs, groups or None, shared, n_groups, scale, ws or None, ws_bytes, stream)
+
+
+def attn_shared_ws(cache: KvCache, q_type, q_heads: int, n_seqs: int, table_width: int, n_groups: int) -> int:
+    """Bytes of attn_shared's workspace; q_type a ggml type id or a torch dtype."""
+    if not isinstance(q_type, int):
+        q_type = _torch_types()[q_type]
+    return lib().qvx_attn_shared_ws(C.byref(cache), q_type, q_heads, n_seqs, table_width, n_groups)
+
+
 def attn_cross(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, offsets: int, n_q: int,
                states: KvStates, lens: int, n_seqs: int, scale: float, ws: int, ws_bytes: int, stream: int = 0) -> int:
     """Cross attention of (ragged) queries to an encoder's states. Status."""
@@ -797,6 +835,60 @@ def attn_paged_t(q, cache: KvCache, table, lens, scale: float | None = None, out
         _check(attn_paged(*_rows(out, "out"), *_rows(q, "q"), heads, cache, tp, width, lp, n,
                           d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(),
                           _stream()), "qvx_attn_paged")
+    return out
+
+
+def _masked_rows(q, cache: KvCache, out, what: str):
+    import torch
+    if q.dtype not in _torch_types() or q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError(f"{what}: q is float32, float16 or bfloat16 [rows, heads, the cache's head_dim]")
+    _beside(cache, q.device, "cache")
+    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.device != q.device):
+        raise ValueError(f"{what}: out is as q")
+    return _torch_types()[q.dtype]
+
+
+def attn_window_t(q, cache: KvCache, table, lens, window: int, sinks: int = 0, offsets=None, scale: float | None = None,
+                  out=None, ws=None):
+    """attn_window on device tensors: q [rows, heads, head_dim] in float32, float16 or bfloat16, table [n, width], lens [n]
+    and offsets [n + 1] int32 (None: equal parts).  Rows past offsets[n] keep out's values, zeros where none is given."""
+    import torch
+    t = _masked_rows(q, cache, out, "attn_window_t")
+    n_q, heads, d = q.shape
+    n, width = table.shape
+    if out is None:
+        out = (torch.empty if offsets is None else torch.zeros)((n_q, heads, d), dtype=q.dtype, device=q.device)
+    op = _int32(offsets, (n + 1,), q.device, "offsets") if offsets is not None else 0
+    tp, lp = _int32(table, (n, width), q.device, "table"), _int32(lens, (n,), q.device, "lens")
+    with torch.cuda.device(q.device):
+        if ws is None:
+            ws = torch.empty(attn_window_ws(cache, t, heads, n_q, n, width, window, sinks), dtype=torch.uint8, device=q.device)
+        _beside(ws, q.device, "ws")
+        _check(attn_window(*_rows(out, "out"), *_rows(q, "q"), t, heads, op, n_q, cache, tp, width, lp, n, window, sinks,
+                           d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream()),
+               "qvx_attn_window")
+    return out
+
+
+def attn_shared_t(q, cache: KvCache, table, lens, shared, groups=None, scale: float | None = None, out=None, ws=None):
+    """attn_shared on device tensors: q [n, heads, head_dim] in float32, float16 or bfloat16, table [n, width] and lens [n],
+    shared [groups] and groups [groups + 1] int32 (None: all sequences are one group)."""
+    import torch
+    t = _masked_rows(q, cache, out, "attn_shared_t")
+    n, heads, d = q.shape
+    width, n_groups = table.shape[-1], shared.shape[0]
+    if out is None:
+        out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
+    tp, lp = _int32(table, (n, width), q.device, "table"), _int32(lens, (n,), q.device, "lens")
+    gp = _int32(groups, (n_groups + 1,), q.device, "groups") if groups is not None else 0
+    sp = _int32(shared, (n_groups,), q.device, "shared")
+    with torch.cuda.device(q.device):
+        if ws is None:
+            ws = torch.empty(attn_shared_ws(cache, t, heads, n, width, n_groups), dtype=torch.uint8, device=q.device)
+        _beside(ws, q.device, "ws")
+        _check(attn_shared(*_rows(out, "out"), *_rows(q, "q"), t, heads, cache, tp, width, lp, n, gp, sp, n_groups,
+                           d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream()),
+               "qvx_attn_shared")
     return out
 
 

@@ -7,6 +7,7 @@
 namespace qvx {
 bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
 void launch_attn_join(const AttnCall& c, hipStream_t s);
+bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s);
 bool launch_attn16(const AttnCall& c, uint32_t type, hipStream_t s);
 bool launch_kv_map(const MapCall& c, bool alias, hipStream_t s);
 void launch_rope_kv(RopeCall c, uint32_t type, bool vec, hipStream_t s);
@@ -34,9 +35,16 @@ constexpr int kAttnWgs = 512, kMinChunk = 8;
 // rows, 8 heads 12.9 against 13.3.
 int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
-// Tiles of the longest sequence that the call allows.
+// Tiles of the longest sequence that the call allows; of a window, of what one of its row tiles may see.
+int64_t tiles_of(const AttnCall& c, int len) {
+  return (int64_t)len / c.page_size * c.page_tiles + (len % c.page_size + kAttnTile - 1) / kAttnTile;
+}
 int64_t most_tiles(const AttnCall& c) {
-  return (int64_t)c.max_len / c.page_size * c.page_tiles + (c.max_len % c.page_size + kAttnTile - 1) / kAttnTile;
+  const int64_t all = tiles_of(c, c.max_len);
+  if (c.mode != kMaskWindow || c.window >= c.max_len) return all;
+  const int64_t near = (int64_t)c.window + attn_span(c.tile_rows, c.group) - 1;
+  return std::min<int64_t>(all, tiles_of(c, std::min(c.sinks, c.max_len)) +
+                                    attn_most_tiles(c.page_size, c.page_tiles, std::max<int64_t>(near, 0)));
 }
 
 // The rest of a partition whose row tiles, target and min_chunk (0: one chunk, whatever the length) are chosen.
@@ -45,6 +53,7 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t tiles = most_tiles(c);
   *join = c.min_chunk && tiles > c.min_chunk;
   const int64_t most = *join ? (tiles + c.min_chunk - 1) / c.min_chunk : 1;  // chunks of a row tile
+  const bool always = c.mode == kMaskPrefix;  // every item leaves a partial result
   const int64_t items = std::min(row_tiles + c.target, row_tiles * most);
   if (items * c.kv_heads > kMostWgs || tiles > kMaxTiles) return false;
   if (!*join) c.min_chunk = 0x7ffffff0;
@@ -54,8 +63,8 @@ bool plan_items(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int d16 = (c.head_dim + 15) / 16 * 16;
   c.small_sum = row_tiles * tiles <= 0x7fffffffll;
   c.read_once = row_tiles <= c.n_seqs;
-  c.slots = (int)std::min<int64_t>(2 * (int64_t)c.target, row_tiles * most);
-  *ws_bytes = *join ? sizeof(AttnPiece) * (1 + (size_t)c.slots) +
+  c.slots = (int)(always ? items : std::min<int64_t>(2 * (int64_t)c.target, row_tiles * most));
+  *ws_bytes = *join || always ? sizeof(AttnPiece) * (1 + (size_t)c.slots) +
                           (size_t)c.slots * c.kv_heads * attn_part(c.tile_rows, d16) * sizeof(float)
                     : 0;
   return true;
@@ -96,8 +105,8 @@ bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   return plan_items(c, row_tiles, join, ws_bytes);
 }
 
-int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width, AttnCall& c, bool* join,
-                size_t* ws_bytes) {
+// A call's cache and table, whatever its queries.
+int check_pages(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width, AttnCall& c) {
   if (n_seqs <= 0) return QVX_E_NVEC;
   if (int rc = check_cache(cache, &c.page_stride); rc != QVX_OK) return rc;
   if (q_heads <= 0 || q_heads % cache->kv_heads || table_width <= 0) return QVX_E_SHAPE;
@@ -120,9 +129,71 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
   c.kv_heads = cache->kv_heads;
   c.group = q_heads / cache->kv_heads;
   c.head_dim = d;
+  return QVX_OK;
+}
+
+int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_width, AttnCall& c, bool* join,
+                size_t* ws_bytes) {
+  if (int rc = check_pages(cache, q_heads, n_seqs, table_width, c); rc != QVX_OK) return rc;
   c.tile_rows = tile_rows(c.group);
   const int64_t row_tiles = (int64_t)n_seqs * ((c.group + c.tile_rows - 1) / c.tile_rows);
   return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+}
+
+bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
+
+int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, int table_width,
+                 int window, int sinks, AttnCall& c, bool* join, size_t* ws_bytes) {
+  if (int rc = check_pages(cache, q_heads, n_seqs, table_width, c); rc != QVX_OK) return rc;
+  if (!q_type_ok(q_type)) return QVX_E_TYPE;
+  if (n_q < 0 || (!ragged && n_q % n_seqs) || window < 0 || sinks < 0) return QVX_E_SHAPE;
+  if ((int64_t)n_q * c.group > 0x7fffff00ll) return QVX_E_RANGE;
+  c.mode = kMaskWindow;
+  c.q_type = q_type;
+  c.n_q = n_q;
+  c.q_each = ragged ? 0 : n_q / n_seqs;
+  c.window = std::min(window, kMaxLen);
+  c.sinks = std::min(sinks, kMaxLen);
+  const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
+  c.tile_rows = tile_rows(ragged ? (rows + n_seqs - 1) / n_seqs : rows);
+  const int64_t row_tiles =
+      ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
+  return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+}
+
+// The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query, its partial
+// results, and the rest's.
+struct SharedPlan {
+  AttnCall prefix{}, rest{};
+  bool join = false;
+  size_t lead_bytes = 0, prefix_bytes = 0, bytes = 0;
+};
+
+int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_seqs, int table_width, int n_groups,
+                 SharedPlan& p) {
+  if (int rc = check_pages(cache, q_heads, n_seqs, table_width, p.rest); rc != QVX_OK) return rc;
+  if (!q_type_ok(q_type)) return QVX_E_TYPE;
+  if (n_groups <= 0) return QVX_E_SHAPE;
+  if (n_groups > n_seqs || (int64_t)n_seqs * p.rest.group > 0x7fffff00ll) return QVX_E_RANGE;
+  p.rest.q_type = q_type;
+  AttnCall& c = p.prefix;
+  c = p.rest;
+  c.mode = kMaskPrefix;
+  c.n_seqs = n_groups;
+  const int64_t rows = (int64_t)n_seqs * c.group;
+  c.tile_rows = tile_rows((rows + n_groups - 1) / n_groups);
+  bool split = false;
+  if (!plan_split(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;
+  AttnCall& r = p.rest;
+  r.mode = kMaskRest;
+  r.lead_rows = c.tile_rows;
+  r.lead_slots = c.slots;
+  r.tile_rows = tile_rows(r.group);
+  size_t rest_bytes = 0;
+  if (!plan_split(r, (int64_t)n_seqs * ((r.group + r.tile_rows - 1) / r.tile_rows), &p.join, &rest_bytes)) return QVX_E_RANGE;
+  p.lead_bytes = sizeof(AttnLead) * (size_t)n_seqs;
+  p.bytes = p.lead_bytes + p.prefix_bytes + rest_bytes;
+  return QVX_OK;
 }
 
 // wide: the call runs on the 16-bit matrix cores (qvx_attn16.hip): q and the states share a 16-bit type, the scale is
@@ -240,6 +311,18 @@ int check_rope(void* d_q_out, int64_t q_out_stride, uint32_t q_out_type, const f
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The rows of q and out of a masked call, which may be the same ones.
+int check_rows(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, AttnCall& c) {
+  const uintptr_t size = c.q_type == T_F32 ? 4 : 2;
+  if (q_stride < 0 || out_stride < (int64_t)c.group * c.kv_heads * c.head_dim) return QVX_E_SHAPE;
+  if (!aligned(d_out, size) || !aligned(d_q, size) || (d_out == d_q && d_q && q_stride != out_stride)) return QVX_E_RANGE;
+  c.q = d_q;
+  c.out = d_out;
+  c.q_stride = q_stride;
+  c.out_stride = out_stride;
+  return QVX_OK;
+}
+
 }  // namespace
 
 #pragma GCC visibility push(default)
@@ -347,6 +430,78 @@ int qvx_attn_paged(float* d_out, int64_t out_stride, const float* d_q, int64_t q
   c.scale2 = scale * kLog2e;
   c.ws = join ? static_cast<float*>(d_ws) : nullptr;
   return attn_status(launch_attn_split(c, cache->type, join, static_cast<hipStream_t>(stream)));
+}
+
+size_t qvx_attn_window_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_q, int n_seqs, int table_width,
+                          int window, int sinks) {
+  size_t most = 0;
+  for (int i = 0; i < 2; ++i) {  // ragged or equal queries
+    AttnCall c{};
+    bool join = false;
+    size_t bytes = 0;
+    if (check_window(cache, q_type, q_heads, i, n_q, n_seqs, table_width, window, sinks, c, &join, &bytes) == QVX_OK)
+      most = std::max(most, bytes);
+  }
+  return most;
+}
+
+int qvx_attn_window(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                    const int32_t* d_offsets, int n_q, const qvx_kv_cache* cache, const int32_t* d_table, int table_width,
+                    const int32_t* d_lens, int n_seqs, int window, int sinks, float scale, void* d_ws, size_t ws_bytes,
+                    void* stream) {
+  AttnCall c{};
+  bool join = false;
+  size_t need = 0;
+  if (int rc = check_window(cache, q_type, q_heads, d_offsets != nullptr, n_q, n_seqs, table_width, window, sinks, c, &join,
+                            &need);
+      rc != QVX_OK)
+    return rc;
+  if (int rc = check_rows(d_out, out_stride, d_q, q_stride, c); rc != QVX_OK) return rc;
+  if (n_q == 0) return QVX_OK;
+  if (!d_out || !d_q || !d_table || !d_lens || (need && !d_ws)) return QVX_E_NULL;
+  if (ws_bytes < need || !aligned(d_ws, 16)) return QVX_E_RANGE;
+  c.q_offsets = d_offsets;
+  c.table = d_table;
+  c.lens = d_lens;
+  c.scale2 = scale * kLog2e;
+  c.ws = join ? static_cast<float*>(d_ws) : nullptr;
+  return attn_status(launch_attn_mask(c, cache->type, join, static_cast<hipStream_t>(stream)));
+}
+
+size_t qvx_attn_shared_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_seqs, int table_width,
+                          int n_groups) {
+  SharedPlan p;
+  return check_shared(cache, q_type, q_heads, n_seqs, table_width, n_groups, p) == QVX_OK ? p.bytes : 0;
+}
+
+int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
+                    const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens, int n_seqs,
+                    const int32_t* d_groups, const int32_t* d_shared, int n_groups, float scale, void* d_ws,
+                    size_t ws_bytes, void* stream) {
+  SharedPlan p;
+  if (int rc = check_shared(cache, q_type, q_heads, n_seqs, table_width, n_groups, p); rc != QVX_OK) return rc;
+  if (int rc = check_rows(d_out, out_stride, d_q, q_stride, p.rest); rc != QVX_OK) return rc;
+  if (!d_out || !d_q || !d_table || !d_lens || (!d_groups && n_groups > 1) || !d_shared || !d_ws) return QVX_E_NULL;
+  if (ws_bytes < p.bytes || !aligned(d_ws, 16)) return QVX_E_RANGE;
+  uint8_t* ws = static_cast<uint8_t*>(d_ws);
+  for (AttnCall* c : {&p.prefix, &p.rest}) {
+    c->q = d_q;
+    c->out = d_out;
+    c->q_stride = q_stride;
+    c->out_stride = out_stride;
+    c->table = d_table;
+    c->lens = d_lens;
+    c->scale2 = scale * kLog2e;
+    c->leads = reinterpret_cast<AttnLead*>(ws);
+  }
+  p.prefix.groups = d_groups;
+  p.prefix.shared = d_shared;
+  p.prefix.ws = reinterpret_cast<float*>(ws + p.lead_bytes);
+  p.rest.lead_ws = p.prefix.ws;
+  p.rest.ws = p.join ? reinterpret_cast<float*>(ws + p.lead_bytes + p.prefix_bytes) : nullptr;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!launch_attn_mask(p.prefix, cache->type, false, s)) return attn_status(false);
+  return attn_status(launch_attn_mask(p.rest, cache->type, p.join, s));
 }
 
 size_t qvx_attn_cross_ws(const qvx_kv_states* states, uint32_t q_type, int q_heads, int n_q, int n_seqs) {

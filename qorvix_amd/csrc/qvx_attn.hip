@@ -8,6 +8,11 @@ bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_f32(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 
+bool launch_attn_mask_f16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_mask_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_mask_f32(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_mask_q8(const AttnCall& c, dim3 grid, hipStream_t s);
+
 void launch_attn_join(const AttnCall& c, hipStream_t s);
 
 namespace {
@@ -112,6 +117,21 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
     case T_BF16: ok = launch_attn_split_bf16(c, grid, s); break;
     case T_F32: ok = launch_attn_split_f32(c, grid, s); break;
     case T_Q8_0: ok = launch_attn_split_q8(c, grid, s); break;
+    default: break;
+  }
+  if (ok && join) launch_attn_join(c, s);
+  return ok;
+}
+
+// The same for masked calls.
+bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s) {
+  const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
+  bool ok = false;
+  switch (type) {
+    case T_F16: ok = launch_attn_mask_f16(c, grid, s); break;
+    case T_BF16: ok = launch_attn_mask_bf16(c, grid, s); break;
+    case T_F32: ok = launch_attn_mask_f32(c, grid, s); break;
+    case T_Q8_0: ok = launch_attn_mask_q8(c, grid, s); break;
     default: break;
   }
   if (ok && join) launch_attn_join(c, s);

@@ -49,6 +49,22 @@ struct AttnCall {
   bool by_length;         // more items than places: the longer rests first
   bool small_sum;         // the tiles of all row tiles stay below 2^31
   float* ws;        // partial results of split sequences
+
+  // Of masked calls alone.  Window: the queries of a sequence are its last tokens, and the one at position p sees the keys
+  // j <= p that are later than p - window or before `sinks`.  Prefix and rest: qvx_attn_shared's two parts.
+  int mode;
+  int window, sinks;
+  const int32_t *groups, *shared;  // prefix: "sequence" g is the group of queries groups[g] .. and its first shared[g] keys
+  struct AttnLead* leads;          // [queries]: what the prefix leaves the rest
+  const float* lead_ws;            // rest: the prefix's workspace
+  int lead_rows, lead_slots;       // its tile_rows and slots
+};
+enum { kNoMask, kMaskWindow, kMaskPrefix, kMaskRest };
+
+// Of a query behind a shared prefix: how many of the prefix's keys it sees, its first row in its group, and where the partial
+// results of that group lie.
+struct AttnLead {
+  int32_t start, row, slot0, chunks;
 };
 
 // What k_attn_join needs to know of a split sequence's item.
@@ -86,10 +102,56 @@ struct AttnSeq {
   int len, q0, nq, row_tiles, tiles;
 };
 
-// R: query rows of a row tile, here and below.
-template <int R> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
+// The tile that key `at` lies in.
+__device__ inline int attn_tile_of(const AttnCall& c, int at) {
+  const int full = at / c.page_size;
+  return full * c.page_tiles + (at - full * c.page_size) / kAttnTile;
+}
+
+// Tiles that `keys` keys in a row touch at most, wherever they begin: x + y keys touch at most one tile more than x and y keys
+// from a page's start (a page's last tile may be short), and the first of them may begin inside a tile.
+__host__ __device__ inline long long attn_most_tiles(int page_size, int page_tiles, long long keys) {
+  return keys / page_size * page_tiles + (keys % page_size + kAttnTile - 1) / kAttnTile + 2;
+}
+// Queries of a row tile at most.
+__host__ __device__ inline int attn_span(int rows, int group) { return (rows + group - 2) / group + 1; }
+
+// A masked call's sequences.
+template <int R> __device__ inline AttnSeq attn_masked_seq(const AttnCall& c, int b) {
+  AttnSeq s{0, 0, 0, 0, 0};
+  if (c.mode == kMaskPrefix) {
+    s.q0 = b && c.groups ? min(max(c.groups[b], 0), c.n_q) : 0;
+    s.nq = max((b + 1 < c.n_seqs && c.groups ? min(max(c.groups[b + 1], 0), c.n_q) : c.n_q) - s.q0, 0);
+    s.len = min(max(c.shared[b], 0), c.max_len);
+    s.tiles = attn_tiles(c, s.len);
+  } else {
+    s.len = min(max(c.lens[b], 0), c.max_len);
+    if (c.mode == kMaskRest) {
+      s.q0 = b;
+      s.nq = 1;
+      const int start = min(max(c.leads[b].start, 0), s.len);
+      s.tiles = s.len > start ? attn_tiles(c, s.len) - attn_tile_of(c, start) : 0;
+    } else {
+      s.q0 = c.q_offsets ? min(max(c.q_offsets[b], 0), c.n_q) : b * c.q_each;
+      s.nq = c.q_offsets ? max(min(max(c.q_offsets[b + 1], 0), c.n_q) - s.q0, 0) : c.q_each;
+      s.tiles = attn_tiles(c, s.len);  // a row tile may see fewer: its chunks end there, or are empty
+      if (c.window < s.len) {
+        const long long near = (long long)c.window + min(attn_span(R, c.group), s.nq) - 1;
+        const long long most =
+            attn_tiles(c, min(c.sinks, s.len)) + attn_most_tiles(c.page_size, c.page_tiles, max(near, 0ll));
+        s.tiles = (int)min((long long)s.tiles, most);
+      }
+    }
+  }
+  s.row_tiles = (s.nq * c.group + R - 1) / R;
+  return s;
+}
+
+// R: query rows of a row tile, M: whether the call is masked, here and below.
+template <int R, bool M> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
   AttnSeq s{0, 0, 0, 0, 0};
   if (b >= c.n_seqs) return s;
+  if constexpr (M) return attn_masked_seq<R>(c, b);
   int len = c.lens ? c.lens[b] : c.max_len;
   s.len = min(max(len, 0), c.max_len);
   if (c.q_offsets) {  // clamped to the rows that the host vouches for
@@ -117,19 +179,21 @@ __device__ inline int attn_chunk(const AttnCall& c, long long total) {
 // against 51.8 with the rests in the order of the sequences.  Where all items find a place at once that order
 // stays (kind 1).  `slots` is the sequence's share of the workspace.
 constexpr int kAttnKinds = 5;
+// Whether every item leaves a partial result, split or not.
+template <bool M> __device__ inline bool attn_parts_always(const AttnCall& c) { return M && c.mode == kMaskPrefix; }
 struct AttnCount {
   int full, rest, kind, slots;  // rest: row_tiles or 0, of that kind
   __device__ int items(int k) const { return k == 0 ? full : k == kind ? rest : 0; }
 };
-__device__ inline AttnCount attn_count(const AttnCall& c, const AttnSeq& s, int chunk) {
+template <bool M> __device__ inline AttnCount attn_count(const AttnCall& c, const AttnSeq& s, int chunk) {
   const int full = s.tiles / chunk, left = s.tiles - full * chunk, rest = left > 0 || s.tiles == 0 ? 1 : 0;
   const int quarter = min(chunk, c.most_tiles) / 4;
   const int kind = c.by_length ? 1 + (left <= 3 * quarter) + (left <= 2 * quarter) + (left <= quarter) : 1;
-  return {s.row_tiles * full, s.row_tiles * rest, kind, full + rest > 1 ? s.row_tiles * (full + rest) : 0};
+  return {s.row_tiles * full, s.row_tiles * rest, kind, full + rest > 1 || attn_parts_always<M>(c) ? s.row_tiles * (full + rest) : 0};
 }
 
 // Item i of sequence b's full (or else short) ones; slot0: its first slot.
-template <int R>
+template <int R, bool M>
 __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b, int chunk, int i, bool full, int slot0) {
   AttnItem it;
   it.seq = b;
@@ -145,7 +209,7 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   it.slot = slot0 + rt * it.chunks + it.chunk;
   // Offsets that are no running sums can wrap the counts: nothing past the rows or the workspace then.
   it.any = i >= 0 && it.row0 >= 0 && it.row0 < it.rows && it.tile0 >= 0 &&
-           (it.chunks == 1 || (unsigned)it.slot < (unsigned)c.slots);
+           ((it.chunks == 1 && !attn_parts_always<M>(c)) || (unsigned)it.slot < (unsigned)c.slots);
   return it;
 }
 
@@ -175,11 +239,11 @@ struct AttnSums {
 // The work item of number `item`, the same in every thread of the workgroup (256 threads); `lds`:
 // 40 words that the caller does not use across the call.
 // Sequences that fit a wave are looked through by every wave for itself, more by the workgroup together.
-template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, AttnSums& sums) {
+template <int R, bool M> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, AttnSums& sums) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   AttnItem none{};
   if (c.n_seqs <= 64) {
-    const AttnSeq s = attn_seq<R>(c, lane);
+    const AttnSeq s = attn_seq<R, M>(c, lane);
     long long total;
     if (c.small_sum) {
       total = __builtin_amdgcn_readlane(attn_scan(s.row_tiles * s.tiles), 63);
@@ -190,7 +254,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
     }
     sums.tiles = attn_uniform(total);
     const int chunk = attn_chunk(c, sums.tiles);
-    const AttnCount n = attn_count(c, s, chunk);
+    const AttnCount n = attn_count<M>(c, s, chunk);
     int slots = 0, i = item, kind = 1, mine, run;
     sums.slots = 0;
     if (c.ws) {  // without a workspace no sequence is split: rests alone
@@ -216,7 +280,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
     t.q0 = __builtin_amdgcn_readlane(s.q0, b);
     t.nq = __builtin_amdgcn_readlane(s.nq, b) * c.group;
     t.tiles = __builtin_amdgcn_readlane(s.tiles, b);
-    return attn_take<R>(c, t, b, chunk, i - __builtin_amdgcn_readlane(run - mine, b), kind == 0,
+    return attn_take<R, M>(c, t, b, chunk, i - __builtin_amdgcn_readlane(run - mine, b), kind == 0,
                         __builtin_amdgcn_readlane(slots - n.slots, b));
   }
   // Every thread takes a run of sequences; the runs' sums are scanned through LDS.
@@ -224,7 +288,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   const int b0 = (int)threadIdx.x * per, b1 = min(b0 + per, c.n_seqs);
   long long total = 0;
   for (int b = b0; b < b1; ++b) {
-    const AttnSeq s = attn_seq<R>(c, b);
+    const AttnSeq s = attn_seq<R, M>(c, b);
     total += (long long)s.row_tiles * s.tiles;
   }
 #pragma unroll
@@ -236,7 +300,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   const int chunk = attn_chunk(c, sums.tiles);
   int items[kAttnKinds] = {}, own = 0;  // own: slots of this thread's sequences
   for (int b = b0; b < b1; ++b) {
-    const AttnCount x = attn_count(c, attn_seq<R>(c, b), chunk);
+    const AttnCount x = attn_count<M>(c, attn_seq<R, M>(c, b), chunk);
 #pragma unroll
     for (int k = 0; k < kAttnKinds; ++k) items[k] += x.items(k);
     own += x.slots;
@@ -275,7 +339,7 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   if (i >= run - mine && i < run) {
     int before = run - mine, slot0 = slots - own;
     for (int b = b0; b < b1; ++b) {
-      const AttnCount x = attn_count(c, attn_seq<R>(c, b), chunk);
+      const AttnCount x = attn_count<M>(c, attn_seq<R, M>(c, b), chunk);
       const int here = x.items(kind);
       if (i < before + here) {
         found[0] = b;
@@ -291,9 +355,60 @@ template <int R> __device__ inline AttnItem attn_item(const AttnCall& c, int ite
   const int b = __builtin_amdgcn_readfirstlane(found[0]), at = __builtin_amdgcn_readfirstlane(found[1]);
   const int slot0 = __builtin_amdgcn_readfirstlane(found[2]);
   if (b < 0) return none;
-  AttnSeq s = attn_seq<R>(c, b);
+  AttnSeq s = attn_seq<R, M>(c, b);
   s.nq *= c.group;
-  return attn_take<R>(c, s, b, chunk, at, kind == 0, slot0);
+  return attn_take<R, M>(c, s, b, chunk, at, kind == 0, slot0);
+}
+
+// What a row tile of a masked call sees: tiles [0, sinks) and [first, end) of its sequence, ordinals one behind the other, and
+// the keys [low, high) and [0, sink_keys) that any of its rows sees.
+struct AttnView {
+  int p0;  // window: the first query's position
+  int sinks, first, end;
+  int low, high, sink_keys;
+  __device__ int tiles() const { return sinks + max(end - first, 0); }
+  __device__ int tile(int t) const { return t < sinks ? t : t - sinks + first; }
+};
+template <int R> __device__ inline AttnView attn_view(const AttnCall& c, const AttnItem& it) {
+  AttnView v{0, 0, 0, 0, 0, it.len, 0};
+  if (c.mode == kMaskRest) {
+    v.low = min(max(c.leads[it.seq].start, 0), it.len);
+    v.first = attn_tile_of(c, v.low);
+  } else if (c.mode == kMaskWindow) {
+    const int nq = it.rows / c.group, qa = it.row0 / c.group, qb = (min(it.row0 + R, it.rows) - 1) / c.group;
+    v.p0 = it.len - nq;
+    v.high = max(v.p0 + qb + 1, 0);
+    v.low = (int)min(max((long long)v.p0 + qa + 1 - c.window, 0ll), (long long)v.high);
+    v.sink_keys = min(c.sinks, v.high);
+    v.first = attn_tile_of(c, v.low);
+    v.sinks = attn_tiles(c, v.sink_keys);
+    if (v.sinks >= v.first) v.first = v.sinks = 0;
+  }
+  v.end = v.high > v.low || v.first == 0 ? attn_tiles(c, v.high) : v.first;
+  return v;
+}
+// The keys that one row sees: those of [low, high) and of [0, sinks).
+struct AttnRange {
+  int low, high, sinks;
+  __device__ bool sees(int key) const { return (key >= low || key < sinks) && key < high; }
+};
+__device__ inline AttnRange attn_range(const AttnCall& c, const AttnItem& it, const AttnView& v, int row) {
+  if (row >= it.rows) return {0, 0, 0};
+  const int query = row / c.group;
+  if (c.mode == kMaskPrefix) return {0, min(max(c.lens[it.q0 + query], 0), it.len), 0};
+  if (c.mode == kMaskRest) return {v.low, it.len, 0};
+  const int p = v.p0 + query;
+  return {(int)max((long long)p + 1 - c.window, 0ll), max(p + 1, 0), c.sinks};
+}
+
+// Leaves the rest what it needs of the prefix: by a row tile's first chunk, for the queries whose first row it holds.
+template <int R>
+__device__ inline void attn_leads(const AttnCall& c, const AttnItem& it, int kvh) {
+  if (kvh != 0 || it.chunk != 0) return;
+  const int first = (it.row0 + c.group - 1) / c.group, end = (min(it.row0 + R, it.rows) + c.group - 1) / c.group;
+  for (int q = first + (int)threadIdx.x; q < end; q += (int)blockDim.x)
+    c.leads[it.q0 + q] = AttnLead{min(max(c.lens[it.q0 + q], 0), it.len), q * c.group,
+                                  it.slot - it.row0 / R * it.chunks, it.chunks};
 }
 
 // Leaves the join what it needs: the number of pieces, and this item's if it is one (of one head, as all

@@ -263,7 +263,7 @@ template <uint32_t T, int DT, bool FULL, int NS> struct AttnTile {
   // [key r][two blocks' scales a word]; kGroup: [key r][this lane's block of round u]
   uint32_t kstep[kQ8 ? 4 : 1][kGroup ? U : kQ8 ? (KS + 1) / 2 : 1];
   uint16_t vstep[kQ8 ? 4 : 1];
-  int live;
+  int live, key0;
 };
 
 __device__ __forceinline__ float attn_half(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -322,8 +322,8 @@ __device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&
 }
 
 // DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.  NS: sets of four
-// rows of a row tile, 1, 2 or 4.
-template <uint32_t T, int DT, bool FULL, int NS>
+// rows of a row tile, 1, 2 or 4.  MASK: rows see parts of their sequence's keys (AttnCall::mode).
+template <uint32_t T, int DT, bool FULL, int NS, bool MASK>
 __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_split(AttnCall c) {
   using Tile = AttnTile<T, DT, FULL, NS>;
   constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN, R = 4 * NS;
@@ -335,26 +335,39 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int col = lane & 15, g = lane >> 4;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
-  const AttnItem it = attn_item<R>(c, item, reinterpret_cast<int*>(lds), sums);
-  attn_note(c, it, item, kvh, sums);
-  if (!it.any) return;
+  AttnItem it = attn_item<R, MASK>(c, item, reinterpret_cast<int*>(lds), sums);
+  AttnView view{};
+  if constexpr (MASK) {
+    if (c.mode != kMaskPrefix) attn_note(c, it, item, kvh, sums);
+    if (!it.any) return;
+    if (c.mode == kMaskPrefix) attn_leads<R>(c, it, kvh);
+    view = attn_view<R>(c, it);
+    it.tile1 = min(it.tile1, view.tiles());  // may end before tile0: a chunk without keys
+    if (c.mode == kMaskPrefix) it.seq = it.q0;  // the table's row
+  } else {
+    attn_note(c, it, item, kvh, sums);
+    if (!it.any) return;
+  }
   // A call that reads more than half the 256 MB memory-side cache finds nothing of it there again, and its
   // loads are marked so: fp16 of 131071 tokens 102 -> 90 us, 128 x 4096 tokens 377 -> 345.  Smaller calls
   // keep the ordinary policy: 47 MB of fp32 in turn with two others like it 17.5 us against 19.3 with the mark.
   const bool once = c.read_once && sums.tiles * (long long)(2 * kAttnTile) * c.key_bytes * c.kv_heads > (128ll << 20);
 
   // The wave takes tiles tile0 + wave, + 4, ...; lane i looks up the i-th of them, 64 at a time.
-  const int tiles = (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
+  const int tiles = MASK && it.tile1 <= it.tile0 ? 0 : (it.tile1 - it.tile0 - wave + kAttnWaves - 1) / kAttnWaves;
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   int64_t at = 0, sat = 0;  // of the tile's keys (and values), and of their scales, from the cache's start
   int live = 0, seen = 0;  // seen: keys that count
+  int key0 = 0;            // masked: the tile's first key
   auto look_up = [&](int n) __attribute__((always_inline)) {
-    const int t = it.tile0 + wave + (n + lane) * kAttnWaves;
+    int t = it.tile0 + wave + (n + lane) * kAttnWaves;
     live = 0;
     if (t < it.tile1) {
+      if constexpr (MASK) t = view.tile(t);
       const int p = t / c.page_tiles, tok = (t - p * c.page_tiles) * kAttnTile;
       int page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
-      live = min(min(kAttnTile, c.page_size - tok), it.len - p * c.page_size - tok);
+      live = min(min(kAttnTile, c.page_size - tok), (MASK ? view.high : it.len) - p * c.page_size - tok);
+      key0 = p * c.page_size + tok;
       if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
       at = page * c.page_stride + kvh * c.head_stride + (int64_t)tok * c.pitch;
       if constexpr (kQ8) sat = page * c.page_stride + c.scale_off + ((int64_t)kvh * c.page_size + tok) * spitch;
@@ -389,6 +402,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     if (n && (n & 63) == 0 && n < tiles) look_up(n);
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
     seen |= x.live;
+    if constexpr (MASK) x.key0 = __builtin_amdgcn_readlane(key0, n & 63);
+    // Masked: keys that no row sees are not read, as if past the end: what is there does not reach the sums.
+    auto hide = [&](int key, uint32_t off) __attribute__((always_inline)) {
+      if constexpr (MASK) return x.key0 + key < view.low && x.key0 + key >= view.sink_keys ? kPastEnd : off;
+      return off;
+    };
     const int64_t ta = of_lane(at, n & 63);
     const uint32_t bytes = (uint32_t)(x.live * c.pitch);
     const __amdgpu_buffer_rsrc_t kr = attn_rsrc(c.k + ta, bytes);
@@ -397,13 +416,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         AttnWords<2 * J> w;
-        w.template load<AUX>(kr, koff[u * J]);
+        w.template load<AUX>(kr, hide(col, koff[u * J]));
 #pragma unroll
         for (int i = 0; i < 2 * J; ++i) x.k[u * J + i / 2].w[i % 2] = w.w[i];
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[s].template load<AUX>(kr, koff[s]);
+      for (int s = 0; s < KS; ++s) x.k[s].template load<AUX>(kr, hide(col, koff[s]));
     }
     if constexpr (kQ8) {
       const int64_t ts = of_lane(sat, n & 63);
@@ -416,29 +435,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
           for (int u = 0; u < U; ++u) {
             const int block = u * NP + col / R;
             x.kstep[r][u] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
-                ks, col / R < NP && 32 * block < d ? soff + r * spitch + 2 * block : kPastEnd, 0, 0);
+                ks, col / R < NP && 32 * block < d ? hide(4 * g + r, soff + r * spitch + 2 * block) : kPastEnd, 0, 0);
           }
         } else if constexpr (FULL) {
           AttnWords<(KS + 1) / 2> w;
-          w.load(ks, soff + r * spitch);
+          w.load(ks, hide(4 * g + r, soff + r * spitch));
 #pragma unroll
           for (int i = 0; i < (KS + 1) / 2; ++i) x.kstep[r][i] = w.w[i];
         } else {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             const uint32_t h =
-                (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? soff + r * spitch + 2 * s : kPastEnd, 0, 0);
+                (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ks, 32 * s < d ? hide(4 * g + r, soff + r * spitch + 2 * s) : kPastEnd, 0, 0);
             x.kstep[r][s / 2] = s % 2 ? x.kstep[r][s / 2] | h << 16 : h;
           }
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x.vstep[r] = __builtin_amdgcn_raw_buffer_load_b16(vs, svoff + r * spitch, 0, 0);
+      for (int r = 0; r < 4; ++r) x.vstep[r] = __builtin_amdgcn_raw_buffer_load_b16(vs, hide(4 * g + r, svoff + r * spitch), 0, 0);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, voff[u] + r * c.pitch);
+      for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, hide(4 * g + r, voff[u] + r * c.pitch));
   };
   // Tiles in registers, one in work and one on its way where they fit: 131071 tokens in bf16 103 us against 111 with one.
   // For eight rows of 128 values they do but for 1 to 22 registers (32 x 2000 tokens in bf16, 7 heads of 80 a group, 45 us
@@ -459,6 +478,16 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     l[t] = 0.0f;
 #pragma unroll
     for (int j = 0; j < VB; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // Masked: what the rows of this lane's weights see.
+  AttnRange range[NT];
+  int saw[NT];  // whether this lane saw a key of the row
+  if constexpr (MASK) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) saw[t] = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) range[t] = attn_range(c, it, view, it.row0 + (kSets ? 4 * t + (lane & 3) : col));
   }
 
   // This lane's query values: row col's pieces; rows and values that are not there are zeros.
@@ -540,7 +569,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
-        if (lane >> 2 >= x.live) p[t] = -INFINITY;
+        bool none = lane >> 2 >= x.live;
+        if constexpr (MASK) {
+          none = none || !range[t].sees(x.key0 + (lane >> 2));
+          saw[t] |= !none;
+        }
+        if (none) p[t] = -INFINITY;
         top[t] = p[t] * muls[t];
         past |= top[t] > m[t] + kSlack;  // m + slack is -inf at the start: any finite logit moves it
       }
@@ -575,7 +609,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       // In every tile: a branch around it right behind the product would lead to reads of sc sooner than the
       // matrix instruction's results are there, and the compiler counts the wait on the other path alone.
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[r] = 4 * g + r >= x.live ? -INFINITY : sc[r];
+      for (int r = 0; r < 4; ++r) {
+        bool none = 4 * g + r >= x.live;
+        if constexpr (MASK) {
+          none = none || !range[0].sees(x.key0 + 4 * g + r);
+          saw[0] |= !none;
+        }
+        sc[r] = none ? -INFINITY : sc[r];
+      }
       const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * mul;
       if (__any(top > m[0] + kSlack)) {
         float t = fmaxf(top, __shfl_xor(top, 16));
@@ -638,7 +679,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     run.template operator()<0>();
 
   // Weightless keys, all at -inf, are keys all the same: their row is 0 / 0, a row without keys zeros.
-  if (seen) {
+  // (Masked rows may see none of the keys that are there: each by its own.)
+  if (!MASK && seen) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) m[t] = fmaxf(m[t], kAttnLow);
   }
@@ -654,6 +696,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int s = 4; s < 64; s *= 2) l[t] += __shfl_xor(l[t], s);
+      if constexpr (MASK) {
+#pragma unroll
+        for (int s = 4; s < 64; s *= 2) saw[t] |= __shfl_xor(saw[t], s);
+        if (saw[t]) m[t] = fmaxf(m[t], kAttnLow);
+      }
       if (lane < 4) {
         lm[wave * R + 4 * t + lane] = m[t];
         ll[wave * R + 4 * t + lane] = l[t];
@@ -678,6 +725,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   } else {
     l[0] += __shfl_xor(l[0], 16);
     l[0] += __shfl_xor(l[0], 32);
+    if constexpr (MASK) {
+      saw[0] |= __shfl_xor(saw[0], 16);
+      saw[0] |= __shfl_xor(saw[0], 32);
+      if (saw[0]) m[0] = fmaxf(m[0], kAttnLow);
+    }
     if (lane < 16) {
       lm[wave * R + lane] = m[0];
       ll[wave * R + lane] = l[0];
@@ -690,7 +742,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   }
   __syncthreads();
   const float* v0 = lds + 2 * kAttnWaves * R;
-  float* part = it.chunks > 1 ? attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
+  const bool whole = it.chunks == 1 && !attn_parts_always<MASK>(c);
+  // The rest of a sequence takes what its shared prefix left into its first chunk.
+  AttnLead lead{0, 0, 0, 0};
+  if constexpr (MASK) {
+    if (c.mode == kMaskRest && it.chunk == 0) {
+      lead = c.leads[it.seq];
+      // groups that are no running sums may have left a query out: nothing past the workspace then
+      if (lead.row < 0 || lead.slot0 < 0 || lead.chunks < 0 || lead.row > c.n_q * c.group ||
+          lead.slot0 + (int64_t)((lead.row + it.rows - 1) / c.lead_rows + 1) * lead.chunks > c.lead_slots)
+        lead.chunks = 0;
+    }
+  }
+  float* part = !whole ? attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
                               : nullptr;
   const int quads = d / 4;
   for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
@@ -709,7 +773,44 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
       for (int k = 0; k < 4; ++k) val[k] += x[k] * f;
     }
-    if (it.chunks == 1) {
+    if constexpr (MASK) {
+      const int row = lead.row + it.row0 + r, tile = lead.chunks ? row / c.lead_rows : 0, rr = row - tile * c.lead_rows;
+      const size_t size = attn_part(c.lead_rows, d16), step = (size_t)c.kv_heads * size;
+      const float* p = lead.chunks ? attn_parts(const_cast<float*>(c.lead_ws), c.lead_slots) +
+                                         ((size_t)(lead.slot0 + tile * lead.chunks) * c.kv_heads + kvh) * size
+                                   : nullptr;
+      for (int j0 = 0; j0 < lead.chunks; j0 += 4) {
+        float mj[4], lj[4];
+        f32x4 vj[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* x = p + min(j0 + k, lead.chunks - 1) * step;
+          mj[k] = x[c.lead_rows * d16 + rr];
+          lj[k] = x[c.lead_rows * (d16 + 1) + rr];
+          vj[k] = *reinterpret_cast<const f32x4*>(x + rr * d16 + i);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (j0 + k >= lead.chunks) mj[k] = -INFINITY;
+          now = fmaxf(now, mj[k]);
+        }
+        const float base = now == -INFINITY ? 0.0f : now, f0 = attn_pow2(top - base);
+        top = now;
+        sum *= f0;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) val[e4] *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (mj[k] == -INFINITY) continue;  // no keys: what its values hold does not count
+          const float f = attn_pow2(mj[k] - base);
+          sum += lj[k] * f;
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) val[e4] += vj[k][e4] * f;
+        }
+      }
+    }
+    if (whole) {
       float o[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = top == -INFINITY ? 0.0f : val[k] / sum;
@@ -725,29 +826,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 }
 
 // Rows of a row tile, 4, 8 or 16: as many as a call's row tiles hold (the launchers' and the join's R).
-template <uint32_t T, int DT, bool FULL, int NS> bool attn_split(const AttnCall& c, dim3 grid, hipStream_t s) {
+template <uint32_t T, int DT, bool FULL, int NS, bool MASK> bool attn_split(const AttnCall& c, dim3 grid, hipStream_t s) {
   static LdsLimit lim;
   const size_t lds = (size_t)kAttnWaves * 4 * NS * (2 + (c.head_dim + 15) / 16 * 16) * sizeof(float);
-  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, DT, FULL, NS>), lim, lds)) return false;
-  k_attn_split<T, DT, FULL, NS><<<grid, 64 * kAttnWaves, lds, s>>>(c);
+  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, DT, FULL, NS, MASK>), lim, lds)) return false;
+  k_attn_split<T, DT, FULL, NS, MASK><<<grid, 64 * kAttnWaves, lds, s>>>(c);
   return true;
 }
 
-template <uint32_t T, int DT, bool FULL> bool attn_split_rows(const AttnCall& c, dim3 grid, hipStream_t s) {
-  if (c.tile_rows == 4) return attn_split<T, DT, FULL, 1>(c, grid, s);
-  if (c.tile_rows == 8) return attn_split<T, DT, FULL, 2>(c, grid, s);
-  return attn_split<T, DT, FULL, 4>(c, grid, s);
+template <uint32_t T, int DT, bool FULL, bool MASK> bool attn_split_rows(const AttnCall& c, dim3 grid, hipStream_t s) {
+  if (c.tile_rows == 4) return attn_split<T, DT, FULL, 1, MASK>(c, grid, s);
+  if (c.tile_rows == 8) return attn_split<T, DT, FULL, 2, MASK>(c, grid, s);
+  return attn_split<T, DT, FULL, 4, MASK>(c, grid, s);
 }
 
-template <uint32_t T> bool attn_split_dt(const AttnCall& c, dim3 grid, hipStream_t s) {
+template <uint32_t T, bool MASK = false> bool attn_split_dt(const AttnCall& c, dim3 grid, hipStream_t s) {
   if constexpr (T == T_Q8_0) {
-    if (c.head_dim == 64) return attn_split_rows<T, 64, true>(c, grid, s);
-    if (c.head_dim == 128) return attn_split_rows<T, 128, true>(c, grid, s);
-    if (c.head_dim == 256) return attn_split_rows<T, 256, true>(c, grid, s);
+    if (c.head_dim == 64) return attn_split_rows<T, 64, true, MASK>(c, grid, s);
+    if (c.head_dim == 128) return attn_split_rows<T, 128, true, MASK>(c, grid, s);
+    if (c.head_dim == 256) return attn_split_rows<T, 256, true, MASK>(c, grid, s);
   }
-  if (c.head_dim <= 64) return attn_split_rows<T, 64, false>(c, grid, s);
-  if (c.head_dim <= 128) return attn_split_rows<T, 128, false>(c, grid, s);
-  return attn_split_rows<T, 256, false>(c, grid, s);
+  if (c.head_dim <= 64) return attn_split_rows<T, 64, false, MASK>(c, grid, s);
+  if (c.head_dim <= 128) return attn_split_rows<T, 128, false, MASK>(c, grid, s);
+  return attn_split_rows<T, 256, false, MASK>(c, grid, s);
 }
 
 }  // namespace qvx
