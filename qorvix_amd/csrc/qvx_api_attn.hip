@@ -142,6 +142,17 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
 
 bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 
+// Whether calls of so many rows a sequence (of a mean one) run on the kernel of many rows, and the partition's geometry
+// there: keys in a row, whatever their pages.
+bool many_rows(const qvx_kv_cache* cache, int64_t rows, AttnCall& c) {
+  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 16) return false;
+  c.table_page = c.page_size;
+  c.page_size = c.max_len;
+  c.page_tiles = (int)(((int64_t)c.max_len + kAttnTile - 1) / kAttnTile);
+  c.tile_rows = kAttnRows16;
+  return true;
+}
+
 int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool ragged, int n_q, int n_seqs, int table_width,
                  int window, int sinks, AttnCall& c, bool* join, size_t* ws_bytes) {
   if (int rc = check_pages(cache, q_heads, n_seqs, table_width, c); rc != QVX_OK) return rc;
@@ -155,10 +166,12 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
   c.window = std::min(window, kMaxLen);
   c.sinks = std::min(sinks, kMaxLen);
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
-  c.tile_rows = tile_rows(ragged ? (rows + n_seqs - 1) / n_seqs : rows);
+  const int64_t mean = ragged ? (rows + n_seqs - 1) / n_seqs : rows;
+  const bool many = many_rows(cache, mean, c);
+  if (!many) c.tile_rows = tile_rows(mean);
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
-  return plan_split(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
+  return (many ? plan16 : plan_split)(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
 // The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query, its partial
@@ -181,9 +194,16 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   c.mode = kMaskPrefix;
   c.n_seqs = n_groups;
   const int64_t rows = (int64_t)n_seqs * c.group;
-  c.tile_rows = tile_rows((rows + n_groups - 1) / n_groups);
+  const int64_t mean = (rows + n_groups - 1) / n_groups;
   bool split = false;
-  if (!plan_split(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;
+  if (many_rows(cache, mean, c)) {  // every chunk leaves its partial results: as many as the CUs, of 256 keys at least
+    c.min_chunk = 16;
+    c.target = std::max(1, kAttnWgs / 2 / c.kv_heads);
+    if (!plan_items(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;
+  } else {
+    c.tile_rows = tile_rows(mean);
+    if (!plan_split(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;
+  }
   AttnCall& r = p.rest;
   r.mode = kMaskRest;
   r.lead_rows = c.tile_rows;
@@ -465,6 +485,8 @@ int qvx_attn_window(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
   c.ws = join ? static_cast<float*>(d_ws) : nullptr;
+  c.q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
+  c.out_wide = aligned(d_out, 8) && out_stride % 4 == 0;
   return attn_status(launch_attn_mask(c, cache->type, join, static_cast<hipStream_t>(stream)));
 }
 
@@ -493,6 +515,7 @@ int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
     c->lens = d_lens;
     c->scale2 = scale * kLog2e;
     c->leads = reinterpret_cast<AttnLead*>(ws);
+    c->q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
   }
   p.prefix.groups = d_groups;
   p.prefix.shared = d_shared;

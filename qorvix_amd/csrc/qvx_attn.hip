@@ -13,6 +13,9 @@ bool launch_attn_mask_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_mask_f32(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_mask_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 
+bool launch_attn_rows_f16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
+bool launch_attn_rows_bf16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
+
 void launch_attn_join(const AttnCall& c, hipStream_t s);
 
 namespace {
@@ -123,10 +126,17 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
   return ok;
 }
 
-// The same for masked calls.
+// The same for masked calls; row tiles of 128 rows are the kernel's of many rows, with 16-bit parts where q is of another
+// type than the cache or its scale does not keep the order of the products.
 bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s) {
   const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
   bool ok = false;
+  if (c.tile_rows == kAttnRows16) {
+    const bool parts = c.q_type != type || !(c.scale2 >= 1e-30f);  // far above the subnormal numbers
+    ok = type == T_F16 ? launch_attn_rows_f16(c, parts, grid, s) : launch_attn_rows_bf16(c, parts, grid, s);
+    if (ok && join) launch_attn_join(c, s);
+    return ok;
+  }
   switch (type) {
     case T_F16: ok = launch_attn_mask_f16(c, grid, s); break;
     case T_BF16: ok = launch_attn_mask_bf16(c, grid, s); break;

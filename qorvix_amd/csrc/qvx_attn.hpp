@@ -54,6 +54,7 @@ struct AttnCall {
   // j <= p that are later than p - window or before `sinks`.  Prefix and rest: qvx_attn_shared's two parts.
   int mode;
   int window, sinks;
+  int table_page;  // many rows: tokens of a page, page_size then standing for the longest sequence
   const int32_t *groups, *shared;  // prefix: "sequence" g is the group of queries groups[g] .. and its first shared[g] keys
   struct AttnLead* leads;          // [queries]: what the prefix leaves the rest
   const float* lead_ws;            // rest: the prefix's workspace
@@ -200,9 +201,12 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   it.len = s.len;
   it.q0 = s.q0;
   it.chunks = max((s.tiles + chunk - 1) / chunk, 1);
-  const int whole = s.tiles / chunk, rt = full ? i / max(whole, 1) : i;
+  const int whole = s.tiles / chunk;
+  int rt = full ? i / max(whole, 1) : i;
   it.chunk = full ? i - rt * whole : whole;
   it.rows = s.nq;
+  // Later queries see more keys: their row tiles come first.
+  if (M && c.mode == kMaskWindow) rt = (s.nq + R - 1) / R - 1 - rt;
   it.row0 = rt * R;
   it.tile0 = it.chunk * chunk;
   it.tile1 = min(it.tile0 + chunk, s.tiles);
