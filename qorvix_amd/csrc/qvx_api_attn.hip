@@ -174,12 +174,12 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
   return (many ? plan16 : plan_split)(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
-// The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query, its partial
-// results, and the rest's.
+// The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query and its
+// counters, its partial results, and the rest's.
 struct SharedPlan {
   AttnCall prefix{}, rest{};
-  bool join = false;
-  size_t lead_bytes = 0, prefix_bytes = 0, bytes = 0;
+  bool join = false;  // the rest may be split
+  size_t arrived_at = 0, lead_bytes = 0, prefix_bytes = 0, bytes = 0;
 };
 
 int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_seqs, int table_width, int n_groups,
@@ -211,7 +211,9 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   r.tile_rows = tile_rows(r.group);
   size_t rest_bytes = 0;
   if (!plan_split(r, (int64_t)n_seqs * ((r.group + r.tile_rows - 1) / r.tile_rows), &p.join, &rest_bytes)) return QVX_E_RANGE;
-  p.lead_bytes = sizeof(AttnLead) * (size_t)n_seqs;
+  r.rest_tiles = c.rest_tiles = (r.group + r.tile_rows - 1) / r.tile_rows;
+  p.arrived_at = sizeof(AttnLead) * (size_t)n_seqs;
+  p.lead_bytes = p.arrived_at + (4 * (size_t)n_seqs * r.rest_tiles * r.kv_heads + 15) / 16 * 16;
   p.bytes = p.lead_bytes + p.prefix_bytes + rest_bytes;
   return QVX_OK;
 }
@@ -515,6 +517,7 @@ int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
     c->lens = d_lens;
     c->scale2 = scale * kLog2e;
     c->leads = reinterpret_cast<AttnLead*>(ws);
+    c->arrived = reinterpret_cast<int*>(ws + p.arrived_at);
     c->q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
   }
   p.prefix.groups = d_groups;
@@ -524,7 +527,7 @@ int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
   p.rest.ws = p.join ? reinterpret_cast<float*>(ws + p.lead_bytes + p.prefix_bytes) : nullptr;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (!launch_attn_mask(p.prefix, cache->type, false, s)) return attn_status(false);
-  return attn_status(launch_attn_mask(p.rest, cache->type, p.join, s));
+  return attn_status(launch_attn_mask(p.rest, cache->type, false, s));  // the rest's chunks join themselves
 }
 
 size_t qvx_attn_cross_ws(const qvx_kv_states* states, uint32_t q_type, int q_heads, int n_q, int n_seqs) {

@@ -8,11 +8,18 @@ bool launch_attn_split_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_f32(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_split_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 
-bool launch_attn_mask_f16(const AttnCall& c, dim3 grid, hipStream_t s);
-bool launch_attn_mask_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
-bool launch_attn_mask_f32(const AttnCall& c, dim3 grid, hipStream_t s);
-bool launch_attn_mask_q8(const AttnCall& c, dim3 grid, hipStream_t s);
-
+bool launch_attn_window_f16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_window_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_window_f32(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_window_q8(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_prefix_f16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_prefix_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_prefix_f32(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_prefix_q8(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_rest_f16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_rest_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_rest_f32(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_rest_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_rows_f16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
 bool launch_attn_rows_bf16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
 
@@ -137,13 +144,16 @@ bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s
     if (ok && join) launch_attn_join(c, s);
     return ok;
   }
+  const bool rest = c.mode == kMaskRest, prefix = c.mode == kMaskPrefix;
+#define QVX_MODE(f) (prefix ? launch_attn_prefix_##f : rest ? launch_attn_rest_##f : launch_attn_window_##f)(c, grid, s)
   switch (type) {
-    case T_F16: ok = launch_attn_mask_f16(c, grid, s); break;
-    case T_BF16: ok = launch_attn_mask_bf16(c, grid, s); break;
-    case T_F32: ok = launch_attn_mask_f32(c, grid, s); break;
-    case T_Q8_0: ok = launch_attn_mask_q8(c, grid, s); break;
+    case T_F16: ok = QVX_MODE(f16); break;
+    case T_BF16: ok = QVX_MODE(bf16); break;
+    case T_F32: ok = QVX_MODE(f32); break;
+    case T_Q8_0: ok = QVX_MODE(q8); break;
     default: break;
   }
+#undef QVX_MODE
   if (ok && join) launch_attn_join(c, s);
   return ok;
 }

@@ -59,6 +59,8 @@ struct AttnCall {
   struct AttnLead* leads;          // [queries]: what the prefix leaves the rest
   const float* lead_ws;            // rest: the prefix's workspace
   int lead_rows, lead_slots;       // its tile_rows and slots
+  int* arrived;                    // [queries][rest_tiles][kv_heads]: chunks of the rest that are done, zeroed by the prefix
+  int rest_tiles;                  // row tiles of a query in the rest
 };
 enum { kNoMask, kMaskWindow, kMaskPrefix, kMaskRest };
 
@@ -118,16 +120,16 @@ __host__ __device__ inline long long attn_most_tiles(int page_size, int page_til
 __host__ __device__ inline int attn_span(int rows, int group) { return (rows + group - 2) / group + 1; }
 
 // A masked call's sequences.
-template <int R> __device__ inline AttnSeq attn_masked_seq(const AttnCall& c, int b) {
+template <int R, int M> __device__ inline AttnSeq attn_masked_seq(const AttnCall& c, int b) {
   AttnSeq s{0, 0, 0, 0, 0};
-  if (c.mode == kMaskPrefix) {
+  if constexpr (M == kMaskPrefix) {
     s.q0 = b && c.groups ? min(max(c.groups[b], 0), c.n_q) : 0;
     s.nq = max((b + 1 < c.n_seqs && c.groups ? min(max(c.groups[b + 1], 0), c.n_q) : c.n_q) - s.q0, 0);
     s.len = min(max(c.shared[b], 0), c.max_len);
     s.tiles = attn_tiles(c, s.len);
   } else {
     s.len = min(max(c.lens[b], 0), c.max_len);
-    if (c.mode == kMaskRest) {
+    if constexpr (M == kMaskRest) {
       s.q0 = b;
       s.nq = 1;
       const int start = min(max(c.leads[b].start, 0), s.len);
@@ -148,11 +150,11 @@ template <int R> __device__ inline AttnSeq attn_masked_seq(const AttnCall& c, in
   return s;
 }
 
-// R: query rows of a row tile, M: whether the call is masked, here and below.
-template <int R, bool M> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
+// R: query rows of a row tile, M: the call's mode, here and below.
+template <int R, int M> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
   AttnSeq s{0, 0, 0, 0, 0};
   if (b >= c.n_seqs) return s;
-  if constexpr (M) return attn_masked_seq<R>(c, b);
+  if constexpr (M != kNoMask) return attn_masked_seq<R, M>(c, b);
   int len = c.lens ? c.lens[b] : c.max_len;
   s.len = min(max(len, 0), c.max_len);
   if (c.q_offsets) {  // clamped to the rows that the host vouches for
@@ -181,20 +183,20 @@ __device__ inline int attn_chunk(const AttnCall& c, long long total) {
 // stays (kind 1).  `slots` is the sequence's share of the workspace.
 constexpr int kAttnKinds = 5;
 // Whether every item leaves a partial result, split or not.
-template <bool M> __device__ inline bool attn_parts_always(const AttnCall& c) { return M && c.mode == kMaskPrefix; }
+template <int M> __device__ constexpr bool attn_parts_always() { return M == kMaskPrefix; }
 struct AttnCount {
   int full, rest, kind, slots;  // rest: row_tiles or 0, of that kind
   __device__ int items(int k) const { return k == 0 ? full : k == kind ? rest : 0; }
 };
-template <bool M> __device__ inline AttnCount attn_count(const AttnCall& c, const AttnSeq& s, int chunk) {
+template <int M> __device__ inline AttnCount attn_count(const AttnCall& c, const AttnSeq& s, int chunk) {
   const int full = s.tiles / chunk, left = s.tiles - full * chunk, rest = left > 0 || s.tiles == 0 ? 1 : 0;
   const int quarter = min(chunk, c.most_tiles) / 4;
   const int kind = c.by_length ? 1 + (left <= 3 * quarter) + (left <= 2 * quarter) + (left <= quarter) : 1;
-  return {s.row_tiles * full, s.row_tiles * rest, kind, full + rest > 1 || attn_parts_always<M>(c) ? s.row_tiles * (full + rest) : 0};
+  return {s.row_tiles * full, s.row_tiles * rest, kind, full + rest > 1 || attn_parts_always<M>() ? s.row_tiles * (full + rest) : 0};
 }
 
 // Item i of sequence b's full (or else short) ones; slot0: its first slot.
-template <int R, bool M>
+template <int R, int M>
 __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b, int chunk, int i, bool full, int slot0) {
   AttnItem it;
   it.seq = b;
@@ -206,14 +208,14 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   it.chunk = full ? i - rt * whole : whole;
   it.rows = s.nq;
   // Later queries see more keys: their row tiles come first.
-  if (M && c.mode == kMaskWindow) rt = (s.nq + R - 1) / R - 1 - rt;
+  if (M == kMaskWindow) rt = (s.nq + R - 1) / R - 1 - rt;
   it.row0 = rt * R;
   it.tile0 = it.chunk * chunk;
   it.tile1 = min(it.tile0 + chunk, s.tiles);
   it.slot = slot0 + rt * it.chunks + it.chunk;
   // Offsets that are no running sums can wrap the counts: nothing past the rows or the workspace then.
   it.any = i >= 0 && it.row0 >= 0 && it.row0 < it.rows && it.tile0 >= 0 &&
-           ((it.chunks == 1 && !attn_parts_always<M>(c)) || (unsigned)it.slot < (unsigned)c.slots);
+           ((it.chunks == 1 && !attn_parts_always<M>()) || (unsigned)it.slot < (unsigned)c.slots);
   return it;
 }
 
@@ -243,7 +245,7 @@ struct AttnSums {
 // The work item of number `item`, the same in every thread of the workgroup (256 threads); `lds`:
 // 40 words that the caller does not use across the call.
 // Sequences that fit a wave are looked through by every wave for itself, more by the workgroup together.
-template <int R, bool M> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, AttnSums& sums) {
+template <int R, int M> __device__ inline AttnItem attn_item(const AttnCall& c, int item, int* lds, AttnSums& sums) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   AttnItem none{};
   if (c.n_seqs <= 64) {
@@ -373,12 +375,12 @@ struct AttnView {
   __device__ int tiles() const { return sinks + max(end - first, 0); }
   __device__ int tile(int t) const { return t < sinks ? t : t - sinks + first; }
 };
-template <int R> __device__ inline AttnView attn_view(const AttnCall& c, const AttnItem& it) {
+template <int R, int M> __device__ inline AttnView attn_view(const AttnCall& c, const AttnItem& it) {
   AttnView v{0, 0, 0, 0, 0, it.len, 0};
-  if (c.mode == kMaskRest) {
+  if constexpr (M == kMaskRest) {
     v.low = min(max(c.leads[it.seq].start, 0), it.len);
     v.first = attn_tile_of(c, v.low);
-  } else if (c.mode == kMaskWindow) {
+  } else if constexpr (M == kMaskWindow) {
     const int nq = it.rows / c.group, qa = it.row0 / c.group, qb = (min(it.row0 + R, it.rows) - 1) / c.group;
     v.p0 = it.len - nq;
     v.high = max(v.p0 + qb + 1, 0);
@@ -396,16 +398,18 @@ struct AttnRange {
   int low, high, sinks;
   __device__ bool sees(int key) const { return (key >= low || key < sinks) && key < high; }
 };
+template <int M>
 __device__ inline AttnRange attn_range(const AttnCall& c, const AttnItem& it, const AttnView& v, int row) {
   if (row >= it.rows) return {0, 0, 0};
   const int query = row / c.group;
-  if (c.mode == kMaskPrefix) return {0, min(max(c.lens[it.q0 + query], 0), it.len), 0};
-  if (c.mode == kMaskRest) return {v.low, it.len, 0};
+  if constexpr (M == kMaskPrefix) return {0, min(max(c.lens[it.q0 + query], 0), it.len), 0};
+  if constexpr (M == kMaskRest) return {v.low, it.len, 0};
   const int p = v.p0 + query;
   return {(int)max((long long)p + 1 - c.window, 0ll), max(p + 1, 0), c.sinks};
 }
 
-// Leaves the rest what it needs of the prefix: by a row tile's first chunk, for the queries whose first row it holds.
+// Leaves the rest what it needs of the prefix, and its counters at zero: by a row tile's first chunk, for the queries whose
+// first row it holds.
 template <int R>
 __device__ inline void attn_leads(const AttnCall& c, const AttnItem& it, int kvh) {
   if (kvh != 0 || it.chunk != 0) return;
@@ -413,6 +417,9 @@ __device__ inline void attn_leads(const AttnCall& c, const AttnItem& it, int kvh
   for (int q = first + (int)threadIdx.x; q < end; q += (int)blockDim.x)
     c.leads[it.q0 + q] = AttnLead{min(max(c.lens[it.q0 + q], 0), it.len), q * c.group,
                                   it.slot - it.row0 / R * it.chunks, it.chunks};
+  const int each = c.rest_tiles * c.kv_heads;
+  for (int64_t e = (int64_t)(it.q0 + first) * each + threadIdx.x; e < (int64_t)(it.q0 + end) * each; e += blockDim.x)
+    c.arrived[e] = 0;
 }
 
 // Leaves the join what it needs: the number of pieces, and this item's if it is one (of one head, as all

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 160 ? 2 : 1) void k_attn1
   const int col = lane & 31, h = lane >> 5;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
-  const AttnItem it = attn_item<kRows16, false>(c, item, reinterpret_cast<int*>(lds16), sums);
+  const AttnItem it = attn_item<kRows16, kNoMask>(c, item, reinterpret_cast<int*>(lds16), sums);
   attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
   __syncthreads();  // the item's words are read before tiles overwrite them

@@ -1,0 +1,11 @@
+// qvx_attn_rest_q8.hip -- the split attention kernel over Q8_0 keys and values (qvx_attn_split.hpp):
+// what is behind a shared prefix.
+#include "qvx_attn_split.hpp"
+
+namespace qvx {
+
+bool launch_attn_rest_q8(const AttnCall& c, dim3 grid, hipStream_t s) {
+  return attn_split_dt<T_Q8_0, kMaskRest>(c, grid, s);
+}
+
+}  // namespace qvx

@@ -6,8 +6,8 @@
 // as in qvx_attn16.hip (128 rows a workgroup, 32 a wave; S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction; K and V
 // tiles staged in LDS, the next one in flight).  What is different:
 //
-// Pages.  Lane i of a wave looks tile t's key i up, two tiles ahead, so a page may hold any number of tokens; the threads
-// that stage a key get its address from that lane.
+// Pages.  The keys' offsets are looked up 512 at a time, half such a block ahead, and stand in LDS, so a page may hold any
+// number of tokens.  Tiles are copied to LDS straight from the pages, NB - 1 tiles ahead.
 //
 // Masks.  The tiles of sixteen keys that any row of the tile sees are numbered one behind the other (AttnView), first tokens
 // before the window, so a row's keys are two ranges of numbers.  Tiles that all rows of a wave see whole take the
@@ -20,6 +20,8 @@
 #pragma once
 
 #include "qvx_attn_split.hpp"
+
+#include <utility>
 
 namespace qvx {
 
@@ -78,10 +80,64 @@ template <int DP, int KT> struct Tile {
   static __device__ __forceinline__ int v_at(int r, int u) { return r * kPitch + 16 * v_unit(r, u); }
 };
 
+constexpr int kBlock = 512;  // keys whose offsets are looked up together
+static_assert(kBlock == 2 * 256);
+
+// Waits until at most N copies to LDS are on their way.
+template <int N> __device__ __forceinline__ void wait_copies() {
+  static_assert(N < 64);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Everyone's LDS accesses done, and nothing moved past it.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int N, class F> __device__ __forceinline__ void unrolled(F f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) {
+    (f.template operator()<I>(), ...);
+  }(std::make_integer_sequence<int, N>{});
+}
+
+// The second product's left operand for N x 32 values: of each two transposing reads, OFF and OFF + STEP bytes behind an LDS
+// address.  Read and waited for in one piece: before a transposing read of its own the compiler would wait for every copy to
+// LDS that is on its way.
+template <int N, int OFF, int STEP> __device__ __forceinline__ void read_values(u32x4 (&v)[N], const uint32_t (&a)[N]) {
+  static_assert(OFF + STEP < 65536);
+  u32x2 l[N], h[N];
+#define QVX_TR(o, at) "ds_read_b64_tr_b16 %" #o ", %" #at
+#define QVX_LO(o, at, n) QVX_TR(o, at) " offset:%" #n "\n\t"
+  if constexpr (N == 1)
+    asm volatile(QVX_LO(0, 2, 3) QVX_LO(1, 2, 4) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(h[0])
+                 : "v"(a[0]), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+  else if constexpr (N == 2)
+    asm volatile(QVX_LO(0, 4, 6) QVX_LO(1, 4, 7) QVX_LO(2, 5, 6) QVX_LO(3, 5, 7) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(h[0]), "=&v"(l[1]), "=&v"(h[1])
+                 : "v"(a[0]), "v"(a[1]), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+  else if constexpr (N == 3)
+    asm volatile(QVX_LO(0, 6, 9) QVX_LO(1, 6, 10) QVX_LO(2, 7, 9) QVX_LO(3, 7, 10) QVX_LO(4, 8, 9) QVX_LO(5, 8, 10)
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(h[0]), "=&v"(l[1]), "=&v"(h[1]), "=&v"(l[2]), "=&v"(h[2])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+  else
+    asm volatile(QVX_LO(0, 8, 12) QVX_LO(1, 8, 13) QVX_LO(2, 9, 12) QVX_LO(3, 9, 13) QVX_LO(4, 10, 12) QVX_LO(5, 10, 13)
+                 QVX_LO(6, 11, 12) QVX_LO(7, 11, 13) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(h[0]), "=&v"(l[1]), "=&v"(h[1]), "=&v"(l[2]), "=&v"(h[2]), "=&v"(l[3]), "=&v"(h[3])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+#undef QVX_LO
+#undef QVX_TR
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = u32x4{l[j][0], l[j][1], h[j][0], h[j][1]};
+}
+
 // What keys that are not there are loaded from.
 __device__ const uint32_t kZeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
-template <uint32_t T, int DP, int KT, bool PARTS, int WGS>
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int WGS>
 __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
   using L = Tile<DP, KT>;
   constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
@@ -91,13 +147,13 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
   const int col = lane & 31, h = lane >> 5;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
-  AttnItem it = attn_item<kRows, true>(c, item, reinterpret_cast<int*>(lds_rows), sums);
-  if (c.mode != kMaskPrefix) attn_note(c, it, item, kvh, sums);
+  AttnItem it = attn_item<kRows, M>(c, item, reinterpret_cast<int*>(lds_rows), sums);
+  if constexpr (M == kMaskWindow) attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
-  if (c.mode == kMaskPrefix) attn_leads<kRows>(c, it, kvh);
-  const AttnView view = attn_view<kRows>(c, it);
+  if constexpr (M == kMaskPrefix) attn_leads<kRows>(c, it, kvh);
+  const AttnView view = attn_view<kRows, M>(c, it);
   it.tile1 = min(it.tile1, view.tiles());
-  if (c.mode == kMaskPrefix) it.seq = it.q0;  // the table's row
+  if constexpr (M == kMaskPrefix) it.seq = it.q0;  // the table's row
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds_rows;
 
@@ -156,7 +212,7 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
 
   // What this lane's row sees, in numbers of keys: [0, first_end) and [low, high); and over the wave's rows.
   const int shift = kAttnTile * (view.first - view.sinks);  // from a number to its key, behind the first tokens' tiles
-  const AttnRange range = attn_range(c, it, view, my_row);
+  const AttnRange range = attn_range<M>(c, it, view, my_row);
   const int first_end = min(range.sinks, range.high), low = range.low - shift;
   const unsigned width = (unsigned)max(range.high - range.low, 0);
   int wave_low = low, wave_high = low + (int)width, most_high = wave_high, least_low = low, most_first = first_end;
@@ -174,25 +230,32 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
   least_low = __builtin_amdgcn_readfirstlane(least_low);
   most_first = __builtin_amdgcn_readfirstlane(most_first);
 
-  // Tile t's keys: number key0 + t KT + lane.  look: asks the table; resolve: the address that it gives, and which keys
-  // are there.
+  // The chunk's keys by number, in blocks of kBlock whose offsets from the cache's start (-1: no such key) stand in LDS, the
+  // next block's looked up in the table while this one is in work: look asks for two keys a thread, place leaves what came.
   const int key0 = it.tile0 * kAttnTile, key_end = it.tile1 * kAttnTile;
+  const int tiles = max(key_end - key0 + KT - 1, 0) / KT;
   const int32_t* table = c.table + (int64_t)it.seq * c.table_width;
   const int64_t head_at = (int64_t)kvh * c.head_stride;
-  int page_id = -1, page_off = 0;
-  int64_t at = -1;
-  auto look = [&](int t) __attribute__((always_inline)) {
-    const int number = key0 + t * KT + (lane & (KT - 1));
-    const int key = number < kAttnTile * view.sinks ? number : number + shift;
-    const bool there = number < key_end && key < view.high && (key >= view.low || key < view.sink_keys);
-    const int column = there ? key / c.table_page : 0;
-    page_off = key - column * c.table_page;
-    page_id = there ? table[column] : -1;
+  int64_t* offsets = reinterpret_cast<int64_t*>(lds_rows + NB * 2 * L::kBytes);  // [2][kBlock]
+  int page_id[2], page_off[2];
+  auto look = [&](int block) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int number = key0 + block * kBlock + 256 * i + tid;
+      const int key = number < kAttnTile * view.sinks ? number : number + shift;
+      const bool there = number < key_end && key < view.high && (key >= view.low || key < view.sink_keys);
+      const int column = there ? key / c.table_page : 0;
+      page_off[i] = key - column * c.table_page;
+      page_id[i] = there ? table[column] : -1;
+    }
   };
-  auto resolve = [&]() __attribute__((always_inline)) {
-    const bool there = (unsigned)page_id < (unsigned)c.n_pages;
-    at = there ? page_id * c.page_stride + head_at + (int64_t)page_off * c.pitch : -1;
-    return (uint64_t)__ballot(there);
+  auto place = [&](int block) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool there = (unsigned)page_id[i] < (unsigned)c.n_pages;
+      offsets[(block & 1) * kBlock + 256 * i + tid] =
+          there ? page_id[i] * c.page_stride + head_at + (int64_t)page_off[i] * c.pitch : -1;
+    }
   };
 
   // Staging, straight to LDS: the lanes of a wave fill 64 slots of 16 bytes in a row, so the swizzle is in what each of
@@ -206,12 +269,12 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
     koff[i] = L::k_unit(r, u) * 8 < d ? 16 * L::k_unit(r, u) : -1;
     voff[i] = L::v_unit(r, u) * 8 < d ? 16 * L::v_unit(r, u) : -1;
   }
-  auto fetch = [&](int buf) __attribute__((always_inline)) {
+  auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+    const int64_t* keys = offsets + t * KT % (2 * kBlock);
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
       if (KT * L::kUnits % 256 != 0 && 64 * (wave + 4 * i) >= KT * L::kUnits) break;
-      const int64_t from = (int64_t)((uint64_t)(uint32_t)__shfl((int)(at >> 32), slot_key[i]) << 32 |
-                                     (uint32_t)__shfl((int)at, slot_key[i]));
+      const int64_t from = keys[slot_key[i]];
       const uint8_t* zeros = reinterpret_cast<const uint8_t*>(kZeros);
       const uint8_t* kp = from >= 0 && koff[i] >= 0 ? c.k + from + koff[i] : zeros;
       const uint8_t* vp = from >= 0 && voff[i] >= 0 ? c.v + from + voff[i] : zeros;
@@ -223,8 +286,14 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
     }
   };
 
-  // Lane addresses of the transposing reads, as in qvx_attn16.hip.
-  const int vrow = 4 * h + (lane & 15) / 4, vcol = 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+  // Lane addresses of the transposing reads, as in qvx_attn16.hip; the swizzle of rows sixteen and eight apart is the same.
+  constexpr int kV = DB % 4 == 0 ? 4 : DB % 3 == 0 ? 3 : DB % 2 == 0 ? 2 : 1;
+  uint32_t value_at[DB];
+#pragma unroll
+  for (int e = 0; e < DB; ++e) {
+    const int vrow = 4 * h + (lane & 15) / 4, vcol = 32 * e + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+    value_at[e] = (uint32_t)(uintptr_t)(lds + L::kBytes) + L::v_at(vrow, vcol / 8) + 2 * (vcol & 7);
+  }
 
   float m = -INFINITY, l = 0.0f;
   bool saw = false;
@@ -234,9 +303,9 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
 
-  // One tile from buffer `buf`; `there`: the keys that are.
-  auto tile = [&]<bool MASKED>(int first, int buf, uint64_t there) __attribute__((always_inline)) {
-    const LdsPtr kb = lds + buf * 2 * L::kBytes, vb = kb + L::kBytes;
+  // One tile from buffer `buf`; `there`: the keys that are; masked: some row of the wave does not see all of them.
+  auto tile = [&](int first, int buf, uint64_t there, bool masked) __attribute__((always_inline)) {
+    const LdsPtr kb = lds + buf * 2 * L::kBytes;
     f32x16 s[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b)
@@ -250,7 +319,12 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
 #pragma unroll
         for (int j = QP - 1; j >= 0; --j) s[b] = mma<T>(a, q[j][i], s[b]);
       }
-    if constexpr (MASKED) {
+    // The mask alone stands in a branch, which changes the products in place: with two versions of the tile the sums change
+    // registers between them.  The products have to be there on either way, and a branch right behind the instruction hides
+    // from the compiler what it has to wait for: twenty wait states, one more than it takes.
+#pragma unroll
+    for (int b = 0; b < KB; ++b) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[b]));
+    if (masked) {
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
         const uint32_t mine = (uint32_t)(there >> (32 * b)) >> (4 * h);
@@ -299,63 +373,70 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
         }
         if constexpr (PARTS) p[PP - 1][b][r / 8][r / 2 % 4] = pack2<T>(x - low2<T>(xy), y - high2<T>(xy));
       }
+    unrolled<2 * KB>([&]<int S>() __attribute__((always_inline)) {  // sixteen keys a step
+      constexpr int B = S / 2, N = S % 2;
+      unrolled<DB / kV>([&]<int E>() __attribute__((always_inline)) {
+        u32x4 v[kV];
+        uint32_t from[kV];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+        for (int j = 0; j < kV; ++j) from[j] = value_at[E * kV + j] + (uint32_t)(buf * 2 * L::kBytes);
+        read_values<kV, 16 * S * L::kPitch, 8 * L::kPitch>(v, from);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int j = 0; j < kV; ++j)
 #pragma unroll
-        for (int e = 0; e < DB; ++e) {
-          const int r0 = 32 * b + 16 * n + vrow, cc = 32 * e + vcol;
-          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) i16x4*)(vb + L::v_at(r0, cc / 8) + 2 * (cc & 7)));
-          const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) i16x4*)(vb + L::v_at(r0 + 8, cc / 8) + 2 * (cc & 7)));
-          const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int j = PP - 1; j >= 0; --j) acc[e] = mma<T>(__builtin_bit_cast(u32x4, v), p[j][b][n], acc[e]);
-        }
+          for (int i = PP - 1; i >= 0; --i) acc[E * kV + j] = mma<T>(v[j], p[i][B][N], acc[E * kV + j]);
+      });
+    });
   };
 
-  const int tiles = max(key_end - key0 + KT - 1, 0) / KT;
   const bool any_row = it.row0 + 32 * wave < it.rows;  // a wave past the rows only stages
   constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
-  uint64_t there = 0, next = 0;
+  constexpr int kTiles = kBlock / KT;  // of a block
+  // Copies a wave has on its way at least for each tile behind the next one: the next one has landed when no more are.
+  constexpr int kBehind = (NB - 2) * 2 * (KT * L::kUnits / 256);
   if (tiles > 0) {
     look(0);
-    there = resolve() & kAll;
-    fetch(0);
-    look(1);
-    next = resolve() & kAll;
+    place(0);
+    if (tiles > kTiles) look(1);
   }
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile is in LDS when everyone passes the barrier
   __syncthreads();
-  for (int t0 = 0; t0 < tiles; t0 += 2) {
 #pragma unroll
-    for (int buf = 0; buf < 2; ++buf) {
-      const int t = t0 + buf;
-      if (t >= tiles) break;
-      if (t + 1 < tiles) fetch(buf ^ 1);  // the buffer that everyone left a barrier ago
-      if (t + 2 < tiles) look(t + 2);
-      const int first = key0 + t * KT;
-      const bool none = !any_row || there == 0 || ((first >= most_high || first + KT <= least_low) && first >= most_first);
-      if (!none) {
-        if (there == kAll && first >= wave_low && first + KT <= wave_high)
-          tile.template operator()<false>(first, buf, there);
-        else
-          tile.template operator()<true>(first, buf, there);
-      }
-      there = next;
-      if (t + 2 < tiles) next = resolve() & kAll;
-      __builtin_amdgcn_s_waitcnt(0x0f70);
-      __syncthreads();
+  for (int t = 0; t < NB - 1; ++t)
+    if (t < tiles) fetch(t, t);
+  if (tiles > NB - 1)
+    wait_copies<kBehind>();
+  else
+    wait_copies<0>();
+  meet();
+  // Buffers by number, not by unrolling: constants of several buffers would be held in registers across the loop.
+  int buf = 0;
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    const int ahead = t + NB - 1;
+    if (ahead < tiles) fetch(ahead, buf == 0 ? NB - 1 : buf - 1);  // the buffer that everyone left a barrier ago
+    const int first = key0 + t * KT;
+    const uint64_t there = __ballot(offsets[t * KT % (2 * kBlock) + (lane & (KT - 1))] >= 0) & kAll;
+    const bool none = !any_row || there == 0 || ((first >= most_high || first + KT <= least_low) && first >= most_first);
+    if (!none) tile(first, buf, there, there != kAll || first < wave_low || first + KT > wave_high);
+    // In the middle of a block the one before is no longer read, and the next one takes its place.
+    if (t % kTiles == kTiles / 2) {
+      const int block = t / kTiles + 1;
+      if (block * kTiles < tiles) place(block);
+      if ((block + 1) * kTiles < tiles) look(block + 1);
     }
+    if (ahead < tiles)
+      wait_copies<kBehind>();
+    else
+      wait_copies<0>();
+    meet();
+    buf = buf == NB - 1 ? 0 : buf + 1;
   }
 
   l += __shfl_xor(l, 32);
   saw = __shfl_xor((int)saw, 32) || saw;
   if (!live) return;
   if (saw) m = fmaxf(m, kAttnLow);
-  if (it.chunks > 1 || c.mode == kMaskPrefix) {  // a part of the keys
+  if (it.chunks > 1 || M == kMaskPrefix) {  // a part of the keys
     const int d16 = (d + 15) & ~15, r16 = row - it.row0;
     float* part = attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(kRows, d16);
     // weights as small as the split kernel's, whose results these are joined with
@@ -387,7 +468,9 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
         const float o[4] = {acc[e][r] * inv, acc[e][r + 1] * inv, acc[e][r + 2] * inv, acc[e][r + 3] * inv};
         attn_store4(c.out, oat + i, c.q_type, o);
       } else {
-        const u32x2 w = {pack2<T>(acc[e][r] * inv, acc[e][r + 1] * inv), pack2<T>(acc[e][r + 2] * inv, acc[e][r + 3] * inv)};
+        uint32_t w0 = pack2<T>(acc[e][r] * inv, acc[e][r + 1] * inv), w1 = pack2<T>(acc[e][r + 2] * inv, acc[e][r + 3] * inv);
+        asm("" : "+v"(w0), "+v"(w1));  // one product and rounding for both stores: a last bit could depend on the stride
+        const u32x2 w = {w0, w1};
         uint16_t* o = static_cast<uint16_t*>(c.out) + oat + i;
         if (c.out_wide) {
           *reinterpret_cast<u32x2*>(o) = w;
@@ -399,31 +482,38 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
     }
 }
 
-template <uint32_t T, int DP, int KT, bool PARTS, int WGS> bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int WGS>
+bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
   static LdsLimit lim;
-  const size_t lds = 4 * (size_t)Tile<DP, KT>::kBytes;
-  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_rows<T, DP, KT, PARTS, WGS>), lim, lds)) return false;
-  k_attn_rows<T, DP, KT, PARTS, WGS><<<grid, 256, lds, s>>>(c);
+  const auto kernel = &k_attn_rows<T, M, DP, KT, NB, PARTS, WGS>;
+  constexpr size_t lds = NB * 2 * (size_t)Tile<DP, KT>::kBytes + 2 * kBlock * sizeof(int64_t);
+  static_assert(WGS * lds <= kLdsPerCU);
+  if (!lds_ready(reinterpret_cast<const void*>(kernel), lim, lds)) return false;
+  kernel<<<grid, 256, lds, s>>>(c);
   return true;
 }
 
 // Registers: with parts a query row alone takes two or three times the others'.
-template <uint32_t T> bool launch_dp(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
+template <uint32_t T, int M> bool launch_dp(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
   const int d = c.head_dim;
   if (!parts) {
-    if (d <= 32) return launch<T, 32, 64, false, 3>(c, grid, s);
-    if (d <= 64) return launch<T, 64, 64, false, 3>(c, grid, s);
-    if (d <= 96) return launch<T, 96, 64, false, 2>(c, grid, s);
-    if (d <= 128) return launch<T, 128, 64, false, 2>(c, grid, s);
-    if (d <= 160) return launch<T, 160, 32, false, 2>(c, grid, s);
-    return launch<T, 256, 32, false, 1>(c, grid, s);
+    if (d <= 32) return launch<T, M, 32, 64, 4, false, 3>(c, grid, s);
+    if (d <= 64) return launch<T, M, 64, 64, 2, false, 3>(c, grid, s);
+    if (d <= 96) return launch<T, M, 96, 64, 2, false, 2>(c, grid, s);
+    if (d <= 128) return launch<T, M, 128, 64, 2, false, 2>(c, grid, s);
+    if (d <= 160) return launch<T, M, 160, 32, 3, false, 2>(c, grid, s);
+    return launch<T, M, 256, 32, 3, false, 1>(c, grid, s);
   }
-  if (d <= 32) return launch<T, 32, 64, true, 2>(c, grid, s);
-  if (d <= 64) return launch<T, 64, 64, true, 2>(c, grid, s);
-  if (d <= 96) return launch<T, 96, 32, true, 2>(c, grid, s);
-  if (d <= 128) return launch<T, 128, 32, true, 2>(c, grid, s);
-  if (d <= 160) return launch<T, 160, 32, true, 1>(c, grid, s);
-  return launch<T, 256, 32, true, 1>(c, grid, s);
+  if (d <= 32) return launch<T, M, 32, 64, 4, true, 2>(c, grid, s);
+  if (d <= 64) return launch<T, M, 64, 64, 3, true, 2>(c, grid, s);
+  if (d <= 96) return launch<T, M, 96, 32, 4, true, 2>(c, grid, s);
+  if (d <= 128) return launch<T, M, 128, 32, 4, true, 2>(c, grid, s);
+  if (d <= 160) return launch<T, M, 160, 32, 3, true, 1>(c, grid, s);
+  return launch<T, M, 256, 32, 3, true, 1>(c, grid, s);
+}
+
+template <uint32_t T> bool launch_mode(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
+  return c.mode == kMaskPrefix ? launch_dp<T, kMaskPrefix>(c, parts, grid, s) : launch_dp<T, kMaskWindow>(c, parts, grid, s);
 }
 
 }  // namespace rows

@@ -4,7 +4,7 @@
 namespace qvx {
 
 bool launch_attn_rows_bf16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
-  return rows::launch_dp<T_BF16>(c, parts, grid, s);
+  return rows::launch_mode<T_BF16>(c, parts, grid, s);
 }
 
 }  // namespace qvx

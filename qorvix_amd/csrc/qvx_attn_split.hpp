@@ -188,6 +188,14 @@ __device__ __forceinline__ int64_t attn_row(const AttnCall& c, int q0, int row, 
   return (int64_t)(q0 + query) * stride + (int64_t)(kvh * c.group + head) * c.head_dim;
 }
 
+// A value that workgroups on other XCDs read, or wrote.
+__device__ __forceinline__ void attn_put(float* p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float attn_get(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 __device__ __forceinline__ float attn_pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The queries as the first product's right operand, KS pieces of 32 values.  F32: fp32 itself, eight
@@ -322,10 +330,12 @@ __device__ __forceinline__ AttnQuery<T_F16, 1>::Key attn_bytes(const uint32_t (&
 }
 
 // DT: head_dim rounded up to 64, 128 or 256.  T: the type of the keys and values.  NS: sets of four
-// rows of a row tile, 1, 2 or 4.  MASK: rows see parts of their sequence's keys (AttnCall::mode).
-template <uint32_t T, int DT, bool FULL, int NS, bool MASK>
+// rows of a row tile, 1, 2 or 4.  M: the call's mode, in which rows may see parts of their
+// sequence's keys.
+template <uint32_t T, int DT, bool FULL, int NS, int M>
 __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_split(AttnCall c) {
   using Tile = AttnTile<T, DT, FULL, NS>;
+  constexpr bool MASK = M != kNoMask;
   constexpr int KS = Tile::KS, VB = Tile::VB, VU = Tile::VU, VN = Tile::VN, R = 4 * NS;
   constexpr int kKeyBytes = AttnRaw<T, 8>::kBytes, kValBytes = AttnRaw<T, VU>::kBytes / VU;
   constexpr bool kQ8 = T == T_Q8_0, kGroup = Tile::kGroup;
@@ -335,15 +345,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int col = lane & 15, g = lane >> 4;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
-  AttnItem it = attn_item<R, MASK>(c, item, reinterpret_cast<int*>(lds), sums);
+  AttnItem it = attn_item<R, M>(c, item, reinterpret_cast<int*>(lds), sums);
   AttnView view{};
   if constexpr (MASK) {
-    if (c.mode != kMaskPrefix) attn_note(c, it, item, kvh, sums);
+    if (M == kMaskWindow) attn_note(c, it, item, kvh, sums);  // what k_attn_join needs
     if (!it.any) return;
-    if (c.mode == kMaskPrefix) attn_leads<R>(c, it, kvh);
-    view = attn_view<R>(c, it);
+    if (M == kMaskPrefix) attn_leads<R>(c, it, kvh);
+    view = attn_view<R, M>(c, it);
     it.tile1 = min(it.tile1, view.tiles());  // may end before tile0: a chunk without keys
-    if (c.mode == kMaskPrefix) it.seq = it.q0;  // the table's row
+    if (M == kMaskPrefix) it.seq = it.q0;  // the table's row
   } else {
     attn_note(c, it, item, kvh, sums);
     if (!it.any) return;
@@ -487,7 +497,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
 #pragma unroll
     for (int t = 0; t < NT; ++t) saw[t] = 0;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) range[t] = attn_range(c, it, view, it.row0 + (kSets ? 4 * t + (lane & 3) : col));
+    for (int t = 0; t < NT; ++t) range[t] = attn_range<M>(c, it, view, it.row0 + (kSets ? 4 * t + (lane & 3) : col));
   }
 
   // This lane's query values: row col's pieces; rows and values that are not there are zeros.
@@ -652,8 +662,73 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       }
     }
   };
+  // The rest of a sequence takes what its shared prefix left into its first chunk: the partial results of the prefix's
+  // chunks, joined by two halves of the workgroup while the first tile is on its way, count as two waves more.
+  const int d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0), quads = d / 4;
+  AttnLead lead{0, 0, 0, 0};
+  if constexpr (M == kMaskRest) {
+    if (it.chunk == 0) {
+      lead = c.leads[it.seq];
+      // groups that are no running sums may have left a query out: nothing past the workspace then
+      if (lead.row < 0 || lead.slot0 < 0 || lead.chunks < 0 || lead.row > c.n_q * c.group ||
+          lead.slot0 + (int64_t)((lead.row + it.rows - 1) / c.lead_rows + 1) * lead.chunks > c.lead_slots)
+        lead.chunks = 0;
+    }
+  }
+  const int ways = kAttnWaves + (M == kMaskRest && lead.chunks ? 2 : 0);
+  float* lm = lds;             // [way][R]
+  float* ll = lds + ways * R;  // [way][R]
+  float* v0 = lds + 2 * ways * R;
+  auto take_lead = [&]() __attribute__((always_inline)) {
+    __syncthreads();  // attn_item's words have been read
+    const int half = threadIdx.x >> 7;
+    const size_t size = attn_part(c.lead_rows, d16), step = (size_t)c.kv_heads * size;
+    for (int e = threadIdx.x & 127; e < nrow * quads; e += 128) {
+      const int r = e / quads, i = 4 * (e - r * quads);
+      const int row = lead.row + it.row0 + r, tile = row / c.lead_rows, rr = row - tile * c.lead_rows;
+      const float* p = attn_parts(const_cast<float*>(c.lead_ws), c.lead_slots) +
+                       ((size_t)(lead.slot0 + tile * lead.chunks) * c.kv_heads + kvh) * size;
+      float top = -INFINITY, sum = 0.0f;
+      f32x4 val = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      constexpr int kBatch = 8;
+      for (int j0 = half; j0 < lead.chunks; j0 += 2 * kBatch) {
+        float mj[kBatch], lj[kBatch];
+        f32x4 vj[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float* x = p + min(j0 + 2 * k, lead.chunks - 1) * step;
+          mj[k] = x[c.lead_rows * d16 + rr];
+          lj[k] = x[c.lead_rows * (d16 + 1) + rr];
+          vj[k] = *reinterpret_cast<const f32x4*>(x + rr * d16 + i);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (j0 + 2 * k >= lead.chunks) mj[k] = -INFINITY;
+          now = fmaxf(now, mj[k]);
+        }
+        const float base = now == -INFINITY ? 0.0f : now, f0 = attn_pow2(top - base);
+        top = now;
+        sum *= f0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) val[x] *= f0;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (mj[k] == -INFINITY) continue;  // no keys
+          const float f = attn_pow2(mj[k] - base);
+          sum += lj[k] * f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) val[x] += vj[k][x] * f;
+        }
+      }
+      *reinterpret_cast<f32x4*>(v0 + ((kAttnWaves + half) * R + r) * d16 + i) = val;
+      if (i == 0) lm[(kAttnWaves + half) * R + r] = top, ll[(kAttnWaves + half) * R + r] = sum;
+    }
+  };
   auto run = [&]<int AUX>() __attribute__((always_inline)) {
     load.template operator()<AUX>(held[0], 0);
+    if constexpr (M == kMaskRest)
+      if (lead.chunks) take_lead();
     set_query();
     for (int n = 0; n < tiles; n += kHeld) {
 #pragma unroll
@@ -686,10 +761,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   }
 
   // Join the waves: m, l and the values of the rows, through LDS.
-  const int d16 = (d + 15) & ~15, nrow = min(R, it.rows - it.row0);
-  float* lm = lds;                   // [wave][R]
-  float* ll = lds + kAttnWaves * R;  // [wave][R]
-  float* lv = lds + 2 * kAttnWaves * R + wave * R * d16;
+  float* lv = v0 + wave * R * d16;
   __syncthreads();  // attn_item's words have been read
   if constexpr (kSets) {
 #pragma unroll
@@ -741,80 +813,43 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         if (col * VB + j < d) lv[(4 * g + r) * d16 + col * VB + j] = acc[0][j][r];
   }
   __syncthreads();
-  const float* v0 = lds + 2 * kAttnWaves * R;
-  const bool whole = it.chunks == 1 && !attn_parts_always<MASK>(c);
-  // The rest of a sequence takes what its shared prefix left into its first chunk.
-  AttnLead lead{0, 0, 0, 0};
-  if constexpr (MASK) {
-    if (c.mode == kMaskRest && it.chunk == 0) {
-      lead = c.leads[it.seq];
-      // groups that are no running sums may have left a query out: nothing past the workspace then
-      if (lead.row < 0 || lead.slot0 < 0 || lead.chunks < 0 || lead.row > c.n_q * c.group ||
-          lead.slot0 + (int64_t)((lead.row + it.rows - 1) / c.lead_rows + 1) * lead.chunks > c.lead_slots)
-        lead.chunks = 0;
-    }
-  }
-  float* part = !whole ? attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16)
-                              : nullptr;
-  const int quads = d / 4;
+  const bool whole = it.chunks == 1 && !attn_parts_always<M>();
+  float* part = whole ? nullptr
+                      : attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(R, d16);
+  // A rest's parts are joined by whichever chunk is done last (below): stored where the others find them, whatever their XCD.
+  const bool met = M == kMaskRest && !whole;
   for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
     const int r = e / quads, i = 4 * (e - r * quads);
     float top = lm[r];
-#pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, lm[w * R + r]);
+    for (int w = 1; w < ways; ++w) top = fmaxf(top, lm[w * R + r]);
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     f32x4 val = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
+    auto add = [&](int w) __attribute__((always_inline)) {
       const float f = attn_pow2(lm[w * R + r] - ref);
       sum += ll[w * R + r] * f;
       const f32x4 x = *reinterpret_cast<const f32x4*>(v0 + (w * R + r) * d16 + i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) val[k] += x[k] * f;
-    }
-    if constexpr (MASK) {
-      const int row = lead.row + it.row0 + r, tile = lead.chunks ? row / c.lead_rows : 0, rr = row - tile * c.lead_rows;
-      const size_t size = attn_part(c.lead_rows, d16), step = (size_t)c.kv_heads * size;
-      const float* p = lead.chunks ? attn_parts(const_cast<float*>(c.lead_ws), c.lead_slots) +
-                                         ((size_t)(lead.slot0 + tile * lead.chunks) * c.kv_heads + kvh) * size
-                                   : nullptr;
-      for (int j0 = 0; j0 < lead.chunks; j0 += 4) {
-        float mj[4], lj[4];
-        f32x4 vj[4];
+    };
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float* x = p + min(j0 + k, lead.chunks - 1) * step;
-          mj[k] = x[c.lead_rows * d16 + rr];
-          lj[k] = x[c.lead_rows * (d16 + 1) + rr];
-          vj[k] = *reinterpret_cast<const f32x4*>(x + rr * d16 + i);
-        }
-        float now = top;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (j0 + k >= lead.chunks) mj[k] = -INFINITY;
-          now = fmaxf(now, mj[k]);
-        }
-        const float base = now == -INFINITY ? 0.0f : now, f0 = attn_pow2(top - base);
-        top = now;
-        sum *= f0;
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) val[e4] *= f0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (mj[k] == -INFINITY) continue;  // no keys: what its values hold does not count
-          const float f = attn_pow2(mj[k] - base);
-          sum += lj[k] * f;
-#pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4) val[e4] += vj[k][e4] * f;
-        }
-      }
+    for (int w = 0; w < kAttnWaves; ++w) add(w);
+    if (M == kMaskRest && ways > kAttnWaves) {
+      add(kAttnWaves);
+      add(kAttnWaves + 1);
     }
     if (whole) {
       float o[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = top == -INFINITY ? 0.0f : val[k] / sum;
       attn_store4(c.out, attn_row(c, it.q0, it.row0 + r, kvh, c.out_stride) + i, c.q_type, o);
+    } else if (met) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) attn_put(part + r * d16 + i + k, val[k]);
+      if (i == 0) {
+        attn_put(part + R * d16 + r, top);
+        attn_put(part + R * (d16 + 1) + r, sum);
+      }
     } else {
       *reinterpret_cast<f32x4*>(part + r * d16 + i) = val;
       if (i == 0) {
@@ -823,32 +858,85 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       }
     }
   }
+  if constexpr (M == kMaskRest) {
+    if (!met) return;
+    // The chunk that finds the others done adds the parts up, in the order of the chunks.  Coherent accesses of device scope, each
+    // wave's stores complete before the barrier and the count behind it, need no fence.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* last = reinterpret_cast<int*>(lds);
+    if (threadIdx.x == 0)
+      *last = __hip_atomic_fetch_add(c.arrived + ((int64_t)it.seq * c.rest_tiles + it.row0 / R) * c.kv_heads + kvh, 1,
+                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*last != it.chunks - 1) return;
+    const size_t size = attn_part(R, d16), step = (size_t)c.kv_heads * size;
+    const float* first = part - it.chunk * step;
+    for (int e = threadIdx.x; e < nrow * quads; e += 64 * kAttnWaves) {
+      const int r = e / quads, i = 4 * (e - r * quads);
+      float top = -INFINITY, sum = 0.0f, val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j0 = 0; j0 < it.chunks; j0 += 4) {
+        float mj[4], lj[4], vj[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* x = first + min(j0 + k, it.chunks - 1) * step;
+          mj[k] = attn_get(x + R * d16 + r);
+          lj[k] = attn_get(x + R * (d16 + 1) + r);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) vj[k][y] = attn_get(x + r * d16 + i + y);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (j0 + k >= it.chunks) mj[k] = -INFINITY;
+          now = fmaxf(now, mj[k]);
+        }
+        const float base = now == -INFINITY ? 0.0f : now, f0 = attn_pow2(top - base);
+        top = now;
+        sum *= f0;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) val[y] *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (mj[k] == -INFINITY) continue;
+          const float f = attn_pow2(mj[k] - base);
+          sum += lj[k] * f;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) val[y] += vj[k][y] * f;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) val[y] = top == -INFINITY ? 0.0f : val[y] / sum;
+      attn_store4(c.out, attn_row(c, it.q0, it.row0 + r, kvh, c.out_stride) + i, c.q_type, val);
+    }
+  }
 }
 
 // Rows of a row tile, 4, 8 or 16: as many as a call's row tiles hold (the launchers' and the join's R).
-template <uint32_t T, int DT, bool FULL, int NS, bool MASK> bool attn_split(const AttnCall& c, dim3 grid, hipStream_t s) {
+template <uint32_t T, int DT, bool FULL, int NS, int M> bool attn_split(const AttnCall& c, dim3 grid, hipStream_t s) {
   static LdsLimit lim;
-  const size_t lds = (size_t)kAttnWaves * 4 * NS * (2 + (c.head_dim + 15) / 16 * 16) * sizeof(float);
-  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, DT, FULL, NS, MASK>), lim, lds)) return false;
-  k_attn_split<T, DT, FULL, NS, MASK><<<grid, 64 * kAttnWaves, lds, s>>>(c);
+  const int ways = kAttnWaves + (M == kMaskRest ? 2 : 0);
+  const size_t lds = (size_t)ways * 4 * NS * (2 + (c.head_dim + 15) / 16 * 16) * sizeof(float);
+  if (!lds_ready(reinterpret_cast<const void*>(&k_attn_split<T, DT, FULL, NS, M>), lim, lds)) return false;
+  k_attn_split<T, DT, FULL, NS, M><<<grid, 64 * kAttnWaves, lds, s>>>(c);
   return true;
 }
 
-template <uint32_t T, int DT, bool FULL, bool MASK> bool attn_split_rows(const AttnCall& c, dim3 grid, hipStream_t s) {
-  if (c.tile_rows == 4) return attn_split<T, DT, FULL, 1, MASK>(c, grid, s);
-  if (c.tile_rows == 8) return attn_split<T, DT, FULL, 2, MASK>(c, grid, s);
-  return attn_split<T, DT, FULL, 4, MASK>(c, grid, s);
+template <uint32_t T, int DT, bool FULL, int M> bool attn_split_rows(const AttnCall& c, dim3 grid, hipStream_t s) {
+  if (c.tile_rows == 4) return attn_split<T, DT, FULL, 1, M>(c, grid, s);
+  if (c.tile_rows == 8) return attn_split<T, DT, FULL, 2, M>(c, grid, s);
+  return attn_split<T, DT, FULL, 4, M>(c, grid, s);
 }
 
-template <uint32_t T, bool MASK = false> bool attn_split_dt(const AttnCall& c, dim3 grid, hipStream_t s) {
+template <uint32_t T, int M = kNoMask> bool attn_split_dt(const AttnCall& c, dim3 grid, hipStream_t s) {
   if constexpr (T == T_Q8_0) {
-    if (c.head_dim == 64) return attn_split_rows<T, 64, true, MASK>(c, grid, s);
-    if (c.head_dim == 128) return attn_split_rows<T, 128, true, MASK>(c, grid, s);
-    if (c.head_dim == 256) return attn_split_rows<T, 256, true, MASK>(c, grid, s);
+    if (c.head_dim == 64) return attn_split_rows<T, 64, true, M>(c, grid, s);
+    if (c.head_dim == 128) return attn_split_rows<T, 128, true, M>(c, grid, s);
+    if (c.head_dim == 256) return attn_split_rows<T, 256, true, M>(c, grid, s);
   }
-  if (c.head_dim <= 64) return attn_split_rows<T, 64, false, MASK>(c, grid, s);
-  if (c.head_dim <= 128) return attn_split_rows<T, 128, false, MASK>(c, grid, s);
-  return attn_split_rows<T, 256, false, MASK>(c, grid, s);
+  if (c.head_dim <= 64) return attn_split_rows<T, 64, false, M>(c, grid, s);
+  if (c.head_dim <= 128) return attn_split_rows<T, 128, false, M>(c, grid, s);
+  return attn_split_rows<T, 256, false, M>(c, grid, s);
 }
 
 }  // namespace qvx
