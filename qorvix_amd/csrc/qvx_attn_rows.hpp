@@ -6,7 +6,7 @@
 // as in qvx_attn16.hip (128 rows a workgroup, 32 a wave; S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction; K and V
 // tiles staged in LDS, the next one in flight).  What is different:
 //
-// Pages.  The keys' offsets are looked up 512 at a time, half such a block ahead, and stand in LDS, so a page may hold any
+// Pages.  The keys' offsets are looked up 1024 at a time, half a block ahead, and stand in LDS, so a page may hold any
 // number of tokens.  Tiles are copied to LDS straight from the pages, NB - 1 tiles ahead.
 //
 // Masks.  The tiles of sixteen keys that any row of the tile sees are numbered one behind the other (AttnView), first tokens
@@ -56,13 +56,15 @@ template <uint32_t T> __device__ __forceinline__ uint32_t pack2(float x, float y
     return __builtin_bit_cast(uint32_t, h);
   }
 }
-template <uint32_t T> __device__ __forceinline__ float low2(uint32_t w) {
-  if constexpr (T == T_F16) return (float)__builtin_bit_cast(f16x2, w).x;
-  return __builtin_bit_cast(float, w << 16);
-}
-template <uint32_t T> __device__ __forceinline__ float high2(uint32_t w) {
-  if constexpr (T == T_F16) return (float)__builtin_bit_cast(f16x2, w).y;
-  return __builtin_bit_cast(float, w & 0xffff0000u);
+// What is left of x and y beside their rounded values in w.
+template <uint32_t T> __device__ __forceinline__ void leave(float& x, float& y, uint32_t w) {
+  if constexpr (T == T_F16) {
+    asm("" : "+v"(w));  // read back, in one instruction a value: left to itself the compiler rounds x and y again
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    x = __builtin_fmaf((float)h.x, -1.0f, x), y = __builtin_fmaf((float)h.y, -1.0f, y);
+  } else {
+    x -= __builtin_bit_cast(float, w << 16), y -= __builtin_bit_cast(float, w & 0xffff0000u);
+  }
 }
 
 // DP: head_dim rounded up to a multiple of 32; KT: keys of a tile.  Swizzled as in qvx_attn16.hip.
@@ -80,8 +82,7 @@ template <int DP, int KT> struct Tile {
   static __device__ __forceinline__ int v_at(int r, int u) { return r * kPitch + 16 * v_unit(r, u); }
 };
 
-constexpr int kBlock = 512;  // keys whose offsets are looked up together
-static_assert(kBlock == 2 * 256);
+constexpr int kBlock = 1024;  // keys whose offsets are looked up together
 
 // Waits until at most N copies to LDS are on their way.
 template <int N> __device__ __forceinline__ void wait_copies() {
@@ -134,11 +135,40 @@ template <int N, int OFF, int STEP> __device__ __forceinline__ void read_values(
   for (int j = 0; j < N; ++j) v[j] = u32x4{l[j][0], l[j][1], h[j][0], h[j][1]};
 }
 
+// N 16-byte LDS reads, waited for together: one by one each of them would be waited for before the product that needs it.
+template <int N> __device__ __forceinline__ void read_keys(u32x4 (&k)[N], const uint32_t (&a)[N]) {
+#define QVX_RD(o, at) "ds_read_b128 %" #o ", %" #at "\n\t"
+  static_assert(N == 4 || N == 5 || N == 6 || N == 8);
+  if constexpr (N == 4)
+    asm volatile(QVX_RD(0, 4) QVX_RD(1, 5) QVX_RD(2, 6) QVX_RD(3, 7) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+                 : "memory");
+  else if constexpr (N == 5)
+    asm volatile(QVX_RD(0, 5) QVX_RD(1, 6) QVX_RD(2, 7) QVX_RD(3, 8) QVX_RD(4, 9) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4])
+                 : "memory");
+  else if constexpr (N == 6)
+    asm volatile(QVX_RD(0, 6) QVX_RD(1, 7) QVX_RD(2, 8) QVX_RD(3, 9) QVX_RD(4, 10) QVX_RD(5, 11) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4]), "=&v"(k[5])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5])
+                 : "memory");
+  else
+    asm volatile(QVX_RD(0, 8) QVX_RD(1, 9) QVX_RD(2, 10) QVX_RD(3, 11) QVX_RD(4, 12) QVX_RD(5, 13) QVX_RD(6, 14)
+                 QVX_RD(7, 15) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4]), "=&v"(k[5]), "=&v"(k[6]), "=&v"(k[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+                 : "memory");
+#undef QVX_RD
+}
+
 // What keys that are not there are loaded from.
 __device__ const uint32_t kZeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
-template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int WGS>
-__global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
+// W: workgroups a CU.
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W>
+__global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   using L = Tile<DP, KT>;
   constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
   constexpr int QP = !PARTS ? 1 : T == T_F16 ? 2 : 3, PP = PARTS ? 2 : 1;
@@ -160,6 +190,116 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
   const int row = it.row0 + 32 * wave + col, my_row = min(row, it.rows - 1);
   const bool live = row < it.rows;
   const int64_t qat = attn_row(c, it.q0, my_row, kvh, c.q_stride);
+  // What this lane's row sees, in numbers of keys: [0, first_end) and [low, high); and over the wave's rows.
+  const int shift = kAttnTile * (view.first - view.sinks);  // from a number to its key, behind the first tokens' tiles
+  const AttnRange range = attn_range<M>(c, it, view, my_row);
+  const int first_end = min(range.sinks, range.high), low = range.low - shift;
+  const unsigned width = (unsigned)max(range.high - range.low, 0);
+  // Over the wave's rows: least_low .. most_high and below most_first some row sees a key, wave_low .. wave_high all do.
+  int wave_low = 0, wave_high = 0, most_high = 0, least_low = 0, most_first = 0;
+  if constexpr (M == kMaskWindow) {  // they rise with the row
+    const int row_a = min(it.row0 + 32 * wave, it.rows - 1), row_b = min(row_a + 31, it.rows - 1);
+    const AttnRange ra = attn_range<M>(c, it, view, row_a), rb = attn_range<M>(c, it, view, row_b);
+    least_low = ra.low - shift;
+    wave_high = least_low + max(ra.high - ra.low, 0);
+    wave_low = rb.low - shift;
+    most_high = wave_low + max(rb.high - rb.low, 0);
+    most_first = min(rb.sinks, rb.high);
+  } else {
+    wave_high = most_high = it.len;
+    if (!__all(range.high == it.len)) {  // sequences that end inside their prefix
+      wave_high = most_high = range.high;
+#pragma unroll
+      for (int x = 1; x < 32; x *= 2) {
+        wave_high = min(wave_high, __shfl_xor(wave_high, x));
+        most_high = max(most_high, __shfl_xor(most_high, x));
+      }
+      wave_high = __builtin_amdgcn_readfirstlane(wave_high);
+      most_high = __builtin_amdgcn_readfirstlane(most_high);
+    }
+  }
+
+  // The chunk's keys by number, in blocks of kBlock whose offsets from the cache's start (-1: no such key) stand in LDS, the
+  // next block's looked up in the table while this one is in work: look asks, place leaves what came.
+  const int key0 = it.tile0 * kAttnTile, key_end = it.tile1 * kAttnTile;
+  const int tiles = max(key_end - key0 + KT - 1, 0) / KT;
+  const int32_t* table = c.table + (int64_t)it.seq * c.table_width;
+  const int64_t head_at = (int64_t)kvh * c.head_stride;
+  int64_t* offsets = reinterpret_cast<int64_t*>(lds_rows + NB * 2 * L::kBytes);  // [2][kBlock]
+  constexpr int kLooks = kBlock / 256;
+  int page_id[kLooks], page_off[kLooks];
+  auto look = [&](int block) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLooks; ++i) {
+      const int number = key0 + block * kBlock + 256 * i + tid;
+      const int key = number < kAttnTile * view.sinks ? number : number + shift;
+      const bool there = number < key_end && key < view.high && (key >= view.low || key < view.sink_keys);
+      const int column = there ? key / c.table_page : 0;
+      page_off[i] = key - column * c.table_page;
+      page_id[i] = there ? table[column] : -1;
+    }
+  };
+  auto place = [&](int block) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLooks; ++i) {
+      const bool there = (unsigned)page_id[i] < (unsigned)c.n_pages;
+      offsets[(block & 1) * kBlock + 256 * i + tid] =
+          there ? page_id[i] * c.page_stride + head_at + (int64_t)page_off[i] * c.pitch : -1;
+    }
+  };
+
+  // Staging, straight to LDS: the lanes of a wave fill 64 slots of 16 bytes in a row, so the swizzle is in what each of
+  // them loads.  Slot e = tid + 256 i of a tile is slot e % kUnits of its key e / kUnits.  Keys that are not there and
+  // values past the head's come from the zeros.
+  int slot_key[L::kLoads], koff[L::kLoads], voff[L::kLoads];
+#pragma unroll
+  for (int i = 0; i < L::kLoads; ++i) {
+    const int e = tid + 256 * i, r = e / L::kUnits, u = e - r * L::kUnits;
+    slot_key[i] = r < KT ? r : 0;
+    koff[i] = L::k_unit(r, u) * 8 < d ? 16 * L::k_unit(r, u) : -1;
+    voff[i] = L::v_unit(r, u) * 8 < d ? 16 * L::v_unit(r, u) : -1;
+  }
+  // ask: where tile t's slots come from, by the offsets in LDS, a round before they are copied: nothing waits for them then.
+  int64_t from[L::kLoads];
+  auto ask = [&](int t) __attribute__((always_inline)) {
+    const int64_t* keys = offsets + t * KT % (2 * kBlock);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) from[i] = keys[slot_key[i]];
+  };
+  auto fetch = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) {
+      if (KT * L::kUnits % 256 != 0 && 64 * (wave + 4 * i) >= KT * L::kUnits) break;
+      const uint8_t* zeros = reinterpret_cast<const uint8_t*>(kZeros);
+      const uint8_t* kp = from[i] >= 0 && koff[i] >= 0 ? c.k + from[i] + koff[i] : zeros;
+      const uint8_t* vp = from[i] >= 0 && voff[i] >= 0 ? c.v + from[i] + voff[i] : zeros;
+      const LdsPtr to = lds + buf * 2 * L::kBytes + 1024 * (wave + 4 * i);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp,
+                                       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp,
+                                       (__attribute__((address_space(3))) void*)(to + L::kBytes), 16, 0, 0);
+    }
+  };
+
+  const bool any_row = it.row0 + 32 * wave < it.rows;  // a wave past the rows only stages
+  constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
+  constexpr int kTiles = kBlock / KT;  // of a block
+  static_assert(kTiles - NB > kTiles / 2);  // a block is in place a tile before its first one is asked for
+  // Copies a wave has on its way at least for each tile behind the next one: the next one has landed when no more are.
+  constexpr int kBehind = (NB - 2) * 2 * (KT * L::kUnits / 256);
+  if (tiles > 0) {
+    look(0);
+    place(0);
+    if (tiles > kTiles) look(1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NB - 1; ++t)
+    if (t < tiles) {
+      ask(t);
+      fetch(t);
+    }
+  // The queries, while the first tiles are on their way.
   u32x4 q[QP][KS];
   float mul = c.scale2;  // of a product to a logit in powers of two
   if constexpr (!PARTS) {
@@ -205,89 +345,15 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
         for (int i = 0; i < QP; ++i) {
           const uint32_t w = pack2<T>(a, b);
           q[i][s][j / 2] = w;
-          a -= low2<T>(w), b -= high2<T>(w);
+          leave<T>(a, b, w);
         }
       }
   }
 
-  // What this lane's row sees, in numbers of keys: [0, first_end) and [low, high); and over the wave's rows.
-  const int shift = kAttnTile * (view.first - view.sinks);  // from a number to its key, behind the first tokens' tiles
-  const AttnRange range = attn_range<M>(c, it, view, my_row);
-  const int first_end = min(range.sinks, range.high), low = range.low - shift;
-  const unsigned width = (unsigned)max(range.high - range.low, 0);
-  int wave_low = low, wave_high = low + (int)width, most_high = wave_high, least_low = low, most_first = first_end;
-#pragma unroll
-  for (int x = 1; x < 32; x *= 2) {
-    wave_low = max(wave_low, __shfl_xor(wave_low, x));
-    wave_high = min(wave_high, __shfl_xor(wave_high, x));
-    most_high = max(most_high, __shfl_xor(most_high, x));
-    least_low = min(least_low, __shfl_xor(least_low, x));
-    most_first = max(most_first, __shfl_xor(most_first, x));
-  }
-  wave_low = __builtin_amdgcn_readfirstlane(wave_low);
-  wave_high = __builtin_amdgcn_readfirstlane(wave_high);
-  most_high = __builtin_amdgcn_readfirstlane(most_high);
-  least_low = __builtin_amdgcn_readfirstlane(least_low);
-  most_first = __builtin_amdgcn_readfirstlane(most_first);
-
-  // The chunk's keys by number, in blocks of kBlock whose offsets from the cache's start (-1: no such key) stand in LDS, the
-  // next block's looked up in the table while this one is in work: look asks for two keys a thread, place leaves what came.
-  const int key0 = it.tile0 * kAttnTile, key_end = it.tile1 * kAttnTile;
-  const int tiles = max(key_end - key0 + KT - 1, 0) / KT;
-  const int32_t* table = c.table + (int64_t)it.seq * c.table_width;
-  const int64_t head_at = (int64_t)kvh * c.head_stride;
-  int64_t* offsets = reinterpret_cast<int64_t*>(lds_rows + NB * 2 * L::kBytes);  // [2][kBlock]
-  int page_id[2], page_off[2];
-  auto look = [&](int block) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int number = key0 + block * kBlock + 256 * i + tid;
-      const int key = number < kAttnTile * view.sinks ? number : number + shift;
-      const bool there = number < key_end && key < view.high && (key >= view.low || key < view.sink_keys);
-      const int column = there ? key / c.table_page : 0;
-      page_off[i] = key - column * c.table_page;
-      page_id[i] = there ? table[column] : -1;
-    }
-  };
-  auto place = [&](int block) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool there = (unsigned)page_id[i] < (unsigned)c.n_pages;
-      offsets[(block & 1) * kBlock + 256 * i + tid] =
-          there ? page_id[i] * c.page_stride + head_at + (int64_t)page_off[i] * c.pitch : -1;
-    }
-  };
-
-  // Staging, straight to LDS: the lanes of a wave fill 64 slots of 16 bytes in a row, so the swizzle is in what each of
-  // them loads.  Slot e = tid + 256 i of a tile is slot e % kUnits of its key e / kUnits.  Keys that are not there and
-  // values past the head's come from the zeros.
-  int slot_key[L::kLoads], koff[L::kLoads], voff[L::kLoads];
-#pragma unroll
-  for (int i = 0; i < L::kLoads; ++i) {
-    const int e = tid + 256 * i, r = e / L::kUnits, u = e - r * L::kUnits;
-    slot_key[i] = r < KT ? r : 0;
-    koff[i] = L::k_unit(r, u) * 8 < d ? 16 * L::k_unit(r, u) : -1;
-    voff[i] = L::v_unit(r, u) * 8 < d ? 16 * L::v_unit(r, u) : -1;
-  }
-  auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
-    const int64_t* keys = offsets + t * KT % (2 * kBlock);
-#pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) {
-      if (KT * L::kUnits % 256 != 0 && 64 * (wave + 4 * i) >= KT * L::kUnits) break;
-      const int64_t from = keys[slot_key[i]];
-      const uint8_t* zeros = reinterpret_cast<const uint8_t*>(kZeros);
-      const uint8_t* kp = from >= 0 && koff[i] >= 0 ? c.k + from + koff[i] : zeros;
-      const uint8_t* vp = from >= 0 && voff[i] >= 0 ? c.v + from + voff[i] : zeros;
-      const LdsPtr to = lds + buf * 2 * L::kBytes + 1024 * (wave + 4 * i);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp,
-                                       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp,
-                                       (__attribute__((address_space(3))) void*)(to + L::kBytes), 16, 0, 0);
-    }
-  };
-
   // Lane addresses of the transposing reads, as in qvx_attn16.hip; the swizzle of rows sixteen and eight apart is the same.
   constexpr int kV = DB % 4 == 0 ? 4 : DB % 3 == 0 ? 3 : DB % 2 == 0 ? 2 : 1;
+  constexpr int kK = QP == 3 && DP >= 128 && KS * KB % 4 == 0 ? 4 : KS * KB % 8 == 0 ? 8 : KS * KB % 6 == 0 ? 6 : KS * KB % 5 == 0 ? 5 : 4;
+  const uint32_t key_at = (uint32_t)(uintptr_t)lds;
   uint32_t value_at[DB];
 #pragma unroll
   for (int e = 0; e < DB; ++e) {
@@ -305,20 +371,27 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
 
   // One tile from buffer `buf`; `there`: the keys that are; masked: some row of the wave does not see all of them.
   auto tile = [&](int first, int buf, uint64_t there, bool masked) __attribute__((always_inline)) {
-    const LdsPtr kb = lds + buf * 2 * L::kBytes;
     f32x16 s[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+    unrolled<KS * KB / kK>([&]<int P>() __attribute__((always_inline)) {
+      u32x4 k[kK];
+      uint32_t from[kK];
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        const u32x4 a = *(__attribute__((address_space(3))) u32x4*)(kb + L::k_at(32 * b + col, 2 * i + h));
-#pragma unroll
-        for (int j = QP - 1; j >= 0; --j) s[b] = mma<T>(a, q[j][i], s[b]);
+      for (int j = 0; j < kK; ++j) {  // read (i, b), the b of a step side by side
+        const int i = (P * kK + j) / KB, b = (P * kK + j) % KB;
+        from[j] = key_at + (uint32_t)(buf * 2 * L::kBytes) + L::k_at(32 * b + col, 2 * i + h);
       }
+      read_keys<kK>(k, from);
+#pragma unroll
+      for (int j = 0; j < kK; ++j) {
+        const int i = (P * kK + j) / KB, b = (P * kK + j) % KB;
+#pragma unroll
+        for (int x = QP - 1; x >= 0; --x) s[b] = mma<T>(k[j], q[x][i], s[b]);
+      }
+    });
     // The mask alone stands in a branch, which changes the products in place: with two versions of the tile the sums change
     // registers between them.  The products have to be there on either way, and a branch right behind the instruction hides
     // from the compiler what it has to wait for: twenty wait states, one more than it takes.
@@ -371,7 +444,10 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
         } else {
           l += x + y;
         }
-        if constexpr (PARTS) p[PP - 1][b][r / 8][r / 2 % 4] = pack2<T>(x - low2<T>(xy), y - high2<T>(xy));
+        if constexpr (PARTS) {
+          leave<T>(x, y, xy);
+          p[PP - 1][b][r / 8][r / 2 % 4] = pack2<T>(x, y);
+        }
       }
     unrolled<2 * KB>([&]<int S>() __attribute__((always_inline)) {  // sixteen keys a step
       constexpr int B = S / 2, N = S % 2;
@@ -389,35 +465,32 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
     });
   };
 
-  const bool any_row = it.row0 + 32 * wave < it.rows;  // a wave past the rows only stages
-  constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
-  constexpr int kTiles = kBlock / KT;  // of a block
-  // Copies a wave has on its way at least for each tile behind the next one: the next one has landed when no more are.
-  constexpr int kBehind = (NB - 2) * 2 * (KT * L::kUnits / 256);
-  if (tiles > 0) {
-    look(0);
-    place(0);
-    if (tiles > kTiles) look(1);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < NB - 1; ++t)
-    if (t < tiles) fetch(t, t);
-  if (tiles > NB - 1)
+  if (NB - 1 < tiles) {
+    ask(NB - 1);
     wait_copies<kBehind>();
-  else
+  } else {
     wait_copies<0>();
+  }
+  auto whole = [&](int t) __attribute__((always_inline)) {
+    return (uint64_t)__ballot(offsets[t * KT % (2 * kBlock) + (lane & (KT - 1))] >= 0) & kAll;
+  };
+  uint64_t there = tiles > 0 ? whole(0) : 0;
   meet();
   // Buffers by number, not by unrolling: constants of several buffers would be held in registers across the loop.
   int buf = 0;
 #pragma unroll 1
   for (int t = 0; t < tiles; ++t) {
     const int ahead = t + NB - 1;
-    if (ahead < tiles) fetch(ahead, buf == 0 ? NB - 1 : buf - 1);  // the buffer that everyone left a barrier ago
+    if (ahead < tiles) {
+      fetch(buf == 0 ? NB - 1 : buf - 1);  // the buffer that everyone left a barrier ago
+      if (ahead + 1 < tiles) ask(ahead + 1);
+    }
     const int first = key0 + t * KT;
-    const uint64_t there = __ballot(offsets[t * KT % (2 * kBlock) + (lane & (KT - 1))] >= 0) & kAll;
-    const bool none = !any_row || there == 0 || ((first >= most_high || first + KT <= least_low) && first >= most_first);
-    if (!none) tile(first, buf, there, there != kAll || first < wave_low || first + KT > wave_high);
+    const uint64_t now = there;
+    if (t + 1 < tiles) there = whole(t + 1);
+    const bool none =
+        !any_row || now == 0 || ((first >= most_high || first + KT <= least_low) && first >= most_first);
+    if (!none) tile(first, buf, now, now != kAll || first < wave_low || first + KT > wave_high);
     // In the middle of a block the one before is no longer read, and the next one takes its place.
     if (t % kTiles == kTiles / 2) {
       const int block = t / kTiles + 1;
@@ -434,8 +507,8 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
 
   l += __shfl_xor(l, 32);
   saw = __shfl_xor((int)saw, 32) || saw;
-  if (!live) return;
   if (saw) m = fmaxf(m, kAttnLow);
+  if (!live) return;
   if (it.chunks > 1 || M == kMaskPrefix) {  // a part of the keys
     const int d16 = (d + 15) & ~15, r16 = row - it.row0;
     float* part = attn_parts(c.ws, c.slots) + ((size_t)it.slot * c.kv_heads + kvh) * attn_part(kRows, d16);
@@ -482,30 +555,31 @@ __global__ __launch_bounds__(256, WGS) void k_attn_rows(AttnCall c) {
     }
 }
 
-template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int WGS>
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W>
 bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
   static LdsLimit lim;
-  const auto kernel = &k_attn_rows<T, M, DP, KT, NB, PARTS, WGS>;
+  const auto kernel = &k_attn_rows<T, M, DP, KT, NB, PARTS, W>;
   constexpr size_t lds = NB * 2 * (size_t)Tile<DP, KT>::kBytes + 2 * kBlock * sizeof(int64_t);
-  static_assert(WGS * lds <= kLdsPerCU);
+  static_assert(W * lds <= kLdsPerCU);
   if (!lds_ready(reinterpret_cast<const void*>(kernel), lim, lds)) return false;
   kernel<<<grid, 256, lds, s>>>(c);
   return true;
 }
 
-// Registers: with parts a query row alone takes two or three times the others'.
+// Tiles of 64 keys where the registers reach, of 32 with more of them on their way where queries in parts take two or three
+// times as many.
 template <uint32_t T, int M> bool launch_dp(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
   const int d = c.head_dim;
   if (!parts) {
-    if (d <= 32) return launch<T, M, 32, 64, 4, false, 3>(c, grid, s);
+    if (d <= 32) return launch<T, M, 32, 64, 2, false, 3>(c, grid, s);
     if (d <= 64) return launch<T, M, 64, 64, 2, false, 3>(c, grid, s);
     if (d <= 96) return launch<T, M, 96, 64, 2, false, 2>(c, grid, s);
     if (d <= 128) return launch<T, M, 128, 64, 2, false, 2>(c, grid, s);
     if (d <= 160) return launch<T, M, 160, 32, 3, false, 2>(c, grid, s);
     return launch<T, M, 256, 32, 3, false, 1>(c, grid, s);
   }
-  if (d <= 32) return launch<T, M, 32, 64, 4, true, 2>(c, grid, s);
-  if (d <= 64) return launch<T, M, 64, 64, 3, true, 2>(c, grid, s);
+  if (d <= 32) return launch<T, M, 32, 64, 2, true, 3>(c, grid, s);
+  if (d <= 64) return launch<T, M, 64, 64, 2, true, 2>(c, grid, s);
   if (d <= 96) return launch<T, M, 96, 32, 4, true, 2>(c, grid, s);
   if (d <= 128) return launch<T, M, 128, 32, 4, true, 2>(c, grid, s);
   if (d <= 160) return launch<T, M, 160, 32, 3, true, 1>(c, grid, s);
