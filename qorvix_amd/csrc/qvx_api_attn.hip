@@ -143,9 +143,11 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
 bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 
 // Whether calls of so many rows a sequence (of a mean one) run on the kernel of many rows, and the partition's geometry
-// there: keys in a row, whatever their pages.
+// there: keys in a row, whatever their pages.  Sequences that share a prefix, 8 key heads, split kernel against that one: fp32
+// queries of 128 values 4000 keys 32 rows 25.4 and 26.4 us, 64 26.9 and 27.6, 96 34.7 and 29.3; 16000 keys 32 35.8 and 38.0, 64
+// 45.3 and 40.6; 1000 keys 64 20.1 and 26.2, 256 34.2 and 32.3; fp16 queries 4000 keys 32 25.2 and 22.8, 64 27.1 and 24.1.
 bool many_rows(const qvx_kv_cache* cache, int64_t rows, AttnCall& c) {
-  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 16) return false;
+  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 48) return false;
   c.table_page = c.page_size;
   c.page_size = c.max_len;
   c.page_tiles = (int)(((int64_t)c.max_len + kAttnTile - 1) / kAttnTile);
@@ -196,9 +198,11 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   const int64_t rows = (int64_t)n_seqs * c.group;
   const int64_t mean = (rows + n_groups - 1) / n_groups;
   bool split = false;
-  if (many_rows(cache, mean, c)) {  // every chunk leaves its partial results: as many as the CUs, of 256 keys at least
-    c.min_chunk = 16;
-    c.target = std::max(1, kAttnWgs / 2 / c.kv_heads);
+  // Every chunk leaves its partial results: two chunks a CU, of 128 keys at least.  64 sequences of 4 heads a group behind 1000
+  // keys 28.6 us, with chunks of 256 32.2, of 512 41.5; 128 behind 8192, fp16, 61.6, with a chunk a CU 66.8.
+  if (many_rows(cache, mean, c)) {
+    c.min_chunk = 8;
+    c.target = std::max(1, kAttnWgs / c.kv_heads);
     if (!plan_items(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;
   } else {
     c.tile_rows = tile_rows(mean);
@@ -209,8 +213,12 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   r.lead_rows = c.tile_rows;
   r.lead_slots = c.slots;
   r.tile_rows = tile_rows(r.group);
+  // Whole up to 512 keys: its chunks meet through memory, 4 us or so.  64 sequences of 1 to 512 own tokens behind 8192 49.9 us,
+  // with chunks of 128 keys 56.9, of 1024 50.7; 5 of 1000 32.6, with 256 30.1, with 1024 35.5.
   size_t rest_bytes = 0;
-  if (!plan_split(r, (int64_t)n_seqs * ((r.group + r.tile_rows - 1) / r.tile_rows), &p.join, &rest_bytes)) return QVX_E_RANGE;
+  r.min_chunk = 32;
+  r.target = std::max(1, kAttnWgs / r.kv_heads);
+  if (!plan_items(r, (int64_t)n_seqs * ((r.group + r.tile_rows - 1) / r.tile_rows), &p.join, &rest_bytes)) return QVX_E_RANGE;
   r.rest_tiles = c.rest_tiles = (r.group + r.tile_rows - 1) / r.tile_rows;
   p.arrived_at = sizeof(AttnLead) * (size_t)n_seqs;
   p.lead_bytes = p.arrived_at + (4 * (size_t)n_seqs * r.rest_tiles * r.kv_heads + 15) / 16 * 16;

@@ -55,7 +55,11 @@ template <int THREADS> __device__ __forceinline__ int block_before(int x, int* p
 // ---- fork --------------------------------------------------------------------------------------------
 //
 // Every workgroup looks all forks through for itself (a few loads a thread): how many want a fresh page before its own,
-// whether the free list reaches, whether any is wrong.  Then it takes forks blockIdx.x, + gridDim.x, ...
+// whether the free list reaches, whether any is wrong.  Then it takes kTogether forks and a column of theirs a thread:
+// forks of one prompt hold the same page there, and one atomic counts all of them.  (An atomic each: 128 forks of 256 shared
+// pages 14.8 us, most of it atomics on the same lines.)
+
+constexpr int kTogether = 16;
 
 // What fork i wants: 1 where its sequence's last page is not full; `bad` gets status bits.
 __device__ __forceinline__ int fork_wants(const ForkCall& c, int i, int& bad) {
@@ -70,11 +74,29 @@ __device__ __forceinline__ int fork_wants(const ForkCall& c, int i, int& bad) {
   return len > 0 && len % c.page_size != 0;
 }
 
+// Pages one behind the other that are counted together; `sign` 1 or -1.
+struct PageRun {
+  int32_t* extra;
+  int n_pages, id = -1, n = 0;
+  __device__ __forceinline__ void flush(int sign) {
+    if (n) atomicAdd(&extra[id], sign * n);
+  }
+  __device__ __forceinline__ void take(int page, int sign) {
+    if (!page_ok(page, n_pages)) return;
+    if (page != id) {
+      flush(sign);
+      id = page, n = 0;
+    }
+    ++n;
+  }
+};
+
 __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
   extern __shared__ int32_t rank[];  // [n] fresh pages of the forks before
-  __shared__ int part[kThreads / 64];
+  __shared__ int part[kThreads / 64], all_bad;
   const int tid = threadIdx.x, taken = c.taken_in[0];
-  int bad = taken < 0 ? QVX_MAP_NEGATIVE : 0, all = 0;
+  if (tid == 0) all_bad = taken < 0 ? QVX_MAP_NEGATIVE : 0;
+  int bad = 0, all = 0;
   for (int i0 = 0; i0 < c.n; i0 += kThreads) {
     const int i = i0 + tid;
     const int wants = i < c.n ? fork_wants(c, i, bad) : 0;
@@ -83,35 +105,49 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
     if (i < c.n) rank[i] = all + before;
     all += total;
   }
-  int status = 0;
-#pragma unroll
-  for (int b = 1; b <= QVX_MAP_SEQUENCE; b *= 2) status |= __syncthreads_or(bad & b) ? b : 0;
+  if (bad) atomicOr(&all_bad, bad);
+  __syncthreads();
+  int status = all_bad;
   if (taken >= 0 && (long long)taken + all > c.n_free) status |= QVX_MAP_PAGES;
-  if ((write & kForkTotals) && blockIdx.x == 0 && tid == 0) {
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0 && tid == 0;
+  if ((write & kForkTotals) && first) {
     c.taken_out[0] = status ? taken : taken + all;
     c.taken_out[1] = status;
     *c.n_pairs = status ? 0 : all;
   }
   if (!(write & kForkRows) || status) return;
-  for (int i = blockIdx.x; i < c.n; i += gridDim.x) {
-    const int from = c.from[i], to = c.to[i], len = c.lens[from];
-    const int full = len / c.page_size, left = len - full * c.page_size;
-    const int32_t* old = c.table + (int64_t)from * c.table_width;
-    int32_t* row = c.table + (int64_t)to * c.table_width;
-    for (int col = tid; col < c.table_width; col += kThreads) {
+  // What the workgroup's forks are is read before anything is stored: the compiler has to assume that a store changes it.
+  __shared__ int from[kTogether], to[kTogether], lens[kTogether], fresh[kTogether], place[kTogether];
+  const int i0 = (int)blockIdx.x * kTogether, n = min(kTogether, c.n - i0);
+  if (tid < kTogether) {
+    const int i = i0 + min(tid, n - 1);
+    from[tid] = c.from[i], to[tid] = c.to[i], lens[tid] = tid < n ? c.lens[c.from[i]] : 0, place[tid] = rank[i];
+    fresh[tid] = taken + rank[i] < c.n_free ? c.free_list[taken + rank[i]] : -1;  // lengths that another fork changes: no place
+  }
+  __syncthreads();
+  for (int col = (int)blockIdx.y * kThreads + tid; col < c.table_width; col += (int)gridDim.y * kThreads) {
+    int ids[kTogether];
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) ids[j] = c.table[(int64_t)from[j] * c.table_width + col];
+    PageRun run{c.extra, c.n_pages};
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) {
+      if (j >= n) continue;
+      const int full = lens[j] / c.page_size;
       int id = -1;
       if (col < full) {
-        id = old[col];
-        if (page_ok(id, c.n_pages)) atomicAdd(&c.extra[id], 1);
-      } else if (col == full && left) {
-        id = taken + rank[i] < c.n_free ? c.free_list[taken + rank[i]] : -1;  // lengths that another fork changes: no place
-        c.pairs[2 * rank[i]] = old[col];
-        c.pairs[2 * rank[i] + 1] = id;
+        id = ids[j];
+        run.take(id, 1);
+      } else if (col == full && lens[j] > full * c.page_size) {
+        id = fresh[j];
+        c.pairs[2 * place[j]] = ids[j];
+        c.pairs[2 * place[j] + 1] = id;
       }
-      row[col] = id;
+      c.table[(int64_t)to[j] * c.table_width + col] = id;
     }
-    if (tid == 0) c.lens[to] = len;
+    run.flush(1);
   }
+  if (blockIdx.y == 0 && tid < n) c.lens[to[tid]] = lens[tid];
 }
 
 // ---- release -----------------------------------------------------------------------------------------
@@ -119,23 +155,34 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
 // First every entry is taken out of the table and one holder from its page, which leaves -1 in extra where there was
 // none beside.  Then those are counted, range by range of ids, and stored in front of what is free.
 
-// Entries of row i, by the threads `at`, at + step, ...
-__device__ __forceinline__ void free_row(const FreeCall& c, int i, int at, int step) {
-  const int row = c.rows[i];
-  if ((unsigned)row >= (unsigned)c.n_rows) return;
-  const int begin = c.begin ? min(max(c.begin[i], 0), c.table_width) : 0, end = c.end ? min(c.end[i], c.table_width) : c.table_width;
-  int32_t* entry = c.table + (int64_t)row * c.table_width;
-  for (int col = begin + at; col < end; col += step) {
-    // by exchange: a row that is listed twice is released once
-    const int id = entry[col] < 0 ? -1 : atomicExch(&entry[col], -1);
-    if (page_ok(id, c.n_pages)) atomicSub(&c.extra[id], 1);
+// Column col of rows i0 .. i0 + n - 1, n up to kTogether.
+__device__ __forceinline__ void free_column(const FreeCall& c, int i0, int n, int col) {
+  int rows[kTogether], ids[kTogether];
+#pragma unroll
+  for (int j = 0; j < kTogether; ++j) {  // all read before the first exchange, which would keep them in order
+    const int i = i0 + min(j, n - 1);
+    rows[j] = j < n ? c.rows[i] : -1;
+    if (c.begin && (col < c.begin[i] || col >= c.end[i])) rows[j] = -1;
+    if ((unsigned)rows[j] >= (unsigned)c.n_rows) rows[j] = -1;
   }
-  if (at == 0 && !c.begin && !c.end) c.lens[row] = 0;
+#pragma unroll
+  for (int j = 0; j < kTogether; ++j)  // by exchange: a row that is listed twice is released once
+    ids[j] = rows[j] < 0 ? -1 : atomicExch(&c.table[(int64_t)rows[j] * c.table_width + col], -1);
+  PageRun run{c.extra, c.n_pages};
+#pragma unroll
+  for (int j = 0; j < kTogether; ++j) run.take(ids[j], -1);
+  run.flush(-1);
+}
+// The lengths of the rows from i0 on that are released whole, by the threads t < n.
+__device__ __forceinline__ void free_lens(const FreeCall& c, int i0, int n, int t) {
+  if (t < n && !c.begin && (unsigned)c.rows[i0 + t] < (unsigned)c.n_rows) c.lens[c.rows[i0 + t]] = 0;
 }
 
 __global__ __launch_bounds__(kThreads) void k_free_mark(FreeCall c) {
-  for (int i = blockIdx.x; i < c.n; i += gridDim.x)
-    free_row(c, i, (int)blockIdx.y * kThreads + threadIdx.x, (int)gridDim.y * kThreads);
+  const int i0 = (int)blockIdx.x * kTogether, n = min(kTogether, c.n - i0);
+  for (int col = (int)blockIdx.y * kThreads + threadIdx.x; col < c.table_width; col += (int)gridDim.y * kThreads)
+    free_column(c, i0, n, col);
+  if (blockIdx.y == 0) free_lens(c, i0, n, threadIdx.x);
 }
 
 // Pages freed in each range of kFreePages.
@@ -150,28 +197,38 @@ __global__ __launch_bounds__(1024) void k_free_count(FreeCall c) {
   if (threadIdx.x == 0 && blockIdx.x == 0) c.counts[gridDim.x] = c.taken_in[0];
 }
 
-// The free list's front and the totals.  ONE: this workgroup is the only one and counts for itself; MARK: it also takes the
+// The free list's front and the totals.  ONE: this workgroup is the only one, for up to 16384 pages; MARK: it also takes the
 // entries out.
 template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_store(FreeCall c) {
-  __shared__ int part[16];
-  const int tid = threadIdx.x, lane = tid & 63;
-  constexpr int kEach = kFreePages / 1024;
+  __shared__ int part[16], bad_row;
+  const int tid = threadIdx.x;
+  constexpr int kEach = (ONE ? 2 : 1) * kFreePages / 1024;
+  if (tid == 0) bad_row = 0;
   if constexpr (MARK) {
-    for (int i = tid >> 6; i < c.n; i += 16) free_row(c, i, lane, 64);
+    const int groups = (c.n + kTogether - 1) / kTogether;
+    for (int e = tid; e < groups * c.table_width; e += 1024) {
+      const int g = e / c.table_width;
+      free_column(c, g * kTogether, min(kTogether, c.n - g * kTogether), e - g * c.table_width);
+    }
+    free_lens(c, 0, c.n, tid);  // at most 1024 rows
     __threadfence();  // the counts are taken where the atomics of all waves have arrived
-    __syncthreads();
   }
-  auto gone = [&](int p) {
-    return MARK ? __hip_atomic_load(&c.extra[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0 : c.extra[p] < 0;
-  };
-  const int p0 = (int)blockIdx.x * kFreePages, end = ONE ? c.n_pages : min(p0 + kFreePages, c.n_pages);
-  int before = 0, all = 0;
-  if constexpr (ONE) {
-    int mine = 0;
-    for (int p = tid; p < end; p += 1024) mine += gone(p);
-    all = block_sum<1024>(mine, part);
-  } else {
-    const int blocks = (c.n_pages + kFreePages - 1) / kFreePages;
+  __syncthreads();
+  // a thread takes kEach pages in a row: one scan for all of them
+  const int p0 = (int)blockIdx.x * kFreePages + tid * kEach;
+  int flags = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (p0 + j >= c.n_pages) break;
+    const int x = MARK ? __hip_atomic_load(&c.extra[p0 + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : c.extra[p0 + j];
+    flags |= (x < 0) << j;
+  }
+  if (blockIdx.x == 0)
+    for (int i = tid; i < c.n; i += 1024)
+      if ((unsigned)c.rows[i] >= (unsigned)c.n_rows) bad_row = 1;
+  int all, at = block_before<1024>(__builtin_popcount(flags), part, all);
+  if constexpr (!ONE) {
+    const int blocks = gridDim.x;
     int mine = 0, past = 0;
     for (int b = tid; b < blocks; b += 1024) {
       const int x = c.counts[b];
@@ -179,31 +236,16 @@ template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_st
       past += b < (int)blockIdx.x ? x : 0;
     }
     all = block_sum<1024>(mine, part);
-    before = block_sum<1024>(past, part);
+    at += block_sum<1024>(past, part);
   }
-  int bad = 0;
-  if (blockIdx.x == 0)
-    for (int i = tid; i < c.n; i += 1024) bad |= (unsigned)c.rows[i] >= (unsigned)c.n_rows;
-  const int bad_row = __syncthreads_or(bad);
-  const int taken = ONE ? c.taken_in[0] : c.counts[gridDim.x], first = taken - all;  // may be negative: ids without a place are lost, and said so
-  for (int q = p0; q < end; q += 1024 * kEach) {
-    // a thread takes kEach pages in a row: one scan for all of them
-    int flags = 0;
+  const int taken = ONE ? c.taken_in[0] : c.counts[gridDim.x], first = taken - all;  // negative: ids without a place are lost
+  at += first;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int p = q + tid * kEach + j;
-      if (p < end && gone(p)) flags |= 1 << j;
-    }
-    int total, at = first + before + block_before<1024>(__builtin_popcount(flags), part, total);
-    before += total;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      if (!(flags >> j & 1)) continue;
-      const int p = q + tid * kEach + j;
-      c.extra[p] = 0;
-      if (at >= 0 && at < c.n_free) c.free_list[at] = p;
-      ++at;
-    }
+  for (int j = 0; j < kEach; ++j) {
+    if (!(flags >> j & 1)) continue;
+    c.extra[p0 + j] = 0;
+    if (at >= 0 && at < c.n_free) c.free_list[at] = p0 + j;
+    ++at;
   }
   if (blockIdx.x == 0 && tid == 0) {
     c.taken_out[0] = max(first, 0);
@@ -322,25 +364,27 @@ __global__ __launch_bounds__(kThreads) void k_compact_list(CompactCall c) {
 
 constexpr int kCopyUnit = 16 << 10, kCopyWgs = 2048;
 
-__global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c) {
-  const int parts = (int)((c.page_bytes + kCopyUnit - 1) / kCopyUnit), each = c.n_caches * 2 * parts;
+__global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c, int parts) {
+  const int each = c.n_caches * 2 * parts;
   const int count = c.count ? min(max(*c.count, 0), c.most) : c.most;
-  for (int64_t u = blockIdx.x; u < (int64_t)count * each; u += gridDim.x) {
-    const int pair = (int)(u / each), rest = (int)(u - (int64_t)pair * each), plane = rest / parts, part = rest - plane * parts;
-    const int src = c.pairs[2 * pair], dst = c.pairs[2 * pair + 1];
+  for (int pair = blockIdx.y; pair < count; pair += (int)gridDim.y) {
+    const int src = c.pairs[2 * (int64_t)pair], dst = c.pairs[2 * (int64_t)pair + 1];
     if (!page_ok(src, c.n_pages) || !page_ok(dst, c.n_pages) || src == dst) continue;
-    const auto& x = c.cache[plane >> 1];
-    uint8_t* base = plane & 1 ? x.v : x.k;
-    const int64_t at = (int64_t)part * kCopyUnit + 16 * threadIdx.x;
-    const uint8_t* from = base + src * x.stride;
-    uint8_t* to = base + dst * x.stride;
-    uint4 w[4];
+    for (int u = blockIdx.x; u < each; u += (int)gridDim.x) {
+      const int plane = u / parts, part = u - plane * parts;
+      const auto& x = c.cache[plane >> 1];
+      uint8_t* base = plane & 1 ? x.v : x.k;
+      const int64_t at = (int64_t)part * kCopyUnit + 16 * threadIdx.x;
+      const uint8_t* from = base + src * x.stride;
+      uint8_t* to = base + dst * x.stride;
+      uint4 w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (at + j * 16 * kThreads < c.page_bytes) w[j] = *reinterpret_cast<const uint4*>(from + at + j * 16 * kThreads);
+      for (int j = 0; j < 4; ++j)
+        if (at + j * 16 * kThreads < c.page_bytes) w[j] = *reinterpret_cast<const uint4*>(from + at + j * 16 * kThreads);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (at + j * 16 * kThreads < c.page_bytes) *reinterpret_cast<uint4*>(to + at + j * 16 * kThreads) = w[j];
+      for (int j = 0; j < 4; ++j)
+        if (at + j * 16 * kThreads < c.page_bytes) *reinterpret_cast<uint4*>(to + at + j * 16 * kThreads) = w[j];
+    }
   }
 }
 
@@ -349,19 +393,20 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c) {
 void launch_kv_fork(const ForkCall& c, bool alias, hipStream_t s) {
   const size_t lds = (size_t)c.n * sizeof(int32_t);  // at most 64 KB
   // Totals that lie on what the others read are stored by a launch behind them.
-  k_kv_fork<<<std::min(c.n, 1024), kThreads, lds, s>>>(c, alias ? kForkRows : kForkRows | kForkTotals);
+  const int groups = (c.n + kTogether - 1) / kTogether, cols = std::min((c.table_width + kThreads - 1) / kThreads, 64);
+  k_kv_fork<<<dim3(groups, cols), kThreads, lds, s>>>(c, alias ? kForkRows : kForkRows | kForkTotals);
   if (alias) k_kv_fork<<<1, kThreads, lds, s>>>(c, kForkTotals);
 }
 
 void launch_kv_free(const FreeCall& c, hipStream_t s) {
   const bool one = c.n_pages <= 2 * kFreePages;
-  const int64_t entries = (int64_t)c.n * ((c.table_width + 63) / 64 * 64);
-  if (one && entries <= 8192) {
+  const int groups = (c.n + kTogether - 1) / kTogether, cols = std::min((c.table_width + kThreads - 1) / kThreads, 64);
+  // One workgroup for all of it up to two columns a thread; its launch alone takes less than two.
+  if (one && (int64_t)groups * c.table_width <= 2048 && c.n <= 1024) {
     k_free_store<true, true><<<1, 1024, 0, s>>>(c);
     return;
   }
-  const int cols = std::min((c.table_width + kThreads - 1) / kThreads, 64);
-  k_free_mark<<<dim3(std::min(c.n, 4096), cols), kThreads, 0, s>>>(c);
+  k_free_mark<<<dim3(groups, cols), kThreads, 0, s>>>(c);
   if (one) {
     k_free_store<true, false><<<1, 1024, 0, s>>>(c);
     return;
@@ -384,8 +429,9 @@ bool launch_kv_compact(const CompactCall& c, bool in_place, hipStream_t s) {
 }
 
 void launch_kv_copy(const CopyCall& c, hipStream_t s) {
-  const int64_t units = (int64_t)c.most * c.n_caches * 2 * ((c.page_bytes + kCopyUnit - 1) / kCopyUnit);
-  k_kv_copy<<<(unsigned)std::min<int64_t>(units, kCopyWgs), kThreads, 0, s>>>(c);
+  const int parts = (int)((c.page_bytes + kCopyUnit - 1) / kCopyUnit), each = c.n_caches * 2 * parts;
+  const int wide = std::min(each, kCopyWgs), high = std::min(c.most, std::max(1, kCopyWgs / wide));
+  k_kv_copy<<<dim3(wide, high), kThreads, 0, s>>>(c, parts);
 }
 
 }  // namespace qvx

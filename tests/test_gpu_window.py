@@ -181,7 +181,12 @@ def test_rows_that_see_nothing(cuda, t, group):
     out = qvx.attn_window_t(q, c.desc, table, lens, 10, 0)  # four each
     assert (out[4:9] == 0).all() and torch.isfinite(out).all()
     alone = qvx.attn_window_t(q[9:].contiguous(), c.desc, table[2:].contiguous(), lens[2:], 10, 0)
-    assert torch.allclose(out[9:], alone, atol=1e-6)
+    # Two calls of other sizes may run on other kernels, each within the bar above of the formula; the one of many rows takes
+    # weights in two 16-bit parts, which leave 2^-18 of a weight (bf16), so at most that part of max |v|.
+    k, v = c.rows(2, 0), c.rows(2, 1)
+    most = float((np.abs(q[9:].cpu().double().numpy().reshape(-1, 64)) @ np.abs(k[0]).T).max()) / 8
+    bar = (2 * 2 * U * (67 * most + 3 + 8) + 2.0 ** -18) * float(np.abs(v).max())
+    assert float((out[9:] - alone).abs().max()) <= bar
     table[0, :] = -1
     assert (qvx.attn_window_t(q, c.desc, table, lens, 10, 0)[:4] == 0).all()
 
