@@ -23,7 +23,9 @@ stand-ins; the FFN's SwiGLU activation is the engine's own.
 
 ``PagedDecodeStep`` is the whole layer: the fused projections with rotary positions, a paged key / value
 cache and its attention between them (``qvx_kv_map``, ``qvx_rope_kv``, ``qvx_attn_paged``), for M
-sequences that each get one token a step.
+sequences that each get one token a step; with norms of q and k where the model has them
+(``qvx_norm_rope_kv``), behind a window (``qvx_attn_window``) or a shared prefix (``qvx_attn_shared``) where
+asked for, and with forks of sequences in between (``qvx_kv_fork``, ``qvx_kv_copy``, ``qvx_kv_free``).
 """
 from __future__ import annotations
 
@@ -151,7 +153,8 @@ class Rotation:
 @dataclass
 class Model:
     """Synthetic Llama-3-8B Q4_K_M weights on the device (``layers[l][name]``, ``lm_head``) and the
-    RMSNorm weights (``norms[l]`` = {"attn_norm", "ffn_norm"} fp32 [d], ``output_norm``)."""
+    RMSNorm weights (``norms[l]`` = {"attn_norm", "ffn_norm"} fp32 [d], ``output_norm``; where a model norms
+    its q and k heads also "q_norm", "k_norm" [head_dim])."""
     layers: list = field(default_factory=list)
     lm_head: DevWeight | None = None
     # name of a stacked weight -> ((part name, rows), ...) in row order (see FUSED)
@@ -281,17 +284,34 @@ class Model:
             import torch
             return f.upload(name, device).data.view(torch.float32)
 
+        # Norms of every q and k head: one weight a value of a head.  Longer ones (a norm over all heads, or weights of their own
+        # for each) stay among what is left out.
+        head_dim = f.arch_u64("attention.key_length") or (d // heads if d and heads else None)
+        taken = set()
+
+        def load_head_norm(name):
+            t = f.tensor(name)
+            if t is None or t.type_raw != F32 or t.n_elements != head_dim:
+                return None
+            import torch
+            taken.add(name)
+            return f.upload(name, device).data.view(torch.float32)
+
         for layer in range(n_layers):
             m.layers.append({k: load(f"blk.{layer}.{names[k]}.weight", *shapes[k]) for k, *_ in LAYER_SPECS})
             m.norms.append({"attn_norm": load_norm(f"blk.{layer}.attn_norm.weight"),
                             "ffn_norm": load_norm(f"blk.{layer}.ffn_norm.weight")})
+            for k, name in (("q_norm", "attn_q_norm"), ("k_norm", "attn_k_norm")):
+                w = load_head_norm(f"blk.{layer}.{name}.weight")
+                if w is not None:
+                    m.norms[-1][k] = w
         head = "output.weight" if f.tensor("output.weight") is not None else "token_embd.weight"
         m.lm_head = load(head, None, d)
         m.output_norm = load_norm("output_norm.weight")
         eps = f.get_f64(f"{f.architecture}.attention.layer_norm_rms_epsilon") if f.architecture else None
         m.eps = float(eps) if eps is not None else NORM_EPS
         m.rotation = Rotation.of_gguf(f, device)
-        m.left_out = Model.not_computed(f)
+        m.left_out = [name for name in Model.not_computed(f) if name not in taken]
         return m
 
     @staticmethod
@@ -582,13 +602,24 @@ class PagedDecodeStep:
 
     heads x head_dim is wo's row length; the cache is ``n_pages`` pages of ``page_size`` tokens a layer, of
     a type of ``KvCache``; the rotation is the model's unless one is given, ``rope_base`` and ``rope_factors`` in
-    place of its base and factors."""
+    place of its base and factors.  q and k heads are normed in layers whose norms have "q_norm" or "k_norm".
+
+    ``window``: every layer's attention sees that many last tokens and the first ``sinks`` (None: all).
+    ``shared_groups``: groups of sequences that share their first tokens, which are then read once a group: the caller
+    keeps ``groups`` [shared_groups + 1] (one group from the start) and ``shared`` [shared_groups] (0), tokens on
+    the pages of the group's first sequence, as ``fork`` leaves them; whole pages alone, since each sequence appends
+    to a last page of its own.  An emptied sequence belongs to a group of its own, or of no shared tokens.
+
+    Between steps, on the current stream: ``fork`` makes sequences copies of others, pages shared as far as they are full,
+    ``release`` empties sequences, ``compact`` brings the pages in use to the front (``taken[0]`` of them).  ``extra`` [n_pages]
+    counts the rows that hold a page beside the first."""
 
     def __init__(self, model: Model, m: int, heads: int, kv_heads: int, n_pages: int, max_pages: int,
                  page_size: int = 16, cache_type: int = F16, rope_base: float | None = None, rope_factors=None,
-                 device="cuda", rotation: Rotation | None = None):
+                 device="cuda", rotation: Rotation | None = None, window: int | None = None, sinks: int = 0,
+                 shared_groups: int = 0):
         import torch
-        from . import KvCache, Rope, attn_paged_ws, kv_page_bytes
+        from . import KvCache, QkNorm, Rope, attn_paged_ws, attn_shared_ws, attn_window_ws, kv_page_bytes
         l0 = model.layers[0]
         if any(k not in l0 for k in ("wo", "ffn_gateup")):
             raise ValueError("PagedDecodeStep needs a Model.fused_ops() model")
@@ -620,6 +651,17 @@ class PagedDecodeStep:
             raise ValueError(f"PagedDecodeStep needs output_norm, of {d} values, for the LM head")
         self.model, self.m, self.heads, self.kv_heads, self.page_size = model, m, heads, kv_heads, page_size
         self.head_dim = hd = width // heads
+        if window is not None and shared_groups:
+            raise ValueError("PagedDecodeStep: a window or shared groups, not both")
+        if (window is not None and window < 1) or sinks < 0 or (sinks and window is None) or not 0 <= shared_groups <= m:
+            raise ValueError("PagedDecodeStep: a window is at least one token, sinks stand beside a window, groups hold sequences")
+        self.window, self.sinks, self.shared_groups = window, sinks, shared_groups
+        self.qk_norms = []
+        for l in range(len(model.layers)):
+            pair = [model.norms[l].get(k) for k in ("q_norm", "k_norm")]
+            if any(w is not None and tuple(w.shape) != (hd,) for w in pair):
+                raise ValueError(f"PagedDecodeStep: norms of the q and k heads of layer {l} are of {hd} values")
+            self.qk_norms.append(QkNorm.of(*pair, model.eps) if any(w is not None for w in pair) else None)
         size = kv_page_bytes(cache_type, kv_heads, page_size, hd)
         if size == 0:
             raise ValueError("PagedDecodeStep: the cache does not take this type or head size")
@@ -642,12 +684,21 @@ class PagedDecodeStep:
         self.taken = torch.zeros(2, **i32)
         self.offsets, self.slots, self.pos = (torch.zeros(n, **i32) for n in (m + 1, m, m))
         self.rope = Rope.of(freq, pairing=turn.pairing, scale=turn.magnitude)
-        self.ws = torch.empty(attn_paged_ws(self.caches[0], heads, m, max_pages), dtype=torch.uint8, device=device)
+        if window is not None:
+            need = attn_window_ws(self.caches[0], F32, heads, m, m, max_pages, window, sinks)
+        elif shared_groups:
+            need = attn_shared_ws(self.caches[0], F32, heads, m, max_pages, shared_groups)
+        else:
+            need = attn_paged_ws(self.caches[0], heads, m, max_pages)
+        self.ws = torch.empty(need, dtype=torch.uint8, device=device)
+        self.extra = torch.zeros(n_pages, **i32)
+        self.groups = torch.tensor([0] + [m] * shared_groups, **i32)
+        self.shared = torch.zeros(max(shared_groups, 1), **i32)
         self.graph = None
 
     def run(self, stream: int) -> None:
         """The step on ``stream``, which is torch's current one (the residual adds are torch's)."""
-        from . import _check, attn_paged, kv_map, rope_kv
+        from . import _check, attn_paged, attn_shared, attn_window, kv_map, norm_rope_kv, rope_kv
         self._on_device()
         so, m, hd, model = lib(), self.m, self.head_dim, self.model
         d, q_row, width = self.x.shape[1], self.heads * self.head_dim, self.qk.shape[1]
@@ -664,11 +715,22 @@ class PagedDecodeStep:
         for l, layer in enumerate(model.layers):
             normed(qk, layer["wqk"], model.norms[l]["attn_norm"])
             normed(v, layer["wv"], model.norms[l]["attn_norm"])
-            _check(rope_kv(qk, width, qk, width, self.heads, qk + 4 * q_row, width, v, self.v.shape[1], m, hd, self.rope,
-                           self.pos.data_ptr(), m, self.caches[l], self.slots.data_ptr(), stream), "qvx_rope_kv")
-            _check(attn_paged(attn, q_row, qk, width, self.heads, self.caches[l], self.table.data_ptr(),
-                              self.table.shape[1], self.lens.data_ptr(), m, hd ** -0.5, self.ws.data_ptr(),
-                              self.ws.numel(), stream), "qvx_attn_paged")
+            kv = (qk + 4 * q_row, width, v, self.v.shape[1], m, hd)
+            at = (self.rope, self.pos.data_ptr(), m, self.caches[l], self.slots.data_ptr(), stream)
+            if self.qk_norms[l] is None:
+                _check(rope_kv(qk, width, qk, width, self.heads, *kv, *at), "qvx_rope_kv")
+            else:
+                _check(norm_rope_kv(qk, width, F32, qk, width, self.heads, *kv, self.qk_norms[l], *at), "qvx_norm_rope_kv")
+            pages = (self.table.data_ptr(), self.table.shape[1], self.lens.data_ptr(), m)
+            end = (hd ** -0.5, self.ws.data_ptr(), self.ws.numel(), stream)
+            if self.window is not None:
+                _check(attn_window(attn, q_row, qk, width, F32, self.heads, 0, m, self.caches[l], *pages, self.window, self.sinks,
+                                   *end), "qvx_attn_window")
+            elif self.shared_groups:
+                _check(attn_shared(attn, q_row, qk, width, F32, self.heads, self.caches[l], *pages, self.groups.data_ptr(),
+                                   self.shared.data_ptr(), self.shared_groups, *end), "qvx_attn_shared")
+            else:
+                _check(attn_paged(attn, q_row, qk, width, self.heads, self.caches[l], *pages, *end), "qvx_attn_paged")
             wmatmul_n(self.o, layer["wo"], self.attn, m, stream)
             self.x.add_(self.o)
             gu = layer["ffn_gateup"]
@@ -688,6 +750,51 @@ class PagedDecodeStep:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.run(torch.cuda.current_stream().cuda_stream)
+
+    def _rows(self, rows, what: str):
+        """Sequence numbers as a device vector; a list is checked here, a tensor on the device."""
+        import torch
+        if not isinstance(rows, torch.Tensor):
+            rows = list(rows)
+            if any(not 0 <= r < self.m for r in rows):
+                raise ValueError(f"PagedDecodeStep: {what} are sequences 0 to {self.m - 1}")
+            rows = torch.tensor(rows, dtype=torch.int32, device=self.x.device)
+        return rows
+
+    def release(self, rows) -> None:
+        """Empties the sequences ``rows``: their pages go back, but those that others hold, and their lengths are 0."""
+        from . import kv_free_t
+        self._on_device()
+        rows = self._rows(rows, "rows")
+        if rows.shape[0]:
+            kv_free_t(rows, self.table, self.lens, self.extra, self.free, self.taken)
+
+    def fork(self, source, to) -> None:
+        """Makes each sequence of ``to``, emptied first, a copy of the one beside it in ``source``: the full pages shared,
+        the last one copied in every layer.  The sequences of ``to`` are distinct and none of them is a source.
+        ``taken[1]`` says whether there were pages for all (then every fork is done; else none, the sequences of ``to``
+        staying empty)."""
+        from . import kv_copy_t, kv_fork_t
+        self._on_device()
+        if not hasattr(source, "data_ptr") and not hasattr(to, "data_ptr"):
+            source, to = list(source), list(to)
+            if len(set(to)) < len(to) or set(to) & set(source) or len(source) != len(to):
+                raise ValueError("PagedDecodeStep.fork: a source for each of the distinct targets, none of them a target")
+        source, to = self._rows(source, "sources"), self._rows(to, "targets")
+        if source.shape != to.shape:
+            raise ValueError("PagedDecodeStep.fork: a source for each target")
+        if to.shape[0] == 0:
+            return
+        self.release(to)
+        pairs, count = kv_fork_t(source, to, self.table, self.page_size, self.lens, self.extra, self.free, self.taken)
+        kv_copy_t(self.caches, pairs, count)
+
+    def compact(self) -> None:
+        """Brings the pages in use to the front, in every layer."""
+        from . import kv_compact_t, kv_copy_t
+        self._on_device()
+        pairs, moved = kv_compact_t(self.table, self.extra, self.free, self.taken)
+        kv_copy_t(self.caches, pairs, moved[:1])
 
     def _on_device(self) -> None:
         """The launches go to the current device, which has to be the buffers'."""
