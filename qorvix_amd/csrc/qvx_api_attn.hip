@@ -40,7 +40,7 @@ int64_t tiles_of(const AttnCall& c, int len) {
   return (int64_t)len / c.page_size * c.page_tiles + (len % c.page_size + kAttnTile - 1) / kAttnTile;
 }
 int64_t most_tiles(const AttnCall& c) {
-  const int64_t all = tiles_of(c, c.max_len);
+  const int64_t all = tiles_of(c, c.max_len) + (c.mode == kMaskWhole);  // where the shared keys end, a tile for both parts
   if (c.mode != kMaskWindow || c.window >= c.max_len) return all;
   const int64_t near = (int64_t)c.window + attn_span(c.tile_rows, c.group) - 1;
   return std::min<int64_t>(all, tiles_of(c, std::min(c.sinks, c.max_len)) +
@@ -176,10 +176,22 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
   return (many ? plan16 : plan_split)(c, row_tiles, join, ws_bytes) ? QVX_OK : QVX_E_RANGE;
 }
 
+// Whether sequences read shared keys each for itself, in one launch (kMaskWhole): reading them once costs another launch and
+// partial results of the prefix, which is worth it where the tables hold more than 128 MB of keys and values in all, or 256 MB in
+// rows of up to 1024 tokens; and every workgroup looks for its group, which in several groups of more sequences than a wave's
+// lanes eats up what it saves.  Once against each for itself, 8 heads of 128 in fp16, 4 queries each: 5 sequences of 740
+// tokens 18.2 and 12.7 us, 8 of 3100 23.0 and 20.9, 32 of 1600 25.0 and 28.2, of 3100 27.3 and 42.5; 64 of 306 24.7 and 12.4, of
+// 740 27.3 and 20.5, of 1600 30.8 and 38.2; 200 of 306 in one group 56.7 and 49.1, in fifty 58.1 and 62.3.
+bool read_whole(const AttnCall& c, int n_groups) {
+  const int64_t bytes = (int64_t)c.n_seqs * c.max_len * 2 * c.key_bytes * c.kv_heads;
+  return bytes <= (c.max_len <= 1024 ? 256ll : 128ll) << 20 && (c.n_seqs <= 64 || n_groups == 1);
+}
+
 // The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query and its
 // counters, its partial results, and the rest's.
 struct SharedPlan {
   AttnCall prefix{}, rest{};
+  bool whole = false;  // `rest` alone, each sequence reading the shared keys for itself
   bool join = false;  // the rest may be split
   size_t arrived_at = 0, lead_bytes = 0, prefix_bytes = 0, bytes = 0;
 };
@@ -191,6 +203,16 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   if (n_groups <= 0) return QVX_E_SHAPE;
   if (n_groups > n_seqs || (int64_t)n_seqs * p.rest.group > 0x7fffff00ll) return QVX_E_RANGE;
   p.rest.q_type = q_type;
+  if (read_whole(p.rest, n_groups)) {
+    p.whole = true;
+    p.rest.mode = kMaskWhole;
+    p.rest.n_groups = n_groups;
+    p.rest.tile_rows = tile_rows(p.rest.group);
+    const int64_t row_tiles = (int64_t)n_seqs * ((p.rest.group + p.rest.tile_rows - 1) / p.rest.tile_rows);
+    if (!plan_split(p.rest, row_tiles, &p.join, &p.bytes)) return QVX_E_RANGE;
+    p.bytes = std::max<size_t>(p.bytes, 16);
+    return QVX_OK;
+  }
   AttnCall& c = p.prefix;
   c = p.rest;
   c.mode = kMaskPrefix;
@@ -528,12 +550,16 @@ int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
     c->arrived = reinterpret_cast<int*>(ws + p.arrived_at);
     c->q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
   }
-  p.prefix.groups = d_groups;
-  p.prefix.shared = d_shared;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  p.prefix.groups = p.rest.groups = d_groups;
+  p.prefix.shared = p.rest.shared = d_shared;
+  if (p.whole) {
+    p.rest.ws = p.join ? static_cast<float*>(d_ws) : nullptr;
+    return attn_status(launch_attn_mask(p.rest, cache->type, p.join, s));
+  }
   p.prefix.ws = reinterpret_cast<float*>(ws + p.lead_bytes);
   p.rest.lead_ws = p.prefix.ws;
   p.rest.ws = p.join ? reinterpret_cast<float*>(ws + p.lead_bytes + p.prefix_bytes) : nullptr;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   if (!launch_attn_mask(p.prefix, cache->type, false, s)) return attn_status(false);
   return attn_status(launch_attn_mask(p.rest, cache->type, false, s));  // the rest's chunks join themselves
 }

@@ -20,6 +20,10 @@ bool launch_attn_rest_f16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_rest_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_rest_f32(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_rest_q8(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_whole_f16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_whole_bf16(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_whole_f32(const AttnCall& c, dim3 grid, hipStream_t s);
+bool launch_attn_whole_q8(const AttnCall& c, dim3 grid, hipStream_t s);
 bool launch_attn_rows_f16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
 bool launch_attn_rows_bf16(const AttnCall& c, bool parts, dim3 grid, hipStream_t s);
 
@@ -144,8 +148,11 @@ bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s
     if (ok && join) launch_attn_join(c, s);
     return ok;
   }
-  const bool rest = c.mode == kMaskRest, prefix = c.mode == kMaskPrefix;
-#define QVX_MODE(f) (prefix ? launch_attn_prefix_##f : rest ? launch_attn_rest_##f : launch_attn_window_##f)(c, grid, s)
+#define QVX_MODE(f)                                       \
+  (c.mode == kMaskPrefix  ? launch_attn_prefix_##f        \
+   : c.mode == kMaskRest  ? launch_attn_rest_##f          \
+   : c.mode == kMaskWhole ? launch_attn_whole_##f         \
+                          : launch_attn_window_##f)(c, grid, s)
   switch (type) {
     case T_F16: ok = QVX_MODE(f16); break;
     case T_BF16: ok = QVX_MODE(bf16); break;

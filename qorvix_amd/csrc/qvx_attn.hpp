@@ -51,18 +51,20 @@ struct AttnCall {
   float* ws;        // partial results of split sequences
 
   // Of masked calls alone.  Window: the queries of a sequence are its last tokens, and the one at position p sees the keys
-  // j <= p that are later than p - window or before `sinks`.  Prefix and rest: qvx_attn_shared's two parts.
+  // j <= p that are later than p - window or before `sinks`.  Prefix and rest: qvx_attn_shared's two parts; whole: all of it at
+  // once, each sequence reading the shared keys for itself.
   int mode;
   int window, sinks;
   int table_page;  // many rows: tokens of a page, page_size then standing for the longest sequence
   const int32_t *groups, *shared;  // prefix: "sequence" g is the group of queries groups[g] .. and its first shared[g] keys
+  int n_groups;                    // whole
   struct AttnLead* leads;          // [queries]: what the prefix leaves the rest
   const float* lead_ws;            // rest: the prefix's workspace
   int lead_rows, lead_slots;       // its tile_rows and slots
   int* arrived;                    // [queries][rest_tiles][kv_heads]: chunks of the rest that are done, zeroed by the prefix
   int rest_tiles;                  // row tiles of a query in the rest
 };
-enum { kNoMask, kMaskWindow, kMaskPrefix, kMaskRest };
+enum { kNoMask, kMaskWindow, kMaskPrefix, kMaskRest, kMaskWhole };
 
 // Of a query behind a shared prefix: how many of the prefix's keys it sees, its first row in its group, and where the partial
 // results of that group lie.
@@ -99,10 +101,12 @@ struct AttnItem {
   int seq, len, q0, rows, row0;  // q0: the sequence's first query; rows: of the whole sequence
   int chunk, chunks, tile0, tile1;
   int slot;  // its place in the workspace, if chunks > 1
+  int lead, start;  // whole: the sequence that holds its first `start` keys
 };
 
 struct AttnSeq {
   int len, q0, nq, row_tiles, tiles;
+  int lead, start;  // whole
 };
 
 // The tile that key `at` lies in.
@@ -121,7 +125,7 @@ __host__ __device__ inline int attn_span(int rows, int group) { return (rows + g
 
 // A masked call's sequences.
 template <int R, int M> __device__ inline AttnSeq attn_masked_seq(const AttnCall& c, int b) {
-  AttnSeq s{0, 0, 0, 0, 0};
+  AttnSeq s{};
   if constexpr (M == kMaskPrefix) {
     s.q0 = b && c.groups ? min(max(c.groups[b], 0), c.n_q) : 0;
     s.nq = max((b + 1 < c.n_seqs && c.groups ? min(max(c.groups[b + 1], 0), c.n_q) : c.n_q) - s.q0, 0);
@@ -129,7 +133,19 @@ template <int R, int M> __device__ inline AttnSeq attn_masked_seq(const AttnCall
     s.tiles = attn_tiles(c, s.len);
   } else {
     s.len = min(max(c.lens[b], 0), c.max_len);
-    if constexpr (M == kMaskRest) {
+    if constexpr (M == kMaskWhole) {
+      s.q0 = b;
+      s.nq = 1;
+      int g = 0, end = c.groups ? c.n_groups : 1;  // the last group that begins at b or before
+      while (end - g > 1) {
+        const int mid = (g + end) / 2;
+        if (c.groups[mid] <= b) g = mid; else end = mid;
+      }
+      s.lead = g ? min(max(c.groups[g], 0), c.n_seqs - 1) : 0;
+      s.start = min(max(c.shared[g], 0), s.len);
+      // the tile in which the shared keys end stands for both parts
+      s.tiles = attn_tiles(c, s.start) + (s.len > s.start ? attn_tiles(c, s.len) - attn_tile_of(c, s.start) : 0);
+    } else if constexpr (M == kMaskRest) {
       s.q0 = b;
       s.nq = 1;
       const int start = min(max(c.leads[b].start, 0), s.len);
@@ -152,7 +168,7 @@ template <int R, int M> __device__ inline AttnSeq attn_masked_seq(const AttnCall
 
 // R: query rows of a row tile, M: the call's mode, here and below.
 template <int R, int M> __device__ inline AttnSeq attn_seq(const AttnCall& c, int b) {
-  AttnSeq s{0, 0, 0, 0, 0};
+  AttnSeq s{};
   if (b >= c.n_seqs) return s;
   if constexpr (M != kNoMask) return attn_masked_seq<R, M>(c, b);
   int len = c.lens ? c.lens[b] : c.max_len;
@@ -213,6 +229,8 @@ __device__ inline AttnItem attn_take(const AttnCall& c, const AttnSeq& s, int b,
   it.tile0 = it.chunk * chunk;
   it.tile1 = min(it.tile0 + chunk, s.tiles);
   it.slot = slot0 + rt * it.chunks + it.chunk;
+  it.lead = s.lead;
+  it.start = s.start;
   // Offsets that are no running sums can wrap the counts: nothing past the rows or the workspace then.
   it.any = i >= 0 && it.row0 >= 0 && it.row0 < it.rows && it.tile0 >= 0 &&
            ((it.chunks == 1 && !attn_parts_always<M>()) || (unsigned)it.slot < (unsigned)c.slots);
@@ -286,6 +304,8 @@ template <int R, int M> __device__ inline AttnItem attn_item(const AttnCall& c, 
     t.q0 = __builtin_amdgcn_readlane(s.q0, b);
     t.nq = __builtin_amdgcn_readlane(s.nq, b) * c.group;
     t.tiles = __builtin_amdgcn_readlane(s.tiles, b);
+    t.lead = M == kMaskWhole ? __builtin_amdgcn_readlane(s.lead, b) : 0;
+    t.start = M == kMaskWhole ? __builtin_amdgcn_readlane(s.start, b) : 0;
     return attn_take<R, M>(c, t, b, chunk, i - __builtin_amdgcn_readlane(run - mine, b), kind == 0,
                         __builtin_amdgcn_readlane(slots - n.slots, b));
   }
@@ -377,7 +397,13 @@ struct AttnView {
 };
 template <int R, int M> __device__ inline AttnView attn_view(const AttnCall& c, const AttnItem& it) {
   AttnView v{0, 0, 0, 0, 0, it.len, 0};
-  if constexpr (M == kMaskRest) {
+  if constexpr (M == kMaskWhole) {  // tiles of the shared keys, then the sequence's own
+    v.low = it.start;
+    v.first = attn_tile_of(c, it.start);
+    v.sinks = attn_tiles(c, it.start);
+    v.end = it.len > it.start ? attn_tiles(c, it.len) : v.first;
+    return v;
+  } else if constexpr (M == kMaskRest) {
     v.low = min(max(c.leads[it.seq].start, 0), it.len);
     v.first = attn_tile_of(c, v.low);
   } else if constexpr (M == kMaskWindow) {
@@ -403,7 +429,7 @@ __device__ inline AttnRange attn_range(const AttnCall& c, const AttnItem& it, co
   if (row >= it.rows) return {0, 0, 0};
   const int query = row / c.group;
   if constexpr (M == kMaskPrefix) return {0, min(max(c.lens[it.q0 + query], 0), it.len), 0};
-  if constexpr (M == kMaskRest) return {v.low, it.len, 0};
+  if constexpr (M == kMaskRest || M == kMaskWhole) return {v.low, it.len, 0};
   const int p = v.p0 + query;
   return {(int)max((long long)p + 1 - c.window, 0ll), max(p + 1, 0), c.sinks};
 }

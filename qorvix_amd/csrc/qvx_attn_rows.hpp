@@ -287,21 +287,9 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   static_assert(kTiles - NB > kTiles / 2);  // a block is in place a tile before its first one is asked for
   // Copies a wave has on its way at least for each tile behind the next one: the next one has landed when no more are.
   constexpr int kBehind = (NB - 2) * 2 * (KT * L::kUnits / 256);
-  if (tiles > 0) {
-    look(0);
-    place(0);
-    if (tiles > kTiles) look(1);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < NB - 1; ++t)
-    if (t < tiles) {
-      ask(t);
-      fetch(t);
-    }
-  // The queries, while the first tiles are on their way.
+  // The queries are asked for before anything that waits for the table, and made ready while the first tiles are on their way.
   u32x4 q[QP][KS];
-  float mul = c.scale2;  // of a product to a logit in powers of two
+  float x[PARTS ? KS : 1][8];
   if constexpr (!PARTS) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -321,8 +309,22 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
     int64_t from[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) from[s] = qat + (16 * s + 8 * h < d ? 16 * s + 8 * h : 0);
-    float x[KS][8];
     attn_load8(x, c.q, from, c.q_type);
+  }
+  if (tiles > 0) {
+    look(0);
+    place(0);
+    if (tiles > kTiles) look(1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NB - 1; ++t)
+    if (t < tiles) {
+      ask(t);
+      fetch(t);
+    }
+  float mul = c.scale2;  // of a product to a logit in powers of two
+  if constexpr (PARTS) {
     float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)

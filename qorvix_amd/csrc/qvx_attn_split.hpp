@@ -271,7 +271,7 @@ template <uint32_t T, int DT, bool FULL, int NS> struct AttnTile {
   // [key r][two blocks' scales a word]; kGroup: [key r][this lane's block of round u]
   uint32_t kstep[kQ8 ? 4 : 1][kGroup ? U : kQ8 ? (KS + 1) / 2 : 1];
   uint16_t vstep[kQ8 ? 4 : 1];
-  int live, key0;
+  int live, key0, low;
 };
 
 __device__ __forceinline__ float attn_half(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   AttnItem it = attn_item<R, M>(c, item, reinterpret_cast<int*>(lds), sums);
   AttnView view{};
   if constexpr (MASK) {
-    if (M == kMaskWindow) attn_note(c, it, item, kvh, sums);  // what k_attn_join needs
+    if (M == kMaskWindow || M == kMaskWhole) attn_note(c, it, item, kvh, sums);  // what k_attn_join needs
     if (!it.any) return;
     if (M == kMaskPrefix) attn_leads<R>(c, it, kvh);
     view = attn_view<R, M>(c, it);
@@ -368,15 +368,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   const int spitch = kQ8 ? d / 16 : 0;  // bytes of a token's scales
   int64_t at = 0, sat = 0;  // of the tile's keys (and values), and of their scales, from the cache's start
   int live = 0, seen = 0;  // seen: keys that count
-  int key0 = 0;            // masked: the tile's first key
+  int key0 = 0, low = 0;   // masked: the tile's first key; whole: the first that counts
   auto look_up = [&](int n) __attribute__((always_inline)) {
     int t = it.tile0 + wave + (n + lane) * kAttnWaves;
     live = 0;
     if (t < it.tile1) {
+      const bool lead = M == kMaskWhole && t < view.sinks;  // a tile of the shared keys
       if constexpr (MASK) t = view.tile(t);
       const int p = t / c.page_tiles, tok = (t - p * c.page_tiles) * kAttnTile;
-      int page = c.table ? c.table[(int64_t)it.seq * c.table_width + p] : it.seq;
-      live = min(min(kAttnTile, c.page_size - tok), (MASK ? view.high : it.len) - p * c.page_size - tok);
+      int page = c.table ? c.table[(int64_t)(lead ? it.lead : it.seq) * c.table_width + p] : it.seq;
+      live = min(min(kAttnTile, c.page_size - tok), (lead ? it.start : MASK ? view.high : it.len) - p * c.page_size - tok);
+      low = lead ? 0 : view.low;
       key0 = p * c.page_size + tok;
       if (page < 0 || page >= c.n_pages) page = 0, live = 0;  // no such page: its keys do not count
       at = page * c.page_stride + kvh * c.head_stride + (int64_t)tok * c.pitch;
@@ -413,8 +415,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
     x.live = n < tiles ? __builtin_amdgcn_readlane(live, n & 63) : 0;
     seen |= x.live;
     if constexpr (MASK) x.key0 = __builtin_amdgcn_readlane(key0, n & 63);
+    if constexpr (M == kMaskWhole) x.low = __builtin_amdgcn_readlane(low, n & 63);
     // Masked: keys that no row sees are not read, as if past the end: what is there does not reach the sums.
     auto hide = [&](int key, uint32_t off) __attribute__((always_inline)) {
+      if constexpr (M == kMaskWhole) return x.key0 + key < x.low ? kPastEnd : off;
       if constexpr (MASK) return x.key0 + key < view.low && x.key0 + key >= view.sink_keys ? kPastEnd : off;
       return off;
     };
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
         p[t] = t == 0 ? attn_gather<0>(sc) : attn_gather<1>(sc);
         bool none = lane >> 2 >= x.live;
         if constexpr (MASK) {
-          none = none || !range[t].sees(x.key0 + (lane >> 2));
+          none = none || (M == kMaskWhole ? x.key0 + (lane >> 2) < x.low : !range[t].sees(x.key0 + (lane >> 2)));
           saw[t] |= !none;
         }
         if (none) p[t] = -INFINITY;
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int r = 0; r < 4; ++r) {
         bool none = 4 * g + r >= x.live;
         if constexpr (MASK) {
-          none = none || !range[0].sees(x.key0 + 4 * g + r);
+          none = none || (M == kMaskWhole ? x.key0 + 4 * g + r < x.low : !range[0].sees(x.key0 + 4 * g + r));
           saw[0] |= !none;
         }
         sc[r] = none ? -INFINITY : sc[r];

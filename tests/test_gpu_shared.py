@@ -13,6 +13,14 @@ from test_gpu_window import HALF, attend
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=["narrow", "wide"])
+def wide(request):
+    """Short tables of few sequences run as one launch, in which each reads the shared keys for itself: the second time round
+    tables are so wide that the sequences could pass that."""
+    global WIDE
+    WIDE = request.param == "wide"
+
+
 def share(torch, c, groups, shared):
     """Every sequence of a group is given its first one's pages for the shared tokens; a page that ends behind them stays
     its own, and holds other values for them, which must not count."""
@@ -21,6 +29,10 @@ def share(torch, c, groups, shared):
         for b in range(groups[g], groups[g + 1]):
             full = min(shared[g], c.lens[b]) // c.page
             c.table[b, :full] = c.table[lead, :full]
+    if WIDE:
+        token = qvx.kv_page_bytes(c.t, c.hk, c.page, c.d) * 2 // c.page * len(c.lens)
+        more = (257 << 20) // token // c.page
+        c.table = np.concatenate([c.table, np.full((len(c.lens), more), -1, c.table.dtype)], 1)
     c.dev_table = torch.from_numpy(c.table).cuda()
 
 
