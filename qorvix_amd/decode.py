@@ -611,7 +611,7 @@ class PagedDecodeStep:
     to a last page of its own.  An emptied sequence belongs to a group of its own, or of no shared tokens.
 
     Between steps, on the current stream: ``fork`` makes sequences copies of others, pages shared as far as they are full,
-    ``release`` empties sequences, ``compact`` brings the pages in use to the front (``taken[0]`` of them).  ``extra`` [n_pages]
+    ``release`` empties sequences, ``trim`` gives back what is behind their windows, ``compact`` brings the pages in use to the front (``taken[0]`` of them).  ``extra`` [n_pages]
     counts the rows that hold a page beside the first."""
 
     def __init__(self, model: Model, m: int, heads: int, kv_heads: int, n_pages: int, max_pages: int,
@@ -788,6 +788,18 @@ class PagedDecodeStep:
         self.release(to)
         pairs, count = kv_fork_t(source, to, self.table, self.page_size, self.lens, self.extra, self.free, self.taken)
         kv_copy_t(self.caches, pairs, count)
+
+    def trim(self) -> None:
+        """Gives the pages back that no later token sees: those whole between the first tokens and the window."""
+        import torch
+        from . import kv_free_t
+        self._on_device()
+        if self.window is None:
+            return
+        rows = torch.arange(self.m, dtype=torch.int32, device=self.x.device)
+        end = (self.lens + 1 - self.window).clamp_(min=0) // self.page_size
+        begin = torch.full_like(end, -(-self.sinks // self.page_size))
+        kv_free_t(rows, self.table, self.lens, self.extra, self.free, self.taken, begin, end)
 
     def compact(self) -> None:
         """Brings the pages in use to the front, in every layer."""

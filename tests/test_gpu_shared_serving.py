@@ -113,6 +113,21 @@ def test_a_window(cuda, window, sinks):
     _both(torch, step, host, 6, replay=True)
 
 
+@pytest.mark.parametrize("window,sinks,page", [(1, 0, 1), (5, 0, 3), (6, 4, 3), (4, 3, 2), (64, 0, 4)])
+def test_pages_behind_a_window_go_back(cuda, window, sinks, page):
+    torch = cuda
+    torch.manual_seed(5)
+    step = decode.PagedDecodeStep(_model(torch, layers=1), 2, heads=8, kv_heads=2, n_pages=2 * (-(-sinks // page) + -(-window // page) + 3),
+                                  max_pages=30, page_size=page, window=window, sinks=sinks)
+    host = HostShared(torch, step, torch.float16, window, sinks)
+    for _ in range(6):
+        _both(torch, step, host, page + 1)
+        step.trim()
+        n = host.t[0]
+        kept = [j for j in range(-(-n // page)) if (j + 1) * page > n - window + 1 or j * page < sinks]
+        assert [j for j in range(30) if int(step.table[0, j]) >= 0] == kept and step.taken.tolist() == [2 * len(kept), 0]
+
+
 @pytest.mark.parametrize("groups", [0, 1, 2])
 def test_forks_between_steps(cuda, groups):
     """Sequences that become copies of others, and go on on their own, in every layer; pages that move in between."""
