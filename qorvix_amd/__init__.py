@@ -730,7 +730,7 @@ def norm_rope_kv_t(q, k, v, pos, norm: QkNorm, rope: Rope, cache: KvCache | None
     n, heads, d = q.shape
     _beside(rope, q.device, "rope")
     _beside(norm, q.device, "norm")
-    for w, h in zip(norm.tensors, (heads, cache.kv_heads if cache is not None else None)):
+    for w, h in zip(getattr(norm, "tensors", ()), (heads, cache.kv_heads if cache is not None else None)):
         if w is not None and (w.shape[-1] != d or (w.dim() == 2 and h is not None and w.shape[0] != h)):
             raise ValueError(f"norm_rope_kv_t: weights of {d} values a head")
     if cache is not None:

@@ -148,6 +148,7 @@ bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 // 45.3 and 40.6; 1000 keys 64 20.1 and 26.2, 256 34.2 and 32.3; fp16 queries 4000 keys 32 25.2 and 22.8, 64 27.1 and 24.1.
 bool many_rows(const qvx_kv_cache* cache, int64_t rows, AttnCall& c) {
   if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 48) return false;
+  if (c.max_len > 0x7ffff000) return false;  // it looks up to 1024 keys past the last one by number
   c.table_page = c.page_size;
   c.page_size = c.max_len;
   c.page_tiles = (int)(((int64_t)c.max_len + kAttnTile - 1) / kAttnTile);

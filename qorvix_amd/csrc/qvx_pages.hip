@@ -95,8 +95,10 @@ struct PageRun {
 };
 
 __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
-  extern __shared__ int32_t rank[];  // [n] fresh pages of the forks before
   __shared__ int part[kThreads / 64], all_bad;
+  __shared__ int from[kTogether], to[kTogether], lens[kTogether], fresh[kTogether];
+  __shared__ int place[kTogether];  // of this workgroup's forks: fresh pages of those before
+  const int own = (int)blockIdx.x * kTogether, n = min(kTogether, c.n - own);
   const int tid = threadIdx.x, taken = c.taken_in[0];
   if (tid == 0) all_bad = taken < 0 ? QVX_MAP_NEGATIVE : 0;
   int bad = 0, all = 0;
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
     const int wants = i < c.n ? fork_wants(c, i, bad) : 0;
     int total;
     const int before = block_before<kThreads>(wants, part, total);
-    if (i < c.n) rank[i] = all + before;
+    if (i >= own && i < own + n) place[i - own] = all + before;
     all += total;
   }
   if (bad) atomicOr(&all_bad, bad);
@@ -120,12 +122,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
   }
   if (!(write & kForkRows) || status) return;
   // What the workgroup's forks are is read before anything is stored: the compiler has to assume that a store changes it.
-  __shared__ int from[kTogether], to[kTogether], lens[kTogether], fresh[kTogether], place[kTogether];
-  const int i0 = (int)blockIdx.x * kTogether, n = min(kTogether, c.n - i0);
-  if (tid < kTogether) {
-    const int i = i0 + min(tid, n - 1);
-    from[tid] = c.from[i], to[tid] = c.to[i], lens[tid] = tid < n ? c.lens[c.from[i]] : 0, place[tid] = rank[i];
-    fresh[tid] = taken + rank[i] < c.n_free ? c.free_list[taken + rank[i]] : -1;  // lengths that another fork changes: no place
+  if (tid < n) {
+    from[tid] = c.from[own + tid], to[tid] = c.to[own + tid], lens[tid] = c.lens[from[tid]];
+    const int at = taken + place[tid];
+    fresh[tid] = at < c.n_free ? c.free_list[at] : -1;  // lengths that another fork changes: no place
+  } else if (tid < kTogether) {
+    from[tid] = c.from[own], lens[tid] = 0;  // read like the others, not used
   }
   __syncthreads();
   for (int col = (int)blockIdx.y * kThreads + tid; col < c.table_width; col += (int)gridDim.y * kThreads) {
@@ -394,11 +396,10 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c, int parts) {
 }  // namespace
 
 void launch_kv_fork(const ForkCall& c, bool alias, hipStream_t s) {
-  const size_t lds = (size_t)c.n * sizeof(int32_t);  // at most 64 KB
   // Totals that lie on what the others read are stored by a launch behind them.
   const int groups = (c.n + kTogether - 1) / kTogether, cols = std::min((c.table_width + kThreads - 1) / kThreads, 64);
-  k_kv_fork<<<dim3(groups, cols), kThreads, lds, s>>>(c, alias ? kForkRows : kForkRows | kForkTotals);
-  if (alias) k_kv_fork<<<1, kThreads, lds, s>>>(c, kForkTotals);
+  k_kv_fork<<<dim3(groups, cols), kThreads, 0, s>>>(c, alias ? kForkRows : kForkRows | kForkTotals);
+  if (alias) k_kv_fork<<<1, kThreads, 0, s>>>(c, kForkTotals);
 }
 
 void launch_kv_free(const FreeCall& c, hipStream_t s) {
