@@ -179,13 +179,13 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
 
 // Whether sequences read shared keys each for itself, in one launch (kMaskWhole): reading them once costs another launch and
 // partial results of the prefix, which is worth it where the tables hold more than 128 MB of keys and values in all, or 256 MB in
-// rows of up to 1024 tokens; and every workgroup looks for its group, which in several groups of more sequences than a wave's
-// lanes eats up what it saves.  Once against each for itself, 8 heads of 128 in fp16, 4 queries each: 5 sequences of 740
-// tokens 18.2 and 12.7 us, 8 of 3100 23.0 and 20.9, 32 of 1600 25.0 and 28.2, of 3100 27.3 and 42.5; 64 of 306 24.7 and 12.4, of
-// 740 27.3 and 20.5, of 1600 30.8 and 38.2; 200 of 306 in one group 56.7 and 49.1, in fifty 58.1 and 62.3.
+// rows of up to 1024 tokens.  Past 256 sequences a thread looks for several groups, again and again.  Once against each for
+// itself, 8 heads of 128 in fp16, 4 queries each: 4 sequences of 1000 tokens 19.0 and 12.8 us, 16 of 1600 21.9 and 20.9, of 3100 24.0
+// and 28.0, 32 of 1600 24.9 and 27.6, 64 of 306 24.8 and 12.2, of 1000 29.8 and 24.8, of 1600 30.9 and 36.9, 100 of 1000 41.1 and
+// 48.1, 200 of 306 54.3 and 43.8, in fifty groups 55.0 and 47.9.
 bool read_whole(const AttnCall& c, int n_groups) {
   const int64_t bytes = (int64_t)c.n_seqs * c.max_len * 2 * c.key_bytes * c.kv_heads;
-  return bytes <= (c.max_len <= 1024 ? 256ll : 128ll) << 20 && (c.n_seqs <= 64 || n_groups == 1);
+  return bytes <= (c.max_len <= 1024 ? 256ll : 128ll) << 20 && (c.n_seqs <= 256 || n_groups == 1);
 }
 
 // The two parts of qvx_attn_shared, and where they lie in its workspace: what the prefix leaves for each query and its
@@ -211,6 +211,7 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
     p.rest.tile_rows = tile_rows(p.rest.group);
     const int64_t row_tiles = (int64_t)n_seqs * ((p.rest.group + p.rest.tile_rows - 1) / p.rest.tile_rows);
     if (!plan_split(p.rest, row_tiles, &p.join, &p.bytes)) return QVX_E_RANGE;
+    p.rest.read_once = false;  // a group's sequences read the same keys
     p.bytes = std::max<size_t>(p.bytes, 16);
     return QVX_OK;
   }

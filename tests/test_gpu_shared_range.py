@@ -7,7 +7,7 @@ import pytest
 
 import qorvix_amd as qvx
 from test_gpu_attention import U, Cache
-from test_gpu_window import attend, check
+from test_gpu_window import HALF, attend, check
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,27 @@ def test_two_graphs_at_once_on_streams_of_their_own(cuda, wide):
             got = [x.clone() for x in outs]
             run()
             assert all(torch.equal(a, b) for a, b in zip(got, outs))
+
+
+@pytest.mark.parametrize("t,q_type", [(qvx.F16, qvx.F16), (qvx.BF16, qvx.F32), (qvx.Q8_0, qvx.F32)])
+@pytest.mark.parametrize("hq,hk", [(150, 1), (260, 2)])
+def test_groups_of_more_heads_than_a_row_tile(cuda, t, q_type, hq, hk):
+    """A query's rows in several row tiles, alone and behind a shared prefix, which the second width reads apart."""
+    torch = cuda
+    check(cuda, Cache(cuda, t, (70, 333, 20, 1), 16, hk, 32, seed=hq), hq, [1, 7, 3, 1], 50, 3, q_type)
+    lens = (300, 291, 400, 290)
+    c = Cache(cuda, t, lens, 16, hk, 32, seed=hq + 1)
+    c.table[:, :18] = c.table[0, :18]
+    q = torch.randn((4, hq, 32), device="cuda").to({qvx.F32: torch.float32, qvx.F16: torch.float16}[q_type])
+    for more in (0, 1 << 17):
+        table = torch.cat([torch.from_numpy(c.table).cuda(), torch.full((4, more), -1, dtype=torch.int32, device="cuda")], 1)
+        got = qvx.attn_shared_t(q, c.desc, table, c.dev_lens, _ints(torch, [288])).double().cpu().numpy()
+        for b, n in enumerate(lens):
+            k, v = (np.concatenate([c.rows(0, i)[:, :288], c.rows(b, i)[:, 288:]], 1) for i in range(2))
+            for h in range(hq):
+                g = h // (hq // hk)
+                want, most = attend(q[b, h: h + 1].double().cpu().numpy(), k[g], v[g], np.ones((1, n), bool), 32 ** -0.5)
+                bar = 2 * U * ((32 + 3) * most + n + 10) * np.abs(v).max() + HALF[q_type] * np.abs(want)
+                # rounded weights, of more than 48 rows a group: half a step of each, or what two bf16 parts leave
+                bar = bar + (HALF[q_type] if q_type == t else 2.0 ** -18 if t == qvx.BF16 else 0.0) * np.abs(v).max()
+                assert (np.abs(got[b, h] - want[0]) <= bar).all()
