@@ -6,10 +6,10 @@
 // free list.  All results are whole numbers and the same in every run: counts meet in integer atomics, whose order does
 // not matter, and pages return in the order of their ids, not of their release.
 //
-// Bound by latency but for the copies, which the bytes bound.  Measured: 128 forks of 256 shared pages 9.3 us, the copy of their
-// last pages in 16 layers 54 (269 MB read and written, 4.9 TB/s; a large copy reaches 4.85), their release 6.5 + 4.8; the compaction of
-// 4500 pages 9 us, its copy in 8 layers 229 (1.13 GB, 4.9 TB/s); 8 forks, copies and releases 6.3, 8.2 and 10.2, chains of
-// dependent loads and atomics.
+// Bound by latency but for the copies, which the bytes bound.  Measured: 128 forks of 256 shared pages 8.4 us, the copy of their
+// last pages in 16 layers 45 (269 MB read and written, 6 TB/s, part of it in the caches; a large copy reaches 4.85), their release
+// 5.8 + 4.7; the compaction of 4500 pages 9 us, its copy in 8 layers 230 (1.13 GB, 4.9 TB/s); 8 forks, copies and releases 6.3, 3.8
+// and 5.8, chains of dependent loads and atomics.
 #include "qvx_pages.hpp"
 
 namespace qvx {
@@ -64,14 +64,13 @@ template <int THREADS> __device__ __forceinline__ int block_before(int x, int* p
 
 constexpr int kTogether = 16;
 
-// What fork i wants: 1 where its sequence's last page is not full; `bad` gets status bits.
-__device__ __forceinline__ int fork_wants(const ForkCall& c, int i, int& bad) {
-  const int from = c.from[i], to = c.to[i];
+// What a fork wants: 1 where its sequence's last page is not full; `bad` gets status bits, `len` the sequence's length.
+__device__ __forceinline__ int fork_wants(const ForkCall& c, int from, int to, int& len, int& bad) {
   if ((unsigned)from >= (unsigned)c.n_rows || (unsigned)to >= (unsigned)c.n_rows || from == to) {
     bad |= QVX_MAP_SEQUENCE;
     return 0;
   }
-  const int len = c.lens[from];
+  len = c.lens[from];
   if (len < 0) bad |= QVX_MAP_NEGATIVE;
   if (len > (long long)c.table_width * c.page_size) bad |= QVX_MAP_COLUMNS;
   return len > 0 && len % c.page_size != 0;
@@ -100,14 +99,16 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
   __shared__ int place[kTogether];  // of this workgroup's forks: fresh pages of those before
   const int own = (int)blockIdx.x * kTogether, n = min(kTogether, c.n - own);
   const int tid = threadIdx.x, taken = c.taken_in[0];
+  if (tid < kTogether) from[tid] = 0, lens[tid] = 0;  // past the last fork: read like the others, not used
   if (tid == 0) all_bad = taken < 0 ? QVX_MAP_NEGATIVE : 0;
   int bad = 0, all = 0;
   for (int i0 = 0; i0 < c.n; i0 += kThreads) {
     const int i = i0 + tid;
-    const int wants = i < c.n ? fork_wants(c, i, bad) : 0;
-    int total;
+    const int source = i < c.n ? c.from[i] : 0, target = i < c.n ? c.to[i] : 0;
+    int total, len = 0;
+    const int wants = i < c.n ? fork_wants(c, source, target, len, bad) : 0;
     const int before = block_before<kThreads>(wants, part, total);
-    if (i >= own && i < own + n) place[i - own] = all + before;
+    if (i >= own && i < own + n) from[i - own] = source, to[i - own] = target, lens[i - own] = len, place[i - own] = all + before;
     all += total;
   }
   if (bad) atomicOr(&all_bad, bad);
@@ -121,13 +122,10 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(ForkCall c, int write) {
     *c.n_pairs = status ? 0 : all;
   }
   if (!(write & kForkRows) || status) return;
-  // What the workgroup's forks are is read before anything is stored: the compiler has to assume that a store changes it.
+  // All of it is read before anything is stored: the compiler has to assume that a store changes it.
   if (tid < n) {
-    from[tid] = c.from[own + tid], to[tid] = c.to[own + tid], lens[tid] = c.lens[from[tid]];
     const int at = taken + place[tid];
-    fresh[tid] = at < c.n_free ? c.free_list[at] : -1;  // lengths that another fork changes: no place
-  } else if (tid < kTogether) {
-    from[tid] = c.from[own], lens[tid] = 0;  // read like the others, not used
+    fresh[tid] = at < c.n_free ? c.free_list[at] : -1;  // a fork that wants none, or whose length another one changes
   }
   __syncthreads();
   for (int col = (int)blockIdx.y * kThreads + tid; col < c.table_width; col += (int)gridDim.y * kThreads) {
@@ -206,7 +204,7 @@ __global__ __launch_bounds__(1024) void k_free_count(FreeCall c) {
 // entries out.
 template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_store(FreeCall c) {
   __shared__ int part[16], bad_row;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, taken = ONE ? c.taken_in[0] : c.counts[gridDim.x];
   constexpr int kEach = (ONE ? 2 : 1) * kFreePages / 1024;
   if (tid == 0) bad_row = 0;
   if constexpr (MARK) {
@@ -216,18 +214,20 @@ template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_st
       free_column(c, g * kTogether, min(kTogether, c.n - g * kTogether), e - g * c.table_width);
     }
     free_lens(c, 0, c.n, tid);  // at most 1024 rows
-    __threadfence();  // the counts are taken where the atomics of all waves have arrived
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the counts are taken where the atomics of all waves have arrived
   }
   __syncthreads();
-  // a thread takes kEach pages in a row: one scan for all of them
-  const int p0 = (int)blockIdx.x * kFreePages + tid * kEach;
-  int flags = 0;
+  // a thread takes up to kEach pages in a row: one scan for all of them; no load waits for another
+  const int each = ONE ? (c.n_pages + 1023) / 1024 : kEach, p0 = (int)blockIdx.x * kFreePages + tid * each;
+  int flags = 0, held[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    if (p0 + j >= c.n_pages) break;
-    const int x = MARK ? __hip_atomic_load(&c.extra[p0 + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : c.extra[p0 + j];
-    flags |= (x < 0) << j;
+    const int* p = &c.extra[min(p0 + j, c.n_pages - 1)];
+    held[j] = 0;
+    if (j < each) held[j] = MARK ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p;
   }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) flags |= (j < each && p0 + j < c.n_pages && held[j] < 0) << j;
   if (blockIdx.x == 0)
     for (int i = tid; i < c.n; i += 1024)
       if ((unsigned)c.rows[i] >= (unsigned)c.n_rows) bad_row = 1;
@@ -243,7 +243,7 @@ template <bool ONE, bool MARK> __global__ __launch_bounds__(1024) void k_free_st
     all = block_sum<1024>(mine, part);
     at += block_sum<1024>(past, part);
   }
-  const int taken = ONE ? c.taken_in[0] : c.counts[gridDim.x], first = taken - all;  // negative: ids without a place are lost
+  const int first = taken - all;  // negative: ids without a place are lost
   at += first;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
@@ -365,9 +365,12 @@ __global__ __launch_bounds__(kThreads) void k_compact_list(CompactCall c) {
 // ---- copies ------------------------------------------------------------------------------------------
 //
 // Units of 16 KB (64 bytes a thread in four loads that go out together) of a pair's page of K or V of a cache, taken in
-// turn by as many workgroups as the card holds: the number of pairs is the device's.
+// turn by as many workgroups as the card holds: the number of pairs is the device's.  What is stored is marked as not needed
+// again: 128 pages of 16 layers 55.9 us with their forks and releases, 59.3 without the mark, 59.9 with loads marked as well;
+// 1080 of 8 layers 237, 239 and 232.
 
 constexpr int kCopyUnit = 16 << 10, kCopyWgs = 2048;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c, int parts) {
   const int each = c.n_caches * 2 * parts;
@@ -382,13 +385,13 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(CopyCall c, int parts) {
       const int64_t at = (int64_t)part * kCopyUnit + 16 * threadIdx.x;
       const uint8_t* from = base + src * x.stride;
       uint8_t* to = base + dst * x.stride;
-      uint4 w[4];
+      u32x4 w[4];  // a vector type of the compiler's: an array of structures is moved to LDS, each load waited for
+#pragma unroll
+      for (int j = 0; j < 4; ++j)  // past the page its last bytes again: a load in a branch would be waited for there
+        w[j] = *reinterpret_cast<const u32x4*>(from + min(at + j * 16 * kThreads, c.page_bytes - 16));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (at + j * 16 * kThreads < c.page_bytes) w[j] = *reinterpret_cast<const uint4*>(from + at + j * 16 * kThreads);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (at + j * 16 * kThreads < c.page_bytes) *reinterpret_cast<uint4*>(to + at + j * 16 * kThreads) = w[j];
+        if (at + j * 16 * kThreads < c.page_bytes) __builtin_nontemporal_store(w[j], reinterpret_cast<u32x4*>(to + at + j * 16 * kThreads));
     }
   }
 }
