@@ -142,12 +142,10 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
 
 bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 
-// Whether calls of so many rows a sequence (of a mean one) run on the kernel of many rows, and the partition's geometry
-// there: keys in a row, whatever their pages.  Sequences that share a prefix, 8 key heads, split kernel against that one: fp32
-// queries of 128 values 4000 keys 32 rows 25.4 and 26.4 us, 64 26.9 and 27.6, 96 34.7 and 29.3; 16000 keys 32 35.8 and 38.0, 64
-// 45.3 and 40.6; 1000 keys 64 20.1 and 26.2, 256 34.2 and 32.3; fp16 queries 4000 keys 32 25.2 and 22.8, 64 27.1 and 24.1.
-bool many_rows(const qvx_kv_cache* cache, int64_t rows, AttnCall& c) {
-  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 48) return false;
+// Whether calls of so many rows a sequence (of a mean one), more than `few`, run on the kernel of many rows, and the partition's
+// geometry there: keys in a row, whatever their pages.
+bool many_rows(const qvx_kv_cache* cache, int64_t rows, int few, AttnCall& c) {
+  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= few) return false;
   if (c.max_len > 0x7ffff000) return false;  // it looks up to 1024 keys past the last one by number
   c.table_page = c.page_size;
   c.page_size = c.max_len;
@@ -170,7 +168,7 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
   c.sinks = std::min(sinks, kMaxLen);
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
   const int64_t mean = ragged ? (rows + n_seqs - 1) / n_seqs : rows;
-  const bool many = many_rows(cache, mean, c);
+  const bool many = many_rows(cache, mean, 48, c);
   if (!many) c.tile_rows = tile_rows(mean);
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
@@ -222,9 +220,13 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   const int64_t rows = (int64_t)n_seqs * c.group;
   const int64_t mean = (rows + n_groups - 1) / n_groups;
   bool split = false;
+  // More than one row tile of the split kernel, which reads the keys again for each: 8 key heads of 128, fp16, 4 queries each, 30000
+  // keys 32 rows 52.8 us there and 41.2, 48 rows 61.4 and 42.8, 4000 keys 23.3 and 21.3, 25.4 and 22.3, 1000 the same.  Up to 64
+  // rows in row tiles of 64, waves in two groups on other keys: 30000 keys of 64 rows 43.8, of 128 rows half empty 51.2.
   // Every chunk leaves its partial results: two chunks a CU, of 128 keys at least.  64 sequences of 4 heads a group behind 1000
   // keys 28.6 us, with chunks of 256 32.2, of 512 41.5; 128 behind 8192, fp16, 61.6, with a chunk a CU 66.8.
-  if (many_rows(cache, mean, c)) {
+  if (many_rows(cache, mean, 16, c)) {
+    if (mean <= kAttnRows16 / 2) c.tile_rows = kAttnRows16 / 2;
     c.min_chunk = 8;
     c.target = std::max(1, kAttnWgs / c.kv_heads);
     if (!plan_items(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;

@@ -142,7 +142,7 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
 bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s) {
   const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
   bool ok = false;
-  if (c.tile_rows == kAttnRows16) {
+  if (c.tile_rows >= kAttnRows16 / 2) {
     const bool parts = c.q_type != type || !(c.scale2 >= 1e-30f);  // far above the subnormal numbers
     ok = type == T_F16 ? launch_attn_rows_f16(c, parts, grid, s) : launch_attn_rows_bf16(c, parts, grid, s);
     if (ok && join) launch_attn_join(c, s);

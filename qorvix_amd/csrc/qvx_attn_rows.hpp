@@ -3,8 +3,9 @@
 //
 //   out[row] = sum_j p_j v_j / sum_j p_j over the keys j that the row sees,  p_j = 2^(s_j - m),  s_j = scale log2(e) q[row] . k_j
 //
-// as in qvx_attn16.hip (128 rows a workgroup, 32 a wave; S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction; K and V
-// tiles staged in LDS, the next one in flight).  What is different:
+// as in qvx_attn16.hip (128 rows a workgroup, 32 a wave, or 64 in two groups of waves that take other keys and join at the end;
+// S^T = K Q^T and O^T = V^T P^T on the 32x32x16 instruction; K and V tiles staged in LDS, the next one in flight).  What is
+// different:
 //
 // Pages.  The keys' offsets are looked up 1024 at a time, half a block ahead, and stand in LDS, so a page may hold any
 // number of tokens.  Tiles are copied to LDS straight from the pages, NB - 1 tiles ahead.
@@ -39,7 +40,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kRows = kAttnRows16;
 constexpr float kSlackRows = 8.0f;
 template <uint32_t T> constexpr float kUpRows = T == T_F16 ? 15.0f : 0.0f;
 
@@ -143,8 +143,10 @@ template <int N, int OFF, int STEP> __device__ __forceinline__ void read_values(
 // N 16-byte LDS reads, waited for together: one by one each of them would be waited for before the product that needs it.
 template <int N> __device__ __forceinline__ void read_keys(u32x4 (&k)[N], const uint32_t (&a)[N]) {
 #define QVX_RD(o, at) "ds_read_b128 %" #o ", %" #at "\n\t"
-  static_assert(N == 4 || N == 5 || N == 6 || N == 8);
-  if constexpr (N == 4)
+  static_assert(N == 2 || N == 4 || N == 5 || N == 6 || N == 8);
+  if constexpr (N == 2)
+    asm volatile(QVX_RD(0, 2) QVX_RD(1, 3) "s_waitcnt lgkmcnt(0)" : "=&v"(k[0]), "=&v"(k[1]) : "v"(a[0]), "v"(a[1]) : "memory");
+  else if constexpr (N == 4)
     asm volatile(QVX_RD(0, 4) QVX_RD(1, 5) QVX_RD(2, 6) QVX_RD(3, 7) "s_waitcnt lgkmcnt(0)"
                  : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3])
                  : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
@@ -171,15 +173,16 @@ template <int N> __device__ __forceinline__ void read_keys(u32x4 (&k)[N], const 
 // What keys that are not there are loaded from.
 __device__ const uint32_t kZeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
-// W: workgroups a CU.
-template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W>
+// KT: keys of a round, of G groups of waves KT / G each, in 128 / G rows; W: workgroups a CU.
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W, int G>
 __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   using L = Tile<DP, KT>;
-  constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  constexpr int kRows = kAttnRows16 / G, KW = KT / G;  // keys of a wave's tile
+  constexpr int KS = DP / 16, DB = DP / 32, KB = KW / 32;
   constexpr int QP = !PARTS ? 1 : T == T_F16 ? 2 : 3, PP = PARTS ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_rows[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, h = lane >> 5;
+  const int col = lane & 31, h = lane >> 5, my_rows = 32 * (wave % (4 / G)), my_keys = wave / (4 / G) * KW;
   const int d = c.head_dim, item = (int)blockIdx.x / c.kv_heads, kvh = (int)blockIdx.x - item * c.kv_heads;
   AttnSums sums;
   AttnItem it = attn_item<kRows, M>(c, item, reinterpret_cast<int*>(lds_rows), sums);
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds_rows;
 
-  const int row = it.row0 + 32 * wave + col, my_row = min(row, it.rows - 1);
+  const int row = it.row0 + my_rows + col, my_row = min(row, it.rows - 1);
   const bool live = row < it.rows;
   const int64_t qat = attn_row(c, it.q0, my_row, kvh, c.q_stride);
   // What this lane's row sees, in numbers of keys: [0, first_end) and [low, high); and over the wave's rows.
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   // Over the wave's rows: least_low .. most_high and below most_first some row sees a key, wave_low .. wave_high all do.
   int wave_low = 0, wave_high = 0, most_high = 0, least_low = 0, most_first = 0;
   if constexpr (M == kMaskWindow) {  // they rise with the row
-    const int row_a = min(it.row0 + 32 * wave, it.rows - 1), row_b = min(row_a + 31, it.rows - 1);
+    const int row_a = min(it.row0 + my_rows, it.rows - 1), row_b = min(row_a + 31, it.rows - 1);
     const AttnRange ra = attn_range<M>(c, it, view, row_a), rb = attn_range<M>(c, it, view, row_b);
     least_low = ra.low - shift;
     wave_high = least_low + max(ra.high - ra.low, 0);
@@ -286,8 +289,8 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
     }
   };
 
-  const bool any_row = it.row0 + 32 * wave < it.rows;  // a wave past the rows only stages
-  constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
+  const bool any_row = it.row0 + my_rows < it.rows;  // a wave past the rows only stages
+  constexpr uint64_t kAll = KW == 64 ? ~0ull : (1ull << KW) - 1;
   constexpr int kTiles = kBlock / KT;  // of a block
   static_assert(kTiles - NB > kTiles / 2);  // a block is in place a tile before its first one is asked for
   // Copies a wave has on its way at least for each tile behind the next one: the next one has landed when no more are.
@@ -359,13 +362,14 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
 
   // Lane addresses of the transposing reads, as in qvx_attn16.hip; the swizzle of rows sixteen and eight apart is the same.
   constexpr int kV = DB % 4 == 0 ? 4 : DB % 3 == 0 ? 3 : DB % 2 == 0 ? 2 : 1;
-  constexpr int kK = QP == 3 && DP >= 128 && KS * KB % 4 == 0 ? 4 : KS * KB % 8 == 0 ? 8 : KS * KB % 6 == 0 ? 6 : KS * KB % 5 == 0 ? 5 : 4;
-  const uint32_t key_at = (uint32_t)(uintptr_t)lds;
+  constexpr int kK = QP == 3 && DP >= 128 && KS * KB % 4 == 0 ? 4 : KS * KB % 8 == 0 ? 8 : KS * KB % 6 == 0 ? 6 : KS * KB % 5 == 0 ? 5 : KS * KB % 4 == 0 ? 4 : 2;
+  static_assert(KS * KB % kK == 0 && DB % kV == 0);
+  const uint32_t key_at = (uint32_t)(uintptr_t)lds + (uint32_t)(my_keys * L::kPitch);
   uint32_t value_at[DB];
 #pragma unroll
   for (int e = 0; e < DB; ++e) {
     const int vrow = 4 * h + (lane & 15) / 4, vcol = 32 * e + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-    value_at[e] = (uint32_t)(uintptr_t)(lds + L::kBytes) + L::v_at(vrow, vcol / 8) + 2 * (vcol & 7);
+    value_at[e] = (uint32_t)(uintptr_t)(lds + L::kBytes) + (uint32_t)(my_keys * L::kPitch) + L::v_at(vrow, vcol / 8) + 2 * (vcol & 7);
   }
 
   float m = -INFINITY, l = 0.0f;
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
     wait_copies<0>();
   }
   auto whole = [&](int t) __attribute__((always_inline)) {
-    return (uint64_t)__ballot(offsets[t * KT % (2 * kBlock) + (lane & (KT - 1))] >= 0) & kAll;
+    return (uint64_t)__ballot(offsets[t * KT % (2 * kBlock) + my_keys + (lane & (KW - 1))] >= 0) & kAll;
   };
   uint64_t there = tiles > 0 ? whole(0) : 0;
   meet();
@@ -492,12 +496,12 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
       fetch(buf == 0 ? NB - 1 : buf - 1);  // the buffer that everyone left a barrier ago
       if (ahead + 1 < tiles) ask(ahead + 1);
     }
-    const int first = key0 + t * KT;
+    const int first = key0 + t * KT + my_keys;
     const uint64_t now = there;
     if (t + 1 < tiles) there = whole(t + 1);
     const bool none =
-        !any_row || now == 0 || ((first >= most_high || first + KT <= least_low) && first >= most_first);
-    if (!none) tile(first, buf, now, now != kAll || first < wave_low || first + KT > wave_high);
+        !any_row || now == 0 || ((first >= most_high || first + KW <= least_low) && first >= most_first);
+    if (!none) tile(first, buf, now, now != kAll || first < wave_low || first + KW > wave_high);
     // In the middle of a block the one before is no longer read, and the next one takes its place.
     if (t % kTiles == kTiles / 2) {
       const int block = t / kTiles + 1;
@@ -515,6 +519,28 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   l += __shfl_xor(l, 32);
   saw = __shfl_xor((int)saw, 32) || saw;
   if (saw) m = fmaxf(m, kAttnLow);
+  if constexpr (G == 2) {  // the second group's sums go to the first one's waves, through the tiles' place
+    static_assert(2 * (16 * DB + 2) * 64 * sizeof(float) <= NB * 2 * L::kBytes);
+    float* other = reinterpret_cast<float*>(lds_rows) + my_rows / 32 * (16 * DB + 2) * 64 + lane;
+    if (my_keys) {
+#pragma unroll
+      for (int e = 0; e < DB; ++e)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) other[(16 * e + r) * 64] = acc[e][r];
+      other[16 * DB * 64] = m;
+      other[(16 * DB + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (my_keys) return;
+    const float m1 = other[16 * DB * 64], l1 = other[(16 * DB + 1) * 64], both = fmaxf(m, m1);
+    const float base = both == -INFINITY ? 0.0f : both, f0 = attn_pow2(m - base), f1 = attn_pow2(m1 - base);
+    m = both;
+    l = l * f0 + l1 * f1;
+#pragma unroll
+    for (int e = 0; e < DB; ++e)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[e][r] = acc[e][r] * f0 + other[(16 * e + r) * 64] * f1;
+  }
   if (!live) return;
   if (it.chunks > 1 || M == kMaskPrefix) {  // a part of the keys
     const int d16 = (d + 15) & ~15, r16 = row - it.row0;
@@ -562,10 +588,10 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
     }
 }
 
-template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W>
+template <uint32_t T, int M, int DP, int KT, int NB, bool PARTS, int W, int G = 1>
 bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
   static LdsLimit lim;
-  const auto kernel = &k_attn_rows<T, M, DP, KT, NB, PARTS, W>;
+  const auto kernel = &k_attn_rows<T, M, DP, KT, NB, PARTS, W, G>;
   constexpr size_t lds = NB * 2 * (size_t)Tile<DP, KT>::kBytes + 2 * kBlock * sizeof(int64_t);
   static_assert(W * lds <= kLdsPerCU);
   if (!lds_ready(reinterpret_cast<const void*>(kernel), lim, lds)) return false;
@@ -573,10 +599,33 @@ bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
   return true;
 }
 
+// Row tiles of 64 rows, each wave's keys half of a round's.
+template <uint32_t T> bool launch_half(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
+  constexpr int M = kMaskPrefix;
+  const int d = c.head_dim;
+  if (!parts) {
+    if (d <= 32) return launch<T, M, 32, 64, 2, false, 3, 2>(c, grid, s);
+    if (d <= 64) return launch<T, M, 64, 64, 2, false, 3, 2>(c, grid, s);
+    if (d <= 96) return launch<T, M, 96, 64, 2, false, 2, 2>(c, grid, s);
+    if (d <= 128) return launch<T, M, 128, 64, 2, false, 2, 2>(c, grid, s);
+    if (d <= 160) return launch<T, M, 160, 64, 2, false, 1, 2>(c, grid, s);
+    return launch<T, M, 256, 64, 2, false, 1, 2>(c, grid, s);
+  }
+  if (d <= 32) return launch<T, M, 32, 64, 2, true, 3, 2>(c, grid, s);
+  if (d <= 64) return launch<T, M, 64, 64, 2, true, 2, 2>(c, grid, s);
+  if (d <= 96) return launch<T, M, 96, 64, 2, true, 2, 2>(c, grid, s);
+  if (d <= 128) return launch<T, M, 128, 64, 2, true, 2, 2>(c, grid, s);
+  if (d <= 160) return launch<T, M, 160, 64, 2, true, 1, 2>(c, grid, s);
+  return launch<T, M, 256, 64, 2, true, 1, 2>(c, grid, s);
+}
+
 // Tiles of 64 keys where the registers reach, of 32 with more of them on their way where queries in parts take two or three
 // times as many.
 template <uint32_t T, int M> bool launch_dp(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
   const int d = c.head_dim;
+  if constexpr (M == kMaskPrefix) {
+    if (c.tile_rows == kAttnRows16 / 2) return launch_half<T>(c, parts, grid, s);
+  }
   if (!parts) {
     if (d <= 32) return launch<T, M, 32, 64, 2, false, 3>(c, grid, s);
     if (d <= 64) return launch<T, M, 64, 64, 2, false, 3>(c, grid, s);

@@ -131,6 +131,18 @@ def test_a_long_prefix(cuda, t, q_same):
     check(cuda, c, 8, [0, 40], [8990], t if q_same and t != qvx.Q8_0 else qvx.F32)
 
 
+@pytest.mark.parametrize("t", (qvx.F16, qvx.BF16))
+@pytest.mark.parametrize("d", [24, 64, 96, 128, 152, 256])
+@pytest.mark.parametrize("n", [5, 9, 16])
+def test_groups_of_up_to_64_rows(cuda, t, d, n):
+    """20 to 64 rows of 16-bit and fp32 queries: waves on other keys of the same rows, prefixes that end in either's."""
+    for shared in (15, 40, 333, 2100):
+        lens = [shared + 5 * i for i in range(n)]
+        lens[1] = max(shared - 20, 0)
+        for q_type in (t, qvx.F32):
+            check(cuda, Cache(cuda, t, lens, 16, 2, d, seed=n), 8, [0, n], [shared], q_type)
+
+
 def test_sharp_logits(cuda):
     """Nearly all the weight on one key, in the prefix or in the rest."""
     for t in CACHE_TYPES:
