@@ -395,7 +395,7 @@ size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int
  * share q_type: F32, F16 or BF16; rows behind the last sequence's are left as they were.  A row that sees no key (positions
  * below 0, a window of 0 without sinks, pages outside the cache, which need not be held behind the window) gets zeros.
  * Keys that no query of the sequence sees are not read; values that another query of it sees are finite, also for those that do
- * not see them.  More than 48 rows (queries times q_heads / kv_heads) a sequence in the
+ * not see them.  More than 16 rows (queries times q_heads / kv_heads) a sequence in the
  * mean of the call over F16 or BF16 run on the 16-bit matrix cores: queries of the cache's own type as they are, at a scale of
  * 1e-30 or more, the softmax weights rounded once to it (2^-11, 2^-8); other queries as in qvx_attn_paged, the weights to 2^-22
  * over F16, 2^-18 over BF16.  All else, q = out, lengths, workspace, is as in qvx_attn_paged. */
@@ -413,7 +413,7 @@ size_t qvx_attn_window_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_head
  * are those on the pages of the group's first sequence, and are read once for all of them; the tokens behind are each
  * sequence's own.  The result is that of the whole rows: joined from the two parts' maxima and sums.  A sequence shorter
  * than d_shared[g] attends the first d_lens[b] of the shared tokens.  q and out share q_type: F32, F16 or BF16; the shared tokens
- * of groups of more than 16 rows in the mean are attended as qvx_attn_window says of its many.  Small batches of short tables read the shared
+ * of groups of more than 16 rows in the mean are attended as qvx_attn_window says.  Small batches of short tables read the shared
  * tokens once a sequence, in one launch, where that is faster.  All else is as in qvx_attn_paged; d_ws is always needed. */
 int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
                     const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens, int n_seqs,

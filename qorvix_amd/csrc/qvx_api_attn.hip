@@ -96,11 +96,10 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 // 45.3 and 68.2.  Chunks for two workgroups a CU: 32 on 4000 27.6 and 35.1 against 21.8 and 28.5; but 4 sequences of 32 rows on
 // 1500, 20 heads of 64, 15.5 against 17.3.
 bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
-  c.tile_rows = kAttnRows16;
   const int64_t whole = row_tiles * c.kv_heads;
   const bool split = whole < kAttnWgs / 2 && most_tiles(c) > 40 + whole / 2;
   c.min_chunk = split ? 16 : 0;
-  const bool sparse = 2 * (int64_t)c.n_q * c.group <= kAttnRows16 * row_tiles;
+  const bool sparse = 2 * (int64_t)c.n_q * c.group <= c.tile_rows * row_tiles;
   c.target = std::max(1, (sparse ? kAttnWgs : kAttnWgs / 2) / c.kv_heads);
   return plan_items(c, row_tiles, join, ws_bytes);
 }
@@ -142,15 +141,19 @@ int check_paged(const qvx_kv_cache* cache, int q_heads, int n_seqs, int table_wi
 
 bool q_type_ok(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 
-// Whether calls of so many rows a sequence (of a mean one), more than `few`, run on the kernel of many rows, and the partition's
-// geometry there: keys in a row, whatever their pages.
-bool many_rows(const qvx_kv_cache* cache, int64_t rows, int few, AttnCall& c) {
-  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= few) return false;
+// Whether calls of so many rows a sequence (of a mean one) run on the kernel of many rows, and the partition's geometry there: keys
+// in a row, whatever their pages.  Those of more than a row tile of the split kernel, which reads the keys again for each; up to 64
+// rows in row tiles of 64, waves in two groups on other keys.  8 key heads of 128 in fp16, split kernel against this one, fp32 and
+// fp16 queries: 8 sequences of 2000 tokens 20 rows 30.7 and 29.0, 30.4 and 28.2 us, 32 rows 30.9 and 32.2, 31.0 and 30.5, 48 rows
+// 47.8 and 34.6, 47.8 and 31.7; 32 of 16000 20 rows 471 and 369, 469 and 444, 48 rows 699 and 431, 694 and 451.  One prefix of 30000
+// tokens, 32 rows 52.8 and 41.2, 48 rows 61.4 and 42.8; 64 rows 43.8, in a row tile of 128 51.2.
+bool many_rows(const qvx_kv_cache* cache, int64_t rows, AttnCall& c) {
+  if ((cache->type != T_F16 && cache->type != T_BF16) || rows <= 16) return false;
   if (c.max_len > 0x7ffff000) return false;  // it looks up to 1024 keys past the last one by number
   c.table_page = c.page_size;
   c.page_size = c.max_len;
   c.page_tiles = (int)(((int64_t)c.max_len + kAttnTile - 1) / kAttnTile);
-  c.tile_rows = kAttnRows16;
+  c.tile_rows = rows <= kAttnRows16 / 2 ? kAttnRows16 / 2 : kAttnRows16;
   return true;
 }
 
@@ -168,7 +171,7 @@ int check_window(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, bool r
   c.sinks = std::min(sinks, kMaxLen);
   const int64_t rows = (int64_t)(ragged ? n_q : n_q / n_seqs) * c.group;
   const int64_t mean = ragged ? (rows + n_seqs - 1) / n_seqs : rows;
-  const bool many = many_rows(cache, mean, 48, c);
+  const bool many = many_rows(cache, mean, c);
   if (!many) c.tile_rows = tile_rows(mean);
   const int64_t row_tiles =
       ragged ? rows / c.tile_rows + n_seqs : n_seqs * ((rows + c.tile_rows - 1) / c.tile_rows);
@@ -220,13 +223,9 @@ int check_shared(const qvx_kv_cache* cache, uint32_t q_type, int q_heads, int n_
   const int64_t rows = (int64_t)n_seqs * c.group;
   const int64_t mean = (rows + n_groups - 1) / n_groups;
   bool split = false;
-  // More than one row tile of the split kernel, which reads the keys again for each: 8 key heads of 128, fp16, 4 queries each, 30000
-  // keys 32 rows 52.8 us there and 41.2, 48 rows 61.4 and 42.8, 4000 keys 23.3 and 21.3, 25.4 and 22.3, 1000 the same.  Up to 64
-  // rows in row tiles of 64, waves in two groups on other keys: 30000 keys of 64 rows 43.8, of 128 rows half empty 51.2.
   // Every chunk leaves its partial results: two chunks a CU, of 128 keys at least.  64 sequences of 4 heads a group behind 1000
   // keys 28.6 us, with chunks of 256 32.2, of 512 41.5; 128 behind 8192, fp16, 61.6, with a chunk a CU 66.8.
-  if (many_rows(cache, mean, 16, c)) {
-    if (mean <= kAttnRows16 / 2) c.tile_rows = kAttnRows16 / 2;
+  if (many_rows(cache, mean, c)) {
     c.min_chunk = 8;
     c.target = std::max(1, kAttnWgs / c.kv_heads);
     if (!plan_items(c, rows / c.tile_rows + n_groups, &split, &p.prefix_bytes)) return QVX_E_RANGE;

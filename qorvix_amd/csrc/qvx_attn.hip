@@ -171,6 +171,7 @@ void launch_attn_join(const AttnCall& c, hipStream_t s) {
     case 4: k_attn_join<4><<<grid, 256, 0, s>>>(c); break;
     case 8: k_attn_join<8><<<grid, 256, 0, s>>>(c); break;
     case 16: k_attn_join<16><<<grid, 256, 0, s>>>(c); break;
+    case kAttnRows16 / 2: k_attn_join<kAttnRows16 / 2><<<dim3(grid.x, grid.y, kJoinShares), 256, 0, s>>>(c); break;
     default: k_attn_join<kAttnRows16><<<dim3(grid.x, grid.y, kJoinShares), 256, 0, s>>>(c); break;
   }
 }

@@ -600,8 +600,7 @@ bool launch(const AttnCall& c, dim3 grid, hipStream_t s) {
 }
 
 // Row tiles of 64 rows, each wave's keys half of a round's.
-template <uint32_t T> bool launch_half(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
-  constexpr int M = kMaskPrefix;
+template <uint32_t T, int M> bool launch_half(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
   const int d = c.head_dim;
   if (!parts) {
     if (d <= 32) return launch<T, M, 32, 64, 2, false, 3, 2>(c, grid, s);
@@ -623,9 +622,7 @@ template <uint32_t T> bool launch_half(const AttnCall& c, bool parts, dim3 grid,
 // times as many.
 template <uint32_t T, int M> bool launch_dp(const AttnCall& c, bool parts, dim3 grid, hipStream_t s) {
   const int d = c.head_dim;
-  if constexpr (M == kMaskPrefix) {
-    if (c.tile_rows == kAttnRows16 / 2) return launch_half<T>(c, parts, grid, s);
-  }
+  if (c.tile_rows == kAttnRows16 / 2) return launch_half<T, M>(c, parts, grid, s);
   if (!parts) {
     if (d <= 32) return launch<T, M, 32, 64, 2, false, 3>(c, grid, s);
     if (d <= 64) return launch<T, M, 64, 64, 2, false, 3>(c, grid, s);
