@@ -394,11 +394,11 @@ size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int
  * n_q / n_seqs queries each (n_q % n_seqs != 0 -> QVX_E_SHAPE).  window and sinks not below 0 (else QVX_E_SHAPE).  q and out
  * share q_type: F32, F16 or BF16; rows behind the last sequence's are left as they were.  A row that sees no key (positions
  * below 0, a window of 0 without sinks, pages outside the cache, which need not be held behind the window) gets zeros.
- * Keys that no query of the sequence sees are not read; values that another query of it sees are finite, also for those that do
- * not see them.  More than 16 rows (queries times q_heads / kv_heads) a sequence in the
- * mean of the call over F16 or BF16 run on the 16-bit matrix cores: queries of the cache's own type as they are, at a scale of
- * 1e-30 or more, the softmax weights rounded once to it (2^-11, 2^-8); other queries as in qvx_attn_paged, the weights to 2^-22
- * over F16, 2^-18 over BF16.  All else, q = out, lengths, workspace, is as in qvx_attn_paged. */
+ * Keys that no query of the sequence sees are not read; values that another query of it sees are finite, also for those that
+ * do not see them.  Calls of more than 16 rows (queries times q_heads / kv_heads) a sequence in the mean over F16 or BF16 run on
+ * the 16-bit matrix cores: queries of the cache's own type as they are, at a scale of 1e-30 or more, the softmax weights rounded
+ * once to it (2^-11, 2^-8); other queries as in qvx_attn_paged, the weights to 2^-22 over F16, 2^-18 over BF16.  All else, q =
+ * out, lengths, workspace, is as in qvx_attn_paged. */
 int qvx_attn_window(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
                     const int32_t* d_offsets, int n_q, const qvx_kv_cache* cache, const int32_t* d_table, int table_width,
                     const int32_t* d_lens, int n_seqs, int window, int sinks, float scale, void* d_ws, size_t ws_bytes,

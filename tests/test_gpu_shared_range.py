@@ -115,6 +115,15 @@ def test_pieces_of_many_sequences(cuda, t, q_type, n):
     check(cuda, Cache(cuda, t, lens, 16, 1, 32, seed=n), 4, new, 40, 5, q_type)
 
 
+@pytest.mark.parametrize("t", (qvx.F16, qvx.BF16))
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 256])
+def test_few_new_tokens_over_a_long_past(cuda, t, d):
+    """17 to 64 rows a sequence whose keys are split over workgroups and joined, a sequence without new tokens between."""
+    for new, window, sinks in (([5, 0, 5], 1 << 20, 0), ([12, 1, 16], 1 << 20, 0), ([16, 0, 9], 700, 33)):
+        for q_type in (t, qvx.F32):
+            check(cuda, Cache(cuda, t, (5000, 40, 2999), 24, 1, d, seed=d), 5, new, window, sinks, q_type)
+
+
 @pytest.mark.parametrize("wide", [False, True])
 def test_two_graphs_at_once_on_streams_of_their_own(cuda, wide):
     """Each with its own workspace: replays beside each other leave what the calls one by one do."""
