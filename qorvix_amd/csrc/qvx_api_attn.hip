@@ -95,12 +95,15 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 // 114 (of one sequence 57.7 and 86.5 against 57.6 and 87.1), but seven ragged ones of 450 queries at most 57.3 and 85.3 against
 // 45.3 and 68.2.  Chunks for two workgroups a CU: 32 on 4000 27.6 and 35.1 against 21.8 and 28.5; but 4 sequences of 32 rows on
 // 1500, 20 heads of 64, 15.5 against 17.3.
+// Row tiles of 64 rows leave the matrix cores time: two chunks a CU, up to one row tile a CU.  60 rows each over 16000 keys, 20
+// sequences of 8 heads 423 us with a chunk a CU and 257 with two, 32 of 20 rows 441 and 364; but 40 of them over 5000 156 and 175.
 bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t whole = row_tiles * c.kv_heads;
-  const bool split = whole < kAttnWgs / 2 && most_tiles(c) > 40 + whole / 2;
+  const bool half = c.tile_rows < kAttnRows16;
+  const bool split = (half ? whole <= kAttnWgs / 2 : whole < kAttnWgs / 2) && most_tiles(c) > 40 + whole / 2;
   c.min_chunk = split ? 16 : 0;
   const bool sparse = 2 * (int64_t)c.n_q * c.group <= c.tile_rows * row_tiles;
-  c.target = std::max(1, (sparse ? kAttnWgs : kAttnWgs / 2) / c.kv_heads);
+  c.target = std::max(1, (sparse || half ? kAttnWgs : kAttnWgs / 2) / c.kv_heads);
   return plan_items(c, row_tiles, join, ws_bytes);
 }
 
