@@ -66,3 +66,21 @@ def test_workspaces_are_bounded(t):
     c = cache(type=t, kv_heads=8, head_dim=128)
     assert qvx.attn_window_ws(c, 0, 32, 4096, 64, 1 << 16, 1 << 30, 0) < 64 << 20
     assert qvx.attn_shared_ws(c, 0, 32, 256, 1 << 13, 1) < 96 << 20
+
+
+@pytest.mark.parametrize("kw", [dict(window=0), dict(window=-3), dict(sinks=1), dict(window=4, sinks=-1), dict(shared_groups=2),
+                                dict(shared_groups=-1), dict(window=4, shared_groups=1)])
+def test_a_step_refuses_masks_that_are_none(kw):
+    from test_decode import _paged_model, _paged_step
+    with pytest.raises(ValueError, match="PagedDecodeStep: a window"):
+        _paged_step(_paged_model(), **kw)
+
+
+def test_a_step_refuses_norms_that_are_not_a_heads():
+    import torch
+    from test_decode import _paged_model, _paged_step
+    for k, size in (("q_norm", 32), ("k_norm", 512)):
+        m = _paged_model()
+        m.norms[1][k] = torch.ones(size)
+        with pytest.raises(ValueError, match="layer 1 are of 64 values"):
+            _paged_step(m)
