@@ -1,5 +1,5 @@
 // qvx_attn_rows.hpp -- attention of many query rows over a paged 16-bit cache on gfx950's matrix cores, rows seeing parts of
-// their sequence's keys: the kernel behind qvx_attn_window for prompts and behind qvx_attn_shared's prefixes.
+// their sequence's keys: the kernel behind qvx_attn_window and behind qvx_attn_shared's prefixes for more than 16 rows.
 //
 //   out[row] = sum_j p_j v_j / sum_j p_j over the keys j that the row sees,  p_j = 2^(s_j - m),  s_j = scale log2(e) q[row] . k_j
 //
@@ -23,6 +23,7 @@
 // us (910 TFLOP/s); three pieces of up to 2500 tokens behind a window of 1024 84 us (510: 688 workgroups on 512 places, and
 // a start of three dependent loads, lengths, table, keys, before the first product, some 7 us each); 64 fp32 queries of 4 heads a
 // group over 8192 shared fp16 keys 35 us, 17.6 of them in the tiles, which is the rate of a large product with the parts counted.
+// Few rows of many sequences are bound by memory: 64 sequences of 16000 fp16 tokens and 5 new ones 693 us (4.2 GB, 6.1 TB/s).
 #pragma once
 
 #include "qvx_attn_split.hpp"
