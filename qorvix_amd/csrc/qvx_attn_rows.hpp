@@ -536,6 +536,7 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
     const float m1 = other[16 * DB * 64], l1 = other[(16 * DB + 1) * 64], both = fmaxf(m, m1);
     const float base = both == -INFINITY ? 0.0f : both, f0 = attn_pow2(m - base), f1 = attn_pow2(m1 - base);
     m = both;
+    saw = both != -INFINITY;  // a group that saw a key stands at kAttnLow or above: the row may have seen the other's alone
     l = l * f0 + l1 * f1;
 #pragma unroll
     for (int e = 0; e < DB; ++e)
