@@ -430,6 +430,18 @@ template <int R, int M> __device__ inline AttnView attn_view(const AttnCall& c, 
   v.end = v.high > v.low || v.first == 0 ? attn_tiles(c, v.high) : v.first;
   return v;
 }
+// A prefix ends where its group's longest sequence does: what stands behind that on the pages is no sequence's.
+__device__ inline void attn_held(const AttnCall& c, AttnItem& it) {
+  int held = min(max(c.lens[it.q0], 0), it.len);
+  const int nq = it.rows / c.group, lane = threadIdx.x & 63;
+  for (int i = 1; i < nq && held < it.len; i += 64) {  // each wave for itself; hardly ever: the first one holds all of it
+    int here = i + lane < nq ? min(max(c.lens[it.q0 + i + lane], 0), it.len) : 0;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) here = max(here, __shfl_xor(here, x));
+    held = max(held, here);
+  }
+  it.len = __builtin_amdgcn_readfirstlane(held);
+}
 // The keys that one row sees: those of [low, high) and of [0, sinks).
 struct AttnRange {
   int low, high, sinks;

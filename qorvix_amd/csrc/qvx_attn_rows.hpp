@@ -189,7 +189,10 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   AttnItem it = attn_item<kRows, M>(c, item, reinterpret_cast<int*>(lds_rows), sums);
   if constexpr (M == kMaskWindow) attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
-  if constexpr (M == kMaskPrefix) attn_leads<kRows>(c, it, kvh);
+  if constexpr (M == kMaskPrefix) {
+    attn_held(c, it);
+    attn_leads<kRows>(c, it, kvh);
+  }
   const AttnView view = attn_view<kRows, M>(c, it);
   it.tile1 = min(it.tile1, view.tiles());
   if constexpr (M == kMaskPrefix) it.seq = it.q0;  // the table's row
