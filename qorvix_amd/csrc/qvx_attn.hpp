@@ -101,7 +101,7 @@ struct AttnItem {
   int seq, len, q0, rows, row0;  // q0: the sequence's first query; rows: of the whole sequence
   int chunk, chunks, tile0, tile1;
   int slot;  // its place in the workspace, if chunks > 1
-  int lead, start;  // whole: the sequence that holds its first `start` keys
+  int lead, start;  // whole: the sequence that holds its first `start` keys, or ~ its group; prefix: that sequence
 };
 
 struct AttnSeq {
@@ -141,8 +141,9 @@ template <int R, int M> __device__ inline AttnSeq attn_masked_seq(const AttnCall
         const int mid = (g + end) / 2;
         if (c.groups[mid] <= b) g = mid; else end = mid;
       }
-      s.lead = g ? min(max(c.groups[g], 0), c.n_seqs - 1) : 0;
-      s.start = min(max(c.shared[g], 0), s.len);
+      const int first = g ? min(max(c.groups[g], 0), c.n_seqs - 1) : 0, keys = min(max(c.shared[g], 0), c.max_len);
+      s.lead = c.lens[first] >= keys ? first : ~g;
+      s.start = min(keys, s.len);
       // the tile in which the shared keys end stands for both parts
       s.tiles = attn_tiles(c, s.start) + (s.len > s.start ? attn_tiles(c, s.len) - attn_tile_of(c, s.start) : 0);
     } else if constexpr (M == kMaskRest) {
@@ -430,17 +431,35 @@ template <int R, int M> __device__ inline AttnView attn_view(const AttnCall& c, 
   v.end = v.high > v.low || v.first == 0 ? attn_tiles(c, v.high) : v.first;
   return v;
 }
-// A prefix ends where its group's longest sequence does: what stands behind that on the pages is no sequence's.
-__device__ inline void attn_held(const AttnCall& c, AttnItem& it) {
-  int held = min(max(c.lens[it.q0], 0), it.len);
-  const int nq = it.rows / c.group, lane = threadIdx.x & 63;
-  for (int i = 1; i < nq && held < it.len; i += 64) {  // each wave for itself; hardly ever: the first one holds all of it
-    int here = i + lane < nq ? min(max(c.lens[it.q0 + i + lane], 0), it.len) : 0;
+// A group's shared keys are read from the pages of the first of its sequences that holds most of them, hardly ever another than
+// the first of all, and end where that one does: what stands behind it is no sequence's.  Each wave looks for itself.
+struct AttnHolder {
+  int row, keys;
+};
+__device__ inline AttnHolder attn_holder(const AttnCall& c, int first, int end, int keys) {
+  AttnHolder h{first, min(max(c.lens[first], 0), keys)};
+  const int lane = threadIdx.x & 63;
+  for (int b0 = first + 1; b0 < end && h.keys < keys; b0 += 64) {
+    const int here = b0 + lane < end ? min(max(c.lens[b0 + lane], 0), keys) : 0;
+    int most = here;
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) here = max(here, __shfl_xor(here, x));
-    held = max(held, here);
+    for (int x = 1; x < 64; x *= 2) most = max(most, __shfl_xor(most, x));
+    most = __builtin_amdgcn_readfirstlane(most);
+    if (most > h.keys) h = {b0 + (int)__builtin_ctzll(__ballot(here == most)), most};
   }
-  it.len = __builtin_amdgcn_readfirstlane(held);
+  return {__builtin_amdgcn_readfirstlane(h.row), __builtin_amdgcn_readfirstlane(h.keys)};
+}
+// Where the item's shared keys are.
+template <int M> __device__ inline void attn_held(const AttnCall& c, AttnItem& it) {
+  if constexpr (M == kMaskPrefix) {
+    const AttnHolder h = attn_holder(c, it.q0, it.q0 + it.rows / c.group, it.len);
+    it.lead = h.row;
+    it.len = h.keys;
+  } else if (it.lead < 0) {
+    const int g = ~it.lead, end = g + 1 < c.n_groups && c.groups ? min(max(c.groups[g + 1], 0), c.n_seqs) : c.n_seqs;
+    const int first = g ? min(max(c.groups[g], 0), c.n_seqs - 1) : 0;
+    it.lead = attn_holder(c, first, end, min(max(c.shared[g], 0), c.max_len)).row;
+  }
 }
 // The keys that one row sees: those of [low, high) and of [0, sinks).
 struct AttnRange {

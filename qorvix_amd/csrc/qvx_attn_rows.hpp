@@ -190,12 +190,12 @@ __global__ __launch_bounds__(256, W) void k_attn_rows(AttnCall c) {
   if constexpr (M == kMaskWindow) attn_note(c, it, item, kvh, sums);
   if (!it.any) return;
   if constexpr (M == kMaskPrefix) {
-    attn_held(c, it);
+    attn_held<M>(c, it);
     attn_leads<kRows>(c, it, kvh);
   }
   const AttnView view = attn_view<kRows, M>(c, it);
   it.tile1 = min(it.tile1, view.tiles());
-  if constexpr (M == kMaskPrefix) it.seq = it.q0;  // the table's row
+  if constexpr (M == kMaskPrefix) it.seq = it.lead;  // the table's row
   __syncthreads();  // the item's words are read before tiles overwrite them
   const LdsPtr lds = (LdsPtr)lds_rows;
 

@@ -359,13 +359,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
   if constexpr (MASK) {
     if (M == kMaskWindow || M == kMaskWhole) attn_note(c, it, item, kvh, sums);  // what k_attn_join needs
     if (!it.any) return;
-    if constexpr (M == kMaskPrefix) {
-      attn_held(c, it);
-      attn_leads<R>(c, it, kvh);
-    }
+    if constexpr (M == kMaskPrefix || M == kMaskWhole) attn_held<M>(c, it);
+    if (M == kMaskPrefix) attn_leads<R>(c, it, kvh);
     view = attn_view<R, M>(c, it);
     it.tile1 = min(it.tile1, view.tiles());  // may end before tile0: a chunk without keys
-    if (M == kMaskPrefix) it.seq = it.q0;  // the table's row
+    if (M == kMaskPrefix) it.seq = it.lead;  // the table's row
   } else {
     attn_note(c, it, item, kvh, sums);
     if (!it.any) return;

@@ -607,8 +607,10 @@ class PagedDecodeStep:
     ``window``: every layer's attention sees that many last tokens and the first ``sinks`` (None: all).
     ``shared_groups``: groups of sequences that share their first tokens, which are then read once a group: the caller
     keeps ``groups`` [shared_groups + 1] (one group from the start) and ``shared`` [shared_groups] (0), tokens on
-    the pages of the group's first sequence, as ``fork`` leaves them; whole pages alone, since each sequence appends
-    to a last page of its own.  An emptied sequence belongs to a group of its own, or of no shared tokens.
+    the pages of the first of the group's sequences that is as long, as ``fork`` leaves them; whole pages alone, since each
+    sequence appends to a last page of its own.  Sequences may be emptied in any order: the others keep their prefix.  What an
+    emptied one holds from then on is its own only in a group of its own, or of no shared tokens, where it belongs before it is as
+    long as the shared ones: from then on they could be taken from its pages.
 
     Between steps, on the current stream: ``fork`` makes sequences copies of others, pages shared as far as they are full,
     ``release`` empties sequences, ``trim`` gives back what is behind their windows, ``compact`` brings the pages in use to the front (``taken[0]`` of them).  ``extra`` [n_pages]

@@ -64,3 +64,31 @@ def test_groups_of_many_rows(cuda, t, q_same, wide, n):
     for shared, longest in ((100, 90), (1500, 1401), (70, 1)):
         lens = [longest] + [max(longest - 7 * i, 0) for i in range(1, n)]
         check(cuda, Cache(cuda, t, lens, 16, 1, 128, seed=n), 4, [0, n], [shared], [0], t if q_same else qvx.F32, wide)
+
+
+def holders(lens, groups, shared):
+    """The first sequence of each group that holds most of its shared tokens."""
+    return [max(range(groups[g], groups[g + 1]), key=lambda b: min(lens[b], shared[g])) for g in range(len(shared))]
+
+
+@pytest.mark.parametrize("wide", (False, True))
+@pytest.mark.parametrize("t", CACHE_TYPES)
+@pytest.mark.parametrize("groups,shared,lens", [
+    ([0, 4], [64], (0, 100, 64, 70)), ([0, 4], [64], (3, 0, 17, 90)), ([0, 5], [300], (10, 200, 250, 40, 250)),
+    ([0, 2, 3, 6], [33, 20, 900], (5, 40, 0, 899, 900, 1000)), ([0, 3, 5], [48, 0], (0, 0, 0, 9, 0))])
+def test_the_first_sequence_is_shorter(cuda, t, wide, groups, shared, lens):
+    """Released and refilled first sequences: the others' tokens are read from one that holds them."""
+    check(cuda, Cache(cuda, t, lens, 16, 2, 64, seed=len(lens)), 8, groups, shared, holders(lens, groups, shared), wide=wide)
+
+
+@pytest.mark.parametrize("wide", (False, True))
+@pytest.mark.parametrize("t,q_type", [(qvx.F16, qvx.F16), (qvx.BF16, qvx.F32), (qvx.Q8_0, qvx.F32)])
+@pytest.mark.parametrize("n,at", [(20, 3), (100, 70), (300, 299)])
+def test_a_holder_far_behind(cuda, t, q_type, wide, n, at):
+    """Past a wave's lanes, and a workgroup's threads; in a group that begins at 0, and behind another."""
+    r = np.random.default_rng(n)
+    for cut in (0, 2):
+        lens = [int(x) for x in r.integers(0, 50, n)]
+        lens[at] = 200
+        groups, shared = ([0, 2, n], [10, 190]) if cut else ([0, n], [190])
+        check(cuda, Cache(cuda, t, lens, 16, 1, 32, seed=n), 4, groups, shared, holders(lens, groups, shared), q_type, wide)
