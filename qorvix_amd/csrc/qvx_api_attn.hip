@@ -337,7 +337,7 @@ int check_rope(void* d_q_out, int64_t q_out_stride, uint32_t q_out_type, const f
   if ((q_heads && (!d_q || !d_q_out)) || (cache && (!d_k || !d_v || !d_slots)) ||
       (rope->rot_dim && (!rope->d_inv_freq || !d_pos)))
     return QVX_E_NULL;
-  if (d_q == d_q_out && (q_stride != q_out_stride || q_out_type != T_F32)) return QVX_E_RANGE;
+  if (q_heads && d_q == d_q_out && (q_stride != q_out_stride || q_out_type != T_F32)) return QVX_E_RANGE;
   const uintptr_t size = q_out_type == T_F32 ? 4 : 2;
   if (q_out_type != T_F32 && !aligned(d_q_out, 2)) return QVX_E_RANGE;
   c.q_out = static_cast<float*>(d_q_out);
