@@ -191,9 +191,9 @@ __global__ __launch_bounds__(kThreads) void k_free_mark(FreeCall c) {
 // Pages freed in each range of kFreePages.
 __global__ __launch_bounds__(1024) void k_free_count(FreeCall c) {
   __shared__ int part[16];
-  const int p0 = (int)blockIdx.x * kFreePages;
+  const int p0 = (int)blockIdx.x * kFreePages, n = min(kFreePages, c.n_pages - p0);  // n_pages may be 2^31 - 1: no sum past it
   int mine = 0;
-  for (int p = p0 + threadIdx.x; p < min(p0 + kFreePages, c.n_pages); p += 1024) mine += c.extra[p] < 0;
+  for (int i = threadIdx.x; i < n; i += 1024) mine += c.extra[p0 + i] < 0;
   mine = block_sum<1024>(mine, part);
   if (threadIdx.x == 0) c.counts[blockIdx.x] = mine;
   // the count taken so far, as the next launch's first workgroup may overwrite it before the others read it
@@ -418,7 +418,7 @@ void launch_kv_free(const FreeCall& c, hipStream_t s) {
     k_free_store<true, false><<<1, 1024, 0, s>>>(c);
     return;
   }
-  const int blocks = (c.n_pages + kFreePages - 1) / kFreePages;
+  const int blocks = (c.n_pages - 1) / kFreePages + 1;
   k_free_count<<<blocks, 1024, 0, s>>>(c);
   k_free_store<false, false><<<blocks, 1024, 0, s>>>(c);
 }
