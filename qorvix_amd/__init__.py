@@ -454,13 +454,18 @@ def attn_paged_ws(cache: KvCache, q_heads: int, n_seqs: int, table_width: int) -
     return lib().qvx_attn_paged_ws(C.byref(cache), q_heads, n_seqs, table_width)
 
 
+def _tokens(n: int) -> int:
+    """A number of tokens as the call takes it: no sequence is longer than 2^31 - 1 (ctypes would cut off what is past 32 bits)."""
+    return max(-1, min(n, 2 ** 31 - 1))
+
+
 def attn_window(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, offsets: int, n_q: int,
                 cache: KvCache, table: int, table_width: int, lens: int, n_seqs: int, window: int, sinks: int, scale: float,
                 ws: int, ws_bytes: int, stream: int = 0) -> int:
     """Attention of each sequence's last tokens over the paged cache, with a window and first tokens that stay visible.
     Status."""
     return lib().qvx_attn_window(out, out_stride, q, q_stride, q_type, q_heads, offsets or None, n_q, C.byref(cache), table,
-                                 table_width, lens, n_seqs, window, sinks, scale, ws or None, ws_bytes, stream)
+                                 table_width, lens, n_seqs, _tokens(window), _tokens(sinks), scale, ws or None, ws_bytes, stream)
 
 
 def attn_window_ws(cache: KvCache, q_type, q_heads: int, n_q: int, n_seqs: int, table_width: int, window: int,
@@ -468,7 +473,7 @@ def attn_window_ws(cache: KvCache, q_type, q_heads: int, n_q: int, n_seqs: int, 
     """Bytes of attn_window's workspace; q_type a ggml type id or a torch dtype."""
     if not isinstance(q_type, int):
         q_type = _torch_types()[q_type]
-    return lib().qvx_attn_window_ws(C.byref(cache), q_type, q_heads, n_q, n_seqs, table_width, window, sinks)
+    return lib().qvx_attn_window_ws(C.byref(cache), q_type, q_heads, n_q, n_seqs, table_width, _tokens(window), _tokens(sinks))
 
 
 def attn_shared(out: int, out_stride: int, q: int, q_stride: int, q_type: int, q_heads: int, cache: KvCache, table: int,

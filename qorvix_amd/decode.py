@@ -657,7 +657,9 @@ class PagedDecodeStep:
             raise ValueError("PagedDecodeStep: a window or shared groups, not both")
         if (window is not None and window < 1) or sinks < 0 or (sinks and window is None) or not 0 <= shared_groups <= m:
             raise ValueError("PagedDecodeStep: a window is at least one token, sinks stand beside a window, groups hold sequences")
-        self.window, self.sinks, self.shared_groups = window, sinks, shared_groups
+        # past 2^31 - 1 tokens, the longest sequence, they are all
+        self.window, self.sinks = (n if n is None else min(n, 2 ** 31 - 1) for n in (window, sinks))
+        self.shared_groups = shared_groups
         self.qk_norms = []
         for l in range(len(model.layers)):
             pair = [model.norms[l].get(k) for k in ("q_norm", "k_norm")]
