@@ -164,13 +164,14 @@ class Model:
     eps: float = NORM_EPS
     rotation: Rotation = field(default_factory=Rotation)
     left_out: list = field(default_factory=list)  # the file's layer tensors that none of these weights stands for
+    sliding_window: int | None = None  # last tokens that the file's layers see, some of them or all
 
     def fused(self) -> "Model":
         """The same weights with each FUSED pair of a layer stacked into one device weight when the
         two share type and row length (the other projections are shared, not copied)."""
         import torch
         m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
-                  rotation=self.rotation, left_out=self.left_out)
+                  rotation=self.rotation, left_out=self.left_out, sliding_window=self.sliding_window)
         for layer in self.layers:
             out, used = {}, set()
             for name, (a, b) in FUSED:
@@ -191,7 +192,7 @@ class Model:
         import torch
         from . import interleave_rows16_t
         m = Model(lm_head=self.lm_head, norms=self.norms, output_norm=self.output_norm, eps=self.eps,
-                  rotation=self.rotation, left_out=self.left_out)
+                  rotation=self.rotation, left_out=self.left_out, sliding_window=self.sliding_window)
         for layer in self.layers:
             out = {k: w for k, w in layer.items() if k not in ("wq", "wk", "ffn_gate", "ffn_up")}
             wq, wk, wg, wu = layer["wq"], layer["wk"], layer["ffn_gate"], layer["ffn_up"]
@@ -312,7 +313,15 @@ class Model:
         m.eps = float(eps) if eps is not None else NORM_EPS
         m.rotation = Rotation.of_gguf(f, device)
         m.left_out = [name for name in Model.not_computed(f) if name not in taken]
+        m.sliding_window = Model.window_of(f)
         return m
+
+    @staticmethod
+    def window_of(f) -> int | None:
+        """A file's <arch>.attention.sliding_window (of several, one a layer, the shortest); None without one, or of 0."""
+        w = f.find(f"{f.architecture}.attention.sliding_window")
+        w = [x for x in (w if isinstance(w, list) else [w]) if type(x) is int and x > 0]
+        return min(w) if w else None
 
     @staticmethod
     def not_computed(f) -> list:
@@ -604,7 +613,8 @@ class PagedDecodeStep:
     a type of ``KvCache``; the rotation is the model's unless one is given, ``rope_base`` and ``rope_factors`` in
     place of its base and factors.  q and k heads are normed in layers whose norms have "q_norm" or "k_norm".
 
-    ``window``: every layer's attention sees that many last tokens and the first ``sinks`` (None: all).
+    ``window``: every layer's attention sees that many last tokens and the first ``sinks`` (None: all).  Of a file whose layers
+    see a window (``model.sliding_window``), a table of more tokens than that needs one, as long as the table for full attention.
     ``shared_groups``: groups of sequences that share their first tokens, which are then read once a group: the caller
     keeps ``groups`` [shared_groups + 1] (one group from the start) and ``shared`` [shared_groups] (0), tokens on
     the pages of the first of the group's sequences that is as long, as ``fork`` leaves them; whole pages alone, since each
@@ -657,6 +667,9 @@ class PagedDecodeStep:
             raise ValueError("PagedDecodeStep: a window or shared groups, not both")
         if (window is not None and window < 1) or sinks < 0 or (sinks and window is None) or not 0 <= shared_groups <= m:
             raise ValueError("PagedDecodeStep: a window is at least one token, sinks stand beside a window, groups hold sequences")
+        if window is None and model.sliding_window and max_pages * page_size > model.sliding_window:
+            raise ValueError(f"PagedDecodeStep: layers of the file see {model.sliding_window} tokens, the table holds "
+                             f"{max_pages * page_size}: pass a window")
         # past 2^31 - 1 tokens, the longest sequence, they are all
         self.window, self.sinks = (n if n is None else min(n, 2 ** 31 - 1) for n in (window, sinks))
         self.shared_groups = shared_groups
