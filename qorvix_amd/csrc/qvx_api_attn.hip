@@ -522,6 +522,7 @@ int qvx_attn_window(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
   c.table = d_table;
   c.lens = d_lens;
   c.scale2 = scale * kLog2e;
+  c.in_order = scale >= kLeastScale;
   c.ws = join ? static_cast<float*>(d_ws) : nullptr;
   c.q_wide = aligned(d_q, 16) && q_stride % 8 == 0;
   c.out_wide = aligned(d_out, 8) && out_stride % 4 == 0;
@@ -552,6 +553,7 @@ int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_
     c->table = d_table;
     c->lens = d_lens;
     c->scale2 = scale * kLog2e;
+    c->in_order = scale >= kLeastScale;
     c->leads = reinterpret_cast<AttnLead*>(ws);
     c->arrived = reinterpret_cast<int*>(ws + p.arrived_at);
     c->q_wide = aligned(d_q, 16) && q_stride % 8 == 0;

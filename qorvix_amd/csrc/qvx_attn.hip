@@ -40,7 +40,7 @@ namespace {
 // The order of the sums is the same in every run.
 // One row at a time throughout took 2048 tokens from 11.3 to 12.0 us, rows together throughout 65536 from 54.4 to 58.0.
 constexpr int kFewChunks = 16;
-constexpr int kJoinShares = 4;  // workgroups a piece of 128 rows: with one 32 row tiles on 700 states 26.4 us against 21.1, with 8 20.0,
+constexpr int kJoinShares = 4;  // workgroups a piece of 64 or 128 rows: of 128, with one 32 row tiles on 700 states 26.4 us against 21.1, with 8 20.0,
                                 // but on 4000 then 44.3 against 35.9
 
 template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
@@ -137,13 +137,13 @@ bool launch_attn_split(const AttnCall& c, uint32_t type, bool join, hipStream_t 
   return ok;
 }
 
-// The same for masked calls; row tiles of 128 rows are the kernel's of many rows, with 16-bit parts where q is of another
+// The same for masked calls; row tiles of 64 and 128 rows are the kernel's of many rows, with 16-bit parts where q is of another
 // type than the cache or its scale does not keep the order of the products.
 bool launch_attn_mask(const AttnCall& c, uint32_t type, bool join, hipStream_t s) {
   const dim3 grid((unsigned)c.items * (unsigned)c.kv_heads);
   bool ok = false;
   if (c.tile_rows >= kAttnRows16 / 2) {
-    const bool parts = c.q_type != type || !(c.scale2 >= 1e-30f);  // far above the subnormal numbers
+    const bool parts = c.q_type != type || !c.in_order;
     ok = type == T_F16 ? launch_attn_rows_f16(c, parts, grid, s) : launch_attn_rows_bf16(c, parts, grid, s);
     if (ok && join) launch_attn_join(c, s);
     return ok;
