@@ -55,9 +55,9 @@ def build(jobs: int | None = None) -> str:
     srcs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
     jobs = jobs or min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        # The largest sources first: qvx_gemv.hip alone takes as long as all others together on eight cores (200 s), and would
-        # otherwise start behind the many small ones.  Those of these that take 20 to 45 s, as they instantiate large headers, end
-        # long before it in any order.
+        # The largest sources first: qvx_gemv.hip takes 200 s, three times as long as all others together on eight cores, and
+        # would otherwise start behind the many small ones.  Small ones that instantiate large headers take 20 to 45 s and end long
+        # before it in any order.
         objs = list(ex.map(_compile, sorted(srcs, key=os.path.getsize, reverse=True)))
     tmp = LIB + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
