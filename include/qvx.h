@@ -409,14 +409,15 @@ size_t qvx_attn_window_ws(const qvx_kv_cache* cache, uint32_t q_type, int q_head
 
 /* Attention of one new token a sequence, as qvx_attn_paged, for batches that share long prefixes (forks, or a server's
  * common instructions): group g is the sequences d_groups[g] .. d_groups[g + 1] - 1 (the first begins at 0 and the last ends at
- * n_seqs, whatever the ends hold; d_groups NULL: one group; at most n_seqs of them, more -> QVX_E_RANGE), whose first d_shared[g] tokens
- * are those on the pages of the first of its sequences that is as long (of the first of the longest, where none is), and are read
- * once for all of them, whatever the others' rows hold there: a group goes on when its first sequence is released.  The tokens
- * behind are each sequence's own.  The result is that of the whole rows: joined from the two parts' maxima and sums.  A sequence shorter
- * than d_shared[g] attends the first d_lens[b] of the shared tokens, and what lies behind the group's longest one is not read; values
- * that another sequence of the group sees are finite, also for those that do not.  q and out share q_type: F32, F16 or BF16; the
- * shared tokens of groups of more than 16 rows in the mean are attended as qvx_attn_window says.  Small batches of short tables
- * read the shared tokens once a sequence, in one launch, where that is faster.  All else is as in qvx_attn_paged; d_ws is always needed. */
+ * n_seqs, whatever the ends hold; d_groups NULL: one group; at most n_seqs of them, more -> QVX_E_RANGE), whose first
+ * d_shared[g] tokens are those on the pages of the first of its sequences that has as many (of the first of the longest, where none
+ * has) and are read once for all of them, whatever the other rows hold there: a group goes on when its first sequence is
+ * released.  The tokens behind are each sequence's own.  The result is that of the whole rows: joined from the two parts' maxima
+ * and sums.  A sequence shorter than d_shared[g] attends the first d_lens[b] of the shared tokens, and what lies behind the group's
+ * longest one is not read; values that another sequence of the group sees are finite, also for those that do not.  q and out
+ * share q_type: F32, F16 or BF16; the shared tokens of groups of more than 16 rows in the mean are attended as qvx_attn_window
+ * says.  Small batches of short tables read the shared tokens once a sequence, in one launch, where that is faster.  All else is as
+ * in qvx_attn_paged; d_ws is always needed. */
 int qvx_attn_shared(void* d_out, int64_t out_stride, const void* d_q, int64_t q_stride, uint32_t q_type, int q_heads,
                     const qvx_kv_cache* cache, const int32_t* d_table, int table_width, const int32_t* d_lens, int n_seqs,
                     const int32_t* d_groups, const int32_t* d_shared, int n_groups, float scale, void* d_ws,

@@ -97,6 +97,8 @@ bool plan_split(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
 // 1500, 20 heads of 64, 15.5 against 17.3.
 // Row tiles of 64 rows leave the matrix cores time: two chunks a CU, up to one row tile a CU.  60 rows each over 16000 keys, 20
 // sequences of 8 heads 423 us with a chunk a CU and 257 with two, 32 of 20 rows 441 and 364; but 40 of them over 5000 156 and 175.
+// (Of as many queries each.  By offsets a row tile more a sequence has to be reckoned with, which passes that bound sooner: the first
+// two 417 and 435 us.)
 bool plan16(AttnCall& c, int64_t row_tiles, bool* join, size_t* ws_bytes) {
   const int64_t whole = row_tiles * c.kv_heads;
   const bool half = c.tile_rows < kAttnRows16;

@@ -40,8 +40,8 @@ namespace {
 // The order of the sums is the same in every run.
 // One row at a time throughout took 2048 tokens from 11.3 to 12.0 us, rows together throughout 65536 from 54.4 to 58.0.
 constexpr int kFewChunks = 16;
-constexpr int kJoinShares = 4;  // workgroups a piece of 64 or 128 rows: of 128, with one 32 row tiles on 700 states 26.4 us against 21.1, with 8 20.0,
-                                // but on 4000 then 44.3 against 35.9
+constexpr int kJoinShares = 4;  // workgroups a piece of 64 or 128 rows: of 128, with one 32 row tiles on 700 states 26.4 us
+                                // against 21.1, with 8 20.0, but on 4000 then 44.3 against 35.9
 
 template <int R> __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
   __shared__ __attribute__((aligned(16))) float4 vals[256];

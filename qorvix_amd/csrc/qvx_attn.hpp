@@ -41,7 +41,7 @@ struct AttnCall {
   int most_tiles;      // of a sequence of that length
   int n_seqs, kv_heads, group, head_dim;
   float scale2;     // scale * log2(e): the kernels work with powers of two
-  int tile_rows;    // query rows of a row tile: 4, 8 or 16 in the split kernel, 64 or 128 in the one of many rows, 128 in the 16-bit one
+  int tile_rows;    // query rows of a row tile: 4, 8 or 16 in the split kernel, 64 or 128 of many rows, 128 in the 16-bit one
   int items;        // bound on the work items of a key / value head; the grid is items * kv_heads
   int target, min_chunk;  // work items aimed at, fewest tiles of a chunk
   int slots;              // bound on the items of split sequences: the workspace's parts

@@ -19,11 +19,12 @@
 // so do the weights: two parts, which leave 2^-22 (fp16) or 2^-18 (bf16) of a weight.  The products of 16-bit values are
 // exact and all sums fp32, so the matrix cores do two to three times the work, an eighth of what fp32 instructions would take.
 //
-// Measured, 32 query and 8 key / value heads of 128, bf16, where a large product reaches 1155 TFLOP/s: a prompt of 8192 tokens 605
-// us (910 TFLOP/s); three pieces of up to 2500 tokens behind a window of 1024 84 us (510: 688 workgroups on 512 places, and
-// a start of three dependent loads, lengths, table, keys, before the first product, some 7 us each); 64 fp32 queries of 4 heads a
-// group over 8192 shared fp16 keys 35 us, 17.6 of them in the tiles, which is the rate of a large product with the parts counted.
-// Few rows of many sequences are bound by memory: 64 sequences of 16000 fp16 tokens and 5 new ones 693 us (4.2 GB, 6.1 TB/s).
+// Measured, 32 query and 8 key / value heads of 128, bf16, where a large product reaches 1155 TFLOP/s: a prompt of 8192 tokens 650
+// us (847 TFLOP/s; the matrix instructions busy a third of the cycles), with fp32 queries 1240; three pieces of up to 2500 tokens
+// behind a window of 1024 84 us (510: 688 workgroups on 512 places, and a start of three dependent loads, lengths, table, keys,
+// before the first product, some 7 us each), with fp32 queries 145; 64 fp32 queries of 4 heads a group over 8192 shared fp16 keys 35
+// us, the matrix instructions busy 6.8 of them.  Few rows of many sequences are bound by memory: 64 sequences of 16000 fp16 tokens
+// and 5 new ones 696 us (4.2 GB, 6.0 TB/s).
 #pragma once
 
 #include "qvx_attn_split.hpp"

@@ -39,7 +39,7 @@
 // order all the same.  kMaskWhole reads the prefix and the rest as one sequence, from two rows of the table.
 // Measured: 48 sequences of up to 32768 tokens behind a window of 4096, fp16, 60 us (248 MB; the join 6 in it), 16 behind
 // 8192 in Q8_0 66 (289 MB); 64 of up to 512 own tokens behind a prefix 18.9 (25 MB of keys and values, 33 of partial
-// results); 5 of 740 with 700 shared read whole 12.2.
+// results); 5 of 740 with 700 shared read whole 12.3.
 #pragma once
 
 #include "qvx_attn.hpp"
@@ -484,8 +484,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DT == 256 ? 1 : 2) void k_attn_spl
       for (int u = 0; u < VN; ++u) x.v[r][u].template load<AUX>(vr, hide(4 * g + r, voff[u] + r * c.pitch));
   };
   // Tiles in registers, one in work and one on its way where they fit: 131071 tokens in bf16 103 us against 111 with one.
-  // For eight rows of 128 values they do but for 1 to 22 registers (32 x 2000 tokens in bf16, 7 heads of 80 a group, 45 us
-  // against 77; 64 x 4096 in Q8_0 139 against 145), but not fp32 (8 heads of 128 a group 175 against 128) or 256 values.
+  // For eight rows of 128 values they do but for 1 to 22 registers, 8 to 50 with masks (32 x 2000 tokens in bf16, 7 heads of 80 a
+  // group, 45 us against 77; 64 x 4096 in Q8_0 139 against 145), but not fp32 (8 heads of 128 a group 175 against 128) or 256
+  // values.
   constexpr int kHeld = Tile::kRegs <= 64 && !(NS == 2 && (DT == 256 || (DT == 128 && T == T_F32))) ? 2 : 1;
   Tile held[kHeld];
   AttnQuery<T, KS> q;

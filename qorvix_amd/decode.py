@@ -623,8 +623,8 @@ class PagedDecodeStep:
     long as the shared ones: from then on they could be taken from its pages.
 
     Between steps, on the current stream: ``fork`` makes sequences copies of others, pages shared as far as they are full,
-    ``release`` empties sequences, ``trim`` gives back what is behind their windows, ``compact`` brings the pages in use to the front (``taken[0]`` of them).  ``extra`` [n_pages]
-    counts the rows that hold a page beside the first."""
+    ``release`` empties sequences, ``trim`` gives back what is behind their windows, ``compact`` brings the pages in use to
+    the front (``taken[0]`` of them).  ``extra`` [n_pages] counts the rows that hold a page beside the first."""
 
     def __init__(self, model: Model, m: int, heads: int, kv_heads: int, n_pages: int, max_pages: int,
                  page_size: int = 16, cache_type: int = F16, rope_base: float | None = None, rope_factors=None,
