@@ -423,7 +423,9 @@ template <int R, int M> __device__ inline AttnView attn_view(const AttnCall& c, 
     const int nq = it.rows / c.group, qa = it.row0 / c.group, qb = (min(it.row0 + R, it.rows) - 1) / c.group;
     v.p0 = it.len - nq;
     v.high = max(v.p0 + qb + 1, 0);
-    v.low = (int)min(max((long long)v.p0 + qa + 1 - c.window, 0ll), (long long)v.high);
+    // from the first row's first key to the last row's last: a row's keys end where the next one's begin, or later, but for a
+    // window of 0, of which no row sees any
+    v.low = c.window ? (int)min(max((long long)v.p0 + qa + 1 - c.window, 0ll), (long long)v.high) : v.high;
     v.sink_keys = min(c.sinks, v.high);
     v.first = attn_tile_of(c, v.low);
     v.sinks = attn_tiles(c, v.sink_keys);
