@@ -395,7 +395,7 @@ size_t qvx_attn_paged_ws(const qvx_kv_cache* cache, int q_heads, int n_seqs, int
  * share q_type: F32, F16 or BF16; rows behind the last sequence's are left as they were.  A row that sees no key (positions
  * below 0, a window of 0 without sinks, pages outside the cache, which need not be held behind the window) gets zeros.
  * Keys that no query of the sequence sees are not read; values that another query of it sees are finite, also for those that
- * do not see them.  Calls of more than 16 rows (queries times q_heads / kv_heads) a sequence in the mean over F16 or BF16 run on
+ * do not see them.  Calls of more than 16 rows (n_q times q_heads / kv_heads) a sequence in the mean over F16 or BF16 run on
  * the 16-bit matrix cores: queries of the cache's own type as they are, at a scale of 1e-30 or more, the softmax weights rounded
  * once to it (2^-11, 2^-8); other queries as in qvx_attn_paged, the weights to 2^-22 over F16, 2^-18 over BF16.  All else, q =
  * out, lengths, workspace, is as in qvx_attn_paged. */

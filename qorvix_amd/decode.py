@@ -614,7 +614,8 @@ class PagedDecodeStep:
     place of its base and factors.  q and k heads are normed in layers whose norms have "q_norm" or "k_norm".
 
     ``window``: every layer's attention sees that many last tokens and the first ``sinks`` (None: all).  Of a file whose layers
-    see a window (``model.sliding_window``), a table of more tokens than that needs one, as long as the table for full attention.
+    see a window (``model.sliding_window``), a table of more tokens than that needs one, as long as the table for full attention (behind shared
+    prefixes, which take no window: ``model.sliding_window = None``).
     ``shared_groups``: groups of sequences that share their first tokens, which are then read once a group: the caller
     keeps ``groups`` [shared_groups + 1] (one group from the start) and ``shared`` [shared_groups] (0), tokens on
     the pages of the first of the group's sequences that is as long, as ``fork`` leaves them; whole pages alone, since each
